@@ -338,6 +338,69 @@ int ltx_adaln(int64_t B, int64_t L, int64_t C, const void* x, int64_t x_bs, int6
               const void* scale, int64_t s_bs, int64_t s_ls, const void* shift, int64_t h_bs,
               int64_t h_ls, float eps, void* stream);
 
+/*
+ * Block-scaled linear layers (no counterpart in the reference, whose linears
+ * are bf16): the operators below hold activations and weights in 8 bits, or
+ * the weight in 4, with scales.
+ *
+ * 8-bit rows [R, K], K a multiple of LTX_MX_BLOCK: OCP e4m3 codes, row after
+ * row, and one E8M0 scale (2^(code - 127)) for every LTX_MX_BLOCK columns,
+ * laid out [ceil(K / 128)][R][4]: the four scales of a row's 128 columns are
+ * neighbours, and so are those of its neighbour rows.  Value = code * scale.
+ * Scale bytes past K are written as 0 and not read.
+ */
+#define LTX_MX_BLOCK 32
+
+/*
+ * ltx_adaln's gated residual update and modulated RMSNorm with the normalised
+ * rows as 8-bit rows: x' = x + y * gate, n = x' * rsqrt(mean x'^2 + eps) *
+ * (1 + scale) + shift, all in float32, x_out = bf16(x'), n rounded once to
+ * e4m3 under the block's scale: the smallest power of two, at least 2^-127,
+ * with which no finite value of the block passes 448.  A value that is not
+ * finite becomes NaN and does not count in its block's maximum.
+ *   Arguments as ltx_adaln.  eps < 0 skips the norm (and takes no scale /
+ *   shift): the rows x' themselves.  C a multiple of 32, at most 8192.
+ *   codes: [B * L, C] bytes, 16-byte aligned; scales: [ceil(C / 128)][B * L][4]
+ *   bytes, 4-byte aligned.
+ */
+int ltx_adaln_mx(int64_t B, int64_t L, int64_t C, const void* x, int64_t x_bs, int64_t x_ls,
+                 const void* y, int64_t y_bs, int64_t y_ls, const void* gate, int64_t g_bs, int64_t g_ls,
+                 void* x_out, int64_t xo_bs, int64_t xo_ls, const void* scale, int64_t s_bs, int64_t s_ls,
+                 const void* shift, int64_t h_bs, int64_t h_ls, float eps, void* codes, void* scales,
+                 void* stream);
+
+/*
+ * Linear layer of 8-bit rows with an 8-bit weight: y = act(a w^T + bias),
+ * products and sums on the scaled matrix cores (float32 accumulators), bias,
+ * activation and one rounding in the epilogue.
+ *   a: 8-bit rows [M, K], w: 8-bit rows [N, K] (codes 16-byte aligned, scales
+ *   4-byte aligned); K a multiple of 32, at most LTX_MX_MAX_K.  bias: bf16 [N]
+ *   or NULL.  act: 0 none, 1 tanh-GELU.
+ *   y_scales NULL: y is bf16 [M, N], rows y_ls elements apart.
+ *   y_scales given: y is 8-bit rows [M, N] (contiguous, y_ls unused; N a
+ *   multiple of 32) quantised as ltx_adaln_mx does.
+ */
+#define LTX_MX_MAX_K (1 << 20)
+int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_codes, const void* a_scales,
+                  const void* w_codes, const void* w_scales, const void* bias, int act, void* y,
+                  int64_t y_ls, void* y_scales, void* stream);
+
+/*
+ * ltx_skinny_linear with the weight in 4 bits: y = act(x) W^T + bias, bf16
+ * rows, float32 sums, W = e2m1 code * scale of its group.
+ *   x [M, K] rows x_ls apart (M <= LTX_GROUP4_MAX_ROWS, K a multiple of 32, at
+ *   most LTX_SKINNY_MAX_K), y [M, N] rows y_ls apart; x rows 16-byte aligned.
+ *   codes: [N, ceil(K / 128) * 64] bytes, 16-byte aligned; the byte c * 64 + p
+ *   * 16 + j * 4 + i of a row holds columns c * 128 + j * 32 + p * 8 + 2 * i (low
+ *   half) and the one after it (p, j, i in [0, 4)); columns past K hold 0.
+ *   scales: bf16 [N, K / group], group 32, 64 or 128 dividing K.
+ *   silu != 0 applies SiLU to x first (float32, rounded to bf16).
+ */
+#define LTX_GROUP4_MAX_ROWS 16
+int ltx_group4_linear(int64_t M, int64_t N, int64_t K, int64_t group, const void* x, int64_t x_ls, int silu,
+                      const void* codes, const void* scales, const void* bias, void* y, int64_t y_ls,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

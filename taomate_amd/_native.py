@@ -17,6 +17,7 @@ LIB_NAME = "libtaomate_ltx.so"
 F32, BF16, F8E4M3 = 0, 1, 2
 MAX_SEGMENTS = 16
 MAX_KEYLEN_BATCH = 16  # LTX_MAX_KEYLEN_BATCH
+GROUP4_MAX_ROWS = 16  # LTX_GROUP4_MAX_ROWS
 NOALLOC_SCRATCH_BYTES = 25 << 20  # LTX_NOALLOC_SCRATCH_BYTES
 ABI_VERSION = 2
 
@@ -63,6 +64,10 @@ SIGNATURES = {
     "ltx_skinny_linear": [_i64, _i64, _i64, _ptr, _i64, _int, _ptr, _i64, _ptr, _ptr, _i64, _ptr],
     "ltx_adaln": [_i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64,
                   _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _f32, _ptr],
+    "ltx_adaln_mx": [_i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64,
+                     _ptr, _i64, _i64, _ptr, _i64, _i64, _f32, _ptr, _ptr, _ptr],
+    "ltx_mx_linear": [_i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _int, _ptr, _i64, _ptr, _ptr],
+    "ltx_group4_linear": [_i64, _i64, _i64, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _i64, _ptr],
 }
 
 

@@ -15,12 +15,14 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -44,6 +46,9 @@ struct Api {
   decltype(&ltx_flash_attn_workspace_size) flash_attn_workspace_size;
   decltype(&ltx_adaln) adaln;
   decltype(&ltx_skinny_linear) skinny_linear;
+  decltype(&ltx_adaln_mx) adaln_mx;
+  decltype(&ltx_mx_linear) mx_linear;
+  decltype(&ltx_group4_linear) group4_linear;
 } api;
 PyObject* native_call_error = nullptr;  // taomate_amd._native.NativeCallError
 
@@ -523,6 +528,120 @@ void skinny_linear(PyObject* const* a) {
        (int)truth(a[4]), ptr(&w), w.stride(0), ptr(bias), ptr(&y), y.stride(0), stream_of(x));
 }
 
+// -------------------------------------------------------- block-scaled linears
+// These calls run on their tensors' device, whichever is current.
+void same_device(const char* what, const at::Tensor& first, std::initializer_list<Opt> others) {
+  need_gpu(&first);
+  for (Opt t : others) {
+    need_gpu(t);
+    if (t != nullptr && t->device() != first.device())
+      value_error(std::string(what) + ": tensors on " + first.device().str() + " and " + t->device().str());
+  }
+}
+
+struct MxRows {
+  int64_t rows, cols;
+};
+// 8-bit rows: codes [..., K] contiguous, scales [ceil(K / 128), rows, 4] contiguous.
+MxRows mx_rows(const char* what, const at::Tensor& codes, const at::Tensor& scales) {
+  if (codes.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kFloat8_e8m0fnu)
+    type_error(std::string(what) + ": 8-bit rows are float8_e4m3fn codes and float8_e8m0fnu scales");
+  if (codes.dim() < 1 || !codes.is_contiguous() || !scales.is_contiguous())
+    value_error(std::string(what) + ": 8-bit rows must be contiguous");
+  const int64_t K = codes.size(-1);
+  int64_t R = 1;
+  for (int64_t d = 0; d + 1 < codes.dim(); ++d) R *= codes.size(d);
+  if (K % LTX_MX_BLOCK != 0 || scales.dim() != 3 || scales.size(0) != (K + 127) / 128 || scales.size(1) != R ||
+      scales.size(2) != 4)
+    value_error(std::string(what) + ": codes " + shape(codes) + " (columns a multiple of 32) need scales [ceil(K / 128), " +
+                std::to_string(R) + ", 4], got " + shape(scales));
+  return {R, K};
+}
+
+// (x, y, gate, x_out, scale, shift, codes, scales, eps)
+void adaln_mx(PyObject* const* a) {
+  static const char* const names[6] = {"x", "y", "gate", "x_out", "scale", "shift"};
+  Opt t[6] = {&tensor(a[0])};
+  for (int i = 1; i < 6; ++i) t[i] = optional(a[i]);
+  const at::Tensor &x = *t[0], &codes = tensor(a[6]), &scales = tensor(a[7]);
+  same_device("adaln_mx", x, {t[1], t[2], t[3], t[4], t[5], &codes, &scales});
+  if (x.dim() != 3 || x.scalar_type() != at::kBFloat16) value_error("adaln_mx: x must be bf16 [B, L, C]");
+  const int64_t B = x.size(0), L = x.size(1), C = x.size(2);
+  struct {
+    void* p;
+    int64_t bs, ls;
+  } r[6] = {};
+  for (int i = 0; i < 6; ++i) {
+    if (t[i] == nullptr) continue;
+    const at::Tensor& o = *t[i];
+    const bool row = i == 2 || i >= 4;  // gate, scale, shift: one row per sample, or per token
+    if (o.scalar_type() != at::kBFloat16 || o.dim() != 3 || o.size(0) != B || o.size(2) != C ||
+        (C > 1 && o.stride(2) != 1) || (o.size(1) != L && !(row && o.size(1) == 1)))
+      value_error(std::string("adaln_mx: ") + names[i] + " must be bf16 [" + std::to_string(B) + ", " +
+                  std::to_string(L) + (row ? " or 1, " : ", ") + std::to_string(C) + "] with contiguous channels, got " +
+                  shape(o));
+    r[i] = {o.data_ptr(), B > 1 ? o.stride(0) : 0, o.size(1) > 1 ? o.stride(1) : 0};
+  }
+  const MxRows n = mx_rows("adaln_mx", codes, scales);
+  if (n.rows != B * L || n.cols != C) value_error("adaln_mx: codes " + shape(codes) + " for rows " + shape(x));
+  const c10::DeviceGuard guard(x.device());
+  call("ltx_adaln_mx", api.adaln_mx, B, L, C, r[0].p, r[0].bs, r[0].ls, r[1].p, r[1].bs, r[1].ls, r[2].p, r[2].bs,
+       r[2].ls, r[3].p, r[3].bs, r[3].ls, r[4].p, r[4].bs, r[4].ls, r[5].p, r[5].bs, r[5].ls,
+       a[8] == Py_None ? -1.0f : (float)real(a[8]), codes.data_ptr(), scales.data_ptr(), stream_of(x));
+}
+
+// (a_codes, a_scales, w_codes, w_scales, bias, y, y_scales, gelu)
+void mx_linear(PyObject* const* a) {
+  const at::Tensor &ac = tensor(a[0]), &as = tensor(a[1]), &wc = tensor(a[2]), &ws = tensor(a[3]), &y = tensor(a[5]);
+  const Opt bias = optional(a[4]), ys = optional(a[6]);
+  same_device("mx_linear", ac, {&as, &wc, &ws, bias, &y, ys});
+  const MxRows x = mx_rows("mx_linear", ac, as), w = mx_rows("mx_linear", wc, ws);
+  if (x.cols != w.cols || wc.dim() != 2)
+    value_error("mx_linear: rows " + shape(ac) + " and weight " + shape(wc) + " do not match");
+  if (bias != nullptr && (bias->scalar_type() != at::kBFloat16 || bias->dim() != 1 || bias->size(0) != w.rows ||
+                          (w.rows > 1 && bias->stride(0) != 1)))
+    value_error("mx_linear: bias must be a contiguous bf16 [" + std::to_string(w.rows) + "] vector");
+  int64_t y_ls = w.rows;
+  if (ys != nullptr) {
+    const MxRows o = mx_rows("mx_linear", y, *ys);
+    if (o.rows != x.rows || o.cols != w.rows)
+      value_error("mx_linear: result " + shape(y) + " for " + std::to_string(x.rows) + " rows of " +
+                  std::to_string(w.rows));
+  } else {
+    if (y.scalar_type() != at::kBFloat16) type_error("mx_linear: the result is bf16");
+    if (y.dim() != 2 || y.size(0) != x.rows || y.size(1) != w.rows || (w.rows > 1 && y.stride(1) != 1))
+      value_error("mx_linear: result " + shape(y) + " for " + std::to_string(x.rows) + " rows of " +
+                  std::to_string(w.rows));
+    if (x.rows > 1) y_ls = y.stride(0);
+  }
+  const c10::DeviceGuard guard(ac.device());
+  call("ltx_mx_linear", api.mx_linear, x.rows, w.rows, x.cols, ac.data_ptr(), as.data_ptr(), wc.data_ptr(),
+       ws.data_ptr(), ptr(bias), (int)truth(a[7]), y.data_ptr(), y_ls, ptr(ys), stream_of(ac));
+}
+
+// (x, codes, scales, bias, y, silu, columns)
+void group4_linear(PyObject* const* a) {
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &s = tensor(a[2]), &y = tensor(a[4]);
+  const Opt bias = optional(a[3]);
+  const int64_t K = integer(a[6]);
+  same_device("group4_linear", x, {&w, &s, bias, &y});
+  for (Opt t : {&x, &s, bias, &y})
+    if (t != nullptr && t->scalar_type() != at::kBFloat16) type_error("group4_linear: x, scales, bias and y must be bf16");
+  if (w.scalar_type() != at::kByte) type_error("group4_linear: codes must be uint8");
+  if (x.dim() != 2 || x.size(1) != K || x.stride(1) != 1 || w.dim() != 2 || !w.is_contiguous() || K < 1 ||
+      w.size(1) != (K + 127) / 128 * 64 || s.dim() != 2 || !s.is_contiguous() || s.size(0) != w.size(0) ||
+      s.size(1) < 1 || K % s.size(1) != 0 || y.dim() != 2 || y.size(0) != x.size(0) || y.size(1) != w.size(0) ||
+      (y.size(1) > 1 && y.stride(1) != 1))
+    value_error("group4_linear: x " + shape(x) + ", codes " + shape(w) + ", scales " + shape(s) + ", y " + shape(y) +
+                " for " + std::to_string(K) + " columns");
+  if (bias != nullptr && (bias->dim() != 1 || bias->size(0) != w.size(0) || (w.size(0) > 1 && bias->stride(0) != 1)))
+    value_error("group4_linear: bias must be a contiguous [N] vector");
+  const c10::DeviceGuard guard(x.device());
+  call("ltx_group4_linear", api.group4_linear, x.size(0), w.size(0), K, K / s.size(1), x.data_ptr(),
+       x.size(0) > 1 ? x.stride(0) : 0, (int)truth(a[5]), w.data_ptr(), s.data_ptr(), ptr(bias), y.data_ptr(),
+       y.size(0) > 1 ? y.stride(0) : 0, stream_of(x));
+}
+
 // is_eager(): whether an op on plain tensors would run as it is written, as far
 // as the thread's state tells: no gradients, autocast, torch function or dispatch
 // mode, function transform or trace (the last two and dispatch modes add keys to
@@ -610,6 +729,9 @@ PyObject* bind(PyObject*, PyObject* args) {
   get("ltx_flash_attn_workspace_size", next.flash_attn_workspace_size);
   get("ltx_adaln", next.adaln);
   get("ltx_skinny_linear", next.skinny_linear);
+  get("ltx_adaln_mx", next.adaln_mx);
+  get("ltx_mx_linear", next.mx_linear);
+  get("ltx_group4_linear", next.group4_linear);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: missing entry point addresses");
     return nullptr;
@@ -628,6 +750,9 @@ PyMethodDef methods[] = {
     {"flash_attn", (PyCFunction)(void*)&entry<flash_attn, 10>, METH_FASTCALL, nullptr},
     {"skinny_linear", (PyCFunction)(void*)&entry<skinny_linear, 5>, METH_FASTCALL, nullptr},
     {"adaln", (PyCFunction)(void*)&entry<adaln, 8>, METH_FASTCALL, nullptr},
+    {"adaln_mx", (PyCFunction)(void*)&entry<adaln_mx, 9>, METH_FASTCALL, nullptr},
+    {"mx_linear", (PyCFunction)(void*)&entry<mx_linear, 8>, METH_FASTCALL, nullptr},
+    {"group4_linear", (PyCFunction)(void*)&entry<group4_linear, 7>, METH_FASTCALL, nullptr},
     {"is_eager", is_eager, METH_NOARGS, nullptr},
     {"row_operands", (PyCFunction)(void*)&row_operands, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

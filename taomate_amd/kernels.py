@@ -11,6 +11,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import _native as N
+from .quant import Group4Weight, MXRows
 
 _DT = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.uint8: N.F8E4M3,
        torch.float8_e4m3fn: N.F8E4M3}
@@ -169,3 +170,46 @@ def adaln(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[torc
     gate), n_out = rms_norm(x_out or x) * (1 + scale) + shift (plain rms_norm
     without scale/shift).  gate/scale/shift are [B, 1 or L, C]."""
     (N._host or N.host()).adaln(x, y, gate, x_out, n_out, scale, shift, eps)
+
+
+def adaln_mx(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+             x_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+             shift: Optional[torch.Tensor] = None, eps: Optional[float] = 1e-6) -> MXRows:
+    """ltx_adaln_mx on bf16 [B, L, C] rows: ``adaln``'s residual update and
+    (modulated) RMS norm with the normalised rows returned in 8 bits, for
+    ``mx_linear``; x_out = x + y * gate in bf16.  float32 between its inputs and
+    outputs (``adaln`` rounds to bf16 where the reference's ops do).  eps None
+    skips the norm: the rows themselves.  C a multiple of 32, at most 8192."""
+    C = x.shape[-1]
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((C + 127) // 128, x.numel() // C if C else 0, 4, dtype=torch.float8_e8m0fnu, device=x.device)
+    (N._host or N.host()).adaln_mx(x, y, gate, x_out, scale, shift, codes, scales, eps)
+    return MXRows(codes, scales)
+
+
+def mx_linear(a: MXRows, weight: MXRows, bias: Optional[torch.Tensor] = None, gelu: bool = False,
+              quantize: bool = False):
+    """ltx_mx_linear: act(a @ weight.T + bias) for 8-bit rows ``a`` [..., K]
+    and an 8-bit ``weight`` [N, K]; bias bf16 [N]; tanh-GELU with ``gelu``.
+    Returns bf16 [..., N], or 8-bit rows with ``quantize`` (N a multiple of 32)."""
+    codes, w = a.codes, weight.codes
+    shape = codes.shape[:-1]
+    n, rows = w.shape[0], a.scales.shape[1]
+    host = N._host or N.host()
+    if quantize:
+        y = torch.empty(*shape, n, dtype=torch.float8_e4m3fn, device=codes.device)
+        ys = torch.empty((n + 127) // 128, rows, 4, dtype=torch.float8_e8m0fnu, device=codes.device)
+        host.mx_linear(codes, a.scales, w, weight.scales, bias, y, ys, gelu)
+        return MXRows(y, ys)
+    y = torch.empty(rows, n, dtype=torch.bfloat16, device=codes.device)
+    host.mx_linear(codes, a.scales, w, weight.scales, bias, y, None, gelu)
+    return y.view(*shape, n)
+
+
+def group4_linear(x: torch.Tensor, weight: Group4Weight, bias: Optional[torch.Tensor] = None,
+                  silu: bool = False) -> torch.Tensor:
+    """ltx_group4_linear: act(x) @ W.T + bias for x [M <= 16, K <= 4096] bf16
+    (SiLU of x first with ``silu``) and a 4-bit weight."""
+    y = torch.empty(x.shape[0], weight.codes.shape[0], dtype=x.dtype, device=x.device)
+    (N._host or N.host()).group4_linear(x, weight.codes, weight.scales, bias, y, silu, weight.columns)
+    return y

@@ -1,0 +1,91 @@
+"""ltx_group4_linear against float64: every row count, K at and around the
+128-column chunks, N around the 16-row tiles, every group, SiLU and bias."""
+import pytest
+import torch
+
+from taomate_amd import _native as N
+from taomate_amd import kernels, quant
+
+from .helpers import gen, randn
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def _weight(n, k, group, g):
+    return quant.quantize_group4(randn((n, k), g) * torch.exp(randn((n, 1), g)) / k ** 0.5, group)
+
+
+def _to(w, dev):
+    return quant.Group4Weight(w.codes.to(dev), w.scales.to(dev), w.columns)
+
+
+def check(x, w, b, silu, y):
+    xd = x.double()
+    # float32 sums of K products: within 2^-20 of the magnitudes; the result's rounding, half a bf16 step
+    extra = 0.0
+    if silu:
+        xd = xd * torch.sigmoid(xd)
+        extra = 2.0 ** -8    # SiLU rounded to bf16
+    wd = w.dequantize().double()
+    ref = xd @ wd.t() + (0 if b is None else b.double())
+    mag = xd.abs() @ wd.abs().t() + (0 if b is None else b.double().abs())
+    assert y.shape == ref.shape and y.dtype == BF
+    assert ((y.double().cpu() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * (2.0 ** -20 + extra) * mag).all()
+
+
+@pytest.mark.parametrize("silu", [False, True], ids=["plain", "silu"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,chunks,n", [(1, 1, 1), (2, 3, 17), (3, 2, 16), (4, 5, 40), (5, 4, 33), (7, 9, 300),
+                                        (8, 32, 130), (9, 8, 64), (15, 12, 47), (16, 32, 100), (2, 16, 4099)])
+def test_group4_linear(dev, M, chunks, n, group, silu):
+    g = gen(M * n + chunks + group)
+    k = group * chunks if group * chunks <= 4096 else 4096
+    x, w = randn((M, k), g, BF), _weight(n, k, group, g)
+    b = randn((n,), g, BF) if n % 2 else None
+    y = kernels.group4_linear(x.to(dev), _to(w, dev), None if b is None else b.to(dev), silu=silu)
+    check(x, w, b, silu, y)
+
+
+def test_strided_rows(dev):
+    g = gen(5)
+    big = randn((5, 512), g, BF)
+    w = _weight(48, 256, 64, g)
+    y = kernels.group4_linear(big.to(dev)[1:4, 128:384], _to(w, dev))
+    check(big[1:4, 128:384], w, None, False, y)
+
+
+def test_rows_do_not_meet(dev):
+    """NaN and infinities in one row of x stay in that row of y."""
+    g = gen(6)
+    x, w = randn((4, 160), g, BF), _weight(70, 160, 32, g)
+    clean = kernels.group4_linear(x.to(dev), _to(w, dev))
+    x[1, 7], x[2, 3] = float("nan"), float("inf")
+    y = kernels.group4_linear(x.to(dev), _to(w, dev))
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+    assert y[1].isnan().all() and not y[2].isfinite().all()
+
+
+def test_empty(dev):
+    w = _to(_weight(16, 64, 32, gen(1)), dev)
+    assert kernels.group4_linear(torch.empty(0, 64, dtype=BF, device=dev), w).shape == (0, 16)
+    none = quant.Group4Weight(w.codes[:0], w.scales[:0], 64)
+    assert kernels.group4_linear(torch.empty(3, 64, dtype=BF, device=dev), none).shape == (3, 0)
+
+
+def test_refusals(dev):
+    w = _to(_weight(16, 64, 32, gen(1)), dev)
+    x = torch.zeros(3, 64, device=dev, dtype=BF)
+    with pytest.raises(N.NativeCallError, match="M must be"):
+        kernels.group4_linear(torch.zeros(17, 64, device=dev, dtype=BF), w)
+    with pytest.raises(N.NativeCallError, match="group must be"):
+        kernels.group4_linear(x, quant.Group4Weight(w.codes, w.scales[:, :1].repeat(1, 4), 64))
+    with pytest.raises(N.NativeCallError, match="16-byte aligned"):
+        kernels.group4_linear(torch.zeros(3, 72, device=dev, dtype=BF)[:, 1:65], w)
+    with pytest.raises(ValueError, match="group4_linear"):
+        kernels.group4_linear(x[:, :32], w)
+    with pytest.raises(ValueError, match="contiguous"):
+        kernels.group4_linear(x, w, torch.zeros(15, device=dev, dtype=BF))
+    with pytest.raises(TypeError):
+        kernels.group4_linear(x.float(), w)

@@ -1,0 +1,121 @@
+"""The packers of the block-scaled linears on the CPU, against the formats'
+definitions written out, and what the wrappers refuse."""
+import math
+
+import pytest
+import torch
+
+from taomate_amd import _native, kernels, quant
+
+from .helpers import gen, randn
+
+BF = torch.bfloat16
+E4M3 = sorted({s * v for s in (1, -1) for v in
+               [m / 8 * 2.0 ** -6 for m in range(8)]
+               + [(1 + m / 8) * 2.0 ** (e - 7) for e in range(1, 16) for m in range(8) if (e, m) != (15, 7)]})
+
+
+def test_8bit_rows_are_the_nearest_values_under_the_smallest_scale():
+    x = randn((3, 5, 96), gen(1)) * torch.exp(4 * randn((96,), gen(2)))
+    x[0, 0, :32] = 0
+    x[0, 1, 0] = 448.0
+    x[0, 1, 1:32] = 1.0
+    x[0, 2, 32:64] = 449.0
+    q = quant.quantize_mx(x)
+    assert q.shape == x.shape and q.scales.shape == (1, 15, 4) and q.codes.dtype == torch.float8_e4m3fn
+    grid = torch.tensor(E4M3, dtype=torch.float64)
+    flat, codes = x.reshape(15, 3, 32).double(), q.codes.reshape(15, 3, 32).double()
+    byte = q.scales.view(torch.uint8)[0]
+    assert (byte[:, 3] == 0).all()
+    for r in range(15):
+        for b in range(3):
+            top = flat[r, b].abs().max().item()
+            k = -127 if top == 0 else max(-127, math.ceil(math.log2(top / 448)))
+            assert byte[r, b] == k + 127
+            t = flat[r, b] / 2.0 ** k
+            best = (t[:, None] - grid).abs().min(1).values
+            assert torch.equal((t - codes[r, b]).abs(), best)
+    d = q.dequantize().reshape(15, 3, 32).double()
+    assert torch.equal(d, codes * torch.exp2(byte[:, :3].double() - 127)[..., None])
+
+
+def test_8bit_rows_of_odd_values():
+    x = torch.zeros(4, 32)
+    x[0, 0], x[0, 1], x[0, 2] = float("nan"), float("inf"), 3.0
+    x[1] = float("-inf")
+    x[2, 0], x[2, 1] = 2.0 ** -149, -0.0
+    x[3, 0] = torch.finfo(torch.float32).max
+    q = quant.quantize_mx(x)
+    d = q.dequantize()
+    assert d[0, :2].isnan().all() and d[0, 2] == 3.0 and (d[0, 3:] == 0).all() and d[1].isnan().all()
+    assert q.scales.view(torch.uint8)[0, :, 0].tolist() == [120, 0, 0, 247] and (d[2] == 0).all()
+    # the nearest code stands for 2^128, which float32 does not hold
+    assert q.codes[3, 0].double() * 2.0 ** 120 == 2.0 ** 128 and d[3, 0].isinf()
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (3, 96, 32), (2, 192, 64), (5, 384, 128), (4, 160, 32)])
+def test_4bit_weight(n, k, group):
+    w = randn((n, k), gen(n + k))
+    w[0, :group] = 0
+    q = quant.quantize_group4(w, group)
+    assert q.shape == (n, k) and q.group == group and q.codes.shape == (n, -(-k // 128) * 64)
+    s = (w.reshape(n, -1, group).abs().amax(-1) / 6).to(BF)
+    assert torch.equal(q.scales, s)
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6])
+    grid = torch.cat([grid, -grid]).double()
+    t = w.double().reshape(n, -1, group)
+    sd = s.double()[..., None]
+    best = (t[..., None] - sd[..., None] * grid).abs().min(-1).values
+    got = (q.dequantize().double().reshape(n, -1, group) - t).abs()
+    assert (got <= best * (1 + 1e-6) + 1e-30).all()
+    # the packed order: byte c*64 + p*16 + j*4 + i of a row holds columns c*128 + j*32 + p*8 + 2i and the next
+    value = q.dequantize()
+    table = [0, .5, 1, 1.5, 2, 3, 4, 6, -0.0, -.5, -1, -1.5, -2, -3, -4, -6]
+    for r in range(n):
+        for at, byte in enumerate(q.codes[r].tolist()):
+            c, p, j, i = at // 64, at // 16 % 4, at // 4 % 4, at % 4
+            col = c * 128 + j * 32 + p * 8 + 2 * i
+            for half, col in ((byte & 15, col), (byte >> 4, col + 1)):
+                want = table[half] * float(s[r, col // group]) if col < k else 0.0
+                assert (float(value[r, col]) if col < k else float(table[half])) == want
+
+
+def test_4bit_ties_go_to_the_even_code():
+    w = torch.zeros(1, 32)
+    w[0, :9] = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -2.5])
+    assert quant.quantize_group4(w).dequantize()[0, :9].tolist() == [6.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, -2.0]
+
+
+def test_no_rows():
+    q = quant.quantize_mx(torch.empty(0, 2, 96))
+    assert q.shape == (0, 2, 96) and q.scales.shape == (1, 0, 4) and q.dequantize().shape == (0, 2, 96)
+    w = quant.quantize_group4(torch.empty(0, 160))
+    assert w.shape == (0, 160) and w.group == 32 and w.dequantize().shape == (0, 160)
+
+
+def test_packers_refuse():
+    with pytest.raises(ValueError, match="multiple of 32"):
+        quant.quantize_mx(torch.zeros(2, 48))
+    with pytest.raises(TypeError):
+        quant.quantize_mx(torch.zeros(2, 32, dtype=torch.int32))
+    with pytest.raises(ValueError, match="group must be"):
+        quant.quantize_group4(torch.zeros(2, 32), 16)
+    with pytest.raises(ValueError, match="multiple of 64"):
+        quant.quantize_group4(torch.zeros(2, 96), 64)
+    with pytest.raises(ValueError, match="not finite"):
+        quant.quantize_group4(torch.full((2, 32), float("inf")))
+    with pytest.raises(ValueError, match="groups must be"):
+        quant.Group4Weight.from_codes(torch.zeros(2, 16, dtype=torch.uint8), torch.zeros(2, 2, dtype=BF))
+
+
+def test_wrappers_refuse_on_the_host():
+    """What never reaches the library: CPU tensors and wrong objects."""
+    rows = quant.quantize_mx(torch.zeros(4, 64))
+    w4 = quant.quantize_group4(torch.zeros(8, 64))
+    for call in (lambda: kernels.adaln_mx(torch.zeros(1, 4, 64, dtype=BF)),
+                 lambda: kernels.mx_linear(rows, rows),
+                 lambda: kernels.group4_linear(torch.zeros(1, 64, dtype=BF), w4)):
+        with pytest.raises(ValueError, match="device tensors"):
+            call()
+    with pytest.raises(TypeError, match="expected 8 arguments"):
+        _native.host().mx_linear(rows.codes)
