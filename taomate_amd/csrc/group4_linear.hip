@@ -1,10 +1,32 @@
 // Linear layers over a few rows with 4-bit weights (gfx950): y = act(x) W^T +
-// bias, W = e2m1 code * bf16 scale of its group of 32, 64 or 128 columns.
+// bias for x [M <= 16, K <= 4096], W = e2m1 code * bf16 scale of its group of 32,
+// 64 or 128 columns: the timestep MLPs' linears with a quarter of the bytes.
+//
+// Bound by the read of W, once: 50 MB of codes and 6 MB of scales (groups of
+// 32) for 4096 -> 24576.  Vector products (one conversion per two weights, then
+// a dot product per row of x) would pass the read's time from about 4 rows on, so
+// the products run on the bf16 matrix cores, whose tile of 16 rows costs the
+// same for 1 row and for 16: a code is exact in bf16, v_cvt_scalef32_pk_bf16_fp4
+// makes two per instruction, and one v_mfma_f32_16x16x32_bf16 multiplies 16 rows
+// of W with all rows of x over the 32 columns of one group (w is the second
+// operand: a lane's four results all belong to one row of W, so the group's
+// scale is one float32 FMA each, unrounded).  That a 16-byte load of a lane holds
+// its 8 columns of four groups is the packed order of the codes.  Rows of x that do
+// not exist repeat the last one: their results are not stored.
+//
+// A workgroup has 8 waves: KS of them share a tile of 16 rows of W, each with up
+// to 4 chunks of 128 columns in flight, and meet in LDS; 8 / KS tiles at a time.
+// x (SiLU applied, rounded to bf16 as the tensor op rounds) is staged in LDS
+// once per workgroup, which then strides over the tiles.
+
 #include "ltx_common.h"
 
 namespace ltx {
 
-constexpr int kG4Threads = 256;
+constexpr int kG4Waves = 8, kG4Chunks = 4;
+
+typedef __bf16 g4_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float g4_f4 __attribute__((ext_vector_type(4)));
 
 struct Group4Args {
   const uint16_t* x;
@@ -15,46 +37,138 @@ struct Group4Args {
   uint16_t* y;
   int64_t y_ls;
   int64_t N;
-  int M, K, group, silu;
+  int M, K, silu;
 };
 
-// One wave per row of W: lanes stride over its 16-byte pieces.
-__global__ void __launch_bounds__(kG4Threads) group4_linear_kernel(const Group4Args a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * (kG4Threads / 64) + (threadIdx.x >> 6);
-  if (n >= a.N) return;
-  const int chunks = (a.K + 127) / 128;
-  float acc[LTX_GROUP4_MAX_ROWS] = {};
-  for (int i = lane; i < chunks * 4; i += 64) {
-    const uint4 w = *reinterpret_cast<const uint4*>(a.codes + n * chunks * 64 + (int64_t)i * 16);
-    for (int j = 0; j < 4; ++j) {
-      const int k = (i >> 2) * 128 + j * 32 + (i & 3) * 8;
-      if (k >= a.K) break;
-      const float s = bf16_bits_to_f32(a.scales[n * (a.K / a.group) + k / a.group]);
-      const uint32_t word = (&w.x)[j];
-      float v[8];
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t c = (word >> (4 * e)) & 15u, m = c & 7u;
-        const float mag = m < 2u ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-        v[e] = (c & 8u) ? -mag * s : mag * s;
+// SiLU through one exp2 and one reciprocal (1 ulp each), rounded to bf16 after.
+__device__ __forceinline__ float g4_silu(float v) {
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
+}
+
+// 8 codes (lower half of byte 0 first) as bf16.
+__device__ __forceinline__ g4_bf16x8 g4_decode(uint32_t w) {
+  const ltx_bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0);
+  const ltx_bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1);
+  const ltx_bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2);
+  const ltx_bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3);
+  const auto ab = __builtin_shufflevector(a, b, 0, 1, 2, 3), cd = __builtin_shufflevector(c, d, 0, 1, 2, 3);
+  return __builtin_shufflevector(ab, cd, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// KS waves per tile, GROUP columns per scale.
+template <int KS, int GROUP>
+__global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Group4Args a) {
+  constexpr int kTiles = kG4Waves / KS, kPer = 128 / GROUP;  // tiles per workgroup; scales per chunk and row
+  extern __shared__ uint4 xs[];                              // [M][chunks * 16 + 1]
+  __shared__ float part[2][kG4Waves][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r16 = lane & 15, p = lane >> 4, kw = wave % KS;
+  const int chunks = (a.K + 127) / 128, groups = a.K / GROUP, row_words = chunks * 16 + 1;
+  const int64_t tiles = (a.N + 15) / 16;
+
+  uint4 w[kG4Chunks];
+  uint16_t s[kG4Chunks][kPer];
+  auto load = [&](int64_t tile) {
+    const int64_t n = tile * 16 + r16 < a.N ? tile * 16 + r16 : a.N - 1;
+#pragma unroll
+    for (int i = 0; i < kG4Chunks; ++i) {
+      const int c = kw + i * KS;
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (c < chunks) w[i] = *reinterpret_cast<const uint4*>(a.codes + (n * chunks + c) * 64 + p * 16);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        s[i][j] = 0;
+        if (c * kPer + j < groups) s[i][j] = a.scales[n * groups + c * kPer + j];
       }
-      for (int m = 0; m < a.M; ++m)
-        for (int e = 0; e < 8; ++e) {
-          float xv = bf16_bits_to_f32(a.x[m * a.x_ls + k + e]);
-          if (a.silu) xv = bf16_bits_to_f32(f32_to_bf16_bits(xv / (1.0f + expf(-xv))));
-          acc[m] = fmaf(xv, v[e], acc[m]);
-        }
     }
+  };
+  int64_t tile = (int64_t)blockIdx.x * kTiles + wave / KS;
+  const int64_t stride = (int64_t)gridDim.x * kTiles;
+  if (tile < tiles) load(tile);  // the first rows of W travel while x is staged
+  for (int i = threadIdx.x; i < a.M * chunks * 16; i += 64 * kG4Waves) {
+    const int m = i / (chunks * 16), c = i - m * (chunks * 16);
+    uint4 v = make_uint4(0, 0, 0, 0);  // columns past K: their codes are 0, so x must be finite there
+    if (c * 8 < a.K) v = *reinterpret_cast<const uint4*>(a.x + m * a.x_ls + c * 8);
+    if (a.silu) {
+      uint32_t* q = &v.x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        q[e] = pack_bf16x2(g4_silu(bf16_bits_to_f32(q[e] & 0xFFFFu)), g4_silu(bf16_bits_to_f32(q[e] >> 16)));
+    }
+    xs[m * row_words + c] = v;
   }
-  for (int m = 0; m < a.M; ++m) {
-    float t = acc[m];
-    for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
-    if (lane == 0) {
-      if (a.bias != nullptr) t += bf16_bits_to_f32(a.bias[n]);
-      a.y[m * a.y_ls + n] = f32_to_bf16_bits(t);
+  __syncthreads();
+  const uint4* xr = xs + min(r16, a.M - 1) * row_words + p;
+  // every workgroup runs the same number of rounds in all its waves
+  const int64_t first = (int64_t)blockIdx.x * kTiles;
+  int buf = 0;
+  for (int64_t t0 = first; t0 < tiles; t0 += stride, tile += stride, buf ^= 1) {
+    g4_f4 acc = {};
+    if (tile < tiles) {
+#pragma unroll
+      for (int i = 0; i < kG4Chunks; ++i) {
+        const int c = kw + i * KS;
+        if (c < chunks) {  // uniform across the wave
+          const uint32_t* wp = &w[i].x;
+          g4_f4 d = {};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const g4_bf16x8 xv = __builtin_bit_cast(g4_bf16x8, xr[c * 16 + j * 4]);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, g4_decode(wp[j]), d, 0, 0, 0);
+            if ((j + 1) * 32 % GROUP == 0) {
+              const float sc = bf16_bits_to_f32(s[i][j * 32 / GROUP]);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[r] = fmaf(d[r], sc, acc[r]);
+              d = g4_f4{};
+            }
+          }
+        }
+      }
+    }
+    if (tile + stride < tiles) load(tile + stride);  // the next rows travel during the reduction
+    // lane: rows 4 p .. + 3 of x, row r16 of the tile
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[buf][wave][p * 4 + r][r16] = acc[r];
+    __syncthreads();  // the buffer written a round ago is read before this barrier, rewritten after it
+    for (int i = threadIdx.x; i < kTiles * 256; i += 64 * kG4Waves) {
+      const int tw = i >> 8, m = (i >> 4) & 15, c = i & 15;
+      const int64_t n = (t0 + tw) * 16 + c;
+      if (m < a.M && n < a.N) {
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) v += part[buf][tw * KS + k][m][c];
+        if (a.bias != nullptr) v += bf16_bits_to_f32(a.bias[n]);
+        a.y[m * a.y_ls + n] = f32_to_bf16_bits(v);
+      }
     }
   }
 }
+
+template <int KS, int GROUP>
+void launch_group4(const Group4Args& a, hipStream_t st) {
+  const int chunks = (a.K + 127) / 128;
+  const size_t lds = (size_t)a.M * (chunks * 16 + 1) * 16;
+  const size_t all = lds + sizeof(float) * 2 * kG4Waves * 16 * 17;
+  // resident workgroups per CU: what the LDS holds, at most 2 (16 waves)
+  const int64_t most = 256 * (all > 80 * 1024 ? 1 : 2), want = ceil_div(ceil_div(a.N, 16), kG4Waves / KS);
+  hipLaunchKernelGGL((group4_linear_kernel<KS, GROUP>), dim3((unsigned)(want < most ? want : most)),
+                     dim3(64 * kG4Waves), lds, st, a);
+}
+
+template <int GROUP>
+void launch_group4(const Group4Args& a, hipStream_t st) {
+  // as few waves per tile as hold its columns in flight (4 chunks of 128 each)
+  const int chunks = (a.K + 127) / 128;
+  if (chunks <= kG4Chunks)
+    launch_group4<1, GROUP>(a, st);
+  else if (chunks <= 2 * kG4Chunks)
+    launch_group4<2, GROUP>(a, st);
+  else if (chunks <= 4 * kG4Chunks)
+    launch_group4<4, GROUP>(a, st);
+  else
+    launch_group4<8, GROUP>(a, st);
+}
+static_assert(LTX_SKINNY_MAX_K <= 8 * kG4Chunks * 128, "8 waves hold a row of W");
 
 }  // namespace ltx
 
@@ -75,9 +189,14 @@ extern "C" int ltx_group4_linear(int64_t M, int64_t N, int64_t K, int64_t group,
   LTX_REQUIRE((uintptr_t)x % 16 == 0 && x_ls % 8 == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 2 == 0,
               "ltx_group4_linear: x rows and codes must be 16-byte aligned");
   Group4Args a{(const uint16_t*)x, x_ls, (const uint8_t*)codes, (const uint16_t*)scales, (const uint16_t*)bias,
-               (uint16_t*)y, y_ls, N, (int)M, (int)K, (int)group, silu};
-  hipLaunchKernelGGL(group4_linear_kernel, dim3((unsigned)ceil_div(N, kG4Threads / 64)), dim3(kG4Threads), 0,
-                     reinterpret_cast<hipStream_t>(stream), a);
+               (uint16_t*)y, y_ls, N, (int)M, (int)K, silu};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (group == 32)
+    launch_group4<32>(a, st);
+  else if (group == 64)
+    launch_group4<64>(a, st);
+  else
+    launch_group4<128>(a, st);
   LTX_LAUNCH_CHECK("ltx_group4_linear");
   return LTX_OK;
 }
