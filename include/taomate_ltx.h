@@ -390,10 +390,11 @@ int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_codes, const vo
  * rows, float32 sums, W = e2m1 code * scale of its group.
  *   x [M, K] rows x_ls apart (M <= LTX_GROUP4_MAX_ROWS, K a multiple of 32, at
  *   most LTX_SKINNY_MAX_K), y [M, N] rows y_ls apart; x rows 16-byte aligned.
- *   codes: [N, ceil(K / 128) * 64] bytes, 16-byte aligned; the byte c * 64 + p
- *   * 16 + j * 4 + i of a row holds columns c * 128 + j * 32 + p * 8 + 2 * i (low
- *   half) and the one after it (p, j, i in [0, 4)); columns past K hold 0.
- *   scales: bf16 [N, K / group], group 32, 64 or 128 dividing K.
+ *   codes: [ceil(N / 16)][ceil(K / 128)][4][16][16] bytes, 16-byte aligned: byte
+ *   [t][c][p][r][4 j + i] holds row 16 t + r, columns 128 c + 32 j + 8 p + 2 i (low
+ *   half) and the one after it (p, j, i in [0, 4)); scales: bf16
+ *   [ceil(N / 16)][ceil(K / 128)][16][128 / group], 8-byte aligned, group 32, 64 or
+ *   128 dividing K.  Codes and scales past N or K are 0.
  *   silu != 0 applies SiLU to x first (float32, rounded to bf16).
  */
 #define LTX_GROUP4_MAX_ROWS 16

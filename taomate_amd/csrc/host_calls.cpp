@@ -628,16 +628,18 @@ void group4_linear(PyObject* const* a) {
   for (Opt t : {&x, &s, bias, &y})
     if (t != nullptr && t->scalar_type() != at::kBFloat16) type_error("group4_linear: x, scales, bias and y must be bf16");
   if (w.scalar_type() != at::kByte) type_error("group4_linear: codes must be uint8");
-  if (x.dim() != 2 || x.size(1) != K || x.stride(1) != 1 || w.dim() != 2 || !w.is_contiguous() || K < 1 ||
-      w.size(1) != (K + 127) / 128 * 64 || s.dim() != 2 || !s.is_contiguous() || s.size(0) != w.size(0) ||
-      s.size(1) < 1 || K % s.size(1) != 0 || y.dim() != 2 || y.size(0) != x.size(0) || y.size(1) != w.size(0) ||
-      (y.size(1) > 1 && y.stride(1) != 1))
+  const int64_t N = y.dim() == 2 ? y.size(1) : -1, tiles = (N + 15) / 16, chunks = (K + 127) / 128;
+  const int64_t per = s.dim() == 4 ? s.size(3) : 0;
+  if (N < 0 || K < 1 || x.dim() != 2 || x.size(1) != K || (K > 1 && x.stride(1) != 1) || y.size(0) != x.size(0) ||
+      (N > 1 && y.stride(1) != 1) || !w.is_contiguous() || w.dim() != 5 || w.size(0) != tiles || w.size(1) != chunks ||
+      w.size(2) != 4 || w.size(3) != 16 || w.size(4) != 16 || !s.is_contiguous() || s.dim() != 4 ||
+      s.size(0) != tiles || s.size(1) != chunks || s.size(2) != 16 || (per != 1 && per != 2 && per != 4))
     value_error("group4_linear: x " + shape(x) + ", codes " + shape(w) + ", scales " + shape(s) + ", y " + shape(y) +
                 " for " + std::to_string(K) + " columns");
-  if (bias != nullptr && (bias->dim() != 1 || bias->size(0) != w.size(0) || (w.size(0) > 1 && bias->stride(0) != 1)))
+  if (bias != nullptr && (bias->dim() != 1 || bias->size(0) != N || (N > 1 && bias->stride(0) != 1)))
     value_error("group4_linear: bias must be a contiguous [N] vector");
   const c10::DeviceGuard guard(x.device());
-  call("ltx_group4_linear", api.group4_linear, x.size(0), w.size(0), K, K / s.size(1), x.data_ptr(),
+  call("ltx_group4_linear", api.group4_linear, x.size(0), N, K, 128 / per, x.data_ptr(),
        x.size(0) > 1 ? x.stride(0) : 0, (int)truth(a[5]), w.data_ptr(), s.data_ptr(), ptr(bias), y.data_ptr(),
        y.size(0) > 1 ? y.stride(0) : 0, stream_of(x));
 }

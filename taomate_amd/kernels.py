@@ -210,6 +210,6 @@ def group4_linear(x: torch.Tensor, weight: Group4Weight, bias: Optional[torch.Te
                   silu: bool = False) -> torch.Tensor:
     """ltx_group4_linear: act(x) @ W.T + bias for x [M <= 16, K <= 4096] bf16
     (SiLU of x first with ``silu``) and a 4-bit weight."""
-    y = torch.empty(x.shape[0], weight.codes.shape[0], dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape[0], weight.rows, dtype=x.dtype, device=x.device)
     (N._host or N.host()).group4_linear(x, weight.codes, weight.scales, bias, y, silu, weight.columns)
     return y

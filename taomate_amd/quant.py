@@ -75,22 +75,23 @@ def quantize_mx(x: torch.Tensor) -> MXRows:
 
 
 class Group4Weight:
-    """A weight [N, columns] in 4 bits: ``codes`` uint8 [N, ceil(K / 128) * 64] in
-    the kernel's order (byte c * 64 + p * 16 + j * 4 + i of a row holds columns
-    c * 128 + j * 32 + p * 8 + 2 i, in the low half, and the next one) and
-    ``scales`` bf16 [N, K / group]."""
-    __slots__ = ("codes", "scales", "columns")
+    """A weight [N, K] in 4 bits, zero-padded to whole tiles of 16 rows and 128
+    columns: ``codes`` uint8 [ceil(N / 16), ceil(K / 128), 4, 16, 16] and
+    ``scales`` bf16 [ceil(N / 16), ceil(K / 128), 16, 128 / group].  Byte
+    [t, c, p, r, 4 j + i] holds row 16 t + r, columns 128 c + 32 j + 8 p + 2 i
+    (low half) and the next one (p, j, i in [0, 4))."""
+    __slots__ = ("codes", "scales", "rows", "columns")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
-        self.codes, self.scales, self.columns = codes, scales, int(columns)
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, columns: int):
+        self.codes, self.scales, self.rows, self.columns = codes, scales, int(rows), int(columns)
 
     @property
     def shape(self) -> torch.Size:
-        return torch.Size((self.codes.shape[0], self.columns))
+        return torch.Size((self.rows, self.columns))
 
     @property
     def group(self) -> int:
-        return self.columns // self.scales.shape[1]
+        return 128 // self.scales.shape[3]
 
     @property
     def device(self) -> torch.device:
@@ -107,20 +108,24 @@ class Group4Weight:
                 or scales.shape[0] != packed.shape[0]:
             raise ValueError("Group4Weight: codes must be uint8 [N, K / 2] and scales bf16 [N, K / group]")
         N, K = packed.shape[0], packed.shape[1] * 2
-        if scales.shape[1] == 0 or K % scales.shape[1] or K // scales.shape[1] not in GROUPS:
+        if K == 0 or scales.shape[1] == 0 or K % scales.shape[1] or K // scales.shape[1] not in GROUPS:
             raise ValueError(f"Group4Weight: {K} columns in {scales.shape[1]} groups: groups must be 32, 64 or 128 columns")
-        chunks = -(-K // 128)
-        rows = F.pad(packed, (0, -packed.shape[1] % 64)).reshape(N, chunks, 4, 4, 4)    # chunk, j, p, i
-        return cls(rows.transpose(2, 3).reshape(N, chunks * 64).contiguous(), scales.contiguous(), K)
+        per, chunks, tiles = 128 * scales.shape[1] // K, -(-K // 128), -(-N // 16)
+        codes = F.pad(packed, (0, chunks * 64 - K // 2, 0, tiles * 16 - N)).reshape(tiles, 16, chunks, 4, 4, 4)
+        # tile, row, chunk, j, p, i -> tile, chunk, p, row, j, i
+        codes = codes.permute(0, 2, 4, 1, 3, 5).reshape(tiles, chunks, 4, 16, 16).contiguous()
+        scales = F.pad(scales, (0, chunks * per - scales.shape[1], 0, tiles * 16 - N)).reshape(tiles, 16, chunks, per)
+        return cls(codes, scales.transpose(1, 2).contiguous(), N, K)
 
     def dequantize(self) -> torch.Tensor:
         """The float32 values that the codes stand for."""
-        N, K = self.shape
-        rows = self.codes.reshape(N, -(-K // 128), 4, 4, 4).transpose(2, 3).flatten(1)[:, :K // 2]
-        code = torch.stack([rows & 15, rows >> 4], -1).reshape(N, K)
+        tiles, chunks = self.codes.shape[:2]
+        rows = self.codes.reshape(tiles, chunks, 4, 16, 4, 4).permute(0, 3, 1, 4, 2, 5).reshape(tiles * 16, chunks * 64)
+        code = torch.stack([rows & 15, rows >> 4], -1).reshape(tiles * 16, chunks * 128)
         grid = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=rows.device)
-        w = grid[code.long()].reshape(N, K // self.group, self.group) * self.scales.to(torch.float32).unsqueeze(-1)
-        return w.reshape(N, K)
+        scales = self.scales.transpose(1, 2).reshape(tiles * 16, chunks * 128 // self.group).to(torch.float32)
+        w = grid[code.long()] * scales.repeat_interleave(self.group, dim=1)
+        return w[:self.rows, :self.columns].contiguous()
 
 
 def quantize_group4(weight: torch.Tensor, group: int = 32) -> Group4Weight:

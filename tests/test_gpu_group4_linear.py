@@ -18,7 +18,7 @@ def _weight(n, k, group, g):
 
 
 def _to(w, dev):
-    return quant.Group4Weight(w.codes.to(dev), w.scales.to(dev), w.columns)
+    return quant.Group4Weight(w.codes.to(dev), w.scales.to(dev), w.rows, w.columns)
 
 
 def check(x, w, b, silu, y):
@@ -70,7 +70,7 @@ def test_rows_do_not_meet(dev):
 def test_empty(dev):
     w = _to(_weight(16, 64, 32, gen(1)), dev)
     assert kernels.group4_linear(torch.empty(0, 64, dtype=BF, device=dev), w).shape == (0, 16)
-    none = quant.Group4Weight(w.codes[:0], w.scales[:0], 64)
+    none = quant.Group4Weight(w.codes[:0], w.scales[:0], 0, 64)
     assert kernels.group4_linear(torch.empty(3, 64, dtype=BF, device=dev), none).shape == (3, 0)
 
 
@@ -79,8 +79,12 @@ def test_refusals(dev):
     x = torch.zeros(3, 64, device=dev, dtype=BF)
     with pytest.raises(N.NativeCallError, match="M must be"):
         kernels.group4_linear(torch.zeros(17, 64, device=dev, dtype=BF), w)
-    with pytest.raises(N.NativeCallError, match="group must be"):
-        kernels.group4_linear(x, quant.Group4Weight(w.codes, w.scales[:, :1].repeat(1, 4), 64))
+    with pytest.raises(N.NativeCallError, match="multiple of the group"):
+        kernels.group4_linear(x, quant.Group4Weight(w.codes, w.scales[..., :1].contiguous(), 16, 64))   # groups of 128
+    with pytest.raises(ValueError, match="group4_linear"):
+        kernels.group4_linear(x, quant.Group4Weight(w.codes, w.scales.repeat(1, 1, 1, 2), 16, 64))   # groups of 16
+    with pytest.raises(ValueError, match="group4_linear"):
+        kernels.group4_linear(x, quant.Group4Weight(w.codes, w.scales, 17, 64))
     with pytest.raises(N.NativeCallError, match="16-byte aligned"):
         kernels.group4_linear(torch.zeros(3, 72, device=dev, dtype=BF)[:, 1:65], w)
     with pytest.raises(ValueError, match="group4_linear"):

@@ -1,5 +1,6 @@
 """The packers of the block-scaled linears on the CPU, against the formats'
 definitions written out, and what the wrappers refuse."""
+import itertools
 import math
 
 import pytest
@@ -58,9 +59,9 @@ def test_4bit_weight(n, k, group):
     w = randn((n, k), gen(n + k))
     w[0, :group] = 0
     q = quant.quantize_group4(w, group)
-    assert q.shape == (n, k) and q.group == group and q.codes.shape == (n, -(-k // 128) * 64)
+    assert q.shape == (n, k) and q.group == group and q.codes.shape == (-(-n // 16), -(-k // 128), 4, 16, 16)
     s = (w.reshape(n, -1, group).abs().amax(-1) / 6).to(BF)
-    assert torch.equal(q.scales, s)
+    assert q.scales.shape == (-(-n // 16), -(-k // 128), 16, 128 // group)
     grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6])
     grid = torch.cat([grid, -grid]).double()
     t = w.double().reshape(n, -1, group)
@@ -68,16 +69,18 @@ def test_4bit_weight(n, k, group):
     best = (t[..., None] - sd[..., None] * grid).abs().min(-1).values
     got = (q.dequantize().double().reshape(n, -1, group) - t).abs()
     assert (got <= best * (1 + 1e-6) + 1e-30).all()
-    # the packed order: byte c*64 + p*16 + j*4 + i of a row holds columns c*128 + j*32 + p*8 + 2i and the next
+    # the packed order, and zeros past the weight
     value = q.dequantize()
+    assert value.shape == (n, k)
     table = [0, .5, 1, 1.5, 2, 3, 4, 6, -0.0, -.5, -1, -1.5, -2, -3, -4, -6]
-    for r in range(n):
-        for at, byte in enumerate(q.codes[r].tolist()):
-            c, p, j, i = at // 64, at // 16 % 4, at // 4 % 4, at % 4
-            col = c * 128 + j * 32 + p * 8 + 2 * i
-            for half, col in ((byte & 15, col), (byte >> 4, col + 1)):
-                want = table[half] * float(s[r, col // group]) if col < k else 0.0
-                assert (float(value[r, col]) if col < k else float(table[half])) == want
+    for (t, c, p, r, at), byte in zip(itertools.product(*map(range, q.codes.shape)), q.codes.flatten().tolist()):
+        row, col = 16 * t + r, 128 * c + 32 * (at // 4) + 8 * p + 2 * (at % 4)
+        for half, col in ((byte & 15, col), (byte >> 4, col + 1)):
+            scale = float(q.scales[t, c, r, col % 128 // group])
+            if row < n and col < k:
+                assert scale == float(s[row, col // group]) and float(value[row, col]) == table[half] * scale
+            else:
+                assert half == 0 and (row < n and col // group < k // group or scale == 0)
 
 
 def test_4bit_ties_go_to_the_even_code():
