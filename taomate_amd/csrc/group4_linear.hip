@@ -21,6 +21,8 @@
 // x (SiLU applied, rounded to bf16 as the tensor op rounds) is staged in LDS
 // once per workgroup, which then strides over the tiles.
 
+#include <type_traits>
+
 #include "ltx_common.h"
 
 namespace ltx {
@@ -69,54 +71,71 @@ __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Grou
   const int64_t tiles = (a.N + 15) / 16;
   const int own = (chunks + KS - 1) / KS, c0 = kw * own, c1 = min(c0 + own, chunks);  // this wave's chunks
 
-  // One tile's rows of W in registers: 4 chunks of codes and their scales.
+  // One tile's rows of W in registers: 4 chunks of codes and their scales.  Every
+  // load of a round is unconditional (a wave with fewer chunks reads its last one
+  // again, one without a tile the last tile): loads that may not have been issued
+  // would make the waits for older ones wait for all.
   struct Rows {
     uint4 w[kG4Chunks];
     uint16_t s[kG4Chunks][kPer];
   };
   auto load = [&](Rows& t, int64_t tile) {
-    const uint8_t* codes = a.codes + tile * chunks * 1024 + lane * 16;
-    const uint16_t* scales = a.scales + (tile * chunks * 16 + r16) * kPer;
+    const int64_t at = (tile < tiles ? tile : tiles - 1) * chunks;
 #pragma unroll
     for (int i = 0; i < kG4Chunks; ++i) {
-      const int c = c0 + i;
-      if (c >= c1) continue;
-      t.w[i] = *reinterpret_cast<const uint4*>(codes + c * 1024);
-      __builtin_memcpy(t.s[i], __builtin_assume_aligned(scales + c * 16 * kPer, kPer * 2), sizeof(t.s[i]));
+      const int64_t c = at + max(min(c0 + i, c1 - 1), 0);
+      t.w[i] = *reinterpret_cast<const uint4*>(a.codes + c * 1024 + lane * 16);
+      __builtin_memcpy(t.s[i], __builtin_assume_aligned(a.scales + (c * 16 + r16) * kPer, kPer * 2), sizeof(t.s[i]));
     }
   };
-  int64_t tile = (int64_t)blockIdx.x * kTiles + wave / KS;
-  const int64_t stride = (int64_t)gridDim.x * kTiles;
-  // the first rows of W travel while x is staged, the next ones while a tile is computed
-  Rows rows[2] = {};
-  if (tile < tiles) load(rows[0], tile);
-  if (tile + stride < tiles) load(rows[1], tile + stride);
-  // a thread keeps its column of x; rows go by in fours, their loads ahead of the first use
+  const int64_t stride = (int64_t)gridDim.x * kTiles, first = (int64_t)blockIdx.x * kTiles;
+  const int64_t tile = first + wave / KS;
+  const int64_t rounds = (tiles - first + stride - 1) / stride;
+  Rows rows[2];
+
+  // x: a thread keeps its column, rows go by in fours.  Loads return in order, so
+  // the last of them are issued ahead of the first rows of W, which then travel
+  // while x is staged.
   const int words = chunks * 16, xrows = 64 * kG4Waves / words;
   const int xm = threadIdx.x / words, xc = threadIdx.x - xm * words;
-  for (int m0 = xm; m0 < a.M && xm < xrows; m0 += 4 * xrows) {
+  for (int m0 = 0; m0 < a.M; m0 += 4 * xrows) {
     uint4 v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+      const int m = m0 + q * xrows + xm;
       v[q] = make_uint4(0, 0, 0, 0);  // columns past K: their codes are 0, so x must be finite there
-      if (m0 + q * xrows < a.M && xc * 8 < a.K)
-        v[q] = *reinterpret_cast<const uint4*>(a.x + (m0 + q * xrows) * a.x_ls + xc * 8);
+      if (xm < xrows && m < a.M && xc * 8 < a.K) v[q] = *reinterpret_cast<const uint4*>(a.x + m * a.x_ls + xc * 8);
+    }
+    if (m0 + 4 * xrows >= a.M) {
+      load(rows[0], tile);
+      if (rounds > 1) load(rows[1], tile + stride);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (m0 + q * xrows >= a.M) break;
+      const int m = m0 + q * xrows + xm;
+      if (xm >= xrows || m >= a.M) break;
       if (a.silu) {
         uint32_t* t = &v[q].x;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           t[e] = pack_bf16x2(g4_silu(bf16_bits_to_f32(t[e] & 0xFFFFu)), g4_silu(bf16_bits_to_f32(t[e] >> 16)));
       }
-      xs[(m0 + q * xrows) * row_words + xc] = v[q];
+      xs[m * row_words + xc] = v[q];
     }
   }
   __syncthreads();
   const uint4* xr = xs + min(r16, a.M - 1) * row_words + p;
-  auto round = [&](Rows& t, int64_t t0, int buf) {
+
+  // the result that this thread stores in a round: row ym of x, column yc of tile yt
+  const int yt = threadIdx.x >> 8, ym = (threadIdx.x >> 4) & 15, yc = threadIdx.x & 15;
+  auto round = [&](Rows& t, int64_t r, auto prefetch) {
+    const int64_t t0 = first + r * stride;
+    float bias[(kTiles + 1) / 2] = {};
+#pragma unroll
+    for (int h = 0; h < (kTiles + 1) / 2; ++h) {
+      const int64_t n = (t0 + h * 2 + yt) * 16 + yc;
+      if (a.bias != nullptr) bias[h] = bf16_bits_to_f32(a.bias[n < a.N ? n : a.N - 1]);
+    }
     g4_f4 acc = {};
 #pragma unroll
     for (int i = 0; i < kG4Chunks; ++i) {
@@ -131,34 +150,45 @@ __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Grou
           if ((j + 1) * 32 % GROUP == 0) {
             const float sc = bf16_bits_to_f32(t.s[i][j * 32 / GROUP]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r] = fmaf(d[r], sc, acc[r]);
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(d[e], sc, acc[e]);
             d = g4_f4{};
           }
         }
       }
     }
-    if (tile + 2 * stride < tiles) load(t, tile + 2 * stride);
-    tile += stride;
+    if (prefetch) load(t, tile + (r + 2) * stride);
     // lane: rows 4 p .. + 3 of x, row r16 of the tile
+    const int buf = (int)(r & 1);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) part[buf][wave][p * 4 + r][r16] = acc[r];
+    for (int e = 0; e < 4; ++e) part[buf][wave][p * 4 + e][r16] = acc[e];
     __syncthreads();  // the other buffer's sums, read a round ago, may be overwritten after it
-    for (int i = threadIdx.x; i < kTiles * 256; i += 64 * kG4Waves) {
-      const int tw = i >> 8, m = (i >> 4) & 15, c = i & 15;
-      const int64_t n = (t0 + tw) * 16 + c;
-      if (m < a.M && n < a.N) {
-        float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) v += part[buf][tw * KS + k][m][c];
-        if (a.bias != nullptr) v += bf16_bits_to_f32(a.bias[n]);
-        a.y[m * a.y_ls + n] = f32_to_bf16_bits(v);
+    for (int h = 0; h < (kTiles + 1) / 2; ++h) {
+      const int tw = h * 2 + yt;
+      const int64_t n = (t0 + tw) * 16 + yc;
+      if (tw < kTiles && ym < a.M && n < a.N) {
+        float v = bias[h];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) v += part[buf][tw * KS + k][ym][yc];
+        a.y[ym * a.y_ls + n] = f32_to_bf16_bits(v);
       }
     }
   };
   // every wave of a workgroup runs the same rounds; one without a tile adds to no stored result
-  for (int64_t t0 = (int64_t)blockIdx.x * kTiles; t0 < tiles; t0 += 2 * stride) {
-    round(rows[0], t0, 0);
-    if (t0 + stride < tiles) round(rows[1], t0 + stride, 1);
+  const std::true_type more;
+  const std::false_type last;
+  int64_t r = 0;
+  for (; r + 3 < rounds; r += 2) {
+    round(rows[0], r, more);
+    round(rows[1], r + 1, more);
+  }
+  if (r + 2 < rounds) {
+    round(rows[0], r, more);
+    round(rows[1], r + 1, last);
+    round(rows[0], r + 2, last);
+  } else {
+    round(rows[0], r, last);
+    if (r + 1 < rounds) round(rows[1], r + 1, last);
   }
 }
 
