@@ -19,6 +19,8 @@
 // group i ends with the 4 NT neighbouring channels 4 NT i ..: contiguous stores,
 // and blocks of 32 for an 8-bit result inside one lane (NT = 8) or a pair (NT = 4).
 
+#include <type_traits>
+
 #include "mx_common.h"
 
 namespace ltx {
@@ -26,7 +28,23 @@ namespace ltx {
 typedef int mx_i4 __attribute__((ext_vector_type(4)));
 typedef int mx_i8 __attribute__((ext_vector_type(8)));
 typedef float mx_f4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void* mx_lds_ptr;
+#define MX_LDS __attribute__((address_space(3)))
+typedef MX_LDS void* mx_lds_ptr;
+// 16 (4) bytes per lane from a buffer's offset straight into LDS: lane l's land at `to` + 16 l (4 l).
+__device__ __forceinline__ void mx_lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t to, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (mx_lds_ptr)(uintptr_t)to, 16, offset, 0, 0, 0);
+}
+__device__ __forceinline__ void mx_lds_load4(__amdgpu_buffer_rsrc_t r, uint32_t to, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (mx_lds_ptr)(uintptr_t)to, 4, offset, 0, 0, 0);
+}
+// The byte column that lane l of a load of 8 rows from `row` on reads: its chunk, exchanged.
+__device__ __forceinline__ int mx_chunk(int l, int row) { return ((l & 7) ^ (((row + (l >> 3)) >> 1) & 7)) * 16; }
+__device__ __forceinline__ const MX_LDS uint8_t* mx_lds(uint32_t at) { return (const MX_LDS uint8_t*)(uintptr_t)at; }
+// A lane's 32 bytes of a fragment: 16 of the row's first 64, 16 of its last.
+__device__ __forceinline__ mx_i8 mx_fragment(const MX_LDS uint8_t* lo, const MX_LDS uint8_t* hi) {
+  const mx_i4 x = *(const MX_LDS mx_i4*)lo, y = *(const MX_LDS mx_i4*)hi;
+  return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
 struct MxLinearArgs {
   const uint8_t* a;
@@ -49,126 +67,240 @@ __device__ __forceinline__ float mx_gelu(float y) {
   return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u));
 }
 
-// MT x NT tiles of 16 x 16 per wave, WM x WN waves, ST buffers of one step.
+constexpr int kGroupM = 4;
+
+// MT x NT tiles of 16 x 16 per wave, WM x WN waves, ST buffers of one step each.
 template <int MT, int NT, int WM, int WN, int ST>
 struct MxTile {
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int kBM = 16 * MT * WM, kBN = 16 * NT * WN, kRows = kBM + kBN;
-  static constexpr int kCodes = kRows * 128, kStage = kCodes + kRows * 4;
-  static constexpr int kPer = (kRows / 8 + kWaves - 1) / kWaves;  // 1 KB loads (8 rows) per wave and step
-  static constexpr int kScalesPer = (kRows + kWaves - 1) / kWaves;
-  static_assert(kScalesPer <= 64 && kRows % 8 == 0, "one scale load per wave");
-  static_assert(ST * kStage <= 160 * 1024, "LDS");
+  static constexpr int kARows = (kBM + 63) / 64 * 64;         // a's rows in the scales: whole loads
+  static constexpr int kCodes = kRows * 128, kStage = kCodes + (kARows + kBN) * 4;
+  // 1 KB loads (8 rows) per step and wave, of each operand
+  static constexpr int kPerA = (kBM / 8 + kWaves - 1) / kWaves, kPerW = (kBN / 8 + kWaves - 1) / kWaves;
+  static constexpr int kScaleLoads = (kARows + kBN) / 64;     // 256 byte loads (64 rows' words) per step
+  static constexpr int kScalePer = (kScaleLoads + kWaves - 1) / kWaves, kParts = kPerA + kPerW + kScalePer;
+  static_assert(kWaves % 2 == 0 && kBM % 8 == 0 && kBN % 64 == 0, "whole loads of one operand");
+  static_assert(ST >= 2 && ST * kStage <= 160 * 1024, "LDS");
 };
 
 template <int MT, int NT, int WM, int WN, int ST, bool GELU>
-__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4 > 0 ? WM * WN / 4 : 1) mx_linear_kernel(const MxLinearArgs p) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLinearArgs p) {
   using T = MxTile<MT, NT, WM, WN, ST>;
   __shared__ __attribute__((aligned(128))) uint8_t lds[ST * T::kStage];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   const int g = lane >> 4, r16 = lane & 15;
-  const int m0 = blockIdx.y * T::kBM, n0 = blockIdx.x * T::kBN;
+  // Workgroups go round-robin to the 8 XCDs: each gets a contiguous run of tiles, walked in
+  // groups of kGroupM rows of tiles, so that those resident on one L2 share rows of a and w.
+  const int tm = (p.M + T::kBM - 1) / T::kBM, tn = gridDim.x / tm;
+  const int per = gridDim.x / 8, rem = gridDim.x % 8, xcd = blockIdx.x % 8;
+  const int tile = xcd * per + min(xcd, rem) + blockIdx.x / 8;
+  const int group = tile / (kGroupM * tn), in = tile - group * kGroupM * tn, gm = min(kGroupM, tm - group * kGroupM);
+  const int m0 = __builtin_amdgcn_readfirstlane((group * kGroupM + in % gm) * T::kBM);
+  const int n0 = __builtin_amdgcn_readfirstlane(in / gm * T::kBN);
   const int steps = (p.K + 127) / 128;
 
-  // Buffer descriptors of the tile's rows: rows past M or N lie past the end and read as zeros.
+  // The channel of the tile that row r of its w rows holds.
+  auto channel = [](int r) {
+    const int s = r % (16 * NT);
+    return r - s + (s % 16 / 4) * 4 * NT + (s / 16) * 4 + s % 4;
+  };
+  // This lane's part of the wave's loads: rows 8 j .. + 7 of load j, a chunk each
   const int mrows = min(p.M - m0, T::kBM), nrows = max(min(p.N - n0, T::kBN), 0);
-  const auto ra =
-      __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + (int64_t)m0 * p.K), (short)0, mrows * p.K, 0x00020000);
-  const auto rw =
-      __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + (int64_t)n0 * p.K), (short)0, nrows * p.K, 0x00020000);
-
-  // This lane's part of the wave's loads: LDS rows 8 j .. of load j, a chunk each.
-  uint32_t voff[T::kPer];
-  uint32_t col[T::kPer];
+  // (a wave whose part lies past an operand's loads repeats the last one: no branch).
+  int aoff[T::kPerA], woff[T::kPerW];
 #pragma unroll
-  for (int q = 0; q < T::kPer; ++q) {
-    const int row = (q * T::kWaves + wave) * 8 + (lane >> 3);
-    const int c = (lane & 7) ^ ((row >> 1) & 7);
-    int src = row;
-    if (row >= T::kBM) {  // w: channel order of the wave's block
-      const int s = (row - T::kBM) % (16 * NT), b = (row - T::kBM) / (16 * NT);
-      src = b * 16 * NT + (s % 16 / 4) * 4 * NT + (s / 16) * 4 + s % 4;
-    }
-    col[q] = (uint32_t)c * 16;
-    voff[q] = (uint32_t)src * (uint32_t)p.K + col[q];
-  }
-  // and of the scales: one word (four blocks) per row of the tile
-  const int srow = wave * T::kScalesPer + lane;
-  const bool sload = lane < T::kScalesPer && srow < T::kRows;
-  const bool sa = srow < T::kBM;
-  int ssrc = srow;
-  if (!sa) {
-    const int s = (srow - T::kBM) % (16 * NT), b = (srow - T::kBM) / (16 * NT);
-    ssrc = b * 16 * NT + (s % 16 / 4) * 4 * NT + (s / 16) * 4 + s % 4;
-  }
-  const uint8_t* sp = sa ? p.as + (int64_t)min(m0 + ssrc, p.M - 1) * 4 : p.ws + (int64_t)min(n0 + ssrc, p.N - 1) * 4;
-  const int64_t sstep = (int64_t)(sa ? p.M : p.N) * 4;
-
-  auto load = [&](int ks) {
-    const uint32_t base = lds0 + (uint32_t)(ks % ST) * T::kStage;
-    const uint32_t k0 = (uint32_t)ks * 128;
+  for (int q = 0; q < T::kPerA; ++q) aoff[q] = (min(q * T::kWaves + wave, T::kBM / 8 - 1) * 8 + (lane >> 3)) * p.K;
 #pragma unroll
-    for (int q = 0; q < T::kPer; ++q) {
-      const int j = q * T::kWaves + wave;
-      if (T::kPer * T::kWaves * 8 == T::kRows || j * 8 < T::kRows) {
-        // columns past K read as zeros: an offset past the end of either operand
-        const uint32_t off = k0 + col[q] < (uint32_t)p.K ? voff[q] + k0 : 0x80000000u;
-        const mx_lds_ptr to = (mx_lds_ptr)(uintptr_t)(base + (uint32_t)j * 1024);
-        if (j * 8 < T::kBM)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, to, 16, off, 0, 0, 0);
+  for (int q = 0; q < T::kPerW; ++q)
+    woff[q] = channel(min(q * T::kWaves + wave, T::kBN / 8 - 1) * 8 + (lane >> 3)) * p.K;
+  int soff[T::kScalePer];
+#pragma unroll
+  for (int i = 0; i < T::kScalePer; ++i) {
+    const int row = min(i * T::kWaves + wave, T::kScaleLoads - 1) * 64 + lane;
+    soff[i] = (row < T::kARows ? row : channel(row - T::kARows)) * 4;
+  }
+  const uint8_t* abase = p.a + (int64_t)m0 * p.K;
+  const uint8_t* wbase = p.w + (int64_t)n0 * p.K;
+  const uint8_t* asbase = p.as + (int64_t)m0 * 4;
+  const uint8_t* wsbase = p.ws + (int64_t)n0 * 4;
+
+  // The loads of a step.  Their buffer descriptors end with the
+  // tile's last row, so rows past M or N, columns past K (by their offset) and steps
+  // past the last (by the descriptor) read as zeros: the loop issues them without a
+  // branch.
+  struct Step {
+    uint32_t base;
+    __amdgpu_buffer_rsrc_t a, w, as, ws;
+    int left;
+  };
+  auto step = [&](int ks, int at) {
+    Step r;
+    r.base = lds0 + at;
+    const int k0 = ks * 128, left = max(p.K - k0, 0);
+    r.a = __builtin_amdgcn_make_buffer_rsrc((void*)(abase + k0), (short)0, left > 0 ? mrows * p.K - k0 : 0, 0x00020000);
+    r.w = __builtin_amdgcn_make_buffer_rsrc((void*)(wbase + k0), (short)0, left > 0 ? max(nrows * p.K - k0, 0) : 0,
+                                            0x00020000);
+    r.as = __builtin_amdgcn_make_buffer_rsrc((void*)(asbase + (int64_t)ks * p.M * 4), (short)0,
+                                             left > 0 ? mrows * 4 : 0, 0x00020000);
+    r.ws = __builtin_amdgcn_make_buffer_rsrc((void*)(wsbase + (int64_t)ks * p.N * 4), (short)0,
+                                             left > 0 ? nrows * 4 : 0, 0x00020000);
+    r.left = left;
+    return r;
+  };
+  auto issue_a = [&](const Step& r, int q) {
+    const int j = min(q * T::kWaves + wave, T::kBM / 8 - 1), col = mx_chunk(lane, j * 8);
+    mx_lds_load16(r.a, r.base + j * 1024, aoff[q] + col + (col < r.left ? 0 : 0x40000000));
+  };
+  auto issue_w = [&](const Step& r, int q) {
+    const int j = min(q * T::kWaves + wave, T::kBN / 8 - 1), col = mx_chunk(lane, T::kBM + j * 8);
+    mx_lds_load16(r.w, r.base + T::kBM * 128 + j * 1024, woff[q] + col + (col < r.left ? 0 : 0x40000000));
+  };
+  auto issue_scales = [&](const Step& r, int q) {
+    const int j = min(q * T::kWaves + wave, T::kScaleLoads - 1);
+    mx_lds_load4(j * 64 < T::kARows ? r.as : r.ws, r.base + T::kCodes + j * 256, soff[q]);
+  };
+  auto issue_all = [&](int ks) {
+    const Step r = step(ks, ks * T::kStage);
+#pragma unroll
+    for (int q = 0; q < T::kPerW; ++q) issue_w(r, q);
+#pragma unroll
+    for (int q = 0; q < T::kPerA; ++q) issue_a(r, q);
+#pragma unroll
+    for (int q = 0; q < T::kScalePer; ++q) issue_scales(r, q);
+  };
+
+  // Fragments and their scales from a step's buffer: rows 16 apart share their chunk exchange.
+  const int sx = (r16 >> 1) & 7;
+  const uint32_t alo = lds0 + (wm * MT * 16 + r16) * 128 + (g ^ sx) * 16;
+  const uint32_t wlo = lds0 + (T::kBM + wn * NT * 16 + r16) * 128 + (g ^ sx) * 16;
+  const uint32_t asc = lds0 + T::kCodes + (wm * MT * 16 + r16) * 4 + g;
+  const uint32_t wsc = lds0 + T::kCodes + (T::kARows + wn * NT * 16 + r16) * 4 + g;
+  struct Buffer {
+    const MX_LDS uint8_t *alo, *ahi, *wlo, *whi, *asc, *wsc;
+  };
+  auto buffer = [&](int at) {
+    return Buffer{mx_lds(alo + at), mx_lds((alo + at) ^ 64), mx_lds(wlo + at), mx_lds((wlo + at) ^ 64),
+                  mx_lds(asc + at), mx_lds(wsc + at)};
+  };
+
+  // One step of a wave.  The fragments of w are held.  The first H tiles of a are
+  // multiplied column by column; after them every wave has its w in registers, and
+  // the loads of the w of the step ST later go out into its place.  The middle tiles
+  // go one by one, those after them read meanwhile.  When the last S are in
+  // registers the waves meet: the next step's data have landed, a's place is free, and
+  // the loads of the a of the step ST later go out.  The last S tiles go column by
+  // column again, and each fragment of w, done after S products, is read for the
+  // next step, as are its first H tiles of a: every read has several products to
+  // arrive in, its own wave's and those of the SIMD's other wave, and w's loads,
+  // which come from further away, more than a step.
+  constexpr int H = MT > 3 ? 2 : 1, S = MT > 4 ? 3 : MT - H, kMid = MT - H - S;
+  mx_f4 acc[MT][NT] = {};
+  mx_i8 fw[NT], fa[MT];
+  int sw[NT], sa[MT];
+  // all but the latest `later` loads of this wave have landed, all its reads too
+  auto meet = [&](auto later) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto read_a = [&](const Buffer& b, int t, int mask) {
+    fa[t] = mx_fragment(b.alo + t * 2048, b.ahi + t * 2048);
+    sa[t] = b.asc[t * 64] & mask;
+  };
+  auto read_w = [&](const Buffer& b, int u, int mask) {
+    fw[u] = mx_fragment(b.wlo + u * 2048, b.whi + u * 2048);
+    sw[u] = b.wsc[u * 64] & mask;
+  };
+  auto product = [&](int t, int u) {
+    acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u], fa[t], acc[t][u], 0, 0, 0, sw[u], 0, sa[t]);
+  };
+  auto first_tiles = [&](const Buffer& b, int mask, const Step* after) {
+#pragma unroll
+    for (int r = 0; r <= kMid; ++r) {
+#pragma unroll
+      for (int t = H + (r * (MT - H) + kMid) / (kMid + 1); t < H + ((r + 1) * (MT - H) + kMid) / (kMid + 1); ++t)
+        read_a(b, t, mask);
+      if (r == 0) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int t = 0; t < H; ++t) product(t, u);
+      } else {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) product(H + r - 1, u);
+        if (after != nullptr)
+#pragma unroll
+          for (int q = (r - 1) * T::kPerW / max(kMid, 1); q < r * T::kPerW / max(kMid, 1); ++q) issue_w(*after, q);
+      }
+#pragma unroll
+      for (int i = 0; i < NT * (r == 0 ? H : 1); ++i) {  // reads and loads between the products
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+        if (r == 0)
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         else
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, to, 16, off, 0, 0, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (r == 0 && after != nullptr) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (kMid == 0)
+#pragma unroll
+          for (int q = 0; q < T::kPerW; ++q) issue_w(*after, q);
       }
     }
   };
-  auto load_scales = [&](int ks) { return sload ? *reinterpret_cast<const uint32_t*>(sp + ks * sstep) : 0u; };
-  auto put_scales = [&](int ks, uint32_t word) {
-    // the scale bytes of blocks past K are not looked at
-    const int left = p.K / 32 - ks * 4;
-    if (left < 4) word &= (1u << (8 * left)) - 1u;
-    if (sload) *reinterpret_cast<uint32_t*>(lds + (ks % ST) * T::kStage + T::kCodes + srow * 4) = word;
-  };
-
-  mx_f4 acc[MT][NT] = {};
-  load(0);
-  put_scales(0, load_scales(0));
-  for (int ks = 0; ks < steps; ++ks) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    uint32_t next_scales = 0;
-    if (ks + 1 < steps) {
-      next_scales = load_scales(ks + 1);
-      load(ks + 1);
-    }
-    const uint8_t* st = lds + (ks % ST) * T::kStage;
-    auto fragment = [&](int row) {
-      const int sw = (row >> 1) & 7;
-      const mx_i4 lo = *reinterpret_cast<const mx_i4*>(st + row * 128 + ((g ^ sw) * 16));
-      const mx_i4 hi = *reinterpret_cast<const mx_i4*>(st + row * 128 + (((g + 4) ^ sw) * 16));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    auto scale = [&](int row) { return (int)st[T::kCodes + row * 4 + g]; };
-    mx_i8 fw[NT];
-    int sw[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int row = T::kBM + (wn * NT + t) * 16 + r16;
-      fw[t] = fragment(row);
-      sw[t] = scale(row);
-    }
+  for (int i = 0; i < ST; ++i) issue_all(i);
+  meet(std::integral_constant<int, (ST - 1) * T::kParts>{});
+  {
+    const Buffer b = buffer(0);
+    const int live = g * 32 < p.K ? 0xFF : 0;  // the scale bytes of blocks past K are not looked at
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int row = (wm * MT + t) * 16 + r16;
-      const mx_i8 fa = fragment(row);
-      const int sc = scale(row);
+    for (int t = 0; t < H; ++t) read_a(b, t, live);
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
-        acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u], fa, acc[t][u], 0, 0, 0, sw[u], 0, sc);
-    }
-    if (ks + 1 < steps) put_scales(ks + 1, next_scales);
+    for (int u = 0; u < NT; ++u) read_w(b, u, live);
   }
+  int at = 0;  // the step's buffer
+  for (int ks = 0; ks + 1 < steps; ++ks) {
+    const int next_at = at + T::kStage == ST * T::kStage ? 0 : at + T::kStage;
+    const Step after = step(ks + ST, at);
+    first_tiles(buffer(at), 0xFF, &after);
+    __builtin_amdgcn_s_setprio(1);
+    meet(std::integral_constant<int, (ST - 2) * T::kParts + T::kPerW>{});
+    const Buffer next = buffer(next_at);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+#pragma unroll
+      for (int t = MT - S; t < MT; ++t) product(t, u);
+#pragma unroll
+      for (int q = u * T::kPerA / NT; q < (u + 1) * T::kPerA / NT; ++q) issue_a(after, q);
+      if (u == NT - 1)
+#pragma unroll
+        for (int q = 0; q < T::kScalePer; ++q) issue_scales(after, q);
+      read_w(next, u, 0xFF);
+      if (u < H) read_a(next, u, 0xFF);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    at = next_at;
+  }
+  const int live = (steps - 1) * 128 + g * 32 < p.K ? 0xFF : 0;
+#pragma unroll
+  for (int u = 0; u < NT; ++u) sw[u] &= live;
+#pragma unroll
+  for (int t = 0; t < H; ++t) sa[t] &= live;
+  first_tiles(buffer(at), live, nullptr);
+#pragma unroll
+  for (int t = MT - S; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) product(t, u);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may land in the LDS of the next workgroup
 
   // Epilogue: lane group g holds channels n .. n + 4 NT - 1 of row m for every tile row.
   const int n = n0 + wn * 16 * NT + g * 4 * NT;
@@ -232,8 +364,33 @@ void launch_mx_linear(const MxLinearArgs& p, hipStream_t st) {
   using T = MxTile<MT, NT, WM, WN, ST>;
   // an 8-bit result's scales are written up to the next 128 columns
   const int64_t cols = p.ys != nullptr ? ceil_div(p.N, 128) * 128 : p.N;
-  const dim3 grid((unsigned)ceil_div(cols, T::kBN), (unsigned)ceil_div(p.M, T::kBM));
+  const dim3 grid((unsigned)(ceil_div(cols, T::kBN) * ceil_div(p.M, T::kBM)));
   hipLaunchKernelGGL((mx_linear_kernel<MT, NT, WM, WN, ST, GELU>), grid, dim3(T::kThreads), 0, st, p);
+}
+
+// The tile height with the least estimated time: rounds of one tile per CU, a step's
+// time times the steps, and what a tile costs beside them.  Step times as
+// measured over 8192 x 8192 x 8192 (us, every CU busy).
+template <bool GELU>
+void launch_tile(const MxLinearArgs& p, hipStream_t st) {
+  struct Height {
+    int rows;
+    float step;
+    void (*launch)(const MxLinearArgs&, hipStream_t);
+  };
+  static const Height heights[] = {
+      {256, 1.41f, launch_mx_linear<8, 4, 2, 4, 2, GELU>}, {192, 1.03f, launch_mx_linear<6, 4, 2, 4, 2, GELU>},
+      {160, 0.94f, launch_mx_linear<5, 4, 2, 4, 2, GELU>}, {128, 0.85f, launch_mx_linear<4, 4, 2, 4, 3, GELU>},
+      {64, 0.60f, launch_mx_linear<2, 4, 2, 4, 3, GELU>},
+  };
+  const Height* best = nullptr;
+  float least = 0.0f;
+  for (const Height& h : heights) {
+    const int64_t tiles = ceil_div(p.M, h.rows) * ceil_div(p.N, 256);
+    const float t = ceil_div(tiles, 256) * (ceil_div(p.K, 128) * h.step + 7.0f);
+    if (best == nullptr || t < least) best = &h, least = t;
+  }
+  best->launch(p, st);
 }
 
 }  // namespace ltx
@@ -262,9 +419,9 @@ extern "C" int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_code
   LTX_REQUIRE(ceil_div(M, 128) <= 65535, "ltx_mx_linear: too many rows");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (act)
-    launch_mx_linear<4, 4, 2, 2, 2, true>(p, st);
+    launch_tile<true>(p, st);
   else
-    launch_mx_linear<4, 4, 2, 2, 2, false>(p, st);
+    launch_tile<false>(p, st);
   LTX_LAUNCH_CHECK("ltx_mx_linear");
   return LTX_OK;
 }
