@@ -19,6 +19,8 @@
 // group i ends with the 4 NT neighbouring channels 4 NT i ..: contiguous stores,
 // and blocks of 32 for an 8-bit result inside one lane (NT = 8) or a pair (NT = 4).
 
+#include <math.h>
+
 #include <type_traits>
 
 #include "mx_common.h"
@@ -46,6 +48,11 @@ __device__ __forceinline__ mx_i8 mx_fragment(const MX_LDS uint8_t* lo, const MX_
   return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+__device__ __forceinline__ mx_i8 mx_fragment(__amdgpu_buffer_rsrc_t r, int lo, int hi) {
+  const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, lo, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b128(r, hi, 0, 0);
+  return __builtin_shufflevector(__builtin_bit_cast(mx_i4, x), __builtin_bit_cast(mx_i4, y), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 struct MxLinearArgs {
   const uint8_t* a;
   const uint8_t* as;
@@ -69,27 +76,29 @@ __device__ __forceinline__ float mx_gelu(float y) {
 
 constexpr int kGroupM = 4;
 
-// MT x NT tiles of 16 x 16 per wave, WM x WN waves, ST buffers of one step each.
-template <int MT, int NT, int WM, int WN, int ST>
+// MT x NT tiles of 16 x 16 per wave, WM x WN waves per group, ST buffers of one step each,
+// KG groups that split the columns of K and meet at the end.
+template <int MT, int NT, int WM, int WN, int ST, int KG>
 struct MxTile {
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves * KG;  // waves of a group
   static constexpr int kBM = 16 * MT * WM, kBN = 16 * NT * WN, kRows = kBM + kBN;
-  static constexpr int kARows = (kBM + 63) / 64 * 64;         // a's rows in the scales: whole loads
-  static constexpr int kCodes = kRows * 128, kStage = kCodes + (kARows + kBN) * 4;
+  static constexpr int kARows = (kBM + 63) / 64 * 64, kWRows = (kBN + 63) / 64 * 64;  // of scales: whole loads
+  static constexpr int kCodes = kRows * 128, kStage = kCodes + (kARows + kWRows) * 4;
   // 1 KB loads (8 rows) per step and wave, of each operand
   static constexpr int kPerA = (kBM / 8 + kWaves - 1) / kWaves, kPerW = (kBN / 8 + kWaves - 1) / kWaves;
-  static constexpr int kScaleLoads = (kARows + kBN) / 64;     // 256 byte loads (64 rows' words) per step
+  static constexpr int kScaleLoads = (kARows + kWRows) / 64;     // 256 byte loads (64 rows' words) per step
   static constexpr int kScalePer = (kScaleLoads + kWaves - 1) / kWaves, kParts = kPerA + kPerW + kScalePer;
-  static_assert(kWaves % 2 == 0 && kBM % 8 == 0 && kBN % 64 == 0, "whole loads of one operand");
-  static_assert(ST >= 2 && ST * kStage <= 160 * 1024, "LDS");
+  static_assert(KG == 1 || KG / 2 * kWaves * MT * NT * 1024 <= KG * ST * kStage, "LDS");
+  static_assert(ST >= 2 && KG * ST * kStage <= 160 * 1024, "LDS");
 };
 
-template <int MT, int NT, int WM, int WN, int ST, bool GELU>
-__global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLinearArgs p) {
-  using T = MxTile<MT, NT, WM, WN, ST>;
-  __shared__ __attribute__((aligned(128))) uint8_t lds[ST * T::kStage];
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+template <int MT, int NT, int WM, int WN, int ST, int KG, bool GELU>
+__global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx_linear_kernel(const MxLinearArgs p) {
+  using T = MxTile<MT, NT, WM, WN, ST, KG>;
+  __shared__ __attribute__((aligned(128))) uint8_t lds[KG * ST * T::kStage];
+  const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave_of_all % T::kWaves, kg = wave_of_all / T::kWaves;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_ptr)lds + kg * ST * T::kStage;
   const int wm = wave % WM, wn = wave / WM;
   const int g = lane >> 4, r16 = lane & 15;
   // Workgroups go round-robin to the 8 XCDs: each gets a contiguous run of tiles, walked in
@@ -100,7 +109,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
   const int group = tile / (kGroupM * tn), in = tile - group * kGroupM * tn, gm = min(kGroupM, tm - group * kGroupM);
   const int m0 = __builtin_amdgcn_readfirstlane((group * kGroupM + in % gm) * T::kBM);
   const int n0 = __builtin_amdgcn_readfirstlane(in / gm * T::kBN);
-  const int steps = (p.K + 127) / 128;
+  // A group's steps; the last group's end with K, and what the first ones have before column 0 reads as zeros.
+  const int all = (p.K + 127) / 128, steps = (all + KG - 1) / KG, first = all - (KG - kg) * steps;
 
   // The channel of the tile that row r of its w rows holds.
   auto channel = [](int r) {
@@ -139,13 +149,13 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
   auto step = [&](int ks, int at) {
     Step r;
     r.base = lds0 + at;
-    const int k0 = ks * 128, left = max(p.K - k0, 0);
+    const int k0 = (first + ks) * 128, left = k0 < 0 || ks >= steps ? 0 : max(p.K - k0, 0);
     r.a = __builtin_amdgcn_make_buffer_rsrc((void*)(abase + k0), (short)0, left > 0 ? mrows * p.K - k0 : 0, 0x00020000);
     r.w = __builtin_amdgcn_make_buffer_rsrc((void*)(wbase + k0), (short)0, left > 0 ? max(nrows * p.K - k0, 0) : 0,
                                             0x00020000);
-    r.as = __builtin_amdgcn_make_buffer_rsrc((void*)(asbase + (int64_t)ks * p.M * 4), (short)0,
+    r.as = __builtin_amdgcn_make_buffer_rsrc((void*)(asbase + (int64_t)(first + ks) * p.M * 4), (short)0,
                                              left > 0 ? mrows * 4 : 0, 0x00020000);
-    r.ws = __builtin_amdgcn_make_buffer_rsrc((void*)(wsbase + (int64_t)ks * p.N * 4), (short)0,
+    r.ws = __builtin_amdgcn_make_buffer_rsrc((void*)(wsbase + (int64_t)(first + ks) * p.N * 4), (short)0,
                                              left > 0 ? nrows * 4 : 0, 0x00020000);
     r.left = left;
     return r;
@@ -260,7 +270,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
   meet(std::integral_constant<int, (ST - 1) * T::kParts>{});
   {
     const Buffer b = buffer(0);
-    const int live = g * 32 < p.K ? 0xFF : 0;  // the scale bytes of blocks past K are not looked at
+    const int live = first * 128 + g * 32 < p.K ? 0xFF : 0;  // the scale bytes of blocks past K are not looked at
 #pragma unroll
     for (int t = 0; t < H; ++t) read_a(b, t, live);
 #pragma unroll
@@ -290,7 +300,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
     __builtin_amdgcn_s_setprio(0);
     at = next_at;
   }
-  const int live = (steps - 1) * 128 + g * 32 < p.K ? 0xFF : 0;
+  const int live = (first + steps - 1) * 128 + g * 32 < p.K ? 0xFF : 0;
 #pragma unroll
   for (int u = 0; u < NT; ++u) sw[u] &= live;
 #pragma unroll
@@ -301,6 +311,26 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
 #pragma unroll
     for (int u = 0; u < NT; ++u) product(t, u);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may land in the LDS of the next workgroup
+  if constexpr (KG > 1) {  // the groups' sums meet in the first one's registers, halving their number
+    mx_f4* part = reinterpret_cast<mx_f4*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int half = KG / 2; half > 0; half /= 2) {
+      if (kg >= half && kg < 2 * half)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) part[((((kg - half) * T::kWaves + wave) * MT + t) * NT + u) * 64 + lane] = acc[t][u];
+      __syncthreads();
+      if (kg < half)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) acc[t][u] += part[(((kg * T::kWaves + wave) * MT + t) * NT + u) * 64 + lane];
+      __syncthreads();
+    }
+    if (kg > 0) return;
+  }
 
   // Epilogue: lane group g holds channels n .. n + 4 NT - 1 of row m for every tile row.
   const int n = n0 + wn * 16 * NT + g * 4 * NT;
@@ -324,19 +354,18 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
         if (n + i >= p.N) v[i] = 0.0f;
         top = fmaxf(top, mx_magnitude(v[i]));
       }
+      static_assert(NT == 2 || NT == 4 || NT == 8, "a block of 32 lies in one, two or four lanes");
       if (NT < 8) top = fmaxf(top, __shfl_xor(top, 16, 64));
-      static_assert(NT == 4 || NT == 8, "a block of 32 lies in one lane or a pair of lanes");
+      if (NT < 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
       const uint32_t code = mx_scale_code(top);
       const float inv = mx_inverse(code);
       if (m < p.M) {
         uint8_t* yp = (uint8_t*)p.y + (int64_t)m * p.N + n;
 #pragma unroll
-        for (int i = 0; i < 4 * NT; i += 16) {
-          const uint4 c = make_uint4(mx_pack4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv),
-                                     mx_pack4(v[i + 4] * inv, v[i + 5] * inv, v[i + 6] * inv, v[i + 7] * inv),
-                                     mx_pack4(v[i + 8] * inv, v[i + 9] * inv, v[i + 10] * inv, v[i + 11] * inv),
-                                     mx_pack4(v[i + 12] * inv, v[i + 13] * inv, v[i + 14] * inv, v[i + 15] * inv));
-          if (n + i < p.N) *reinterpret_cast<uint4*>(yp + i) = c;
+        for (int i = 0; i < 4 * NT; i += 8) {
+          const uint2 c = make_uint2(mx_pack4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv),
+                                     mx_pack4(v[i + 4] * inv, v[i + 5] * inv, v[i + 6] * inv, v[i + 7] * inv));
+          if (n + i < p.N) *reinterpret_cast<uint2*>(yp + i) = c;
         }
         // blocks past N up to the next 128 columns are written as 0
         if (n / 128 < (p.N + 127) / 128 && n % 32 == 0)
@@ -359,35 +388,202 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) mx_linear_kernel(const MxLine
   }
 }
 
-template <int MT, int NT, int WM, int WN, int ST, bool GELU>
+template <int MT, int NT, int WM, int WN, int ST, int KG, bool GELU>
 void launch_mx_linear(const MxLinearArgs& p, hipStream_t st) {
-  using T = MxTile<MT, NT, WM, WN, ST>;
+  using T = MxTile<MT, NT, WM, WN, ST, KG>;
   // an 8-bit result's scales are written up to the next 128 columns
   const int64_t cols = p.ys != nullptr ? ceil_div(p.N, 128) * 128 : p.N;
   const dim3 grid((unsigned)(ceil_div(cols, T::kBN) * ceil_div(p.M, T::kBM)));
-  hipLaunchKernelGGL((mx_linear_kernel<MT, NT, WM, WN, ST, GELU>), grid, dim3(T::kThreads), 0, st, p);
+  hipLaunchKernelGGL((mx_linear_kernel<MT, NT, WM, WN, ST, KG, GELU>), grid, dim3(T::kThreads), 0, st, p);
 }
 
-// The tile height with the least estimated time: rounds of one tile per CU, a step's
-// time times the steps, and what a tile costs beside them.  Step times as
-// measured over 8192 x 8192 x 8192 (us, every CU busy).
+// Few rows: a workgroup's 8 waves share a tile of 16 MT rows of y by 16 NT channels and
+// split its columns of K.  They have no operand in common, so fragments go from HBM
+// straight to registers, the next step's while this one's are multiplied; a
+// problem whose steps one after the other would each wait for memory waits an eighth as
+// often.  The partial sums meet in LDS: the upper four waves' are added to the lower
+// four's, then 512 threads add four each, 8 neighbouring channels of a row at a time.
+constexpr int kRowWaves = 8;
+
+template <int MT, int NT, bool GELU>
+__global__ void __launch_bounds__(64 * kRowWaves, 2) mx_linear_rows_kernel(const MxLinearArgs p) {
+  constexpr int kBM = 16 * MT, kBN = 16 * NT, kLine = kBN + 4;
+  __shared__ __attribute__((aligned(16))) float part[kRowWaves / 2][kBM][kLine];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r16 = lane & 15;
+  // workgroups of one XCD share channels: the rows of y go by first
+  const int tm = (p.M + kBM - 1) / kBM;
+  const int per = gridDim.x / 8, rem = gridDim.x % 8, xcd = blockIdx.x % 8;
+  const int tile = xcd * per + min(xcd, rem) + blockIdx.x / 8;
+  const int m0 = __builtin_amdgcn_readfirstlane(tile % tm * kBM), n0 = __builtin_amdgcn_readfirstlane(tile / tm * kBN);
+  const int steps = (p.K + 127) / 128, own = (steps + kRowWaves - 1) / kRowWaves;
+  const int first = wave * own, last = min(first + own, steps);
+
+  const int mrows = min(p.M - m0, kBM), nrows = max(min(p.N - n0, kBN), 0);
+  const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + (int64_t)m0 * p.K), (short)0, mrows * p.K, 0x00020000);
+  const auto rw = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + (int64_t)n0 * p.K), (short)0, nrows * p.K, 0x00020000);
+  struct Fragments {
+    mx_i8 a[MT], w[NT];
+    int sa[MT], sw[NT];
+  };
+  // rows past the operand's last, and columns past K by their offset, read as zeros
+  auto load = [&](Fragments& f, int ks) {
+    const int lo = ks * 128 + g * 16, hi = lo + 64;
+    const int plo = lo < p.K ? lo : 0x40000000, phi = hi < p.K ? hi : 0x40000000;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) f.a[t] = mx_fragment(ra, (t * 16 + r16) * p.K + plo, (t * 16 + r16) * p.K + phi);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) f.w[u] = mx_fragment(rw, (u * 16 + r16) * p.K + plo, (u * 16 + r16) * p.K + phi);
+    const bool live = ks * 128 + g * 32 < p.K;  // the scale bytes of blocks past K are not looked at
+    const uint8_t* as = p.as + ((int64_t)ks * p.M + m0) * 4 + g;
+    const uint8_t* ws = p.ws + ((int64_t)ks * p.N + n0) * 4 + g;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) f.sa[t] = live && t * 16 + r16 < mrows ? as[(t * 16 + r16) * 4] : 0;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) f.sw[u] = live && u * 16 + r16 < nrows ? ws[(u * 16 + r16) * 4] : 0;
+  };
+  mx_f4 acc[MT][NT] = {};
+  auto products = [&](const Fragments& f) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+        acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.w[u], f.a[t], acc[t][u], 0, 0, 0, f.sw[u], 0, f.sa[t]);
+  };
+  Fragments f[2];
+  if (first < last) load(f[0], first);
+  int ks = first;
+  for (; ks + 2 < last; ks += 2) {
+    load(f[1], ks + 1);
+    products(f[0]);
+    load(f[0], ks + 2);
+    products(f[1]);
+  }
+  if (ks + 1 < last) {
+    load(f[1], ks + 1);
+    products(f[0]);
+    products(f[1]);
+  } else if (ks < last) {
+    products(f[0]);
+  }
+
+  // lane: channels 16 u + 4 g .. + 3 of row 16 t + r16
+  if (wave >= kRowWaves / 2)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+        *reinterpret_cast<mx_f4*>(&part[wave - kRowWaves / 2][t * 16 + r16][u * 16 + g * 4]) = acc[t][u];
+  __syncthreads();
+  if (wave < kRowWaves / 2)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        mx_f4* to = reinterpret_cast<mx_f4*>(&part[wave][t * 16 + r16][u * 16 + g * 4]);
+        *to = *to + acc[t][u];
+      }
+  __syncthreads();
+  constexpr int kItems = kBM * kBN / 8, kCols = kBN / 8;
+#pragma unroll
+  for (int i0 = 0; i0 < kItems; i0 += 64 * kRowWaves) {
+    const int i = i0 + threadIdx.x;
+    if (kItems % (64 * kRowWaves) != 0 && i >= kItems) break;  // whole blocks of 4 threads
+    const int row = i / kCols, c = i % kCols * 8, m = m0 + row, n = n0 + c;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const mx_f4 x = *reinterpret_cast<const mx_f4*>(&part[0][row][c + e]), y = *reinterpret_cast<const mx_f4*>(&part[1][row][c + e]);
+      const mx_f4 z = *reinterpret_cast<const mx_f4*>(&part[2][row][c + e]), w = *reinterpret_cast<const mx_f4*>(&part[3][row][c + e]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[e + k] = (x[k] + y[k]) + (z[k] + w[k]);
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] += p.bias != nullptr && n + e < p.N ? bf16_bits_to_f32(p.bias[n + e]) : 0.0f;
+      if (GELU) v[e] = mx_gelu(v[e]);
+      if (n + e >= p.N) v[e] = 0.0f;
+      top = fmaxf(top, mx_magnitude(v[e]));
+    }
+    if (p.ys != nullptr) {
+      if constexpr (NT % 2 == 0) {
+        top = fmaxf(top, __shfl_xor(top, 1, 64));
+        top = fmaxf(top, __shfl_xor(top, 2, 64));
+        const uint32_t code = mx_scale_code(top);
+        const float inv = mx_inverse(code);
+        if (m < p.M) {
+          if (n < p.N)
+            *reinterpret_cast<uint2*>((uint8_t*)p.y + (int64_t)m * p.N + n) =
+                make_uint2(mx_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                           mx_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+          // blocks past N up to the next 128 columns are written as 0
+          if (n % 32 == 0 && n / 128 < (p.N + 127) / 128)
+            p.ys[((int64_t)(n / 128) * p.M + m) * 4 + n / 32 % 4] = (uint8_t)code;
+        }
+      }
+    } else if (m < p.M) {
+      uint16_t* yp = (uint16_t*)p.y + (int64_t)m * p.y_ls + n;
+      if (p.vec && n + 8 <= p.N) {
+        *reinterpret_cast<uint4*>(yp) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                   pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < p.N) yp[e] = f32_to_bf16_bits(v[e]);
+      }
+    }
+  }
+}
+
+template <int MT, int NT, bool GELU>
+void launch_mx_rows(const MxLinearArgs& p, hipStream_t st) {
+  const int64_t cols = p.ys != nullptr ? ceil_div(p.N, 128) * 128 : p.N;
+  const dim3 grid((unsigned)(ceil_div(cols, 16 * NT) * ceil_div(p.M, 16 * MT)));
+  hipLaunchKernelGGL((mx_linear_rows_kernel<MT, NT, GELU>), grid, dim3(64 * kRowWaves), 0, st, p);
+}
+
+// The kernels by their tile of y and the groups that split K, with an estimate of
+// their time in us, fitted to 75 shapes of 1 to 2304 rows, 128 to 16384 columns and 32
+// to 16384 channels: `once`, then for every round of workgroups `round` plus `step` for
+// each step of a group (`each` per 256 tiles and step instead where many tiles
+// share a CU), never below what the bytes take at 5.3 TB/s.  Over those shapes the
+// choice is within 4 % of the fastest of 17 tiles in the mean.  What the ends are for: at 2
+// rows of 4096 -> 16384 the 64-row tile without groups takes 21.4 us where the rows
+// kernel and the 32 x 64 tile take 13.6 and 14.5 (the weight's bytes 13.2); at 2304 rows
+// of 4096 -> 12288 the 256-row tile takes 113 us, the 192-row one 124, at 16384
+// channels 156 and 145; at 150 rows of 2048 -> 8192 80 x 64 takes 10.4, 128 x 256 19.1.
+struct MxShape {
+  int rows, cols, groups;
+  float once, round, step, each;
+  void (*launch)(const MxLinearArgs&, hipStream_t);
+};
+
 template <bool GELU>
-void launch_tile(const MxLinearArgs& p, hipStream_t st) {
-  struct Height {
-    int rows;
-    float step;
-    void (*launch)(const MxLinearArgs&, hipStream_t);
+void launch_mx(const MxLinearArgs& p, hipStream_t st) {
+  static const MxShape shapes[] = {
+      {16, 16, 8, 3.22f, 0.0f, 0.36f, 0.77f, launch_mx_rows<1, 1, GELU>},  // bf16 results
+      {16, 32, 8, 3.11f, 0.0f, 0.63f, 1.34f, launch_mx_rows<1, 2, GELU>},  // 8-bit ones: whole blocks
+      {32, 32, 4, 1.45f, 3.23f, 0.39f, 0.0f, launch_mx_linear<2, 2, 1, 1, 3, 4, GELU>},
+      {32, 64, 4, 1.13f, 3.64f, 0.61f, 0.0f, launch_mx_linear<2, 2, 1, 2, 3, 4, GELU>},
+      {64, 64, 2, 1.17f, 3.60f, 0.48f, 0.0f, launch_mx_linear<2, 2, 2, 2, 3, 2, GELU>},
+      {80, 64, 4, 0.76f, 4.89f, 0.84f, 0.0f, launch_mx_linear<5, 2, 1, 2, 2, 4, GELU>},
+      {160, 64, 2, 0.0f, 5.19f, 0.71f, 0.0f, launch_mx_linear<5, 2, 2, 2, 2, 2, GELU>},
+      {128, 128, 2, 0.0f, 6.70f, 0.87f, 0.0f, launch_mx_linear<4, 4, 2, 2, 2, 2, GELU>},
+      {128, 256, 1, 0.0f, 6.21f, 0.78f, 0.0f, launch_mx_linear<4, 4, 2, 4, 3, 1, GELU>},
+      {192, 256, 1, 0.0f, 6.22f, 0.94f, 0.0f, launch_mx_linear<6, 4, 2, 4, 2, 1, GELU>},
+      {256, 256, 1, 0.0f, 8.21f, 1.09f, 0.0f, launch_mx_linear<8, 4, 2, 4, 2, 1, GELU>},
   };
-  static const Height heights[] = {
-      {256, 1.41f, launch_mx_linear<8, 4, 2, 4, 2, GELU>}, {192, 1.03f, launch_mx_linear<6, 4, 2, 4, 2, GELU>},
-      {160, 0.94f, launch_mx_linear<5, 4, 2, 4, 2, GELU>}, {128, 0.85f, launch_mx_linear<4, 4, 2, 4, 3, GELU>},
-      {64, 0.60f, launch_mx_linear<2, 4, 2, 4, 3, GELU>},
-  };
-  const Height* best = nullptr;
+  const float bytes = ((float)p.M + p.N) * p.K * 1.03f + 2.0f * p.M * p.N, floor = 2.5f + bytes / 5.3e6f;
+  const MxShape* best = nullptr;
   float least = 0.0f;
-  for (const Height& h : heights) {
-    const int64_t tiles = ceil_div(p.M, h.rows) * ceil_div(p.N, 256);
-    const float t = ceil_div(tiles, 256) * (ceil_div(p.K, 128) * h.step + 7.0f);
+  for (const MxShape& h : shapes) {
+    if (h.cols == (p.ys != nullptr ? 16 : 32) && h.each > 0.0f) continue;
+    const float tiles = (float)(ceil_div(p.M, h.rows) * ceil_div(p.N, h.cols));
+    const float steps = (float)ceil_div(ceil_div(p.K, 128), h.groups);
+    const float rounds = h.each > 0.0f ? 1.0f : ceilf(tiles / 256.0f);
+    const float own = h.once + rounds * (h.round + steps * h.step) + tiles / 256.0f * steps * h.each;
+    const float t = fmaxf(own, floor) + 0.1f * own;  // between those at the floor, the one with least of its own
     if (best == nullptr || t < least) best = &h, least = t;
   }
   best->launch(p, st);
@@ -419,9 +615,9 @@ extern "C" int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_code
   LTX_REQUIRE(ceil_div(M, 128) <= 65535, "ltx_mx_linear: too many rows");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (act)
-    launch_tile<true>(p, st);
+    launch_mx<true>(p, st);
   else
-    launch_tile<false>(p, st);
+    launch_mx<false>(p, st);
   LTX_LAUNCH_CHECK("ltx_mx_linear");
   return LTX_OK;
 }
