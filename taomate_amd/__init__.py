@@ -18,6 +18,8 @@ The public names mirror the reference's drop-in surface:
   update, retention)
 * ``LearnedMemoryState``, ``StreamingMemory`` (taomate/runtime_support/learned_memory.py,
   taomate/inference/memory.py)
+* ``AVModel.quantize_linears_`` (feed-forwards in 8 bits, timestep linears in 4: ``quant``; no
+  counterpart in the reference)
 * ``load_generator`` / ``save_generator`` (taomate/inference/model_runtime.py:182-425) and the
   interactive prefix state (taomate/inference/streaming_runtime.py:1404-1500)
 
@@ -37,7 +39,8 @@ from .runtime import StreamingGenerator, denoising_sigmas
 from .rope import CausalRopeType, apply_split_rotary_emb, causal_precompute_freqs_cis, generate_freq_grid
 from .streaming import ChunkStream, retain_pinned_recent
 from .memory import LearnedMemoryState, StreamingMemory
-from . import dit
+from . import dit, quant
+from .quant import Group4Weight, MXRows, quantize_group4, quantize_mx
 from .checkpoint import load_generator, save_generator
 from .prefix_state import build_prefix_state_payload, load_prefix_state, save_prefix_state
 
@@ -51,4 +54,5 @@ __all__ = [
     "LearnedMemoryState", "StreamingMemory", "load_generator", "save_generator", "build_prefix_state_payload",
     "load_prefix_state", "save_prefix_state", "attach_arena", "attach_block_arenas", "ArenaPlan",
     "Installation", "init_kv_cache_for", "install", "StreamingGenerator", "denoising_sigmas",
+    "Group4Weight", "MXRows", "quantize_group4", "quantize_mx",
 ]

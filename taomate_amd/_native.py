@@ -18,6 +18,7 @@ F32, BF16, F8E4M3 = 0, 1, 2
 MAX_SEGMENTS = 16
 MAX_KEYLEN_BATCH = 16  # LTX_MAX_KEYLEN_BATCH
 GROUP4_MAX_ROWS = 16  # LTX_GROUP4_MAX_ROWS
+GROUP4_MAX_COLUMNS = 4096  # LTX_SKINNY_MAX_K
 NOALLOC_SCRATCH_BYTES = 25 << 20  # LTX_NOALLOC_SCRATCH_BYTES
 ABI_VERSION = 2
 

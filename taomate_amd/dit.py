@@ -38,7 +38,7 @@ import torch.nn.functional as F
 import torch.nn.modules.module as nn_module
 from torch.autograd import forward_ad
 
-from . import _native, kernels
+from . import _native, kernels, quant
 from .attention import CausalLTXAttention, attention_with_cache, standard_attention_forward
 from .kv_cache import LayerKVCache, _cat_cache
 
@@ -72,7 +72,54 @@ class FeedForward(nn.Module):
         inner = int(dim * mult)
         self.net = nn.Sequential(GELUApprox(dim, inner), nn.Identity(), nn.Linear(inner, dim_out))
 
+    def quantize_(self, enabled: bool = True) -> "FeedForward":
+        """Run the two linears in 8 bits (``kernels.mx_linear``): the weights are
+        packed into 8-bit rows beside the bf16 parameters, which keep their
+        names and values; the activations are quantised by the norm before
+        and by the first linear's epilogue.  Anything that changes or replaces a
+        weight afterwards ends it and the bf16 linears run again; so do calls
+        that something else would see (gradients, autocast, hooks, compilation).
+        Both widths must be multiples of 32, the input's at most 8192."""
+        self.__dict__.pop("_mx", None)
+        if not enabled:
+            return self
+        up, down = self.net[0].proj, self.net[2]
+        for lin in (up, down):
+            if not _is_plain(lin, nn.Linear) or lin.weight.dtype != torch.bfloat16:
+                raise TypeError("quantize_: both linears must be plain bf16 nn.Linear modules")
+        if up.in_features > kernels.ADALN_MX_MAX_COLUMNS:
+            raise ValueError(f"quantize_: inputs of at most {kernels.ADALN_MX_MAX_COLUMNS} channels, "
+                             f"got {up.in_features}")
+        self._mx = tuple(quant.Packed(lin, quant.quantize_mx(lin.weight)) for lin in (up, down))
+        return self
+
+    def quantized(self) -> bool:
+        """Whether a call now runs in 8 bits, as ``quantize_`` describes."""
+        mx = self.__dict__.get("_mx")
+        if mx is None:
+            return False
+        act, mid, down = self.net[0], self.net[1], self.net[2]
+        if not (_is_plain(self, FeedForward) and _is_plain(self.net, nn.Sequential) and len(self.net) == 3
+                and _is_plain(act, GELUApprox) and _is_plain(act.proj, nn.Linear) and _is_plain(mid, nn.Identity)
+                and _is_plain(down, nn.Linear) and _is_eager()):
+            return False
+        if not (mx[0].holds(act.proj) and mx[1].holds(down)):
+            del self._mx   # a weight was changed or replaced: drop the stale rows
+            return False
+        return act.proj.weight.is_cuda
+
+    def forward_rows(self, rows: quant.MXRows) -> torch.Tensor:
+        """The feed-forward of 8-bit rows (``quantized()`` must hold)."""
+        up, down = self._mx
+        h = kernels.mx_linear(rows, up.rows, self.net[0].proj.bias, gelu=True, quantize=True)
+        return kernels.mx_linear(h, down.rows, self.net[2].bias)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.is_cuda and x.dtype == torch.bfloat16 and "_mx" in self.__dict__ and self.quantized():
+            rows = x.reshape(1, -1, x.shape[-1]).contiguous()
+            if rows.data_ptr() % 16:
+                rows = rows.clone()
+            return self.forward_rows(kernels.adaln_mx(rows, eps=None)).view(*x.shape[:-1], self.net[2].out_features)
         return self.net(x)
 
 
@@ -108,9 +155,25 @@ def _row_linear(lin: nn.Module, x: torch.Tensor, act: Optional[nn.Module] = None
     if (x.is_cuda and _is_plain(lin, nn.Linear) and (act is None or _is_plain(act, nn.SiLU) and not act.inplace)
             and _is_eager()):
         w, b = lin.weight, lin.bias
+        packed = lin.__dict__.get("_group4")
+        if packed is not None and x.dim() == 2 and x.shape[0] <= _native.GROUP4_MAX_ROWS and x.dtype == torch.bfloat16:
+            if packed.holds(lin):
+                x = x.contiguous()
+                return kernels.group4_linear(x.clone() if x.data_ptr() % 16 else x, packed.rows, b, silu=act is not None)
+            del lin._group4   # the weight was changed or replaced: drop the stale codes
         if _native._host.row_operands(x, w, b):
             return kernels.skinny_linear(x, w, b, silu=act is not None)
     return lin(x if act is None else act(x))
+
+
+def _pack_group4(lin: nn.Linear, group: int) -> None:
+    """Hold ``lin``'s weight in 4 bits beside its parameter for ``_row_linear``."""
+    if not _is_plain(lin, nn.Linear) or lin.weight.dtype != torch.bfloat16:
+        raise TypeError("4-bit timestep linears must be plain bf16 nn.Linear modules")
+    if lin.in_features > _native.GROUP4_MAX_COLUMNS:
+        raise ValueError(f"4-bit timestep linears take at most {_native.GROUP4_MAX_COLUMNS} columns, "
+                         f"got {lin.in_features}")
+    lin._group4 = quant.Packed(lin, quant.quantize_group4(lin.weight, group))
 
 
 class TimestepEmbedding(nn.Module):
@@ -317,6 +380,27 @@ def _residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor] = N
     return xo, n
 
 
+def _residual_rows(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor,
+                   eps: float) -> Tuple[torch.Tensor, quant.MXRows]:
+    """``_residual`` with the modulated norm in 8 bits (ltx_adaln_mx)."""
+    xo = torch.empty_like(x)
+    return xo, kernels.adaln_mx(x, y, gate, xo, scale, shift, eps=eps)
+
+
+def _feed_forward(ff: FeedForward, x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, scale: torch.Tensor,
+                  shift: torch.Tensor, ff_gate: torch.Tensor, eps: float) -> torch.Tensor:
+    """x' = x + y * gate, then x' + ff(rms_norm(x') * (1 + scale) + shift) * ff_gate:
+    the cross-modal residual, the feed-forward's input norm, the feed-forward
+    (in 8 bits where it is quantised) and its residual."""
+    if isinstance(ff, FeedForward) and ff.quantized():
+        x, rows = _residual_rows(x, y, gate, scale, shift, eps)
+        out = ff.forward_rows(rows)
+    else:
+        x, n = _residual(x, y, gate, norm=True, scale=scale, shift=shift, eps=eps)
+        out = ff(n)
+    return _residual(x, out, ff_gate, eps=eps)[0]
+
+
 def _apply_memory(x: torch.Tensor, n: Optional[torch.Tensor], steps, eps: float, need_norm: bool):
     """x + adapter(rms_norm(x), arg) for each (adapter, arg) in ``steps``
     (causal_block.py:489-505), each residual fused with the next norm.  ``n``
@@ -478,13 +562,11 @@ def block_forward_with_cache(block: AVBlock, vx: torch.Tensor, ax: torch.Tensor,
                                                  video_cross_pe, cache.v2a_k, cache.v2a_v)
     # cross-modal residuals fused with the feed-forward input norms
     sh, sc, g = ada["v"][3:6] if ada else block.get_ada_values(block.scale_shift_table, B, v_ts, slice(3, 6))
-    vx, vn = _residual(vx, a2v, gate_a2v, norm=True, scale=sc, shift=sh, eps=eps)
-    vx, _ = _residual(vx, block.ff(vn), g, eps=eps)
+    vx = _feed_forward(block.ff, vx, a2v, gate_a2v, sc, sh, g, eps)
     with on_audio():
         sh, sc, g = ada["a"][3:6] if ada else block.get_ada_values(block.audio_scale_shift_table, B, a_ts,
                                                                    slice(3, 6))
-        ax, an = _residual(ax, v2a, gate_v2a, norm=True, scale=sc, shift=sh, eps=eps)
-        ax, _ = _residual(ax, block.audio_ff(an), g, eps=eps)
+        ax = _feed_forward(block.audio_ff, ax, v2a, gate_v2a, sc, sh, g, eps)
     new_cache = LayerKVCache(
         video_self_k=_cat_cache(cache.video_self_k, vs_k), video_self_v=_cat_cache(cache.video_self_v, vs_v),
         audio_self_k=_cat_cache(cache.audio_self_k, as_k), audio_self_v=_cat_cache(cache.audio_self_v, as_v),
@@ -564,6 +646,24 @@ class AVModel(nn.Module):
         for m in self.modules():
             if isinstance(m, CausalLTXAttention):
                 m.fuse_qkv_()
+        return self
+
+    def quantize_linears_(self, feed_forward: bool = True, timestep: bool = True, group: int = 32) -> "AVModel":
+        """Hold weights in fewer bits beside the bf16 parameters, whose names and
+        values stay: every block's video and audio feed-forward in 8 bits
+        (``FeedForward.quantize_``), and the linears of the timestep embeddings
+        and modulations in 4 bits with a bf16 scale for every ``group`` columns,
+        for calls of up to 16 rows (one per sample or frame; more rows run in
+        bf16).  False ends either.  Load the weights before; a weight that is
+        changed or replaced afterwards runs in bf16 again until the next call."""
+        for m in self.modules():
+            if isinstance(m, FeedForward):
+                m.quantize_(feed_forward)
+            elif isinstance(m, (TimestepEmbedding, AdaLayerNormSingle)):
+                for lin in (m.linear_1, m.linear_2) if isinstance(m, TimestepEmbedding) else (m.linear,):
+                    lin.__dict__.pop("_group4", None)
+                    if timestep:
+                        _pack_group4(lin, group)
         return self
 
     def overlap_audio_(self, enabled: bool = True) -> "AVModel":

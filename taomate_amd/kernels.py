@@ -17,6 +17,9 @@ _DT = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.uint8: N.F8E4M3,
        torch.float8_e4m3fn: N.F8E4M3}
 
 
+ADALN_MX_MAX_COLUMNS = 8192   # ltx_adaln_mx
+
+
 def _code(t: torch.Tensor) -> int:
     try:
         return _DT[t.dtype]

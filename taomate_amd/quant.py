@@ -150,3 +150,21 @@ def quantize_group4(weight: torch.Tensor, group: int = 32) -> Group4Weight:
     code = torch.where(on & (code % 2 == 1) & (code < 7), code + 1, code).to(torch.uint8)
     code = (code | ((w < 0).to(torch.uint8) << 3)).reshape(N, K // 2, 2)
     return Group4Weight.from_codes(code[..., 0] | (code[..., 1] << 4), scales)
+
+
+class Packed:
+    """What a linear's weight was packed into, as long as it holds: ``holds(lin)``
+    tells whether ``lin.weight`` is still the parameter, in the memory and at the
+    version, that was packed (a change through ``.data`` in place goes unseen).
+    Keeps the packed memory alive, so that nothing else can come to lie there."""
+    __slots__ = ("rows", "source", "version")
+
+    def __init__(self, lin: torch.nn.Linear, rows):
+        self.rows = rows
+        self.source = lin.weight.detach()
+        self.version = lin.weight._version
+
+    def holds(self, lin: torch.nn.Linear) -> bool:
+        w = lin._parameters.get("weight")
+        return (w is not None and w._version == self.version and w.data_ptr() == self.source.data_ptr()
+                and w.shape == self.source.shape and w.dtype == self.source.dtype and w.device == self.source.device)

@@ -287,3 +287,146 @@ def test_refusals(dev):
         kernels.adaln_mx(x, x_out=x)
     with pytest.raises(N.NativeCallError, match="8192"):
         kernels.adaln_mx(torch.zeros(1, 1, 8224, dtype=BF, device=dev))
+
+
+# ------------------------------------------------------------ every tile, larger
+def _on_gpu(dev, M, K, N, seed, gelu, bias=True):
+    """A case of any size with its float64 result and the error bound, on the GPU."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    a = quant.quantize_mx(rand(M, K) * torch.exp(rand(K)))
+    w = quant.quantize_mx(rand(N, K) / K ** 0.5)
+    b = (0.1 * rand(N)).to(BF) if bias else None
+    ad, wd = a.dequantize().double(), w.dequantize().double()
+    y = ad @ wd.t()
+    err = MFMA * (ad.abs() @ wd.abs().t())
+    if bias:
+        y = y + b.double()
+    err = 1.01 * (err + 2.0 ** -23 * y.abs())
+    if gelu:
+        err = 1.13 * err + 2.0 ** -20 * y.abs()
+        y = torch.nn.functional.gelu(y, approximate="tanh")
+    return a, w, b, y, err
+
+
+def _check_bf16(y, ref, err):
+    d = (y.double() - ref).abs()
+    assert y.dtype == BF and (d <= 2.0 ** -8 * ref.abs() + err).all()
+    assert d.norm() <= 2.0 ** -8 * ref.norm()
+
+
+# sizes at which every tile and K split of the kernels is the one that runs (for the
+# large tiles also with more steps than buffers), none of them a multiple of it
+TILES = [(6, 576, 633), (1, 32, 40), (3, 8256, 197), (19, 512, 5707), (17, 64, 8300), (29, 1120, 8001), (387, 544, 1177),
+         (300, 1952, 1180), (2111, 192, 226), (17, 64, 8290), (120, 288, 5003), (822, 864, 1367), (65, 288, 8248),
+         (150, 2080, 8190), (285, 640, 8646), (179, 160, 8245), (900, 1504, 2050), (801, 160, 8954), (162, 64, 8328),
+         (390, 4128, 16300), (545, 320, 2505), (69, 64, 8299), (331, 1056, 4099), (2211, 384, 4110), (1045, 64, 7289),
+         (2290, 4192, 16390), (1556, 384, 7823), (1348, 64, 8311), (2301, 2336, 12290)]
+
+
+@pytest.mark.parametrize("M,K,N", TILES)
+def test_every_tile(dev, M, K, N):
+    gelu = (M + N) % 2 == 0
+    a, w, b, ref, err = _on_gpu(dev, M, K, N, M + K + N, gelu, bias=M % 3 != 0)
+    _check_bf16(kernels.mx_linear(a, w, b, gelu=gelu), ref, err)
+
+
+@pytest.mark.parametrize("M,K,N", TILES)
+def test_every_tile_8bit_result(dev, M, K, N):
+    N = N // 32 * 32
+    gelu = (M + N // 32) % 2 == 0
+    a, w, b, ref, err = _on_gpu(dev, M, K, N, M + K + N, gelu, bias=M % 3 != 0)
+    y = kernels.mx_linear(a, w, b, gelu=gelu, quantize=True)
+    rows = torch.arange(M) if M * N < 1 << 20 else torch.randint(0, M, (64,), generator=gen(1)).unique()
+    part = quant.MXRows(y.codes[rows.to(dev)], y.scales[:, rows.to(dev)].contiguous())
+    check_mx(part, ref[rows.to(dev)].cpu(), err[rows.to(dev)].cpu(), f"{M}x{K}x{N}")
+    # every value of the result, against the bf16 one of the same call
+    plain = kernels.mx_linear(a, w, b, gelu=gelu).float()
+    S = torch.exp2(y.scales.view(torch.uint8).transpose(0, 1).flatten(1)[:, :N // 32].float() - 127.0)
+    half = torch.maximum(2.0 ** -4 * 1.01 * plain.abs(), (2.0 ** -10 * S).repeat_interleave(32, 1))
+    # both round the same float32 value, half a step each
+    assert ((y.dequantize() - plain).abs() <= half + 2.0 ** -8 * plain.abs()).all()
+
+
+def test_rows_of_a_wider_result(dev):
+    """Rows of y further apart than N (aligned and not): the rest stays as it was."""
+    from taomate_amd import _native
+    a, w, b, ref, err = _on_gpu(dev, 70, 160, 200, 9, False)
+    for ls, at in ((256, 8), (203, 1)):
+        big = torch.full((70, ls), 7.0, dtype=BF, device=dev)
+        y = big[:, at:] if at + 200 >= ls else big[:, at:at + 200]
+        _native.host().mx_linear(a.codes, a.scales, w.codes, w.scales, b, y[:, :200], None, False)
+        _check_bf16(y[:, :200], ref, err)
+        y[:, :200] = 7.0
+        assert (big == 7.0).all()
+
+
+def test_feed_forward_chain(dev):
+    """norm -> up + GELU in 8 bits -> down, as a block runs them, each step against
+    float64 from what it was given."""
+    g = gen(21)
+    B, L, C, inner = 2, 75, 256, 1024
+    x, y = randn((B, L, C), g, BF), randn((B, L, C), g, BF)
+    gate, sc, sh = (randn((B, 1, C), g, BF, 0.4) for _ in range(3))
+    w1 = _to(quant.quantize_mx(randn((inner, C), g) / 16), dev)
+    w2 = _to(quant.quantize_mx(randn((C, inner), g) / 32), dev)
+    b1, b2 = randn((inner,), g, BF, 0.1), randn((C,), g, BF, 0.1)
+    xo = torch.empty(B, L, C, dtype=BF, device=dev)
+    n = kernels.adaln_mx(x.to(dev), y.to(dev), gate.to(dev), xo, sc.to(dev), sh.to(dev), eps=EPS)
+    h = kernels.mx_linear(n, w1, b1.to(dev), gelu=True, quantize=True)
+    out = kernels.mx_linear(h, w2, b2.to(dev))
+    xd = x.double() + y.double() * gate.double()
+    nd = xd / torch.sqrt(xd.square().mean(-1, keepdim=True) + EPS)
+    mag = nd.abs() * (1 + sc.double()).abs() + sh.double().abs()
+    check_mx(n, nd * (1 + sc.double()) + sh.double(), 2.0 ** -17 * mag)   # x' may cancel up to a factor 4
+    ref, err = _exact_linear(n, w1, b1, True)
+    check_mx(h, ref, 1.01 * err)
+    ref, err = _exact_linear(h, w2, b2, False)
+    d = (out.double().cpu().view(-1, C) - ref).abs()
+    assert out.shape == (B, L, C) and (d <= 2.0 ** -8 * ref.abs() + 1.01 * err).all()
+
+
+def test_captured_calls_replay(dev):
+    """The chain and the 4-bit linear captured into one graph: every replay, between
+    eager work and on new inputs in the same buffers, equals the eager calls."""
+    g = gen(22)
+    x = randn((1, 40, 512), g, BF).to(dev)
+    w1 = _to(quant.quantize_mx(randn((2048, 512), g) / 22), dev)
+    w2 = _to(quant.quantize_mx(randn((512, 2048), g) / 45), dev)
+    w4 = quant.quantize_group4(randn((1024, 512), g) / 22, 64)
+    w4 = quant.Group4Weight(w4.codes.to(dev), w4.scales.to(dev), w4.rows, w4.columns)
+
+    def run():
+        n = kernels.adaln_mx(x)
+        out = kernels.mx_linear(kernels.mx_linear(n, w1, gelu=True, quantize=True), w2)
+        return out, kernels.group4_linear(x[0, :5], w4, silu=True)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        held = run()
+    for i in range(4):
+        x.copy_(randn((1, 40, 512), gen(30 + i), BF))
+        eager = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, eager):
+            assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    cases = [_on_gpu(dev, 200, 1056, 1000, s, True) for s in (1, 2)]
+    want = [kernels.mx_linear(a, w, b, gelu=True) for a, w, b, _, _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (st, (a, w, b, _, _)) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(st):
+                got[i].append(kernels.mx_linear(a, w, b, gelu=True))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(t, want[i]) for t in got[i])

@@ -1,0 +1,101 @@
+"""When a linear's packed weight holds, and what quantising a module leaves as it
+was, on the CPU."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+from taomate_amd import dit as D
+from taomate_amd import quant
+
+BF = torch.bfloat16
+CFG = D.AVConfig(num_layers=1, video_dim=128, audio_dim=64, video_heads=2, audio_heads=1, video_d_head=64,
+                 audio_d_head=64)
+
+
+def _lin():
+    return nn.Linear(64, 32, dtype=BF)
+
+
+def _replace(lin):
+    lin.weight = nn.Parameter(lin.weight.detach().clone())
+
+
+def _in_place(lin):
+    with torch.no_grad():
+        lin.weight.mul_(2)
+
+
+def _load(lin):
+    lin.load_state_dict({k: v.clone() for k, v in lin.state_dict().items()})
+
+
+def _assign(lin):
+    lin.load_state_dict({k: v.clone() for k, v in lin.state_dict().items()}, assign=True)
+
+
+def _data(lin):
+    lin.weight.data = lin.weight.data.clone()
+
+
+def _weight_norm(lin):
+    nn.utils.parametrizations.weight_norm(lin)
+
+
+def _dtype(lin):
+    lin.float()
+
+
+@pytest.mark.parametrize("change", [_replace, _in_place, _load, _assign, _data, _weight_norm, _dtype])
+def test_a_changed_weight_ends_the_packing(change):
+    lin = _lin()
+    packed = quant.Packed(lin, quant.quantize_mx(lin.weight))
+    assert packed.holds(lin)
+    change(lin)
+    assert not packed.holds(lin)
+
+
+def test_freed_memory_does_not_come_back_as_the_packed_weight():
+    """Weights replaced twice: the first one's memory is held, so no later weight lies there."""
+    lin = _lin()
+    packed = quant.Packed(lin, quant.quantize_mx(lin.weight))
+    at = lin.weight.data_ptr()
+    for _ in range(50):
+        lin.weight.data = torch.randn(32, 64).to(BF)
+        assert lin.weight.data_ptr() != at and not packed.holds(lin)
+
+
+def test_quantising_keeps_names_values_and_modules():
+    m = D.build_model(CFG, "cpu", seed=1)
+    before = {k: v.clone() for k, v in m.state_dict().items()}
+    assert m.quantize_linears_(group=64) is m
+    after = m.state_dict()
+    assert list(after) == list(before) and all(torch.equal(after[k], before[k]) for k in before)
+    ff = m.transformer_blocks[0].ff
+    assert ff._mx[0].rows.shape == (512, 128) and m.adaln_single.linear._group4.rows.group == 64
+    assert m.adaln_single.emb.timestep_embedder.linear_1._group4.rows.shape == (128, 256)
+    x = torch.randn(2, 3, 128).to(BF)
+    with torch.no_grad():
+        assert not ff.quantized() and torch.equal(ff(x), ff.net(x))   # no GPU here: the modules run
+    c = copy.deepcopy(m)
+    assert torch.equal(c.state_dict()["adaln_single.linear.weight"], before["adaln_single.linear.weight"])
+    m.quantize_linears_(feed_forward=False, timestep=False)
+    assert "_mx" not in ff.__dict__ and "_group4" not in m.adaln_single.linear.__dict__
+
+
+def test_what_cannot_be_quantised_is_refused():
+    with pytest.raises(ValueError, match="multiple of 32"):
+        D.FeedForward(48, 48).to(BF).quantize_()
+    with pytest.raises(TypeError, match="plain bf16"):
+        D.FeedForward(64, 64).quantize_()
+    ff = D.FeedForward(64, 64).to(BF)
+    ff.net[2].register_forward_hook(lambda *_: None)
+    with pytest.raises(TypeError, match="plain bf16"):
+        ff.quantize_()
+    with pytest.raises(ValueError, match="at most 8192"):
+        D.FeedForward(8224, 32, mult=0.0078125).to(BF).quantize_()
+    with pytest.raises(ValueError, match="at most 4096"):
+        D._pack_group4(nn.Linear(4224, 8, dtype=BF), 32)
+    with pytest.raises(ValueError, match="multiple of 128"):
+        D._pack_group4(nn.Linear(64, 8, dtype=BF), 128)
