@@ -27,6 +27,7 @@
 #include <mutex>
 #include <optional>
 #include <string>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -558,15 +559,29 @@ MxRows mx_rows(const char* what, const at::Tensor& codes, const at::Tensor& scal
   return {R, K};
 }
 
-// (x, y, gate, x_out, scale, shift, codes, scales, eps)
-void adaln_mx(PyObject* const* a) {
+// New 8-bit rows of `shape` beside `like`: (codes, scales).
+struct NewRows {
+  at::Tensor codes, scales;
+  NewRows(at::IntArrayRef shape, int64_t rows, int64_t cols, const at::Tensor& like)
+      : codes(at::empty(shape, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(like.device()))),
+        scales(at::empty({(cols + 127) / 128, rows, 4},
+                         at::TensorOptions().dtype(at::kFloat8_e8m0fnu).device(like.device()))) {}
+  PyObject* pair() const {
+    Ref c(THPVariable_Wrap(codes)), s(THPVariable_Wrap(scales));
+    return PyTuple_Pack(2, c.o, s.o);
+  }
+};
+
+// (x, y, gate, x_out, scale, shift, eps) -> (codes, scales)
+PyObject* adaln_mx(PyObject* const* a) {
   static const char* const names[6] = {"x", "y", "gate", "x_out", "scale", "shift"};
   Opt t[6] = {&tensor(a[0])};
   for (int i = 1; i < 6; ++i) t[i] = optional(a[i]);
-  const at::Tensor &x = *t[0], &codes = tensor(a[6]), &scales = tensor(a[7]);
-  same_device("adaln_mx", x, {t[1], t[2], t[3], t[4], t[5], &codes, &scales});
+  const at::Tensor& x = *t[0];
+  same_device("adaln_mx", x, {t[1], t[2], t[3], t[4], t[5]});
   if (x.dim() != 3 || x.scalar_type() != at::kBFloat16) value_error("adaln_mx: x must be bf16 [B, L, C]");
   const int64_t B = x.size(0), L = x.size(1), C = x.size(2);
+  if (C == 0 || C % LTX_MX_BLOCK != 0) value_error("adaln_mx: channels must be a multiple of 32, got " + std::to_string(C));
   struct {
     void* p;
     int64_t bs, ls;
@@ -582,66 +597,81 @@ void adaln_mx(PyObject* const* a) {
                   shape(o));
     r[i] = {o.data_ptr(), B > 1 ? o.stride(0) : 0, o.size(1) > 1 ? o.stride(1) : 0};
   }
-  const MxRows n = mx_rows("adaln_mx", codes, scales);
-  if (n.rows != B * L || n.cols != C) value_error("adaln_mx: codes " + shape(codes) + " for rows " + shape(x));
+  const float eps = a[6] == Py_None ? -1.0f : (float)real(a[6]);
+  if (a[6] != Py_None && !(eps >= 0.0f)) value_error("adaln_mx: eps must not be negative");
   const c10::DeviceGuard guard(x.device());
+  const NewRows n(x.sizes(), B * L, C, x);
   call("ltx_adaln_mx", api.adaln_mx, B, L, C, r[0].p, r[0].bs, r[0].ls, r[1].p, r[1].bs, r[1].ls, r[2].p, r[2].bs,
-       r[2].ls, r[3].p, r[3].bs, r[3].ls, r[4].p, r[4].bs, r[4].ls, r[5].p, r[5].bs, r[5].ls,
-       a[8] == Py_None ? -1.0f : (float)real(a[8]), codes.data_ptr(), scales.data_ptr(), stream_of(x));
+       r[2].ls, r[3].p, r[3].bs, r[3].ls, r[4].p, r[4].bs, r[4].ls, r[5].p, r[5].bs, r[5].ls, eps, n.codes.data_ptr(),
+       n.scales.data_ptr(), stream_of(x));
+  return n.pair();
 }
 
-// (a_codes, a_scales, w_codes, w_scales, bias, y, y_scales, gelu)
-void mx_linear(PyObject* const* a) {
-  const at::Tensor &ac = tensor(a[0]), &as = tensor(a[1]), &wc = tensor(a[2]), &ws = tensor(a[3]), &y = tensor(a[5]);
-  const Opt bias = optional(a[4]), ys = optional(a[6]);
-  same_device("mx_linear", ac, {&as, &wc, &ws, bias, &y, ys});
+// (a_codes, a_scales, w_codes, w_scales, bias, gelu, quantize, out) -> y or (codes, scales)
+PyObject* mx_linear(PyObject* const* a) {
+  const at::Tensor &ac = tensor(a[0]), &as = tensor(a[1]), &wc = tensor(a[2]), &ws = tensor(a[3]);
+  const Opt bias = optional(a[4]), out = optional(a[7]);
+  const bool quantize = truth(a[6]);
+  same_device("mx_linear", ac, {&as, &wc, &ws, bias, out});
   const MxRows x = mx_rows("mx_linear", ac, as), w = mx_rows("mx_linear", wc, ws);
   if (x.cols != w.cols || wc.dim() != 2)
     value_error("mx_linear: rows " + shape(ac) + " and weight " + shape(wc) + " do not match");
   if (bias != nullptr && (bias->scalar_type() != at::kBFloat16 || bias->dim() != 1 || bias->size(0) != w.rows ||
                           (w.rows > 1 && bias->stride(0) != 1)))
     value_error("mx_linear: bias must be a contiguous bf16 [" + std::to_string(w.rows) + "] vector");
-  int64_t y_ls = w.rows;
-  if (ys != nullptr) {
-    const MxRows o = mx_rows("mx_linear", y, *ys);
-    if (o.rows != x.rows || o.cols != w.rows)
-      value_error("mx_linear: result " + shape(y) + " for " + std::to_string(x.rows) + " rows of " +
-                  std::to_string(w.rows));
-  } else {
-    if (y.scalar_type() != at::kBFloat16) type_error("mx_linear: the result is bf16");
-    if (y.dim() != 2 || y.size(0) != x.rows || y.size(1) != w.rows || (w.rows > 1 && y.stride(1) != 1))
-      value_error("mx_linear: result " + shape(y) + " for " + std::to_string(x.rows) + " rows of " +
-                  std::to_string(w.rows));
-    if (x.rows > 1) y_ls = y.stride(0);
-  }
+  c10::SmallVector<int64_t, 8> sizes(ac.sizes().begin(), ac.sizes().end());
+  sizes.back() = w.rows;
   const c10::DeviceGuard guard(ac.device());
-  call("ltx_mx_linear", api.mx_linear, x.rows, w.rows, x.cols, ac.data_ptr(), as.data_ptr(), wc.data_ptr(),
-       ws.data_ptr(), ptr(bias), (int)truth(a[7]), y.data_ptr(), y_ls, ptr(ys), stream_of(ac));
+  const auto run = [&](void* y, int64_t y_ls, void* ys) {
+    call("ltx_mx_linear", api.mx_linear, x.rows, w.rows, x.cols, ac.data_ptr(), as.data_ptr(), wc.data_ptr(),
+         ws.data_ptr(), ptr(bias), (int)truth(a[5]), y, y_ls, ys, stream_of(ac));
+  };
+  if (quantize) {
+    if (out != nullptr) value_error("mx_linear: out takes bf16 results");
+    if (w.rows % LTX_MX_BLOCK != 0)
+      value_error("mx_linear: an 8-bit result needs a multiple of 32 channels, got " + std::to_string(w.rows));
+    const NewRows y(sizes, x.rows, w.rows, ac);
+    run(y.codes.data_ptr(), w.rows, y.scales.data_ptr());
+    return y.pair();
+  }
+  if (out != nullptr) {
+    if (out->scalar_type() != at::kBFloat16) type_error("mx_linear: out must be bf16");
+    if (out->dim() != 2 || out->size(0) != x.rows || out->size(1) != w.rows || (w.rows > 1 && out->stride(1) != 1))
+      value_error("mx_linear: out " + shape(*out) + " for " + std::to_string(x.rows) + " rows of " +
+                  std::to_string(w.rows));
+    run(out->data_ptr(), x.rows > 1 ? out->stride(0) : w.rows, nullptr);
+    Py_INCREF(a[7]);
+    return a[7];
+  }
+  const at::Tensor y = at::empty(sizes, at::TensorOptions().dtype(at::kBFloat16).device(ac.device()));
+  run(y.data_ptr(), w.rows, nullptr);
+  return THPVariable_Wrap(y);
 }
 
-// (x, codes, scales, bias, y, silu, columns)
-void group4_linear(PyObject* const* a) {
-  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &s = tensor(a[2]), &y = tensor(a[4]);
+// (x, codes, scales, bias, silu, rows, columns) -> y
+PyObject* group4_linear(PyObject* const* a) {
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &s = tensor(a[2]);
   const Opt bias = optional(a[3]);
-  const int64_t K = integer(a[6]);
-  same_device("group4_linear", x, {&w, &s, bias, &y});
-  for (Opt t : {&x, &s, bias, &y})
-    if (t != nullptr && t->scalar_type() != at::kBFloat16) type_error("group4_linear: x, scales, bias and y must be bf16");
+  const int64_t N = integer(a[5]), K = integer(a[6]);
+  same_device("group4_linear", x, {&w, &s, bias});
+  for (Opt t : {&x, &s, bias})
+    if (t != nullptr && t->scalar_type() != at::kBFloat16) type_error("group4_linear: x, scales and bias must be bf16");
   if (w.scalar_type() != at::kByte) type_error("group4_linear: codes must be uint8");
-  const int64_t N = y.dim() == 2 ? y.size(1) : -1, tiles = (N + 15) / 16, chunks = (K + 127) / 128;
-  const int64_t per = s.dim() == 4 ? s.size(3) : 0;
-  if (N < 0 || K < 1 || x.dim() != 2 || x.size(1) != K || (K > 1 && x.stride(1) != 1) || y.size(0) != x.size(0) ||
-      (N > 1 && y.stride(1) != 1) || !w.is_contiguous() || w.dim() != 5 || w.size(0) != tiles || w.size(1) != chunks ||
-      w.size(2) != 4 || w.size(3) != 16 || w.size(4) != 16 || !s.is_contiguous() || s.dim() != 4 ||
-      s.size(0) != tiles || s.size(1) != chunks || s.size(2) != 16 || (per != 1 && per != 2 && per != 4))
-    value_error("group4_linear: x " + shape(x) + ", codes " + shape(w) + ", scales " + shape(s) + ", y " + shape(y) +
-                " for " + std::to_string(K) + " columns");
+  const int64_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, per = s.dim() == 4 ? s.size(3) : 0;
+  if (N < 0 || K < 1 || x.dim() != 2 || x.size(1) != K || (K > 1 && x.stride(1) != 1) || !w.is_contiguous() ||
+      w.dim() != 5 || w.size(0) != tiles || w.size(1) != chunks || w.size(2) != 4 || w.size(3) != 16 ||
+      w.size(4) != 16 || !s.is_contiguous() || s.dim() != 4 || s.size(0) != tiles || s.size(1) != chunks ||
+      s.size(2) != 16 || (per != 1 && per != 2 && per != 4))
+    value_error("group4_linear: x " + shape(x) + ", codes " + shape(w) + ", scales " + shape(s) + " for a weight [" +
+                std::to_string(N) + ", " + std::to_string(K) + "]");
   if (bias != nullptr && (bias->dim() != 1 || bias->size(0) != N || (N > 1 && bias->stride(0) != 1)))
     value_error("group4_linear: bias must be a contiguous [N] vector");
   const c10::DeviceGuard guard(x.device());
+  const at::Tensor y = at::empty({x.size(0), N}, x.options());
   call("ltx_group4_linear", api.group4_linear, x.size(0), N, K, 128 / per, x.data_ptr(),
-       x.size(0) > 1 ? x.stride(0) : 0, (int)truth(a[5]), w.data_ptr(), s.data_ptr(), ptr(bias), y.data_ptr(),
-       y.size(0) > 1 ? y.stride(0) : 0, stream_of(x));
+       x.size(0) > 1 ? x.stride(0) : 0, (int)truth(a[4]), w.data_ptr(), s.data_ptr(), ptr(bias), y.data_ptr(), N,
+       stream_of(x));
+  return THPVariable_Wrap(y);
 }
 
 // is_eager(): whether an op on plain tensors would run as it is written, as far
@@ -689,15 +719,19 @@ PyObject* row_operands(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ------------------------------------------------------------------- bindings
-template <void (*Fn)(PyObject* const*), Py_ssize_t N>
+template <auto Fn, Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != N) {
     PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", N, nargs);
     return nullptr;
   }
   try {
-    Fn(args);
-    Py_RETURN_NONE;
+    if constexpr (std::is_void_v<decltype(Fn(args))>) {
+      Fn(args);
+      Py_RETURN_NONE;
+    } else {
+      return Fn(args);
+    }
   } catch (const Refused& r) {
     if (r.type != nullptr) PyErr_SetString(r.type, r.msg.c_str());
   } catch (const c10::IndexError& e) {
@@ -752,7 +786,7 @@ PyMethodDef methods[] = {
     {"flash_attn", (PyCFunction)(void*)&entry<flash_attn, 10>, METH_FASTCALL, nullptr},
     {"skinny_linear", (PyCFunction)(void*)&entry<skinny_linear, 5>, METH_FASTCALL, nullptr},
     {"adaln", (PyCFunction)(void*)&entry<adaln, 8>, METH_FASTCALL, nullptr},
-    {"adaln_mx", (PyCFunction)(void*)&entry<adaln_mx, 9>, METH_FASTCALL, nullptr},
+    {"adaln_mx", (PyCFunction)(void*)&entry<adaln_mx, 7>, METH_FASTCALL, nullptr},
     {"mx_linear", (PyCFunction)(void*)&entry<mx_linear, 8>, METH_FASTCALL, nullptr},
     {"group4_linear", (PyCFunction)(void*)&entry<group4_linear, 7>, METH_FASTCALL, nullptr},
     {"is_eager", is_eager, METH_NOARGS, nullptr},

@@ -183,36 +183,21 @@ def adaln_mx(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[t
     ``mx_linear``; x_out = x + y * gate in bf16.  float32 between its inputs and
     outputs (``adaln`` rounds to bf16 where the reference's ops do).  eps None
     skips the norm: the rows themselves.  C a multiple of 32, at most 8192."""
-    C = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((C + 127) // 128, x.numel() // C if C else 0, 4, dtype=torch.float8_e8m0fnu, device=x.device)
-    (N._host or N.host()).adaln_mx(x, y, gate, x_out, scale, shift, codes, scales, eps)
-    return MXRows(codes, scales)
+    return MXRows(*(N._host or N.host()).adaln_mx(x, y, gate, x_out, scale, shift, eps))
 
 
 def mx_linear(a: MXRows, weight: MXRows, bias: Optional[torch.Tensor] = None, gelu: bool = False,
-              quantize: bool = False):
+              quantize: bool = False, out: Optional[torch.Tensor] = None):
     """ltx_mx_linear: act(a @ weight.T + bias) for 8-bit rows ``a`` [..., K]
     and an 8-bit ``weight`` [N, K]; bias bf16 [N]; tanh-GELU with ``gelu``.
-    Returns bf16 [..., N], or 8-bit rows with ``quantize`` (N a multiple of 32)."""
-    codes, w = a.codes, weight.codes
-    shape = codes.shape[:-1]
-    n, rows = w.shape[0], a.scales.shape[1]
-    host = N._host or N.host()
-    if quantize:
-        y = torch.empty(*shape, n, dtype=torch.float8_e4m3fn, device=codes.device)
-        ys = torch.empty((n + 127) // 128, rows, 4, dtype=torch.float8_e8m0fnu, device=codes.device)
-        host.mx_linear(codes, a.scales, w, weight.scales, bias, y, ys, gelu)
-        return MXRows(y, ys)
-    y = torch.empty(rows, n, dtype=torch.bfloat16, device=codes.device)
-    host.mx_linear(codes, a.scales, w, weight.scales, bias, y, None, gelu)
-    return y.view(*shape, n)
+    Returns bf16 [..., N], or 8-bit rows with ``quantize`` (N a multiple of 32).
+    ``out``: bf16 [rows, N] with contiguous channels to write instead of a new tensor."""
+    y = (N._host or N.host()).mx_linear(a.codes, a.scales, weight.codes, weight.scales, bias, gelu, quantize, out)
+    return MXRows(*y) if quantize else y
 
 
 def group4_linear(x: torch.Tensor, weight: Group4Weight, bias: Optional[torch.Tensor] = None,
                   silu: bool = False) -> torch.Tensor:
     """ltx_group4_linear: act(x) @ W.T + bias for x [M <= 16, K <= 4096] bf16
     (SiLU of x first with ``silu``) and a 4-bit weight."""
-    y = torch.empty(x.shape[0], weight.rows, dtype=x.dtype, device=x.device)
-    (N._host or N.host()).group4_linear(x, weight.codes, weight.scales, bias, y, silu, weight.columns)
-    return y
+    return (N._host or N.host()).group4_linear(x, weight.codes, weight.scales, bias, silu, weight.rows, weight.columns)

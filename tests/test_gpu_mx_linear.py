@@ -274,7 +274,17 @@ def test_refusals(dev):
         kernels.adaln_mx(x, y=x[:, :2])
     with pytest.raises(ValueError, match="multiple of 32"):
         kernels.adaln_mx(x[..., :40].contiguous())
+    with pytest.raises(ValueError, match="out takes bf16"):
+        kernels.mx_linear(a, _to(quant.quantize_mx(torch.zeros(32, 64)), dev), quantize=True, out=x[0])
+    with pytest.raises(ValueError, match="out"):
+        kernels.mx_linear(a, w, b, out=torch.empty(4, 47, dtype=BF, device=dev))
+    with pytest.raises(TypeError, match="out must be"):
+        kernels.mx_linear(a, w, b, out=torch.empty(4, 48, device=dev))
+    with pytest.raises(ValueError, match="negative"):
+        kernels.adaln_mx(x, eps=-1.0)
     from taomate_amd import _native as N
+    with pytest.raises(N.NativeCallError, match="overlap"):
+        kernels.mx_linear(a, w, b, out=torch.empty(1, 48, dtype=BF, device=dev).expand(4, 48))
     with pytest.raises(N.NativeCallError, match="aligned"):
         kernels.adaln_mx(torch.zeros(1, 2, 104, dtype=BF, device=dev)[..., 4:100])
     with pytest.raises(N.NativeCallError, match="a gate needs"):
@@ -350,12 +360,12 @@ def test_every_tile_8bit_result(dev, M, K, N):
 
 def test_rows_of_a_wider_result(dev):
     """Rows of y further apart than N (aligned and not): the rest stays as it was."""
-    from taomate_amd import _native
     a, w, b, ref, err = _on_gpu(dev, 70, 160, 200, 9, False)
     for ls, at in ((256, 8), (203, 1)):
         big = torch.full((70, ls), 7.0, dtype=BF, device=dev)
         y = big[:, at:] if at + 200 >= ls else big[:, at:at + 200]
-        _native.host().mx_linear(a.codes, a.scales, w.codes, w.scales, b, y[:, :200], None, False)
+        out = y[:, :200]
+        assert kernels.mx_linear(a, w, b, out=out) is out
         _check_bf16(y[:, :200], ref, err)
         y[:, :200] = 7.0
         assert (big == 7.0).all()
