@@ -16,10 +16,19 @@ namespace ltx {
 
 constexpr int kMxBlock = LTX_MX_BLOCK;
 
-// |v| as it counts in a block's maximum.
-__device__ __forceinline__ float mx_magnitude(float v) {
-  const float a = fabsf(v);
-  return a < __builtin_inff() ? a : 0.0f;
+// The largest finite magnitude of N values.  A maximum passes over NaN by itself;
+// only one that is infinite is taken again without the infinities.
+template <int N>
+__device__ __forceinline__ float mx_top(const float (&v)[N]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) top = fmaxf(top, fmaxf(fabsf(v[i]), fabsf(v[i + 1])));
+  if (top == __builtin_inff()) {
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(v[i]) < __builtin_inff() ? fabsf(v[i]) : 0.0f);
+  }
+  return top;
 }
 
 // The E8M0 code of a block with maximum `top` (finite, >= 0): the exponent of

@@ -64,13 +64,14 @@ struct MxLinearArgs {
   int64_t y_ls;
   int M, N, K;
   int vec;               // bf16 rows of y take 16-byte stores
+  int bias_vec;          // bias takes 16-byte loads: 16-byte aligned, N a multiple of 8
 };
 
 // tanh-GELU: y sigmoid(2 u), u = sqrt(2 / pi) (y + 0.044715 y^3).  The sigmoid
 // through one exp2 and one reciprocal (1 ulp each).
 __device__ __forceinline__ float mx_gelu(float y) {
   const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
-  const float u = c * (y + 0.044715f * y * y * y);
+  const float u = y * fmaf(y * y, 0.044715f * c, c);
   return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u));
 }
 
@@ -300,6 +301,20 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx_linear_kernel(const M
     __builtin_amdgcn_s_setprio(0);
     at = next_at;
   }
+  // the bias travels during the last step, as pairs of bf16
+  const int n = n0 + wn * 16 * NT + g * 4 * NT;
+  uint32_t bias[2 * NT] = {};
+  if (p.bias != nullptr) {
+    if (p.bias_vec) {
+#pragma unroll
+      for (int i = 0; i < 2 * NT; i += 4)
+        if (n + 2 * i < p.N) __builtin_memcpy(bias + i, __builtin_assume_aligned(p.bias + n + 2 * i, 16), 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i)
+        if (n + i < p.N) bias[i / 2] |= (uint32_t)p.bias[n + i] << (16 * (i % 2));
+    }
+  }
   const int live = (first + steps - 1) * 128 + g * 32 < p.K ? 0xFF : 0;
 #pragma unroll
   for (int u = 0; u < NT; ++u) sw[u] &= live;
@@ -333,40 +348,34 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx_linear_kernel(const M
   }
 
   // Epilogue: lane group g holds channels n .. n + 4 NT - 1 of row m for every tile row.
-  const int n = n0 + wn * 16 * NT + g * 4 * NT;
-  float bias[4 * NT];
-#pragma unroll
-  for (int i = 0; i < 4 * NT; ++i)
-    bias[i] = p.bias != nullptr && n + i < p.N ? bf16_bits_to_f32(p.bias[n + i]) : 0.0f;
+  // Channels past N are zeros (NaN beside one in a): they count in no block's maximum.
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int m = m0 + (wm * MT + t) * 16 + r16;
     float v[4 * NT];
 #pragma unroll
     for (int i = 0; i < 4 * NT; ++i) {
-      v[i] = acc[t][i / 4][i % 4] + bias[i];
+      const uint32_t b = bias[i / 2];
+      v[i] = acc[t][i / 4][i % 4] + __uint_as_float(i % 2 ? b & 0xFFFF0000u : b << 16);
       if (GELU) v[i] = mx_gelu(v[i]);
     }
     if (p.ys != nullptr) {
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) {
-        if (n + i >= p.N) v[i] = 0.0f;
-        top = fmaxf(top, mx_magnitude(v[i]));
-      }
       static_assert(NT == 2 || NT == 4 || NT == 8, "a block of 32 lies in one, two or four lanes");
+      float top = mx_top(v);
       if (NT < 8) top = fmaxf(top, __shfl_xor(top, 16, 64));
       if (NT < 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
       const uint32_t code = mx_scale_code(top);
       const float inv = mx_inverse(code);
       if (m < p.M) {
         uint8_t* yp = (uint8_t*)p.y + (int64_t)m * p.N + n;
+        constexpr int kStore = NT == 2 ? 8 : 16;  // N is a multiple of 32, n one of 4 NT: whole stores
+        uint32_t c[NT];
 #pragma unroll
-        for (int i = 0; i < 4 * NT; i += 8) {
-          const uint2 c = make_uint2(mx_pack4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv),
-                                     mx_pack4(v[i + 4] * inv, v[i + 5] * inv, v[i + 6] * inv, v[i + 7] * inv));
-          if (n + i < p.N) *reinterpret_cast<uint2*>(yp + i) = c;
-        }
+        for (int i = 0; i < NT; ++i)
+          c[i] = mx_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+#pragma unroll
+        for (int i = 0; i < 4 * NT; i += kStore)
+          if (n + i < p.N) __builtin_memcpy(__builtin_assume_aligned(yp + i, kStore), c + i / 4, kStore);
         // blocks past N up to the next 128 columns are written as 0
         if (n / 128 < (p.N + 127) / 128 && n % 32 == 0)
           p.ys[((int64_t)(n / 128) * p.M + m) * 4 + n / 32 % 4] = (uint8_t)code;
@@ -498,16 +507,14 @@ __global__ void __launch_bounds__(64 * kRowWaves, 2) mx_linear_rows_kernel(const
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[e + k] = (x[k] + y[k]) + (z[k] + w[k]);
     }
-    float top = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[e] += p.bias != nullptr && n + e < p.N ? bf16_bits_to_f32(p.bias[n + e]) : 0.0f;
       if (GELU) v[e] = mx_gelu(v[e]);
-      if (n + e >= p.N) v[e] = 0.0f;
-      top = fmaxf(top, mx_magnitude(v[e]));
     }
     if (p.ys != nullptr) {
       if constexpr (NT % 2 == 0) {
+        float top = mx_top(v);
         top = fmaxf(top, __shfl_xor(top, 1, 64));
         top = fmaxf(top, __shfl_xor(top, 2, 64));
         const uint32_t code = mx_scale_code(top);
@@ -611,7 +618,7 @@ extern "C" int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_code
   LTX_REQUIRE(y_scales != nullptr || M == 1 || y_ls >= N, "ltx_mx_linear: rows of y overlap");
   MxLinearArgs p{(const uint8_t*)a_codes, (const uint8_t*)a_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales,
                  (const uint16_t*)bias, y, (uint8_t*)y_scales, y_ls, (int)M, (int)N, (int)K,
-                 (uintptr_t)y % 16 == 0 && y_ls % 8 == 0};
+                 (uintptr_t)y % 16 == 0 && y_ls % 8 == 0, (uintptr_t)bias % 16 == 0 && N % 8 == 0};
   LTX_REQUIRE(ceil_div(M, 128) <= 65535, "ltx_mx_linear: too many rows");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (act)

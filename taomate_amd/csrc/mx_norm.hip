@@ -116,9 +116,7 @@ __global__ void __launch_bounds__(1024 / NV) adaln_mx_kernel(const MxNormArgs a)
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float top = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, mx_magnitude(x[i][e]));
+    float top = mx_top(x[i]);
     top = fmaxf(top, __shfl_xor(top, 1, 64));
     top = fmaxf(top, __shfl_xor(top, 2, 64));
     const uint32_t code = mx_scale_code(top);
