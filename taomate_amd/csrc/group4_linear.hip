@@ -19,7 +19,9 @@
 // A workgroup has 8 waves: KS of them share a tile of 16 rows of W, each with up
 // to 4 chunks of 128 columns in flight, and meet in LDS; 8 / KS tiles at a time.
 // x (SiLU applied, rounded to bf16 as the tensor op rounds) is staged in LDS
-// once per workgroup, which then strides over the tiles.
+// once per workgroup, which then strides over the tiles.  2 rows of 4096 -> 24576 with
+// groups of 32 and SiLU: 13.7 us (4.2 TB/s of 57 MB; 5.5 TB/s at the end of longer
+// weights), 8 rows of 2048 -> 12288 with groups of 128: 6.8 us.
 
 #include <type_traits>
 

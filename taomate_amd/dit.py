@@ -648,14 +648,21 @@ class AVModel(nn.Module):
                 m.fuse_qkv_()
         return self
 
-    def quantize_linears_(self, feed_forward: bool = True, timestep: bool = True, group: int = 32) -> "AVModel":
+    def quantize_linears_(self, feed_forward: bool = True, timestep: bool = False, group: int = 32) -> "AVModel":
         """Hold weights in fewer bits beside the bf16 parameters, whose names and
         values stay: every block's video and audio feed-forward in 8 bits
-        (``FeedForward.quantize_``), and the linears of the timestep embeddings
-        and modulations in 4 bits with a bf16 scale for every ``group`` columns,
-        for calls of up to 16 rows (one per sample or frame; more rows run in
-        bf16).  False ends either.  Load the weights before; a weight that is
-        changed or replaced afterwards runs in bf16 again until the next call."""
+        (``FeedForward.quantize_``), and with ``timestep`` the linears of the
+        timestep embeddings and modulations in 4 bits with a bf16 scale for every
+        ``group`` columns, for calls of up to 16 rows (one per sample or frame;
+        more rows run in bf16).  False ends either.  Load the weights before; a
+        weight that is changed or replaced afterwards runs in bf16 again until
+        the next call.
+
+        Measured on random weights at the 512x768 chunk, 48 blocks: the feed-forwards
+        take a step from 79.7 to 70.7 ms, its outputs to a cosine of 0.995 with
+        the bf16 step's.  The 4-bit modulations reach every block's norms: cosine
+        0.96, for 0.1 ms of the 79 (half of the timestep linears' time, a
+        quarter of the bytes they read)."""
         for m in self.modules():
             if isinstance(m, FeedForward):
                 m.quantize_(feed_forward)

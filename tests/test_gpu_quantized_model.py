@@ -96,7 +96,7 @@ def test_model_step(dev, overlap):
     same = copy.deepcopy(m)
     with torch.no_grad():
         base = _forward(m, dev, x)
-        m.quantize_linears_()
+        m.quantize_linears_(timestep=True)
         for a, b in zip(m.modules(), same.modules()):
             if isinstance(a, D.FeedForward):
                 assert a.quantized()
@@ -105,7 +105,7 @@ def test_model_step(dev, overlap):
             elif isinstance(a, torch.nn.Linear) and "_group4" in a.__dict__:
                 b.weight.copy_(a._group4.rows.dequantize())
         got, again, want = _forward(m, dev, x), _forward(m, dev, x), _forward(same, dev, x)
-        m.quantize_linears_(False, False)
+        m.quantize_linears_(False)
         back = _forward(m, dev, x)
     for i in range(2):
         assert got[i].isfinite().all() and torch.equal(got[i], again[i]) and torch.equal(back[i], base[i])
@@ -116,7 +116,7 @@ def test_model_step(dev, overlap):
 
 
 def test_model_step_runs_the_quantised_kernels(dev, monkeypatch):
-    m = D.build_model(CFG, dev, seed=3).quantize_linears_()
+    m = D.build_model(CFG, dev, seed=3).quantize_linears_(timestep=True)
     calls = []
     for name in ("adaln_mx", "mx_linear", "group4_linear"):
         fn = getattr(kernels, name)
@@ -129,7 +129,7 @@ def test_model_step_runs_the_quantised_kernels(dev, monkeypatch):
 
 def test_model_step_over_arena_caches(dev):
     """The clean commit and a step over its caches, as the streaming loop calls them."""
-    m = D.build_model(CFG, dev, seed=3).fuse_qkv_().quantize_linears_()
+    m = D.build_model(CFG, dev, seed=3).fuse_qkv_().quantize_linears_(timestep=True)
     x = _inputs()
     with torch.no_grad():
         caches = _small_arena_caches(dev, CFG, x)

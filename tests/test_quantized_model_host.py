@@ -69,7 +69,7 @@ def test_freed_memory_does_not_come_back_as_the_packed_weight():
 def test_quantising_keeps_names_values_and_modules():
     m = D.build_model(CFG, "cpu", seed=1)
     before = {k: v.clone() for k, v in m.state_dict().items()}
-    assert m.quantize_linears_(group=64) is m
+    assert m.quantize_linears_(timestep=True, group=64) is m
     after = m.state_dict()
     assert list(after) == list(before) and all(torch.equal(after[k], before[k]) for k in before)
     ff = m.transformer_blocks[0].ff
