@@ -156,15 +156,28 @@ class Packed:
     """What a linear's weight was packed into, as long as it holds: ``holds(lin)``
     tells whether ``lin.weight`` is still the parameter, in the memory and at the
     version, that was packed (a change through ``.data`` in place goes unseen).
-    Keeps the packed memory alive, so that nothing else can come to lie there."""
-    __slots__ = ("rows", "source", "version")
+    Keeps the packed memory alive, so that nothing else can come to lie there.
+    A deep copy or pickle carries no rows and never holds: versions count anew there."""
+    __slots__ = ("rows", "weight", "source", "version")
 
     def __init__(self, lin: torch.nn.Linear, rows):
+        if lin.weight.is_inference():
+            raise ValueError("a weight made in inference mode does not tell when it is changed: it cannot be packed")
         self.rows = rows
+        self.weight = lin.weight
         self.source = lin.weight.detach()
         self.version = lin.weight._version
 
+    @classmethod
+    def _lapsed(cls) -> "Packed":
+        p = cls.__new__(cls)
+        p.rows = p.weight = p.source = p.version = None
+        return p
+
+    def __reduce__(self):
+        return Packed._lapsed, ()
+
     def holds(self, lin: torch.nn.Linear) -> bool:
         w = lin._parameters.get("weight")
-        return (w is not None and w._version == self.version and w.data_ptr() == self.source.data_ptr()
+        return (w is not None and w is self.weight and w.data_ptr() == self.source.data_ptr() and w._version == self.version
                 and w.shape == self.source.shape and w.dtype == self.source.dtype and w.device == self.source.device)

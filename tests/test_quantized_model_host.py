@@ -1,6 +1,7 @@
 """When a linear's packed weight holds, and what quantising a module leaves as it
 was, on the CPU."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -64,6 +65,49 @@ def test_freed_memory_does_not_come_back_as_the_packed_weight():
     for _ in range(50):
         lin.weight.data = torch.randn(32, 64).to(BF)
         assert lin.weight.data_ptr() != at and not packed.holds(lin)
+
+
+def test_a_new_parameter_over_the_same_memory_ends_the_packing():
+    lin = _lin()
+    packed = quant.Packed(lin, quant.quantize_mx(lin.weight))
+    old = lin.weight._version
+    lin.weight = nn.Parameter(lin.weight.data)
+    for _ in range(old + 2):
+        assert not packed.holds(lin)
+        with torch.no_grad():
+            lin.weight.mul_(2)
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda m: pickle.loads(pickle.dumps(m))], ids=["deepcopy", "pickle"])
+def test_a_copy_is_not_packed(how):
+    """A copy's version count begins anew: changed up to the packed version it must not hold."""
+    ff = D.FeedForward(64, 64).to(BF)
+    lin = ff.net[2]
+    with torch.no_grad():
+        lin.weight.mul_(2)
+    ff.quantize_()
+    two = how(ff)
+    assert ff._mx[1].holds(lin)
+    for _ in range(lin.weight._version + 2):
+        assert not any(p.holds(m) for p, m in zip(two._mx, (two.net[0].proj, two.net[2])))
+        with torch.no_grad():
+            two.net[0].proj.weight.mul_(2)
+            two.net[2].weight.mul_(2)
+    with torch.no_grad():
+        assert not two.quantized() and two.quantize_() is two
+
+
+def test_inference_mode_weights():
+    with torch.inference_mode():
+        made = _lin()
+    with pytest.raises(ValueError, match="inference mode"):
+        quant.Packed(made, quant.quantize_mx(made.weight))
+    lin = _lin()
+    packed = quant.Packed(lin, quant.quantize_mx(lin.weight))
+    with torch.inference_mode():
+        assert packed.holds(lin)
+    lin.weight = made.weight
+    assert not packed.holds(lin)
 
 
 def test_quantising_keeps_names_values_and_modules():
