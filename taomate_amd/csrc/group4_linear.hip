@@ -238,6 +238,7 @@ extern "C" int ltx_group4_linear(int64_t M, int64_t N, int64_t K, int64_t group,
               "ltx_group4_linear: null pointer");
   LTX_REQUIRE((uintptr_t)x % 16 == 0 && x_ls % 8 == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 8 == 0,
               "ltx_group4_linear: x rows and codes must be 16-byte aligned, scales 8-byte");
+  LTX_REQUIRE(M == 1 || y_ls >= N, "ltx_group4_linear: rows of y overlap");
   Group4Args a{(const uint16_t*)x, x_ls, (const uint8_t*)codes, (const uint16_t*)scales, (const uint16_t*)bias,
                (uint16_t*)y, y_ls, N, (int)M, (int)K, silu};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

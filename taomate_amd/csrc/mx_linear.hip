@@ -575,8 +575,9 @@ struct MxShape {
   void (*launch)(const MxLinearArgs&, hipStream_t);
 };
 
+// False if every tile makes more workgroups than a grid of 512 threads each may have (2^32 threads).
 template <bool GELU>
-void launch_mx(const MxLinearArgs& p, hipStream_t st) {
+bool launch_mx(const MxLinearArgs& p, hipStream_t st) {
   static const MxShape shapes[] = {
       {16, 16, 8, 3.22f, 0.0f, 0.36f, 0.77f, launch_mx_rows<1, 1, GELU>},  // bf16 results
       {16, 32, 8, 3.11f, 0.0f, 0.63f, 1.34f, launch_mx_rows<1, 2, GELU>},  // 8-bit ones: whole blocks
@@ -591,18 +592,22 @@ void launch_mx(const MxLinearArgs& p, hipStream_t st) {
       {256, 256, 1, 0.0f, 8.21f, 1.09f, 0.0f, launch_mx_linear<8, 4, 2, 4, 2, 1, GELU>},
   };
   const float bytes = ((float)p.M + p.N) * p.K * 1.03f + 2.0f * p.M * p.N, floor = 2.5f + bytes / 5.3e6f;
+  const int64_t cols = p.ys != nullptr ? ceil_div(p.N, 128) * 128 : p.N;
   const MxShape* best = nullptr;
   float least = 0.0f;
   for (const MxShape& h : shapes) {
     if (h.cols == (p.ys != nullptr ? 16 : 32) && h.each > 0.0f) continue;
-    const float tiles = (float)(ceil_div(p.M, h.rows) * ceil_div(p.N, h.cols));
+    const int64_t count = ceil_div(p.M, h.rows) * ceil_div(cols, h.cols);
+    if (count >= (int64_t{1} << 32) / 512) continue;
+    const float tiles = (float)count;
     const float steps = (float)ceil_div(ceil_div(p.K, 128), h.groups);
     const float rounds = h.each > 0.0f ? 1.0f : ceilf(tiles / 256.0f);
     const float own = h.once + rounds * (h.round + steps * h.step) + tiles / 256.0f * steps * h.each;
     const float t = fmaxf(own, floor) + 0.1f * own;  // between those at the floor, the one with least of its own
     if (best == nullptr || t < least) best = &h, least = t;
   }
-  best->launch(p, st);
+  if (best != nullptr) best->launch(p, st);
+  return best != nullptr;
 }
 
 }  // namespace ltx
@@ -628,12 +633,8 @@ extern "C" int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_code
   MxLinearArgs p{(const uint8_t*)a_codes, (const uint8_t*)a_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales,
                  (const uint16_t*)bias, y, (uint8_t*)y_scales, y_ls, (int)M, (int)N, (int)K,
                  (uintptr_t)y % 16 == 0 && y_ls % 8 == 0, (uintptr_t)bias % 16 == 0 && N % 8 == 0};
-  LTX_REQUIRE(ceil_div(M, 128) <= 65535, "ltx_mx_linear: too many rows");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (act)
-    launch_mx<true>(p, st);
-  else
-    launch_mx<false>(p, st);
+  LTX_REQUIRE(act ? launch_mx<true>(p, st) : launch_mx<false>(p, st), "ltx_mx_linear: the result is too large");
   LTX_LAUNCH_CHECK("ltx_mx_linear");
   return LTX_OK;
 }

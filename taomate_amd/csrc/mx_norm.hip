@@ -147,13 +147,15 @@ extern "C" int ltx_adaln_mx(int64_t B, int64_t L, int64_t C, const void* x, int6
   clear_error();
   LTX_REQUIRE(B >= 0 && L >= 0 && C >= kMxBlock && C % kMxBlock == 0 && C <= 8192,
               "ltx_adaln_mx: C must be a multiple of %d in [%d, 8192]", kMxBlock, kMxBlock);
-  LTX_REQUIRE(B <= 0x7FFFFFFF && L <= 0x7FFFFFFF && B * L <= 0x7FFFFFFF, "ltx_adaln_mx: too many rows");
+  // a grid holds fewer than 2^32 threads along L, at most 512 a row
+  LTX_REQUIRE(B <= 0x7FFFFFFF && L < (int64_t{1} << 32) / 512 && B * L <= 0x7FFFFFFF, "ltx_adaln_mx: too many rows");
   if (B * L == 0) return LTX_OK;
   LTX_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr, "ltx_adaln_mx: null pointer");
   LTX_REQUIRE(gate == nullptr || y != nullptr, "ltx_adaln_mx: a gate needs a residual branch y");
   LTX_REQUIRE((scale == nullptr) == (shift == nullptr), "ltx_adaln_mx: scale and shift go together");
   LTX_REQUIRE(scale == nullptr || eps >= 0.0f, "ltx_adaln_mx: modulation needs the norm");
   LTX_REQUIRE(x_out == nullptr || y != nullptr, "ltx_adaln_mx: x_out without a residual branch");
+  LTX_REQUIRE(x_out == nullptr || ((L == 1 || xo_ls >= C) && (B == 1 || xo_bs >= C)), "ltx_adaln_mx: rows of x_out overlap");
   auto ok = [](const void* p, int64_t bs, int64_t ls) {
     return p == nullptr || (((uintptr_t)p % 16) == 0 && bs % 8 == 0 && ls % 8 == 0);
   };

@@ -180,9 +180,10 @@ def adaln_mx(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[t
              shift: Optional[torch.Tensor] = None, eps: Optional[float] = 1e-6) -> MXRows:
     """ltx_adaln_mx on bf16 [B, L, C] rows: ``adaln``'s residual update and
     (modulated) RMS norm with the normalised rows returned in 8 bits, for
-    ``mx_linear``; x_out = x + y * gate in bf16.  float32 between its inputs and
-    outputs (``adaln`` rounds to bf16 where the reference's ops do).  eps None
-    skips the norm: the rows themselves.  C a multiple of 32, at most 8192."""
+    ``mx_linear``; x_out = x + y * gate in bf16 (x_out may be x or y).  float32
+    between its inputs and outputs (``adaln`` rounds to bf16 where the
+    reference's ops do).  eps None skips the norm: the rows themselves.  C a
+    multiple of 32, at most 8192; fewer than 2^23 rows a sample."""
     return MXRows(*(N._host or N.host()).adaln_mx(x, y, gate, x_out, scale, shift, eps))
 
 

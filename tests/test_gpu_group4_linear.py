@@ -93,3 +93,28 @@ def test_refusals(dev):
         kernels.group4_linear(x, w, torch.zeros(15, device=dev, dtype=BF))
     with pytest.raises(TypeError):
         kernels.group4_linear(x.float(), w)
+
+
+def test_one_row_expanded(dev):
+    g = gen(7)
+    x, w = randn((1, 256), g, BF), _weight(100, 256, 64, g)
+    y = kernels.group4_linear(x.to(dev).expand(5, 256), _to(w, dev))
+    assert torch.equal(y, kernels.group4_linear(x.to(dev), _to(w, dev)).expand(5, 100))
+
+
+def test_a_long_weight(dev):
+    """Codes past 2^32 bytes."""
+    tiles, chunks = 70_000, 64 // 2
+    codes = torch.empty(tiles, chunks, 4, 16, 16, dtype=torch.uint8, device=dev)
+    g = torch.Generator(device=dev).manual_seed(3)
+    for i in range(0, tiles, 10_000):
+        codes[i:i + 10_000] = torch.randint(0, 256, (min(10_000, tiles - i), chunks, 4, 16, 16), generator=g, device=dev,
+                                            dtype=torch.uint8)
+    scales = torch.rand(tiles, chunks, 16, 1, generator=g, device=dev).to(BF)
+    K = chunks * 128
+    w = quant.Group4Weight(codes, scales, tiles * 16, K)
+    x = torch.randn(2, K, generator=g, device=dev).to(BF)
+    y = kernels.group4_linear(x, w)
+    for t in (0, 32_767, 32_768, 65_536, tiles - 1):
+        part = quant.Group4Weight(codes[t:t + 1].contiguous(), scales[t:t + 1].contiguous(), 16, K)
+        check(x.cpu(), quant.Group4Weight(part.codes.cpu(), part.scales.cpu(), 16, K), None, False, y[:, t * 16:t * 16 + 16])

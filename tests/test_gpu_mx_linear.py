@@ -440,3 +440,57 @@ def test_calls_on_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(t, want[i]) for t in got[i])
+
+
+@pytest.mark.parametrize("into", ["x", "y"])
+def test_adaln_mx_in_place(dev, into):
+    g = gen(40)
+    x, y = randn((2, 9, 2048), g, BF).to(dev), randn((2, 9, 2048), g, BF).to(dev)
+    gate = randn((2, 1, 2048), g, BF).to(dev)
+    xo = torch.empty_like(x)
+    n = kernels.adaln_mx(x, y, gate, xo)
+    target = {"x": x, "y": y}[into]
+    m = kernels.adaln_mx(x, y, gate, target)
+    assert torch.equal(target, xo) and torch.equal(m.codes.view(torch.uint8), n.codes.view(torch.uint8))
+
+
+def test_many_samples(dev):
+    """More samples than one grid dimension holds."""
+    x = randn((70001, 1, 32), gen(41), BF)
+    n = kernels.adaln_mx(x.to(dev))
+    xd = x.double()
+    check_mx(n, xd / torch.sqrt(xd.square().mean(-1, keepdim=True) + EPS), torch.tensor(2.0 ** -17))
+
+
+def test_many_rows(dev):
+    """A tall product: rows past 2^20, few columns and channels."""
+    M = (1 << 20) + 37
+    a, w, b, ref, err = _on_gpu(dev, M, 32, 40, 42, False)
+    _check_bf16(kernels.mx_linear(a, w, b), ref, err)
+
+
+def test_a_weight_past_two_gigabytes(dev):
+    """Byte offsets of w and of the result past 2^31 and 2^32."""
+    N, K = 1_100_000, 4096
+    w = torch.empty(N, K, dtype=torch.uint8, device=dev)
+    step = 100_000
+    g = torch.Generator(device=dev).manual_seed(3)
+    for i in range(0, N, step):   # finite codes
+        w[i:i + step] = torch.randint(0, 120, (min(step, N - i), K), generator=g, device=dev, dtype=torch.uint8)
+    scales = torch.full((K // 128, N, 4), 118, dtype=torch.uint8, device=dev)
+    weight = quant.MXRows(w.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
+    for M in (3, 130):
+        a = quant.quantize_mx(torch.randn(M, K, generator=g, device=dev))
+        y = kernels.mx_linear(a, weight)
+        rows = torch.tensor([0, 1, 524_287, 524_288, 800_001, 1_048_576, N - 1], device=dev)
+        part = quant.MXRows(weight.codes.view(torch.uint8)[rows].view(torch.float8_e4m3fn), scales[:, rows].contiguous().view(torch.float8_e8m0fnu))
+        ad, wd = a.dequantize().double(), part.dequantize().double()
+        ref, err = ad @ wd.t(), 1.01 * MFMA * (ad.abs() @ wd.abs().t())
+        assert ((y[:, rows].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + err).all()
+
+
+def test_one_row_without_leading_dimensions(dev):
+    a, w, b = _linear_case(1, 96, 64, 43)
+    one = quant.MXRows(a.codes.view(96).to(dev), a.scales.to(dev))
+    y = kernels.mx_linear(one, _to(w, dev), b.to(dev))
+    assert y.shape == (64,) and torch.equal(y, kernels.mx_linear(_to(a, dev), _to(w, dev), b.to(dev))[0])

@@ -1,5 +1,6 @@
 """The packers of the block-scaled linears on the CPU, against the formats'
 definitions written out, and what the wrappers refuse."""
+import ctypes
 import itertools
 import math
 
@@ -122,3 +123,49 @@ def test_wrappers_refuse_on_the_host():
             call()
     with pytest.raises(TypeError, match="expected 8 arguments"):
         _native.host().mx_linear(rows.codes)
+
+
+P = ctypes.c_void_p(4096)   # never read: each call below is refused before a launch
+BIG = 1 << 30
+
+
+def _adaln_mx(B, L, C, x_out=None, xo=(0, 0), eps=1e-6, y=P):
+    _native.call("ltx_adaln_mx", B, L, C, P, L * C, C, y, L * C, C, None, 0, 0, x_out, *xo, None, 0, 0, None, 0, 0, eps,
+                 P, P, None)
+
+
+def _mx_linear(M, N, K, y_ls=None, y_scales=None, act=0, a=P):
+    _native.call("ltx_mx_linear", M, N, K, a, P, P, P, None, act, P, N if y_ls is None else y_ls, y_scales, None)
+
+
+def _group4_linear(M, N, K, group=32, y_ls=None, x_ls=None, x=P):
+    _native.call("ltx_group4_linear", M, N, K, group, x, K if x_ls is None else x_ls, 0, P, P, None, P,
+                 N if y_ls is None else y_ls, None)
+
+
+@pytest.mark.parametrize("match,call", [
+    ("multiple of 32", lambda: _adaln_mx(1, 1, 40)),
+    ("multiple of 32", lambda: _adaln_mx(1, 1, 8224)),
+    ("too many rows", lambda: _adaln_mx(1, 1 << 23, 32)),
+    ("too many rows", lambda: _adaln_mx(1 << 20, 1 << 12, 32)),
+    ("x_out without", lambda: _adaln_mx(1, 1, 32, P, y=None)),
+    ("rows of x_out overlap", lambda: _adaln_mx(2, 3, 64, P, (0, 64))),
+    ("rows of x_out overlap", lambda: _adaln_mx(2, 3, 64, P, (192, 0))),
+    ("null pointer", lambda: _mx_linear(1, 32, 32, a=None)),
+    ("16-byte aligned", lambda: _mx_linear(1, 32, 32, a=ctypes.c_void_p(4104))),
+    ("bad M or N", lambda: _mx_linear(BIG, 32, 32)),
+    ("too large", lambda: _mx_linear(BIG - 1, BIG - 1, 32)),
+    ("too large", lambda: _mx_linear(BIG - 1, 1 << 20, 4096, act=1)),
+    ("too large", lambda: _mx_linear(1 << 20, BIG - 32, 4096, y_scales=P)),
+    ("rows of y overlap", lambda: _mx_linear(2, 64, 32, 63)),
+    ("multiple of 32", lambda: _mx_linear(2, 40, 32, y_scales=P)),
+    ("K must be", lambda: _mx_linear(2, 32, (1 << 20) + 32)),
+    ("rows of y overlap", lambda: _group4_linear(2, 64, 32, y_ls=63)),
+    ("16-byte aligned", lambda: _group4_linear(2, 64, 32, x_ls=36)),
+    ("M must be", lambda: _group4_linear(17, 64, 32)),
+    ("group must be", lambda: _group4_linear(2, 64, 32, group=16)),
+    ("K must be", lambda: _group4_linear(2, 64, 4128)),
+])
+def test_entry_points_refuse(match, call):
+    with pytest.raises(_native.NativeCallError, match=match):
+        call()
