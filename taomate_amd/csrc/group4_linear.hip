@@ -18,10 +18,14 @@
 //
 // A workgroup has 8 waves: KS of them share a tile of 16 rows of W, each with up
 // to 4 chunks of 128 columns in flight, and meet in LDS; 8 / KS tiles at a time.
-// x (SiLU applied, rounded to bf16 as the tensor op rounds) is staged in LDS
-// once per workgroup, which then strides over the tiles.  2 rows of 4096 -> 24576 with
-// groups of 32 and SiLU: 13.7 us (4.2 TB/s of 57 MB; 5.5 TB/s at the end of longer
-// weights), 8 rows of 2048 -> 12288 with groups of 128: 6.8 us.
+// x is staged in LDS once per workgroup, which then strides over the tiles.  SiLU(x)
+// is held unrounded, to 2^-18, as two rows of the matrix cores' 16: its bf16 and the
+// bf16 of what that leaves, whose sums meet in the epilogue.  (Rounded to bf16 once it
+// would add as much error again as the result's own rounding.)  Those are free up to 8
+// rows; more go by halves, two workgroups of one XCD over the same tiles, so that
+// the second read of W comes from their L2 (16 rows of 4096 -> 24576: 25.7 us; rounded once 20.8).  2 rows of 4096 -> 24576 with
+// groups of 32 and SiLU: 13.9 us (4.1 TB/s of 57 MB; 5.5 TB/s at the end of longer
+// weights), 8 rows of 2048 -> 12288 with groups of 128: 7.5 us.
 
 #include <type_traits>
 
@@ -43,10 +47,10 @@ struct Group4Args {
   uint16_t* y;
   int64_t y_ls;
   int64_t N;
-  int M, K, silu;
+  int M, K;
 };
 
-// SiLU through one exp2 and one reciprocal (1 ulp each), rounded to bf16 after.
+// SiLU through one exp2 and one reciprocal (1 ulp each).
 __device__ __forceinline__ float g4_silu(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
 }
@@ -61,12 +65,13 @@ __device__ __forceinline__ g4_bf16x8 g4_decode(uint32_t w) {
   return __builtin_shufflevector(ab, cd, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// KS waves per tile, GROUP columns per scale.
-template <int KS, int GROUP>
+// KS waves per tile, GROUP columns per scale.  With SILU, rows 4 i + 2 h + l of the
+// matrix cores' 16 (h, l of {0, 1}) are part h of row 2 i + l of x: a lane has both sums.
+template <int KS, int GROUP, bool SILU>
 __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Group4Args a) {
   constexpr int kTiles = kG4Waves / KS, kPer = 128 / GROUP;  // tiles per workgroup; scales per chunk and row
-  extern __shared__ uint4 xs[];                              // [M][chunks * 16 + 1]
-  __shared__ float part[2][kG4Waves][16][17];
+  extern __shared__ uint4 xs[];                              // [M, with SiLU 2 M][chunks * 16 + 1]
+  __shared__ float part[2][kG4Waves][SILU ? 8 : 16][17];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, p = lane >> 4, kw = wave % KS;
   const int chunks = (a.K + 127) / 128, row_words = chunks * 16 + 1;
@@ -90,7 +95,16 @@ __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Grou
       __builtin_memcpy(t.s[i], __builtin_assume_aligned(a.scales + (c * 16 + r16) * kPer, kPer * 2), sizeof(t.s[i]));
     }
   };
-  const int64_t stride = (int64_t)gridDim.x * kTiles, first = (int64_t)blockIdx.x * kTiles;
+  int m_first = 0, M = a.M, block = blockIdx.x, blocks = gridDim.x;
+  if (SILU && a.M > 8) {  // halves of the rows: workgroups 8 apart, of one XCD
+    const int per = (a.M + 1) >> 1;
+    m_first = block & 8 ? per : 0;
+    M = min(a.M - m_first, per);
+    block = (block >> 4) * 8 + (block & 7);
+    blocks >>= 1;
+  }
+  const uint16_t* x = a.x + m_first * a.x_ls;
+  const int64_t stride = (int64_t)blocks * kTiles, first = (int64_t)block * kTiles;
   const int64_t tile = first + wave / KS;
   const int64_t rounds = (tiles - first + stride - 1) / stride;
   Rows rows[2];
@@ -100,33 +114,40 @@ __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Grou
   // while x is staged.
   const int words = chunks * 16, xrows = 64 * kG4Waves / words;
   const int xm = threadIdx.x / words, xc = threadIdx.x - xm * words;
-  for (int m0 = 0; m0 < a.M; m0 += 4 * xrows) {
+  for (int m0 = 0; m0 < M; m0 += 4 * xrows) {
     uint4 v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int m = m0 + q * xrows + xm;
       v[q] = make_uint4(0, 0, 0, 0);  // columns past K: their codes are 0, so x must be finite there
-      if (xm < xrows && m < a.M && xc * 8 < a.K) v[q] = *reinterpret_cast<const uint4*>(a.x + m * a.x_ls + xc * 8);
+      if (xm < xrows && m < M && xc * 8 < a.K) v[q] = *reinterpret_cast<const uint4*>(x + m * a.x_ls + xc * 8);
     }
-    if (m0 + 4 * xrows >= a.M) {
+    if (m0 + 4 * xrows >= M) {
       load(rows[0], tile);
       if (rounds > 1) load(rows[1], tile + stride);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int m = m0 + q * xrows + xm;
-      if (xm >= xrows || m >= a.M) break;
-      if (a.silu) {
-        uint32_t* t = &v[q].x;
+      if (xm >= xrows || m >= M) break;
+      if constexpr (SILU) {
+        uint4 rest;
+        uint32_t *t = &v[q].x, *d = &rest.x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          t[e] = pack_bf16x2(g4_silu(bf16_bits_to_f32(t[e] & 0xFFFFu)), g4_silu(bf16_bits_to_f32(t[e] >> 16)));
+        for (int e = 0; e < 4; ++e) {
+          const float lo = g4_silu(bf16_bits_to_f32(t[e] & 0xFFFFu)), hi = g4_silu(bf16_bits_to_f32(t[e] >> 16));
+          t[e] = pack_bf16x2(lo, hi);
+          const float blo = bf16_bits_to_f32(t[e] & 0xFFFFu), bhi = bf16_bits_to_f32(t[e] >> 16);
+          d[e] = pack_bf16x2(lo == blo ? 0.0f : lo - blo, hi == bhi ? 0.0f : hi - bhi);  // infinity leaves nothing
+        }
+        xs[(M + m) * row_words + xc] = rest;
       }
       xs[m * row_words + xc] = v[q];
     }
   }
   __syncthreads();
-  const uint4* xr = xs + min(r16, a.M - 1) * row_words + p;
+  const int xrow = SILU ? (r16 >> 1 & 1) * M + min((r16 >> 2) * 2 + (r16 & 1), M - 1) : min(r16, M - 1);
+  const uint4* xr = xs + xrow * row_words + p;
 
   // the result that this thread stores in a round: row ym of x, column yc of tile yt
   const int yt = threadIdx.x >> 8, ym = (threadIdx.x >> 4) & 15, yc = threadIdx.x & 15;
@@ -159,20 +180,21 @@ __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Grou
       }
     }
     if (prefetch) load(t, tile + (r + 2) * stride);
-    // lane: rows 4 p .. + 3 of x, row r16 of the tile
+    // lane: rows 4 p .. + 3 of x (with SILU 2 p and 2 p + 1), row r16 of the tile
     const int buf = (int)(r & 1);
+    constexpr int kOwn = SILU ? 2 : 4;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[buf][wave][p * 4 + e][r16] = acc[e];
+    for (int e = 0; e < kOwn; ++e) part[buf][wave][p * kOwn + e][r16] = SILU ? acc[e] + acc[e + 4 - kOwn] : acc[e];
     __syncthreads();  // the other buffer's sums, read a round ago, may be overwritten after it
 #pragma unroll
     for (int h = 0; h < (kTiles + 1) / 2; ++h) {
       const int tw = h * 2 + yt;
       const int64_t n = (t0 + tw) * 16 + yc;
-      if (tw < kTiles && ym < a.M && n < a.N) {
+      if (tw < kTiles && ym < M && n < a.N) {
         float v = bias[h];
 #pragma unroll
         for (int k = 0; k < KS; ++k) v += part[buf][tw * KS + k][ym][yc];
-        a.y[ym * a.y_ls + n] = f32_to_bf16_bits(v);
+        a.y[(m_first + ym) * a.y_ls + n] = f32_to_bf16_bits(v);
       }
     }
   };
@@ -194,29 +216,33 @@ __global__ void __launch_bounds__(64 * kG4Waves) group4_linear_kernel(const Grou
   }
 }
 
-template <int KS, int GROUP>
+template <int KS, int GROUP, bool SILU>
 void launch_group4(const Group4Args& a, hipStream_t st) {
   const int chunks = (a.K + 127) / 128;
-  const size_t lds = (size_t)a.M * (chunks * 16 + 1) * 16;
-  const size_t all = lds + sizeof(float) * 2 * kG4Waves * 16 * 17;
-  // resident workgroups per CU: what the LDS holds, at most 2 (16 waves)
-  const int64_t most = 256 * (all > 80 * 1024 ? 1 : 2), want = ceil_div(ceil_div(a.N, 16), kG4Waves / KS);
-  hipLaunchKernelGGL((group4_linear_kernel<KS, GROUP>), dim3((unsigned)(want < most ? want : most)),
-                     dim3(64 * kG4Waves), lds, st, a);
+  const size_t lds = (size_t)(!SILU ? a.M : a.M > 8 ? a.M + 1 : 2 * a.M) * (chunks * 16 + 1) * 16;
+  const size_t all = lds + sizeof(float) * 2 * kG4Waves * (SILU ? 8 : 16) * 17;
+  // Resident workgroups per CU: two (16 waves) where the LDS holds them (4 rows of 4096
+  // -> 24576 in 15.5 us, one at a time 17.2).  Each stages x, so a large x takes one
+  // where two would have no more than a round each (8 rows of 2048 -> 12288: 7.5 us, two 8.1).
+  const int64_t want = ceil_div(ceil_div(a.N, 16), kG4Waves / KS);
+  const int64_t most = all > 80 * 1024 || (all > 48 * 1024 && want <= 512) ? 256 : 512;
+  int64_t grid = want < most ? want : most;
+  if (SILU && a.M > 8) grid = 2 * (want < most / 2 ? ceil_div(want, 8) * 8 : most / 2);  // whole groups of 8, 8 apart
+  hipLaunchKernelGGL((group4_linear_kernel<KS, GROUP, SILU>), dim3((unsigned)grid), dim3(64 * kG4Waves), lds, st, a);
 }
 
-template <int GROUP>
+template <int GROUP, bool SILU>
 void launch_group4(const Group4Args& a, hipStream_t st) {
   // as few waves per tile as hold its columns in flight (4 chunks of 128 each)
   const int chunks = (a.K + 127) / 128;
   if (chunks <= kG4Chunks)
-    launch_group4<1, GROUP>(a, st);
+    launch_group4<1, GROUP, SILU>(a, st);
   else if (chunks <= 2 * kG4Chunks)
-    launch_group4<2, GROUP>(a, st);
+    launch_group4<2, GROUP, SILU>(a, st);
   else if (chunks <= 4 * kG4Chunks)
-    launch_group4<4, GROUP>(a, st);
+    launch_group4<4, GROUP, SILU>(a, st);
   else
-    launch_group4<8, GROUP>(a, st);
+    launch_group4<8, GROUP, SILU>(a, st);
 }
 static_assert(LTX_SKINNY_MAX_K <= 8 * kG4Chunks * 128, "8 waves hold a row of W");
 
@@ -240,14 +266,14 @@ extern "C" int ltx_group4_linear(int64_t M, int64_t N, int64_t K, int64_t group,
               "ltx_group4_linear: x rows and codes must be 16-byte aligned, scales 8-byte");
   LTX_REQUIRE(M == 1 || y_ls >= N, "ltx_group4_linear: rows of y overlap");
   Group4Args a{(const uint16_t*)x, x_ls, (const uint8_t*)codes, (const uint16_t*)scales, (const uint16_t*)bias,
-               (uint16_t*)y, y_ls, N, (int)M, (int)K, silu};
+               (uint16_t*)y, y_ls, N, (int)M, (int)K};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (group == 32)
-    launch_group4<32>(a, st);
+    silu ? launch_group4<32, true>(a, st) : launch_group4<32, false>(a, st);
   else if (group == 64)
-    launch_group4<64>(a, st);
+    silu ? launch_group4<64, true>(a, st) : launch_group4<64, false>(a, st);
   else
-    launch_group4<128>(a, st);
+    silu ? launch_group4<128, true>(a, st) : launch_group4<128, false>(a, st);
   LTX_LAUNCH_CHECK("ltx_group4_linear");
   return LTX_OK;
 }

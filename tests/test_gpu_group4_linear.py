@@ -118,3 +118,31 @@ def test_a_long_weight(dev):
     for t in (0, 32_767, 32_768, 65_536, tiles - 1):
         part = quant.Group4Weight(codes[t:t + 1].contiguous(), scales[t:t + 1].contiguous(), 16, K)
         check(x.cpu(), quant.Group4Weight(part.codes.cpu(), part.scales.cpu(), 16, K), None, False, y[:, t * 16:t * 16 + 16])
+
+
+@pytest.mark.parametrize("M,K,n,group", [(1, 64, 5, 64), (3, 4096, 40, 32), (8, 2048, 300, 128), (9, 4096, 130, 64),
+                                         (12, 160, 17, 32), (16, 32, 1, 32), (16, 4096, 4099, 128), (13, 1152, 9001, 32)])
+def test_silu_is_not_rounded(dev, M, K, n, group):
+    """Only the sums and the result's rounding: SiLU of |x| < 6 in float32 is within
+    2^-20 (exp2's argument |x| 2^-23.4, exp2, reciprocal and product 1 ulp each), and
+    what two bf16 hold of it within 2^-18: 2^-17 together, of each product."""
+    g = gen(M + K + n)
+    x, w = randn((M, K), g, BF).clamp(-6, 6), _weight(n, K, group, g)
+    b = randn((n,), g, BF)
+    y = kernels.group4_linear(x.to(dev), _to(w, dev), b.to(dev), silu=True).double().cpu()
+    xd, wd = torch.nn.functional.silu(x.double()), w.dequantize().double()
+    ref, mag = xd @ wd.t() + b.double(), xd.abs() @ wd.abs().t() + b.double().abs()
+    assert ((y - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * (2.0 ** -17 + 2.0 ** -20) * mag).all()
+
+
+@pytest.mark.parametrize("M", [4, 11])
+def test_silu_of_infinities(dev, M):
+    """+inf keeps its sign of the weights, NaN and -inf (0 * inf) are NaN, in their rows."""
+    g = gen(M)
+    x, w = randn((M, 128), g, BF), _weight(64, 128, 32, g)
+    w = quant.quantize_group4(w.dequantize().abs() + 0.1 * w.dequantize().abs().amax(), 32)   # no code 0
+    clean = kernels.group4_linear(x.to(dev), _to(w, dev), silu=True)
+    x[0, 5], x[1, 7], x[M - 1, 9] = float("inf"), float("-inf"), float("nan")
+    y = kernels.group4_linear(x.to(dev), _to(w, dev), silu=True)
+    assert (w.dequantize()[:, 5] > 0).all() and (y[0] == float("inf")).all()
+    assert y[1].isnan().all() and y[M - 1].isnan().all() and torch.equal(y[2:M - 1], clean[2:M - 1])
