@@ -494,3 +494,46 @@ def test_one_row_without_leading_dimensions(dev):
     one = quant.MXRows(a.codes.view(96).to(dev), a.scales.to(dev))
     y = kernels.mx_linear(one, _to(w, dev), b.to(dev))
     assert y.shape == (64,) and torch.equal(y, kernels.mx_linear(_to(a, dev), _to(w, dev), b.to(dev))[0])
+
+
+def test_results_are_ordinary_tensors(dev):
+    """Their memory is the caching allocator's, codes and scales of one allocation, freed
+    with the last of them; they are inference tensors where torch's own would be."""
+    x = randn((2, 3, 160), gen(44), BF).to(dev)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    n = kernels.adaln_mx(x)
+    scales = n.scales
+    assert torch.cuda.memory_allocated() > before
+    for t in n.tensors():
+        assert t.device == x.device and t.is_contiguous() and not t.requires_grad and not t.is_inference()
+        assert torch.equal(t.view(torch.uint8).clone(), t.view(torch.uint8).cpu().to(dev))
+    side = torch.cuda.Stream()
+    n.codes.record_stream(side)
+    del n, t
+    assert torch.cuda.memory_allocated() > before
+    del scales
+    torch.cuda.synchronize()
+    kernels.adaln_mx(x)   # events of recorded streams are looked at by the next allocation
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+    with torch.inference_mode():
+        assert kernels.adaln_mx(x).codes.is_inference() and kernels.adaln_mx(x).scales.is_inference()
+
+
+def test_no_memory_left(dev):
+    """The allocator's own error, and the next call works."""
+    x = randn((1, 2048, 4096), gen(45), BF).to(dev)
+    w = quant.quantize_mx(torch.ones(65536, 4096, device=dev, dtype=BF))
+    rows = kernels.adaln_mx(x)
+    total = torch.cuda.get_device_properties(dev).total_memory
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):   # 256 MB
+            kernels.mx_linear(rows, w)
+        with pytest.raises(torch.OutOfMemoryError):   # 128 MB
+            kernels.mx_linear(rows, w, quantize=True)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert kernels.mx_linear(rows, w).shape == (1, 2048, 65536)
