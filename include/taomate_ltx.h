@@ -396,7 +396,7 @@ int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_codes, const vo
  *   half) and the one after it (p, j, i in [0, 4)); scales: bf16
  *   [ceil(N / 16)][ceil(K / 128)][16][128 / group], 8-byte aligned, group 32, 64 or
  *   128 dividing K.  Codes and scales past N or K are 0.
- *   silu != 0 applies SiLU to x first, in float32 and not rounded (to 2^-18).
+ *   silu != 0 applies SiLU to x first, in float32 and not rounded (to 2^-16).
  */
 #define LTX_GROUP4_MAX_ROWS 16
 int ltx_group4_linear(int64_t M, int64_t N, int64_t K, int64_t group, const void* x, int64_t x_ls, int silu,

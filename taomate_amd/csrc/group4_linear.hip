@@ -19,13 +19,14 @@
 // A workgroup has 8 waves: KS of them share a tile of 16 rows of W, each with up
 // to 4 chunks of 128 columns in flight, and meet in LDS; 8 / KS tiles at a time.
 // x is staged in LDS once per workgroup, which then strides over the tiles.  SiLU(x)
-// is held unrounded, to 2^-18, as two rows of the matrix cores' 16: its bf16 and the
-// bf16 of what that leaves, whose sums meet in the epilogue.  (Rounded to bf16 once it
-// would add as much error again as the result's own rounding.)  Those are free up to 8
-// rows; more go by halves, two workgroups of one XCD over the same tiles, so that
-// the second read of W comes from their L2 (16 rows of 4096 -> 24576: 25.7 us; rounded once 20.8).  2 rows of 4096 -> 24576 with
-// groups of 32 and SiLU: 13.9 us (4.1 TB/s of 57 MB; 5.5 TB/s at the end of longer
-// weights), 8 rows of 2048 -> 12288 with groups of 128: 7.5 us.
+// is held to 2^-16 as two rows of the matrix cores' 16: its bf16 and the bf16 of what
+// that leaves, whose sums meet in the epilogue.  (Rounded to bf16 once it would add
+// as much error again as the result's own rounding.)  That costs no products up to 8
+// rows; more go by halves, two workgroups of one XCD over the same tiles, so that the
+// second read of W comes from their L2 (16 rows of 4096 -> 24576: 25.7 us; rounded
+// once 20.8).  2 rows of 4096 -> 24576 with groups of 32 and SiLU: 13.8 us (4.1 TB/s
+// of 57 MB; 5.5 TB/s at the end of longer weights), 8 rows of 2048 -> 12288 with groups
+// of 128: 7.5 us, of which computing SiLU(x) in every workgroup takes about 1.
 
 #include <type_traits>
 
