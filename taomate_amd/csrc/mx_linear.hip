@@ -564,11 +564,13 @@ void launch_mx_rows(const MxLinearArgs& p, hipStream_t st) {
 // to 16384 channels: `once`, then for every round of workgroups `round` plus `step` for
 // each step of a group (`each` per 256 tiles and step instead where many tiles
 // share a CU), never below what the bytes take at 5.3 TB/s.  Over those shapes the
-// choice is within 4 % of the fastest of 17 tiles in the mean.  What the ends are for: at 2
-// rows of 4096 -> 16384 the 64-row tile without groups takes 21.4 us where the rows
-// kernel and the 32 x 64 tile take 13.6 and 14.5 (the weight's bytes 13.2); at 2304 rows
-// of 4096 -> 12288 the 256-row tile takes 113 us, the 192-row one 124, at 16384
-// channels 156 and 145; at 150 rows of 2048 -> 8192 80 x 64 takes 9.3, 128 x 256 19.1.
+// choice is within 1 % of the fastest of 19 tiles in the mean.  What each is for, the
+// next best beside it: 1 row of 16384 -> 4096 16 x 16 14.2 us (32 x 32 15.8); 8 rows of
+// 4096 -> 4096 32 x 32 6.9 (48 x 32 7.6); 75 rows of 2048 -> 8192 48 x 64 7.4 (80 x 64 8.6),
+// 150 rows 80 x 64 9.2 (160 x 64 10.7), of 8192 -> 2048 48 x 32 12.0 (32 x 64 14.3); 331 rows of
+// 1056 -> 4099 160 x 64 9.2 (128 x 128 11.2); 768 rows of 16384 -> 4096 128 x 128 64 (48 x 64 and
+// 80 x 64 88 and more); 384 rows of 4096 -> 16384 128 x 256 34.6 (192 x 256 36.8); 2304 rows 192 x 256
+// 146 (256 x 256 150), to 12288 channels 256 x 256 111 (192 x 256 121).
 struct MxShape {
   int rows, cols, groups;
   float once, round, step, each;
@@ -579,17 +581,18 @@ struct MxShape {
 template <bool GELU>
 bool launch_mx(const MxLinearArgs& p, hipStream_t st) {
   static const MxShape shapes[] = {
-      {16, 16, 8, 3.22f, 0.0f, 0.36f, 0.77f, launch_mx_rows<1, 1, GELU>},  // bf16 results
-      {16, 32, 8, 3.11f, 0.0f, 0.63f, 1.34f, launch_mx_rows<1, 2, GELU>},  // 8-bit ones: whole blocks
-      {32, 32, 4, 1.45f, 3.23f, 0.39f, 0.0f, launch_mx_linear<2, 2, 1, 1, 3, 4, GELU>},
-      {32, 64, 4, 1.13f, 3.64f, 0.61f, 0.0f, launch_mx_linear<2, 2, 1, 2, 3, 4, GELU>},
-      {64, 64, 2, 1.17f, 3.60f, 0.48f, 0.0f, launch_mx_linear<2, 2, 2, 2, 3, 2, GELU>},
-      {80, 64, 4, 0.76f, 4.89f, 0.84f, 0.0f, launch_mx_linear<5, 2, 1, 2, 2, 4, GELU>},
-      {160, 64, 2, 0.0f, 5.19f, 0.71f, 0.0f, launch_mx_linear<5, 2, 2, 2, 2, 2, GELU>},
-      {128, 128, 2, 0.0f, 6.70f, 0.87f, 0.0f, launch_mx_linear<4, 4, 2, 2, 2, 2, GELU>},
-      {128, 256, 1, 0.0f, 6.21f, 0.78f, 0.0f, launch_mx_linear<4, 4, 2, 4, 3, 1, GELU>},
-      {192, 256, 1, 0.0f, 6.22f, 0.94f, 0.0f, launch_mx_linear<6, 4, 2, 4, 2, 1, GELU>},
-      {256, 256, 1, 0.0f, 8.21f, 1.09f, 0.0f, launch_mx_linear<8, 4, 2, 4, 2, 1, GELU>},
+      {16, 16, 8, 3.13f, 0.0f, 0.37f, 0.76f, launch_mx_rows<1, 1, GELU>},  // bf16 results
+      {16, 32, 8, 2.98f, 0.0f, 0.65f, 1.32f, launch_mx_rows<1, 2, GELU>},  // 8-bit ones: whole blocks
+      {32, 32, 4, 1.84f, 2.06f, 0.39f, 0.0f, launch_mx_linear<2, 2, 1, 1, 3, 4, GELU>},
+      {32, 64, 4, 1.66f, 2.59f, 0.60f, 0.0f, launch_mx_linear<2, 2, 1, 2, 3, 4, GELU>},
+      {48, 32, 4, 1.70f, 2.38f, 0.47f, 0.0f, launch_mx_linear<3, 2, 1, 1, 3, 4, GELU>},
+      {48, 64, 4, 1.48f, 2.38f, 0.68f, 0.0f, launch_mx_linear<3, 2, 1, 2, 2, 4, GELU>},
+      {80, 64, 4, 1.19f, 3.14f, 0.85f, 0.0f, launch_mx_linear<5, 2, 1, 2, 2, 4, GELU>},
+      {160, 64, 2, 0.0f, 4.16f, 0.70f, 0.0f, launch_mx_linear<5, 2, 2, 2, 2, 2, GELU>},
+      {128, 128, 2, 0.0f, 4.95f, 0.86f, 0.0f, launch_mx_linear<4, 4, 2, 2, 2, 2, GELU>},
+      {128, 256, 1, 0.0f, 5.39f, 0.77f, 0.0f, launch_mx_linear<4, 4, 2, 4, 3, 1, GELU>},
+      {192, 256, 1, 0.0f, 5.22f, 0.91f, 0.0f, launch_mx_linear<6, 4, 2, 4, 2, 1, GELU>},
+      {256, 256, 1, 0.0f, 6.34f, 1.05f, 0.0f, launch_mx_linear<8, 4, 2, 4, 2, 1, GELU>},
   };
   const float bytes = ((float)p.M + p.N) * p.K * 1.03f + 2.0f * p.M * p.N, floor = 2.5f + bytes / 5.3e6f;
   const int64_t cols = p.ys != nullptr ? ceil_div(p.N, 128) * 128 : p.N;

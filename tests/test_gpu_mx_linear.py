@@ -537,3 +537,28 @@ def test_no_memory_left(dev):
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert kernels.mx_linear(rows, w).shape == (1, 2048, 65536)
+
+
+# of the tiles of 48 rows and of 32 x 64, steps short of, at and past their buffers
+TILES_OF_48 = [(137, 2144, 2096), (533, 1120, 906), (34, 544, 4109), (10, 64, 10058), (92, 10336, 8769), (75, 2048, 8190),
+               (150, 8160, 2050), (41, 1568, 4131), (13, 96, 9999)]
+
+
+@pytest.mark.parametrize("M,K,N", TILES_OF_48)
+def test_tiles_of_48_rows(dev, M, K, N):
+    test_every_tile(dev, M, K, N)
+    test_every_tile_8bit_result(dev, M, K, N)
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3])
+@pytest.mark.parametrize("M,K,N", [(5, 192, 40), (40, 1088, 999), (331, 1056, 515), (700, 320, 1000)])
+def test_rows_of_any_alignment(dev, M, K, N, shift):
+    """y and bias at odd elements, rows an odd number apart: what lies between them stays."""
+    a, w, b, ref, err = _on_gpu(dev, M, K, N, M + N + shift, False, bias=True)
+    flat = torch.full((M * (N + 5) + 8,), 7.0, dtype=BF, device=dev)
+    y = flat[shift:shift + M * (N + 5)].view(M, N + 5)[:, :N]
+    bias = torch.empty(N + 3, dtype=BF, device=dev)[shift:shift + N].copy_(b)
+    assert kernels.mx_linear(a, w, bias, out=y) is y
+    _check_bf16(y, ref, err)
+    assert (flat[:shift] == 7).all() and (flat[shift + M * (N + 5):] == 7).all()
+    assert (flat[shift:shift + M * (N + 5)].view(M, N + 5)[:, N:] == 7).all()
