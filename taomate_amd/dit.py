@@ -660,10 +660,10 @@ class AVModel(nn.Module):
         the next call; so does a deep copy or pickle of the model.
 
         Measured on random weights at the 512x768 chunk, 48 blocks: the feed-forwards
-        take a step from 79.7 to 70.7 ms, its outputs to a cosine of 0.995 with
+        take a step from 82.0 to 70.5 ms, its outputs to a cosine of 0.995 with
         the bf16 step's.  The 4-bit modulations reach every block's norms: cosine
-        0.96, for 0.1 ms of the 79 (half of the timestep linears' time, a
-        quarter of the bytes they read)."""
+        0.96, for a quarter of the bytes that the timestep linears read and no
+        measurable part of the step's time."""
         for m in self.modules():
             if isinstance(m, FeedForward):
                 m.quantize_(feed_forward)
