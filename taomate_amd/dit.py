@@ -76,13 +76,16 @@ class FeedForward(nn.Module):
         """Run the two linears in 8 bits (``kernels.mx_linear``): the weights are
         packed into 8-bit rows beside the bf16 parameters, which keep their
         names and values; the activations are quantised by the norm before
-        and by the first linear's epilogue.  Anything that changes or replaces a
-        weight afterwards ends it and the bf16 linears run again; so do calls
-        that something else would see (gradients, autocast, hooks, compilation).
-        A deep copy or pickle of the module runs in bf16.
+        and by the first linear's epilogue.  Call it on the device it is to run
+        on.  Anything that changes, moves or replaces a weight afterwards ends it
+        and the bf16 linears run again; so do calls that something else would see
+        (gradients, autocast, hooks, compilation).  A deep copy or pickle of the
+        module runs in bf16.  A captured graph keeps to the packed rows: another
+        ``quantize_()`` packs the weights' new values into the same memory, and
+        ``quantize_(False)`` frees it, after which such a graph must not be replayed.
         Both widths must be multiples of 32, the input's at most 8192."""
-        self.__dict__.pop("_mx", None)
         if not enabled:
+            self.__dict__.pop("_mx", None)
             return self
         up, down = self.net[0].proj, self.net[2]
         for lin in (up, down):
@@ -91,7 +94,9 @@ class FeedForward(nn.Module):
         if up.in_features > kernels.ADALN_MX_MAX_COLUMNS:
             raise ValueError(f"quantize_: inputs of at most {kernels.ADALN_MX_MAX_COLUMNS} channels, "
                              f"got {up.in_features}")
-        self._mx = tuple(quant.Packed(lin, quant.quantize_mx(lin.weight)) for lin in (up, down))
+        old = self.__dict__.get("_mx", (None, None))
+        with torch.inference_mode(False), torch.no_grad():
+            self._mx = tuple(quant.Packed(lin, quant.quantize_mx(lin.weight), o) for lin, o in zip((up, down), old))
         return self
 
     def quantized(self) -> bool:
@@ -104,10 +109,7 @@ class FeedForward(nn.Module):
                 and _is_plain(act, GELUApprox) and _is_plain(act.proj, nn.Linear) and _is_plain(mid, nn.Identity)
                 and _is_plain(down, nn.Linear) and _is_eager()):
             return False
-        if not (mx[0].holds(act.proj) and mx[1].holds(down)):
-            self.__dict__.pop("_mx", None)   # a weight was changed or replaced: drop the stale rows
-            return False
-        return act.proj.weight.is_cuda
+        return mx[0].holds(act.proj) and mx[1].holds(down) and act.proj.weight.is_cuda
 
     def forward_rows(self, rows: quant.MXRows) -> torch.Tensor:
         """The feed-forward of 8-bit rows (``quantized()`` must hold)."""
@@ -161,7 +163,6 @@ def _row_linear(lin: nn.Module, x: torch.Tensor, act: Optional[nn.Module] = None
             if packed.holds(lin):
                 x = x.contiguous()
                 return kernels.group4_linear(x.clone() if x.data_ptr() % 16 else x, packed.rows, b, silu=act is not None)
-            lin.__dict__.pop("_group4", None)   # the weight was changed or replaced: drop the stale codes
         if _native._host.row_operands(x, w, b):
             return kernels.skinny_linear(x, w, b, silu=act is not None)
     return lin(x if act is None else act(x))
@@ -174,7 +175,8 @@ def _pack_group4(lin: nn.Linear, group: int) -> None:
     if lin.in_features > _native.GROUP4_MAX_COLUMNS:
         raise ValueError(f"4-bit timestep linears take at most {_native.GROUP4_MAX_COLUMNS} columns, "
                          f"got {lin.in_features}")
-    lin._group4 = quant.Packed(lin, quant.quantize_group4(lin.weight, group))
+    with torch.inference_mode(False), torch.no_grad():
+        lin._group4 = quant.Packed(lin, quant.quantize_group4(lin.weight, group), lin.__dict__.get("_group4"))
 
 
 class TimestepEmbedding(nn.Module):
@@ -655,9 +657,10 @@ class AVModel(nn.Module):
         (``FeedForward.quantize_``), and with ``timestep`` the linears of the
         timestep embeddings and modulations in 4 bits with a bf16 scale for every
         ``group`` columns, for calls of up to 16 rows (one per sample or frame;
-        more rows run in bf16).  False ends either.  Load the weights before; a
-        weight that is changed or replaced afterwards runs in bf16 again until
-        the next call; so does a deep copy or pickle of the model.
+        more rows run in bf16).  False ends either.  Load the weights and move the
+        model before; a weight that is changed, moved or replaced afterwards runs
+        in bf16 again until the next call; so does a deep copy or pickle of the
+        model.  What holds of captured graphs is at ``FeedForward.quantize_``.
 
         Measured on random weights at the 512x768 chunk, 48 blocks: the feed-forwards
         take a step from 82.0 to 70.5 ms, its outputs to a cosine of 0.995 with
@@ -669,9 +672,10 @@ class AVModel(nn.Module):
                 m.quantize_(feed_forward)
             elif isinstance(m, (TimestepEmbedding, AdaLayerNormSingle)):
                 for lin in (m.linear_1, m.linear_2) if isinstance(m, TimestepEmbedding) else (m.linear,):
-                    lin.__dict__.pop("_group4", None)
                     if timestep:
                         _pack_group4(lin, group)
+                    else:
+                        lin.__dict__.pop("_group4", None)
         return self
 
     def overlap_audio_(self, enabled: bool = True) -> "AVModel":

@@ -157,12 +157,20 @@ class Packed:
     tells whether ``lin.weight`` is still the parameter, in the memory and at the
     version, that was packed (a change through ``.data`` in place goes unseen).
     Keeps the packed memory alive, so that nothing else can come to lie there.
-    A deep copy or pickle carries no rows and never holds: versions count anew there."""
+    ``into``: an earlier packing whose rows are overwritten where they have the
+    same layout, so that captured graphs read the new ones.  A deep copy or pickle
+    carries no rows and never holds: versions count anew there."""
     __slots__ = ("rows", "weight", "source", "version")
 
-    def __init__(self, lin: torch.nn.Linear, rows):
+    def __init__(self, lin: torch.nn.Linear, rows, into: "Packed | None" = None):
         if lin.weight.is_inference():
             raise ValueError("a weight made in inference mode does not tell when it is changed: it cannot be packed")
+        old = None if into is None else into.rows
+        if old is not None and old.shape == rows.shape and all(
+                a.shape == b.shape and a.device == b.device for a, b in zip(old.tensors(), rows.tensors())):
+            for a, b in zip(old.tensors(), rows.tensors()):
+                a.view(torch.uint8).copy_(b.view(torch.uint8))
+            rows = old
         self.rows = rows
         self.weight = lin.weight
         self.source = lin.weight.detach()

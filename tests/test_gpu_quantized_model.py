@@ -137,3 +137,34 @@ def test_model_step_over_arena_caches(dev):
         v, a, _ = _forward(m, dev, x, caches)
     assert v.shape == (B, NF * GH * GW, CFG.out_channels) and a.shape == (B, LA, CFG.out_channels)
     assert v.isfinite().all() and a.isfinite().all() and LT > 0
+
+
+def test_a_captured_feed_forward_follows_packing_again(dev):
+    """Replays read the packed weights: the old ones after a change, the new ones once packed
+    again, whatever eager calls in between allocate."""
+    ff = D.FeedForward(128, 128).to(dev, BF).quantize_()
+    x = randn((1, 16, 128), gen(3), BF).to(dev)
+    with torch.no_grad():
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            ff(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            held = ff(x)
+        first = ff(x).clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, first)
+        ff.net[2].weight.mul_(-2.0)
+        assert not ff.quantized() and torch.equal(ff(x), ff.net(x))
+        junk = [torch.full((1 << n,), 255, dtype=torch.uint8, device=dev) for n in range(6, 20)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, first)
+        ff.quantize_()
+        second = ff(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, second) and not torch.equal(second, first) and len(junk) == 14

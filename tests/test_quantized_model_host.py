@@ -97,6 +97,33 @@ def test_a_copy_is_not_packed(how):
         assert not two.quantized() and two.quantize_() is two
 
 
+def test_packing_again_keeps_the_memory():
+    """What a captured graph reads stays in place and gets the new values; another layout or
+    device has memory of its own.  Packing in inference mode makes ordinary tensors."""
+    ff = D.FeedForward(64, 64).to(BF)
+    with torch.inference_mode():
+        ff.quantize_()
+    at = [t.data_ptr() for p in ff._mx for t in p.rows.tensors()]
+    old = ff._mx[1].rows.dequantize()
+    with torch.no_grad():
+        ff.net[2].weight.mul_(-3)
+    assert not ff._mx[1].holds(ff.net[2]) and ff._mx[0].holds(ff.net[0].proj)
+    ff.quantize_()
+    assert [t.data_ptr() for p in ff._mx for t in p.rows.tensors()] == at
+    assert ff._mx[1].holds(ff.net[2])
+    want = quant.quantize_mx(ff.net[2].weight)
+    assert torch.equal(ff._mx[1].rows.dequantize(), want.dequantize()) and not torch.equal(want.dequantize(), old)
+    lin = nn.Linear(128, 32, dtype=BF)
+    D._pack_group4(lin, 32)
+    first = lin._group4.rows
+    with torch.no_grad():
+        lin.weight.neg_()
+    D._pack_group4(lin, 32)
+    assert lin._group4.rows is first and torch.equal(first.dequantize(), quant.quantize_group4(lin.weight, 32).dequantize())
+    D._pack_group4(lin, 64)
+    assert lin._group4.rows is not first and lin._group4.rows.group == 64
+
+
 def test_inference_mode_weights():
     with torch.inference_mode():
         made = _lin()
