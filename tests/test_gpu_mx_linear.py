@@ -523,20 +523,22 @@ def test_results_are_ordinary_tensors(dev):
 
 def test_no_memory_left(dev):
     """The allocator's own error, and the next call works."""
-    x = randn((1, 2048, 4096), gen(45), BF).to(dev)
-    w = quant.quantize_mx(torch.ones(65536, 4096, device=dev, dtype=BF))
-    rows = kernels.adaln_mx(x)
-    total = torch.cuda.get_device_properties(dev).total_memory
     torch.cuda.empty_cache()
-    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+    total = torch.cuda.get_device_properties(dev).total_memory
+    allowed = torch.cuda.memory_reserved() + (1 << 30)
+    M = allowed // 65536 + 1   # codes of M rows of 65536 channels alone are more than is allowed
+    w = quant.quantize_mx(torch.ones(65536, 32, device=dev, dtype=BF))
+    rows = kernels.adaln_mx(torch.ones(1, M, 32, device=dev, dtype=BF))
+    torch.cuda.set_per_process_memory_fraction(allowed / total)
     try:
-        with pytest.raises(torch.OutOfMemoryError):   # 256 MB
+        with pytest.raises(torch.OutOfMemoryError):
             kernels.mx_linear(rows, w)
-        with pytest.raises(torch.OutOfMemoryError):   # 128 MB
+        with pytest.raises(torch.OutOfMemoryError):
             kernels.mx_linear(rows, w, quantize=True)
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
-    assert kernels.mx_linear(rows, w).shape == (1, 2048, 65536)
+    few = kernels.adaln_mx(torch.ones(1, 8, 32, device=dev, dtype=BF))
+    assert kernels.mx_linear(few, w).shape == (1, 8, 65536)
 
 
 # of the tiles of 48 rows and of 32 x 64, steps short of, at and past their buffers
