@@ -49,7 +49,8 @@ class MXRows:
         K, rows = self.codes.shape[-1], self.scales.shape[1]
         s = self.scales.view(torch.uint8).transpose(0, 1).flatten(1)[:, :K // MX_BLOCK].to(torch.int32) - 127
         v = self.codes.to(torch.float32).reshape(rows, K // MX_BLOCK, MX_BLOCK)
-        return torch.ldexp(v, s.unsqueeze(-1)).reshape(self.codes.shape)
+        v = torch.ldexp(v, s.unsqueeze(-1)).masked_fill((s == 128).unsqueeze(-1), float("nan"))   # byte 255
+        return v.reshape(self.codes.shape)
 
 
 def quantize_mx(x: torch.Tensor) -> MXRows:
@@ -111,11 +112,14 @@ class Group4Weight:
         if K == 0 or scales.shape[1] == 0 or K % scales.shape[1] or K // scales.shape[1] not in GROUPS:
             raise ValueError(f"Group4Weight: {K} columns in {scales.shape[1]} groups: groups must be 32, 64 or 128 columns")
         per, chunks, tiles = 128 * scales.shape[1] // K, -(-K // 128), -(-N // 16)
-        codes = F.pad(packed, (0, chunks * 64 - K // 2, 0, tiles * 16 - N)).reshape(tiles, 16, chunks, 4, 4, 4)
+        if K % 128 or N % 16:
+            packed = F.pad(packed, (0, chunks * 64 - K // 2, 0, tiles * 16 - N))
+            scales = F.pad(scales, (0, chunks * per - scales.shape[1], 0, tiles * 16 - N))
+        codes = packed.reshape(tiles, 16, chunks, 4, 4, 4)
         # tile, row, chunk, j, p, i -> tile, chunk, p, row, j, i
         codes = codes.permute(0, 2, 4, 1, 3, 5).reshape(tiles, chunks, 4, 16, 16).contiguous()
-        scales = F.pad(scales, (0, chunks * per - scales.shape[1], 0, tiles * 16 - N)).reshape(tiles, 16, chunks, per)
-        return cls(codes, scales.transpose(1, 2).contiguous(), N, K)
+        scales = scales.reshape(tiles, 16, chunks, per).transpose(1, 2).clone(memory_format=torch.contiguous_format)
+        return cls(codes, scales, N, K)
 
     def dequantize(self) -> torch.Tensor:
         """The float32 values that the codes stand for."""

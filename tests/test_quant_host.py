@@ -125,6 +125,26 @@ def test_wrappers_refuse_on_the_host():
         _native.host().mx_linear(rows.codes)
 
 
+def test_a_scale_that_is_not_a_number():
+    """E8M0's byte 255 is NaN: so is what its block stands for, and nothing else."""
+    q = quant.quantize_mx(torch.ones(3, 96))
+    q.scales.view(torch.uint8)[0, 1, 2] = 255
+    v = q.dequantize()
+    assert v[1, 64:].isnan().all() and v.isnan().sum() == 32
+
+
+def test_packing_leaves_its_input():
+    """A weight of whole tiles is not padded: the packed tensors must still be their own."""
+    for n, group in ((16, 128), (16, 32), (32, 64)):
+        codes = torch.randint(0, 256, (n, 64), dtype=torch.uint8)
+        scales = torch.rand(n, 128 // group).to(BF)
+        w = quant.Group4Weight.from_codes(codes, scales)
+        was = w.dequantize()
+        codes.zero_()
+        scales.zero_()
+        assert torch.equal(w.dequantize(), was) and was.any()
+
+
 P = ctypes.c_void_p(4096)   # never read: each call below is refused before a launch
 BIG = 1 << 30
 
