@@ -564,3 +564,23 @@ def test_rows_of_any_alignment(dev, M, K, N, shift):
     _check_bf16(y, ref, err)
     assert (flat[:shift] == 7).all() and (flat[shift + M * (N + 5):] == 7).all()
     assert (flat[shift:shift + M * (N + 5)].view(M, N + 5)[:, N:] == 7).all()
+
+
+@pytest.mark.parametrize("M,N", [(2, 40), (33, 64), (300, 96)])
+def test_the_longest_rows(dev, M, N):
+    a, w, b, ref, err = _on_gpu(dev, M, 1 << 20, N, M, False, bias=True)
+    _check_bf16(kernels.mx_linear(a, w, b), ref, err)
+
+
+def test_no_rows_of_several_kinds(dev):
+    """Empty results of every form, and a next call that works."""
+    w = _to(quant.quantize_mx(randn((64, 96), gen(1))), dev)
+    for lead in ((0,), (0, 3), (2, 0)):
+        e = kernels.adaln_mx(torch.empty(1, 0, 96, dtype=BF, device=dev))
+        e = quant.MXRows(e.codes.view(*lead, 96), e.scales)
+        assert kernels.mx_linear(e, w).shape == (*lead, 64)
+        q = kernels.mx_linear(e, w, quantize=True, gelu=True)
+        assert q.shape == (*lead, 64) and q.scales.shape == (1, 0, 4)
+    none = quant.MXRows(w.codes[:0].contiguous(), w.scales[:, :0].contiguous())
+    assert kernels.mx_linear(w, none).shape == (64, 0)
+    assert kernels.mx_linear(w, w).isfinite().all()
