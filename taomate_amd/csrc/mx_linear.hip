@@ -565,8 +565,8 @@ void launch_mx_rows(const MxLinearArgs& p, hipStream_t st) {
 // each step of a group (`each` per 256 tiles and step instead where many tiles
 // share a CU), never below what the bytes take at 5.3 TB/s.  Over those shapes the
 // choice is within 1 % of the fastest of 19 tiles in the mean.  What each is for, the
-// next best beside it: 1 row of 16384 -> 4096 16 x 16 14.2 us (32 x 32 15.8); 8 rows of
-// 4096 -> 4096 32 x 32 6.9 (48 x 32 7.6); 75 rows of 2048 -> 8192 48 x 64 7.4 (80 x 64 8.6),
+// next best beside it: 1 row of 8256 -> 195 16 x 16 7.0 us (16 x 32, whose tiles hold the blocks
+// of an 8-bit result, and 32 x 32 9.8); 8 rows of 4096 -> 4096 32 x 32 6.9 (16 x 16 7.1); 75 rows of 2048 -> 8192 48 x 64 7.4 (80 x 64 8.6),
 // 150 rows 80 x 64 9.2 (160 x 64 10.7), of 8192 -> 2048 48 x 32 12.0 (32 x 64 14.3); 331 rows of
 // 1056 -> 4099 160 x 64 9.2 (128 x 128 11.2); 768 rows of 16384 -> 4096 128 x 128 64 (48 x 64 and
 // 80 x 64 88 and more); 384 rows of 4096 -> 16384 128 x 256 34.6 (192 x 256 36.8); 2304 rows 192 x 256
