@@ -83,7 +83,8 @@ class FeedForward(nn.Module):
         module runs in bf16.  A captured graph keeps to the packed rows: another
         ``quantize_()`` packs the weights' new values into the same memory, and
         ``quantize_(False)`` frees it, after which such a graph must not be replayed.
-        Both widths must be multiples of 32, the input's at most 8192."""
+        A weight that has come to another shape or GPU since needs ``quantize_(False)``
+        first.  Both widths must be multiples of 32, the input's at most 8192."""
         if not enabled:
             self.__dict__.pop("_mx", None)
             return self
@@ -168,8 +169,18 @@ def _row_linear(lin: nn.Module, x: torch.Tensor, act: Optional[nn.Module] = None
     return lin(x if act is None else act(x))
 
 
-def _pack_group4(lin: nn.Linear, group: int) -> None:
-    """Hold ``lin``'s weight in 4 bits beside its parameter for ``_row_linear``."""
+def _group4_rows(lin: nn.Linear) -> Optional[quant.Group4Weight]:
+    """What ``lin``'s weight was last packed into, whether or not that still holds."""
+    packed = lin.__dict__.get("_group4")
+    return None if packed is None else packed.rows
+
+
+def _pack_group4(lin: nn.Linear, group: Optional[int] = None) -> None:
+    """Hold ``lin``'s weight in 4 bits beside its parameter for ``_row_linear``, in
+    ``group`` columns a scale: without one, those of its last packing, or 32."""
+    rows = _group4_rows(lin)
+    if group is None:
+        group = 32 if rows is None else rows.group
     if not _is_plain(lin, nn.Linear) or lin.weight.dtype != torch.bfloat16:
         raise TypeError("4-bit timestep linears must be plain bf16 nn.Linear modules")
     if lin.in_features > _native.GROUP4_MAX_COLUMNS:
@@ -651,16 +662,23 @@ class AVModel(nn.Module):
                 m.fuse_qkv_()
         return self
 
-    def quantize_linears_(self, feed_forward: bool = True, timestep: bool = False, group: int = 32) -> "AVModel":
+    def quantize_linears_(self, feed_forward: bool = True, timestep: Optional[bool] = None,
+                          group: Optional[int] = None) -> "AVModel":
         """Hold weights in fewer bits beside the bf16 parameters, whose names and
         values stay: every block's video and audio feed-forward in 8 bits
         (``FeedForward.quantize_``), and with ``timestep`` the linears of the
         timestep embeddings and modulations in 4 bits with a bf16 scale for every
-        ``group`` columns, for calls of up to 16 rows (one per sample or frame;
-        more rows run in bf16).  False ends either.  Load the weights and move the
-        model before; a weight that is changed, moved or replaced afterwards runs
-        in bf16 again until the next call; so does a deep copy or pickle of the
-        model.  What holds of captured graphs is at ``FeedForward.quantize_``.
+        ``group`` columns (32), for calls of up to 16 rows (one per sample or frame;
+        more rows run in bf16).  Load the weights and move the model before; a weight
+        that is changed, moved or replaced afterwards runs in bf16 again until the
+        next call; so does a deep copy or pickle of the model.
+
+        A captured graph reads the packed rows.  The next call packs all that was
+        packed into the same memory, the 4-bit rows too where ``timestep`` is not
+        given; only False frees rows: ``quantize_linears_(timestep=False)`` the 4-bit
+        ones, ``quantize_linears_(False)`` all of them (with ``timestep=True`` only
+        the 8-bit ones).  Another ``group`` for linears that are packed is refused
+        until they are dropped.
 
         Measured on random weights at the 512x768 chunk, 48 blocks: the feed-forwards
         take a step from 82.0 to 70.5 ms, its outputs to a cosine of 0.995 with
@@ -672,7 +690,7 @@ class AVModel(nn.Module):
                 m.quantize_(feed_forward)
             elif isinstance(m, (TimestepEmbedding, AdaLayerNormSingle)):
                 for lin in (m.linear_1, m.linear_2) if isinstance(m, TimestepEmbedding) else (m.linear,):
-                    if timestep:
+                    if timestep or timestep is None and feed_forward and _group4_rows(lin) is not None:
                         _pack_group4(lin, group)
                     else:
                         lin.__dict__.pop("_group4", None)

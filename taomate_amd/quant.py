@@ -161,9 +161,10 @@ class Packed:
     tells whether ``lin.weight`` is still the parameter, in the memory and at the
     version, that was packed (a change through ``.data`` in place goes unseen).
     Keeps the packed memory alive, so that nothing else can come to lie there.
-    ``into``: an earlier packing whose rows are overwritten where they have the
-    same layout, so that captured graphs read the new ones.  A deep copy or pickle
-    carries no rows and never holds: versions count anew there."""
+    ``into``: an earlier packing whose rows are overwritten, so that captured graphs
+    read the new ones.  Rows on a GPU that have another layout (shape, group or
+    device) are refused instead of being freed under such a graph.  A deep copy or
+    pickle carries no rows and never holds: versions count anew there."""
     __slots__ = ("rows", "weight", "source", "version")
 
     def __init__(self, lin: torch.nn.Linear, rows, into: "Packed | None" = None):
@@ -175,6 +176,9 @@ class Packed:
             for a, b in zip(old.tensors(), rows.tensors()):
                 a.view(torch.uint8).copy_(b.view(torch.uint8))
             rows = old
+        elif old is not None and old.device.type == "cuda":
+            raise ValueError(f"packed rows {tuple(old.shape)} on {old.device} have another layout, and a captured graph "
+                             "may read them: drop them first (False)")
         self.rows = rows
         self.weight = lin.weight
         self.source = lin.weight.detach()

@@ -168,3 +168,36 @@ def test_a_captured_feed_forward_follows_packing_again(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, second) and not torch.equal(second, first) and len(junk) == 14
+
+
+def test_captured_timestep_linears_follow_packing_again(dev):
+    """``quantize_linears_()`` as documented after new weights: replays read the new 4-bit rows,
+    whatever has been allocated since."""
+    m = D.build_model(CFG, dev, seed=3).quantize_linears_(timestep=True, group=64)
+    emb = m.adaln_single.emb.timestep_embedder
+    x = randn((2, 256), gen(5), BF).to(dev)
+    with torch.no_grad():
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            emb(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            held = emb(x)
+        first = emb(x).clone()
+        for factor in (-2.0, 0.5):
+            emb.linear_2.weight.mul_(factor)
+            m.quantize_linears_()
+            junk = [torch.full((1 << n,), 255, dtype=torch.uint8, device=dev) for n in range(6, 20)]
+            now = emb(x)
+            assert emb.linear_2._group4.holds(emb.linear_2) and not torch.equal(now, first) and len(junk) == 14
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, now)
+        with pytest.raises(ValueError, match="another layout"):
+            m.quantize_linears_(timestep=True, group=32)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, now)
+        assert m.quantize_linears_(timestep=False).quantize_linears_(timestep=True, group=32) is m

@@ -170,3 +170,60 @@ def test_what_cannot_be_quantised_is_refused():
         D._pack_group4(nn.Linear(4224, 8, dtype=BF), 32)
     with pytest.raises(ValueError, match="multiple of 128"):
         D._pack_group4(nn.Linear(64, 8, dtype=BF), 128)
+
+
+def _packed_at(m):
+    return {n: [t.data_ptr() for t in lin._group4.rows.tensors()] for n, lin in m.named_modules() if "_group4" in lin.__dict__}
+
+
+def test_quantising_again_frees_no_rows():
+    """A captured graph reads the packed rows: the documented call after new weights packs all of
+    them into the same memory, the 4-bit ones too, in the group that they have."""
+    m = D.build_model(CFG, "cpu", seed=1).quantize_linears_(timestep=True, group=64)
+    at, lin = _packed_at(m), m.adaln_single.linear
+    rows = [r for x in m.modules() if isinstance(x, D.FeedForward) for p in x._mx for r in p.rows.tensors()]
+    assert len(at) == 18
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(2)
+    assert not lin._group4.holds(lin)
+    m.quantize_linears_()
+    assert _packed_at(m) == at and lin._group4.holds(lin) and lin._group4.rows.group == 64
+    assert torch.equal(lin._group4.rows.dequantize(), quant.quantize_group4(lin.weight, 64).dequantize())
+    again = [r for x in m.modules() if isinstance(x, D.FeedForward) for p in x._mx for r in p.rows.tensors()]
+    assert all(a is b for a, b in zip(rows, again))
+    # a model without 4-bit linears gets none, a copy's are gone with its own first packing
+    assert not _packed_at(D.build_model(CFG, "cpu", seed=1).quantize_linears_())
+    c = copy.deepcopy(m).quantize_linears_()
+    assert not _packed_at(c) and c.transformer_blocks[0].ff._mx[0].holds(c.transformer_blocks[0].ff.net[0].proj)
+    # only False ends them
+    m.quantize_linears_(timestep=False)
+    assert not _packed_at(m) and "_mx" in m.transformer_blocks[0].ff.__dict__
+    m.quantize_linears_(timestep=True)
+    assert lin._group4.rows.group == 32
+    m.quantize_linears_(False)
+    assert not _packed_at(m) and "_mx" not in m.transformer_blocks[0].ff.__dict__
+
+
+class _Elsewhere:
+    """Rows as on a GPU, which a graph there may read."""
+    def __init__(self, rows):
+        self.rows = rows
+
+    def __getattr__(self, name):
+        return getattr(self.rows, name)
+
+    @property
+    def device(self):
+        return torch.device("cuda:0")
+
+
+def test_another_layout_does_not_replace_rows_on_a_gpu():
+    lin = _lin()
+    packed = quant.Packed(lin, quant.quantize_group4(lin.weight, 32))
+    held = packed.rows = _Elsewhere(packed.rows)
+    with pytest.raises(ValueError, match="another layout"):
+        quant.Packed(lin, quant.quantize_group4(lin.weight, 64), packed)
+    assert packed.rows is held
+    same = quant.Packed(lin, quant.quantize_group4(lin.weight, 32), packed)
+    assert same.rows is held
