@@ -165,7 +165,7 @@ class Packed:
     read the new ones.  Rows on a GPU that have another layout (shape, group or
     device) are refused instead of being freed under such a graph.  A deep copy or
     pickle carries no rows and never holds: versions count anew there."""
-    __slots__ = ("rows", "weight", "source", "version")
+    __slots__ = ("rows", "weight", "source", "at", "version")
 
     def __init__(self, lin: torch.nn.Linear, rows, into: "Packed | None" = None):
         if lin.weight.is_inference():
@@ -182,12 +182,13 @@ class Packed:
         self.rows = rows
         self.weight = lin.weight
         self.source = lin.weight.detach()
+        self.at = self.source.data_ptr()   # source itself follows a storage that is allocated anew
         self.version = lin.weight._version
 
     @classmethod
     def _lapsed(cls) -> "Packed":
         p = cls.__new__(cls)
-        p.rows = p.weight = p.source = p.version = None
+        p.rows = p.weight = p.source = p.at = p.version = None
         return p
 
     def __reduce__(self):
@@ -195,5 +196,5 @@ class Packed:
 
     def holds(self, lin: torch.nn.Linear) -> bool:
         w = lin._parameters.get("weight")
-        return (w is not None and w is self.weight and w.data_ptr() == self.source.data_ptr() and w._version == self.version
+        return (w is not None and w is self.weight and w.data_ptr() == self.at and w._version == self.version
                 and w.shape == self.source.shape and w.dtype == self.source.dtype and w.device == self.source.device)

@@ -227,3 +227,17 @@ def test_another_layout_does_not_replace_rows_on_a_gpu():
     assert packed.rows is held
     same = quant.Packed(lin, quant.quantize_group4(lin.weight, 32), packed)
     assert same.rows is held
+
+
+def test_a_weight_whose_memory_was_exchanged_ends_the_packing():
+    """Its storage freed and allocated again elsewhere, as sharded parameters are."""
+    lin = _lin()
+    packed = quant.Packed(lin, quant.quantize_mx(lin.weight))
+    store, at = lin.weight.untyped_storage(), lin.weight.data_ptr()
+    size = store.nbytes()
+    store.resize_(0)
+    assert not packed.holds(lin)
+    others = [torch.empty(size, dtype=torch.uint8) for _ in range(8)]   # the old place is taken
+    store.resize_(size)
+    if any(t.data_ptr() == at for t in others):
+        assert lin.weight.data_ptr() != at and not packed.holds(lin)
