@@ -64,7 +64,24 @@ class GELUApprox(nn.Module):
         return F.gelu(self.proj(x), approximate="tanh")
 
 
-class FeedForward(nn.Module):
+class _Packs(nn.Module):
+    """A module that holds packed weights, its own (``_mx``) or its linears'
+    (``_group4``).  What moves or casts it lets go of the old weights at once."""
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        linears = [m for m in self.modules() if isinstance(m, nn.Linear)]
+        for p in self.__dict__.get("_mx", ()):
+            if not any(p.holds(m) for m in linears):
+                p.lapse()
+        for m in linears:
+            p = m.__dict__.get("_group4")
+            if p is not None and not p.holds(m):
+                p.lapse()
+        return self
+
+
+class FeedForward(_Packs):
     """compat.py:46-71: Linear -> tanh-GELU -> Linear, inner width mult * dim."""
 
     def __init__(self, dim: int, dim_out: int, mult: int = 4):
@@ -79,8 +96,12 @@ class FeedForward(nn.Module):
         and by the first linear's epilogue.  Call it on the device it is to run
         on.  Anything that changes, moves or replaces a weight afterwards ends it
         and the bf16 linears run again; so do calls that something else would see
-        (gradients, autocast, hooks, compilation).  A deep copy or pickle of the
-        module runs in bf16.  A captured graph keeps to the packed rows: another
+        (gradients, autocast, hooks, compilation).  The old
+        weight's memory is let go by ``to`` and the like, or by the first call after
+        the change, which ends the packing for good; the packed rows stay until
+        ``quantize_(False)``.  A change in place through ``.data`` goes unseen: call
+        ``quantize_()`` again after one.  A deep copy or pickle of the module runs in
+        bf16.  A captured graph keeps to the packed rows: another
         ``quantize_()`` packs the weights' new values into the same memory, and
         ``quantize_(False)`` frees it, after which such a graph must not be replayed.
         A weight that has come to another shape or GPU since needs ``quantize_(False)``
@@ -110,7 +131,11 @@ class FeedForward(nn.Module):
                 and _is_plain(act, GELUApprox) and _is_plain(act.proj, nn.Linear) and _is_plain(mid, nn.Identity)
                 and _is_plain(down, nn.Linear) and _is_eager()):
             return False
-        return mx[0].holds(act.proj) and mx[1].holds(down) and act.proj.weight.is_cuda
+        if mx[0].holds(act.proj) and mx[1].holds(down):
+            return act.proj.weight.is_cuda
+        for p in mx:
+            p.lapse()
+        return False
 
     def forward_rows(self, rows: quant.MXRows) -> torch.Tensor:
         """The feed-forward of 8-bit rows (``quantized()`` must hold)."""
@@ -119,7 +144,7 @@ class FeedForward(nn.Module):
         return kernels.mx_linear(h, down.rows, self.net[2].bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.is_cuda and x.dtype == torch.bfloat16 and "_mx" in self.__dict__ and self.quantized():
+        if "_mx" in self.__dict__ and self.quantized() and x.is_cuda and x.dtype == torch.bfloat16:
             rows = x.reshape(1, -1, x.shape[-1]).contiguous()
             if rows.data_ptr() % 16:
                 rows = rows.clone()
@@ -156,14 +181,16 @@ def _row_linear(lin: nn.Module, x: torch.Tensor, act: Optional[nn.Module] = None
     """``lin(act(x))`` for a few rows (one per sample or frame): a plain bf16
     nn.Linear in plain eager mode reads its weight once (ltx_skinny_linear);
     anything else runs as modules."""
+    packed = lin.__dict__.get("_group4")
+    if packed is not None and _is_eager() and not packed.holds(lin):   # a trace's stand-in for the weight ends nothing
+        packed.lapse()
+        packed = None
     if (x.is_cuda and _is_plain(lin, nn.Linear) and (act is None or _is_plain(act, nn.SiLU) and not act.inplace)
             and _is_eager()):
         w, b = lin.weight, lin.bias
-        packed = lin.__dict__.get("_group4")
         if packed is not None and x.dim() == 2 and x.shape[0] <= _native.GROUP4_MAX_ROWS and x.dtype == torch.bfloat16:
-            if packed.holds(lin):
-                x = x.contiguous()
-                return kernels.group4_linear(x.clone() if x.data_ptr() % 16 else x, packed.rows, b, silu=act is not None)
+            x = x.contiguous()
+            return kernels.group4_linear(x.clone() if x.data_ptr() % 16 else x, packed.rows, b, silu=act is not None)
         if _native._host.row_operands(x, w, b):
             return kernels.skinny_linear(x, w, b, silu=act is not None)
     return lin(x if act is None else act(x))
@@ -190,7 +217,7 @@ def _pack_group4(lin: nn.Linear, group: Optional[int] = None) -> None:
         lin._group4 = quant.Packed(lin, quant.quantize_group4(lin.weight, group), lin.__dict__.get("_group4"))
 
 
-class TimestepEmbedding(nn.Module):
+class TimestepEmbedding(_Packs):
     def __init__(self, in_channels: int, dim: int):
         super().__init__()
         self.linear_1 = nn.Linear(in_channels, dim)
@@ -210,7 +237,7 @@ class _CombinedEmbedding(nn.Module):
         return self.timestep_embedder(timestep_embedding(t).to(dtype))
 
 
-class AdaLayerNormSingle(nn.Module):
+class AdaLayerNormSingle(_Packs):
     """compat.py:212-275: timestep -> (coefficient * dim modulation, dim embedding)."""
 
     def __init__(self, dim: int, coefficient: int = 6):
@@ -671,7 +698,9 @@ class AVModel(nn.Module):
         ``group`` columns (32), for calls of up to 16 rows (one per sample or frame;
         more rows run in bf16).  Load the weights and move the model before; a weight
         that is changed, moved or replaced afterwards runs in bf16 again until the
-        next call; so does a deep copy or pickle of the model.
+        next call; so does a deep copy or pickle of the model.  The packed weights
+        come on top of the bf16 ones: half as much again for a feed-forward, between
+        a quarter and a third for a timestep linear.
 
         A captured graph reads the packed rows.  The next call packs all that was
         packed into the same memory, the 4-bit rows too where ``timestep`` is not

@@ -160,7 +160,9 @@ class Packed:
     """What a linear's weight was packed into, as long as it holds: ``holds(lin)``
     tells whether ``lin.weight`` is still the parameter, in the memory and at the
     version, that was packed (a change through ``.data`` in place goes unseen).
-    Keeps the packed memory alive, so that nothing else can come to lie there.
+    Keeps the memory of the weight alive, so that nothing else can come to lie there,
+    until ``lapse``: the caller's, once the packing holds no more.  The rows stay for
+    captured graphs, and the packing never holds again.
     ``into``: an earlier packing whose rows are overwritten, so that captured graphs
     read the new ones.  Rows on a GPU that have another layout (shape, group or
     device) are refused instead of being freed under such a graph.  A deep copy or
@@ -184,6 +186,9 @@ class Packed:
         self.source = lin.weight.detach()
         self.at = self.source.data_ptr()   # source itself follows a storage that is allocated anew
         self.version = lin.weight._version
+
+    def lapse(self) -> None:
+        self.weight = self.source = None
 
     @classmethod
     def _lapsed(cls) -> "Packed":

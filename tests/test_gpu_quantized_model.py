@@ -201,3 +201,16 @@ def test_captured_timestep_linears_follow_packing_again(dev):
         torch.cuda.synchronize()
         assert torch.equal(held, now)
         assert m.quantize_linears_(timestep=False).quantize_linears_(timestep=True, group=32) is m
+
+
+def test_a_moved_feed_forward_frees_its_weights(dev):
+    ff = D.FeedForward(512, 512).to(dev, BF)
+    weights = sum(m.weight.untyped_storage().nbytes() for m in (ff.net[0].proj, ff.net[2]))
+    torch.cuda.synchronize()
+    ff.quantize_()
+    before = torch.cuda.memory_allocated()
+    ff.to("cpu")
+    assert before - torch.cuda.memory_allocated() >= weights
+    before = torch.cuda.memory_allocated()
+    ff.quantize_(False)
+    assert before - torch.cuda.memory_allocated() >= weights // 2   # the 8-bit rows

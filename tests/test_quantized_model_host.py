@@ -6,6 +6,7 @@ import pickle
 import pytest
 import torch
 import torch.nn as nn
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from taomate_amd import dit as D
 from taomate_amd import quant
@@ -241,3 +242,78 @@ def test_a_weight_whose_memory_was_exchanged_ends_the_packing():
     store.resize_(size)
     if any(t.data_ptr() == at for t in others):
         assert lin.weight.data_ptr() != at and not packed.holds(lin)
+
+
+def _memory(t):
+    """A weak reference to a tensor's memory; ``expired()`` once it is freed."""
+    return StorageWeakRef(t.untyped_storage())
+
+
+@pytest.mark.parametrize("change", [_replace, _assign, _data], ids=["parameter", "state dict", "data"])
+def test_replaced_weights_are_let_go(change):
+    """The first call after a change sees that the packing lapsed and lets go of the old weights;
+    the rows, which a captured graph may read, stay until they are dropped."""
+    ff = D.FeedForward(64, 64).to(BF).quantize_()
+    lins = (ff.net[0].proj, ff.net[2])
+    old, rows = [_memory(m.weight) for m in lins], [_memory(t) for p in ff._mx for t in p.rows.tensors()]
+    for m in lins:
+        change(m)
+    with torch.no_grad():
+        ff(torch.zeros(2, 64, dtype=BF))
+        assert not ff.quantized() and all(m.expired() for m in old) and not any(r.expired() for r in rows)
+        assert not any(p.holds(m) for p, m in zip(ff._mx, lins))
+        ff.quantize_()
+        assert all(p.holds(m) for p, m in zip(ff._mx, lins)) and not any(r.expired() for r in rows)
+    ff.quantize_(False)
+    assert all(r.expired() for r in rows)
+
+
+def test_one_replaced_weight_lets_go_of_both():
+    ff = D.FeedForward(64, 64).to(BF).quantize_()
+    old = _memory(ff.net[0].proj.weight)
+    _replace(ff.net[0].proj)
+    with torch.no_grad():
+        ff(torch.zeros(2, 64, dtype=BF))
+    assert old.expired() and not ff._mx[1].holds(ff.net[2])
+
+
+@pytest.mark.parametrize("part", ["model", "block", "feed-forward", "adaln"])
+def test_moved_weights_are_let_go_at_once(part):
+    """A model that is cast or moved keeps none of its old weights, whether or not it is called again."""
+    m = D.build_model(CFG, "cpu", seed=1).quantize_linears_(timestep=True)
+    block = m.transformer_blocks[0]
+    of = {"model": m, "block": block, "feed-forward": block.ff, "adaln": m.adaln_single}[part]
+    old = [_memory(p) for p in of.parameters()]
+    of.to(torch.float32)
+    assert len(old) >= 4 and all(r.expired() for r in old)
+    of.to(BF)
+    with torch.no_grad():
+        assert not block.ff.quantized() or part == "adaln"
+    m.quantize_linears_()
+    assert m.adaln_single.linear._group4.holds(m.adaln_single.linear) and block.ff._mx[0].holds(block.ff.net[0].proj)
+
+
+def test_replaced_timestep_weights_are_let_go():
+    m = D.build_model(CFG, "cpu", seed=1).quantize_linears_(timestep=True)
+    lins = [m.adaln_single.linear, m.adaln_single.emb.timestep_embedder.linear_1]
+    old = [_memory(x.weight) for x in lins]
+    for x in lins:
+        _replace(x)
+    with torch.no_grad():
+        m.adaln_single(torch.zeros(17), BF)
+    assert all(r.expired() for r in old)
+
+
+def test_a_trace_does_not_end_the_packing():
+    """Calls that see stand-ins for the weights run the modules and leave the packing as it is."""
+    m = D.build_model(CFG, "cpu", seed=1).quantize_linears_(timestep=True)
+    emb, ff = m.adaln_single.emb.timestep_embedder, m.transformer_blocks[0].ff
+    x, y = torch.zeros(2, 256, dtype=BF), torch.zeros(2, 128, dtype=BF)
+    for mod, arg in ((emb, x), (ff, y)):
+        other = {k: v.detach().clone() for k, v in mod.named_parameters()}
+        torch.func.functional_call(mod, other, (arg,))      # gradients are on
+        torch.export.export(mod, (arg,), strict=False)
+        with torch.no_grad():
+            mod(arg)
+    assert emb.linear_1._group4.holds(emb.linear_1) and emb.linear_2._group4.holds(emb.linear_2)
+    assert ff._mx[0].holds(ff.net[0].proj) and ff._mx[1].holds(ff.net[2])
