@@ -358,8 +358,8 @@ int ltx_adaln(int64_t B, int64_t L, int64_t C, const void* x, int64_t x_bs, int6
  * e4m3 under the block's scale: the smallest power of two, at least 2^-127,
  * with which no finite value of the block passes 448.  A value that is not
  * finite becomes NaN and does not count in its block's maximum.
- *   Arguments as ltx_adaln (x_out may equal x or y; fewer than 2^23 rows a
- *   sample).  eps < 0 skips the norm (and takes no scale / shift): the rows x'
+ *   Arguments as ltx_adaln (x_out may equal x or y, its rows must not overlap;
+ *   fewer than 2^23 rows a sample).  eps < 0 skips the norm (and takes no scale / shift): the rows x'
  *   themselves.  C a multiple of 32, at most 8192.
  *   codes: [B * L, C] bytes, 16-byte aligned; scales: [ceil(C / 128)][B * L][4]
  *   bytes, 4-byte aligned.

@@ -155,7 +155,12 @@ extern "C" int ltx_adaln_mx(int64_t B, int64_t L, int64_t C, const void* x, int6
   LTX_REQUIRE((scale == nullptr) == (shift == nullptr), "ltx_adaln_mx: scale and shift go together");
   LTX_REQUIRE(scale == nullptr || eps >= 0.0f, "ltx_adaln_mx: modulation needs the norm");
   LTX_REQUIRE(x_out == nullptr || y != nullptr, "ltx_adaln_mx: x_out without a residual branch");
-  LTX_REQUIRE(x_out == nullptr || ((L == 1 || xo_ls >= C) && (B == 1 || xo_bs >= C)), "ltx_adaln_mx: rows of x_out overlap");
+  // one sample after the other, or one token's samples after the other's
+  const auto apart = [&](int64_t n, int64_t step) { return n == 1 || step >= C; };
+  const auto nested = [&](int64_t n, int64_t inner, int64_t outer) { return (outer - C) / (n - 1) >= inner; };
+  LTX_REQUIRE(x_out == nullptr || (apart(L, xo_ls) && apart(B, xo_bs) &&
+                                   (L == 1 || B == 1 || nested(L, xo_ls, xo_bs) || nested(B, xo_bs, xo_ls))),
+              "ltx_adaln_mx: rows of x_out overlap");
   auto ok = [](const void* p, int64_t bs, int64_t ls) {
     return p == nullptr || (((uintptr_t)p % 16) == 0 && bs % 8 == 0 && ls % 8 == 0);
   };

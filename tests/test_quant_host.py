@@ -189,3 +189,23 @@ def _group4_linear(M, N, K, group=32, y_ls=None, x_ls=None, x=P):
 def test_entry_points_refuse(match, call):
     with pytest.raises(_native.NativeCallError, match=match):
         call()
+
+
+@pytest.mark.parametrize("B,L,C,bs,ls", [(2, 2, 64, 64, 64), (2, 3, 64, 128, 64), (2, 3, 64, 184, 64), (3, 2, 64, 64, 128),
+                                         (3, 2, 64, 64, 184), (2, 2, 64, 96, 64), (4, 4, 32, 64, 64)])
+def test_rows_of_x_out_that_overlap_across_samples(B, L, C, bs, ls):
+    """Two workgroups would store to one address."""
+    at = sorted(b * bs + l * ls for b in range(B) for l in range(L))
+    assert any(q - p < C for p, q in zip(at, at[1:]))
+    with pytest.raises(_native.NativeCallError, match="rows of x_out overlap"):
+        _adaln_mx(B, L, C, P, (bs, ls))
+
+
+@pytest.mark.parametrize("B,L,C,bs,ls", [(2, 3, 64, 192, 64), (2, 3, 64, 64, 128), (2, 3, 64, 72, 136), (1, 3, 64, 0, 64),
+                                         (3, 1, 64, 64, 0), (1, 1, 64, 0, 0), (2, 2, 64, 1 << 60, 64)])
+def test_rows_of_x_out_side_by_side(B, L, C, bs, ls):
+    """Refused for the alignment of its x only, which is looked at last."""
+    odd = ctypes.c_void_p(4104)
+    with pytest.raises(_native.NativeCallError, match="16-byte aligned"):
+        _native.call("ltx_adaln_mx", B, L, C, odd, L * C, C, P, L * C, C, None, 0, 0, P, bs, ls, None, 0, 0, None, 0, 0, 1e-6,
+                     P, P, None)
