@@ -531,8 +531,16 @@ void skinny_linear(PyObject* const* a) {
 }
 
 // -------------------------------------------------------- block-scaled linears
-// These calls run on their tensors' device, whichever is current.
+// These calls run on their tensors' device, whichever is current.  Their results are
+// new tensors without a history, so inputs that want gradients are refused.
 void same_device(const char* what, const at::Tensor& first, std::initializer_list<Opt> others) {
+  const bool grad = at::GradMode::is_enabled();
+  const auto wants = [&](Opt t) { return t != nullptr && ((grad && t->requires_grad()) || t->_fw_grad(0).defined()); };
+  bool any = wants(&first);
+  for (Opt t : others) any |= wants(t);
+  if (any)
+    throw Refused{PyExc_RuntimeError, std::string(what) + " computes no gradients, and a tensor that it was given wants them: "
+                                                          "call it under torch.no_grad() or on detached tensors"};
   need_gpu(&first);
   for (Opt t : others) {
     need_gpu(t);

@@ -183,7 +183,8 @@ def adaln_mx(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[t
     ``mx_linear``; x_out = x + y * gate in bf16 (x_out may be x or y).  float32
     between its inputs and outputs (``adaln`` rounds to bf16 where the
     reference's ops do).  eps None skips the norm: the rows themselves.  C a
-    multiple of 32, at most 8192; fewer than 2^23 rows a sample."""
+    multiple of 32, at most 8192; fewer than 2^23 rows a sample.  Computes no
+    gradients: refuses tensors that want them, as the two below do."""
     return MXRows(*(N._host or N.host()).adaln_mx(x, y, gate, x_out, scale, shift, eps))
 
 
@@ -192,7 +193,8 @@ def mx_linear(a: MXRows, weight: MXRows, bias: Optional[torch.Tensor] = None, ge
     """ltx_mx_linear: act(a @ weight.T + bias) for 8-bit rows ``a`` [..., K]
     and an 8-bit ``weight`` [N, K]; bias bf16 [N]; tanh-GELU with ``gelu``.
     Returns bf16 [..., N], or 8-bit rows with ``quantize`` (N a multiple of 32).
-    ``out``: bf16 [rows, N] with contiguous channels to write instead of a new tensor."""
+    ``out``: bf16 [rows, N] with contiguous channels to write instead of a new tensor.
+    Computes no gradients."""
     y = (N._host or N.host()).mx_linear(a.codes, a.scales, weight.codes, weight.scales, bias, gelu, quantize, out)
     return MXRows(*y) if quantize else y
 
@@ -200,5 +202,5 @@ def mx_linear(a: MXRows, weight: MXRows, bias: Optional[torch.Tensor] = None, ge
 def group4_linear(x: torch.Tensor, weight: Group4Weight, bias: Optional[torch.Tensor] = None,
                   silu: bool = False) -> torch.Tensor:
     """ltx_group4_linear: act(x) @ W.T + bias for x [M <= 16, K <= 4096] bf16
-    (SiLU of x first with ``silu``) and a 4-bit weight."""
+    (SiLU of x first with ``silu``) and a 4-bit weight.  Computes no gradients."""
     return (N._host or N.host()).group4_linear(x, weight.codes, weight.scales, bias, silu, weight.rows, weight.columns)

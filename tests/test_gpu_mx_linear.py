@@ -584,3 +584,16 @@ def test_no_rows_of_several_kinds(dev):
     none = quant.MXRows(w.codes[:0].contiguous(), w.scales[:, :0].contiguous())
     assert kernels.mx_linear(w, none).shape == (64, 0)
     assert kernels.mx_linear(w, w).isfinite().all()
+
+
+def test_gradients_are_refused(dev):
+    a, w, b = (t.to(dev) if isinstance(t, torch.Tensor) else _to(t, dev) for t in _linear_case(4, 64, 32, 5))
+    bias = torch.nn.Parameter(b)
+    for quantize in (False, True):
+        with pytest.raises(RuntimeError, match="mx_linear computes no gradients"):
+            kernels.mx_linear(a, w, bias, quantize=quantize)
+    with torch.no_grad():
+        y = kernels.mx_linear(a, w, bias)
+    assert torch.equal(y, kernels.mx_linear(a, w, bias.detach())) and not y.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(kernels.mx_linear(a, w, bias), y)

@@ -209,3 +209,30 @@ def test_rows_of_x_out_side_by_side(B, L, C, bs, ls):
     with pytest.raises(_native.NativeCallError, match="16-byte aligned"):
         _native.call("ltx_adaln_mx", B, L, C, odd, L * C, C, P, L * C, C, None, 0, 0, P, bs, ls, None, 0, 0, None, 0, 0, 1e-6,
                      P, P, None)
+
+
+def _calls_that_want_gradients(x, make):
+    """Each public call with one tensor of each kind made by ``make``."""
+    rows, w4 = quant.quantize_mx(torch.zeros(4, 64)), quant.quantize_group4(torch.zeros(8, 64))
+    bias, big = torch.zeros(8, dtype=BF), x.new_zeros(4, 4)
+    return [lambda: kernels.adaln_mx(make(x)), lambda: kernels.adaln_mx(x, y=make(x)),
+            lambda: kernels.adaln_mx(x, y=x, gate=make(x)), lambda: kernels.adaln_mx(x, y=x, x_out=make(x)),
+            lambda: kernels.adaln_mx(x, scale=make(x), shift=x), lambda: kernels.adaln_mx(x, scale=x, shift=make(x)),
+            lambda: kernels.mx_linear(rows, rows, make(bias[:4])), lambda: kernels.mx_linear(rows, rows, out=make(big)),
+            lambda: kernels.group4_linear(make(x[0]), w4), lambda: kernels.group4_linear(x[0], w4, make(bias))]
+
+
+def test_tensors_that_want_gradients_are_refused():
+    """The results have no history: a gradient would be lost without a word."""
+    x = torch.zeros(1, 4, 64, dtype=BF)
+    calls = _calls_that_want_gradients(x, lambda t: t.clone().requires_grad_())
+    for call in calls:
+        with pytest.raises(RuntimeError, match="computes no gradients"):
+            call()
+    for call in calls:
+        with torch.no_grad(), pytest.raises(ValueError, match="device tensors"):
+            call()
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        for call in _calls_that_want_gradients(x, lambda t: torch.autograd.forward_ad.make_dual(t, t)):
+            with pytest.raises(RuntimeError, match="computes no gradients"):
+                call()
