@@ -16,6 +16,7 @@
 #include <ATen/EmptyTensor.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
+#include <ATen/ops/empty_ops.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -572,7 +573,12 @@ MxRows mx_rows(const char* what, const at::Tensor& codes, const at::Tensor& scal
 // the current device (a guard's), from the allocator that at::empty takes.
 const c10::DispatchKeySet kPlain{c10::DispatchKey::CUDA};
 c10::Allocator* device_memory() {
-  static c10::Allocator* const memory = at::empty({1}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA)).storage().allocator();
+  // the backend's own at::empty: a mode that is on (fake tensors, a trace) would hand out another allocator
+  static c10::Allocator* const memory =
+      at::_ops::empty_memory_format::redispatch(kPlain, c10::SymIntArrayRef(c10::SymInt(1)), at::kByte, std::nullopt,
+                                                at::Device(at::kCUDA), std::nullopt, std::nullopt)
+          .storage()
+          .allocator();
   return memory;
 }
 

@@ -1,5 +1,9 @@
 """The 8-bit rows and block-scaled linears against float64: the residual + norm
 that writes 8-bit rows, and the linear that reads and writes them."""
+import pathlib
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -597,3 +601,26 @@ def test_gradients_are_refused(dev):
     assert torch.equal(y, kernels.mx_linear(a, w, bias.detach())) and not y.requires_grad
     with torch.inference_mode():
         assert torch.equal(kernels.mx_linear(a, w, bias), y)
+
+
+_FIRST_CALL_UNDER_A_MODE = """
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from taomate_amd import kernels
+x = torch.ones(1, 2, 32, dtype=torch.bfloat16, device="cuda")
+with FakeTensorMode(allow_non_fake_inputs=True):
+    first = kernels.adaln_mx(x)
+n = kernels.adaln_mx(x)
+for rows in (first, n):
+    assert type(rows.codes) is torch.Tensor and rows.codes.is_cuda and rows.codes.data_ptr() != 0
+    assert (rows.dequantize() == 1).all()
+print("right")
+"""
+
+
+def test_a_first_call_while_a_mode_is_on(dev):
+    """The results' allocator is looked up once: not through a mode, whose tensors have another."""
+    root = pathlib.Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", _FIRST_CALL_UNDER_A_MODE], cwd=root, capture_output=True, text=True,
+                          timeout=100)
+    assert done.returncode == 0 and "right" in done.stdout, done.stderr[-2000:]
