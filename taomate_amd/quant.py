@@ -145,7 +145,7 @@ def quantize_group4(weight: torch.Tensor, group: int = 32) -> Group4Weight:
     if not bool(w.isfinite().all()):
         raise ValueError("quantize_group4: the weight holds values that are not finite (4-bit codes have none)")
     scales = (w.abs().amax(-1) / E2M1_MAX).to(torch.bfloat16)
-    t = w.abs() / scales.to(torch.float32).clamp_min(torch.finfo(torch.float32).tiny).unsqueeze(-1)
+    t = w.abs() / scales.to(torch.float32).clamp_min(2.0 ** -133).unsqueeze(-1)   # bf16's smallest
     grid = torch.tensor(_E2M1, device=w.device)
     mid = (grid[1:] + grid[:-1]) / 2
     # below or on a midpoint: the lower code; on one whose lower code is odd: the upper

@@ -236,3 +236,16 @@ def test_tensors_that_want_gradients_are_refused():
         for call in _calls_that_want_gradients(x, lambda t: torch.autograd.forward_ad.make_dual(t, t)):
             with pytest.raises(RuntimeError, match="computes no gradients"):
                 call()
+
+
+@pytest.mark.parametrize("top", [6e-38, 6e-39, 3e-40, 2.0 ** -133, 2.0 ** -149, 1.2e-38])
+def test_4bit_weights_near_the_smallest_scales(top):
+    """Scales below 2^-126, which bf16 holds to 2^-133: each value is still the nearest."""
+    w = (torch.linspace(-1, 1, 32, dtype=torch.float64) * top).to(torch.float32)[None]
+    q = quant.quantize_group4(w)
+    s = (w.abs().amax() / 6).to(BF)
+    assert q.scales[0, 0, 0, 0] == s
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+    best = (w.double().abs()[..., None] - s.double() * grid).abs().amin(-1)
+    # the value that a code stands for is a product in float32, to half of 2^-149
+    assert ((q.dequantize().double() - w.double()).abs() <= best + 2.0 ** -150).all()
