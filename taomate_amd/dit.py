@@ -105,7 +105,8 @@ class FeedForward(_Packs):
         ``quantize_()`` packs the weights' new values into the same memory, and
         ``quantize_(False)`` frees it, after which such a graph must not be replayed.
         A weight that has come to another shape or GPU since needs ``quantize_(False)``
-        first.  Both widths must be multiples of 32, the input's at most 8192."""
+        first.  Both widths must be multiples of 32, the input's at most 8192; a call
+        of 2^23 rows or more runs in bf16."""
         if not enabled:
             self.__dict__.pop("_mx", None)
             return self
@@ -144,7 +145,8 @@ class FeedForward(_Packs):
         return kernels.mx_linear(h, down.rows, self.net[2].bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if "_mx" in self.__dict__ and self.quantized() and x.is_cuda and x.dtype == torch.bfloat16:
+        if ("_mx" in self.__dict__ and self.quantized() and x.is_cuda and x.dtype == torch.bfloat16
+                and x.numel() < x.shape[-1] << 23):   # fewer rows than one call of adaln_mx refuses
             rows = x.reshape(1, -1, x.shape[-1]).contiguous()
             if rows.data_ptr() % 16:
                 rows = rows.clone()

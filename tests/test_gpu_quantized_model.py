@@ -214,3 +214,16 @@ def test_a_moved_feed_forward_frees_its_weights(dev):
     before = torch.cuda.memory_allocated()
     ff.quantize_(False)
     assert before - torch.cuda.memory_allocated() >= weights // 2   # the 8-bit rows
+
+
+def test_more_rows_than_a_call_takes(dev):
+    """2^23 rows and more run in bf16 instead of being refused; one row fewer in 8 bits."""
+    ff = D.FeedForward(32, 32).to(dev, BF).quantize_()
+    few = randn((16, 32), gen(9), BF).to(dev)
+    rows = 1 << 23
+    x = few.repeat(rows // 16, 1)
+    with torch.no_grad():
+        y = ff(x)
+        assert y.shape == x.shape and torch.equal(y, ff.net(x))
+        y = ff(x[:rows - 1])
+        assert torch.equal(y[:16], ff(few)) and torch.equal(y[-15:], y[:15]) and not torch.equal(y[:16], ff.net(few))
