@@ -26,7 +26,7 @@
 // 16 different 16-byte columns of the LDS.  Tile t of a wave's w rows holds the
 // channels 4 NT i + 4 t + r (i, r in [0, 4)) in its rows 4 i + r, so that lane
 // group i ends with the 4 NT neighbouring channels 4 NT i ..: contiguous stores,
-// and blocks of 32 for an 8-bit result inside one lane (NT = 8) or a pair (NT = 4).
+// and blocks of 32 for an 8-bit result inside a pair of lanes (NT = 4) or four (NT = 2).
 
 #include <math.h>
 
@@ -366,10 +366,10 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx_linear_kernel(const M
       if (GELU) v[i] = mx_gelu(v[i]);
     }
     if (p.ys != nullptr) {
-      static_assert(NT == 2 || NT == 4 || NT == 8, "a block of 32 lies in one, two or four lanes");
+      static_assert(NT == 2 || NT == 4, "a block of 32 lies in two or four lanes");
       float top = mx_top(v);
-      if (NT < 8) top = fmaxf(top, __shfl_xor(top, 16, 64));
-      if (NT < 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      if (NT == 2) top = fmaxf(top, __shfl_xor(top, 32, 64));
       const uint32_t code = mx_scale_code(top);
       const float inv = mx_inverse(code);
       if (m < p.M) {
