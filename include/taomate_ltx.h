@@ -387,6 +387,14 @@ int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_codes, const vo
                   int64_t y_ls, void* y_scales, void* stream);
 
 /*
+ * The tile of y that ltx_mx_linear takes for these sizes (y_scales given:
+ * quantized != 0), without a GPU: tile[0] rows, tile[1] channels, tile[2] groups of
+ * waves that split K, tile[3] its number among the tile[4] that such a result can
+ * take.
+ */
+int ltx_mx_linear_tile(int64_t M, int64_t N, int64_t K, int quantized, int64_t* tile);
+
+/*
  * ltx_skinny_linear with the weight in 4 bits: y = act(x) W^T + bias, bf16
  * rows, float32 sums, W = e2m1 code * scale of its group.
  *   x [M, K] rows x_ls apart (M <= LTX_GROUP4_MAX_ROWS, K a multiple of 32, at

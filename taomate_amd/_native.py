@@ -68,6 +68,7 @@ SIGNATURES = {
     "ltx_adaln_mx": [_i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64,
                      _ptr, _i64, _i64, _ptr, _i64, _i64, _f32, _ptr, _ptr, _ptr],
     "ltx_mx_linear": [_i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _int, _ptr, _i64, _ptr, _ptr],
+    "ltx_mx_linear_tile": [_i64, _i64, _i64, _int, _ptr],
     "ltx_group4_linear": [_i64, _i64, _i64, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _i64, _ptr],
 }
 

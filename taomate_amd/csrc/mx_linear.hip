@@ -574,56 +574,77 @@ void launch_mx_rows(const MxLinearArgs& p, hipStream_t st) {
 struct MxShape {
   int rows, cols, groups;
   float once, round, step, each;
-  void (*launch)(const MxLinearArgs&, hipStream_t);
+  void (*launch[2])(const MxLinearArgs&, hipStream_t);  // plain, with GELU
+};
+constexpr MxShape kMxShapes[] = {
+    // bf16 results
+    {16, 16, 8, 3.13f, 0.0f, 0.37f, 0.76f, {launch_mx_rows<1, 1, false>, launch_mx_rows<1, 1, true>}},
+    // 8-bit ones: whole blocks
+    {16, 32, 8, 2.98f, 0.0f, 0.65f, 1.32f, {launch_mx_rows<1, 2, false>, launch_mx_rows<1, 2, true>}},
+    {32, 32, 4, 1.84f, 2.06f, 0.39f, 0.0f, {launch_mx_linear<2, 2, 1, 1, 3, 4, false>, launch_mx_linear<2, 2, 1, 1, 3, 4, true>}},
+    {32, 64, 4, 1.66f, 2.59f, 0.60f, 0.0f, {launch_mx_linear<2, 2, 1, 2, 3, 4, false>, launch_mx_linear<2, 2, 1, 2, 3, 4, true>}},
+    {48, 32, 4, 1.70f, 2.38f, 0.47f, 0.0f, {launch_mx_linear<3, 2, 1, 1, 3, 4, false>, launch_mx_linear<3, 2, 1, 1, 3, 4, true>}},
+    {48, 64, 4, 1.48f, 2.38f, 0.68f, 0.0f, {launch_mx_linear<3, 2, 1, 2, 2, 4, false>, launch_mx_linear<3, 2, 1, 2, 2, 4, true>}},
+    {80, 64, 4, 1.19f, 3.14f, 0.85f, 0.0f, {launch_mx_linear<5, 2, 1, 2, 2, 4, false>, launch_mx_linear<5, 2, 1, 2, 2, 4, true>}},
+    {160, 64, 2, 0.0f, 4.16f, 0.70f, 0.0f, {launch_mx_linear<5, 2, 2, 2, 2, 2, false>, launch_mx_linear<5, 2, 2, 2, 2, 2, true>}},
+    {128, 128, 2, 0.0f, 4.95f, 0.86f, 0.0f, {launch_mx_linear<4, 4, 2, 2, 2, 2, false>, launch_mx_linear<4, 4, 2, 2, 2, 2, true>}},
+    {128, 256, 1, 0.0f, 5.39f, 0.77f, 0.0f, {launch_mx_linear<4, 4, 2, 4, 3, 1, false>, launch_mx_linear<4, 4, 2, 4, 3, 1, true>}},
+    {192, 256, 1, 0.0f, 5.22f, 0.91f, 0.0f, {launch_mx_linear<6, 4, 2, 4, 2, 1, false>, launch_mx_linear<6, 4, 2, 4, 2, 1, true>}},
+    {256, 256, 1, 0.0f, 6.34f, 1.05f, 0.0f, {launch_mx_linear<8, 4, 2, 4, 2, 1, false>, launch_mx_linear<8, 4, 2, 4, 2, 1, true>}},
 };
 
-// False if every tile makes more workgroups than a grid of 512 threads each may have (2^32 threads).
-template <bool GELU>
-bool launch_mx(const MxLinearArgs& p, hipStream_t st) {
-  static const MxShape shapes[] = {
-      {16, 16, 8, 3.13f, 0.0f, 0.37f, 0.76f, launch_mx_rows<1, 1, GELU>},  // bf16 results
-      {16, 32, 8, 2.98f, 0.0f, 0.65f, 1.32f, launch_mx_rows<1, 2, GELU>},  // 8-bit ones: whole blocks
-      {32, 32, 4, 1.84f, 2.06f, 0.39f, 0.0f, launch_mx_linear<2, 2, 1, 1, 3, 4, GELU>},
-      {32, 64, 4, 1.66f, 2.59f, 0.60f, 0.0f, launch_mx_linear<2, 2, 1, 2, 3, 4, GELU>},
-      {48, 32, 4, 1.70f, 2.38f, 0.47f, 0.0f, launch_mx_linear<3, 2, 1, 1, 3, 4, GELU>},
-      {48, 64, 4, 1.48f, 2.38f, 0.68f, 0.0f, launch_mx_linear<3, 2, 1, 2, 2, 4, GELU>},
-      {80, 64, 4, 1.19f, 3.14f, 0.85f, 0.0f, launch_mx_linear<5, 2, 1, 2, 2, 4, GELU>},
-      {160, 64, 2, 0.0f, 4.16f, 0.70f, 0.0f, launch_mx_linear<5, 2, 2, 2, 2, 2, GELU>},
-      {128, 128, 2, 0.0f, 4.95f, 0.86f, 0.0f, launch_mx_linear<4, 4, 2, 2, 2, 2, GELU>},
-      {128, 256, 1, 0.0f, 5.39f, 0.77f, 0.0f, launch_mx_linear<4, 4, 2, 4, 3, 1, GELU>},
-      {192, 256, 1, 0.0f, 5.22f, 0.91f, 0.0f, launch_mx_linear<6, 4, 2, 4, 2, 1, GELU>},
-      {256, 256, 1, 0.0f, 6.34f, 1.05f, 0.0f, launch_mx_linear<8, 4, 2, 4, 2, 1, GELU>},
-  };
-  const float bytes = ((float)p.M + p.N) * p.K * 1.03f + 2.0f * p.M * p.N, floor = 2.5f + bytes / 5.3e6f;
-  const int64_t cols = p.ys != nullptr ? ceil_div(p.N, 128) * 128 : p.N;
+// Whether a tile can hold such a result: the smallest exist once for either kind.
+bool mx_admits(const MxShape& h, bool quantized) { return h.each == 0.0f || h.cols == (quantized ? 32 : 16); }
+
+// Null if every tile makes more workgroups than a grid of 512 threads each may have (2^32 threads).
+const MxShape* choose_mx(int64_t M, int64_t N, int64_t K, bool quantized) {
+  const float bytes = ((float)M + N) * K * 1.03f + 2.0f * M * N, floor = 2.5f + bytes / 5.3e6f;
+  const int64_t cols = quantized ? ceil_div(N, 128) * 128 : N;
   const MxShape* best = nullptr;
   float least = 0.0f;
-  for (const MxShape& h : shapes) {
-    if (h.cols == (p.ys != nullptr ? 16 : 32) && h.each > 0.0f) continue;
-    const int64_t count = ceil_div(p.M, h.rows) * ceil_div(cols, h.cols);
+  for (const MxShape& h : kMxShapes) {
+    if (!mx_admits(h, quantized)) continue;
+    const int64_t count = ceil_div(M, h.rows) * ceil_div(cols, h.cols);
     if (count >= (int64_t{1} << 32) / 512) continue;
     const float tiles = (float)count;
-    const float steps = (float)ceil_div(ceil_div(p.K, 128), h.groups);
+    const float steps = (float)ceil_div(ceil_div(K, 128), h.groups);
     const float rounds = h.each > 0.0f ? 1.0f : ceilf(tiles / 256.0f);
     const float own = h.once + rounds * (h.round + steps * h.step) + tiles / 256.0f * steps * h.each;
     const float t = fmaxf(own, floor) + 0.1f * own;  // between those at the floor, the one with least of its own
     if (best == nullptr || t < least) best = &h, least = t;
   }
-  if (best != nullptr) best->launch(p, st);
-  return best != nullptr;
+  return best;
 }
 
 }  // namespace ltx
 
 using namespace ltx;
 
+#define LTX_REQUIRE_MX_SIZES(name)                                                                               \
+  LTX_REQUIRE(M >= 0 && M <= 0x3FFFFFFF && N >= 0 && N <= 0x3FFFFFFF, name ": bad M or N");                       \
+  LTX_REQUIRE(K >= kMxBlock && K % kMxBlock == 0 && K <= LTX_MX_MAX_K,                                            \
+              name ": K must be a multiple of %d, at most %d", kMxBlock, LTX_MX_MAX_K)
+
+extern "C" int ltx_mx_linear_tile(int64_t M, int64_t N, int64_t K, int quantized, int64_t* tile) {
+  clear_error();
+  LTX_REQUIRE_MX_SIZES("ltx_mx_linear_tile");
+  LTX_REQUIRE(tile != nullptr, "ltx_mx_linear_tile: null pointer");
+  const MxShape* const h = M * N == 0 ? nullptr : choose_mx(M, N, K, quantized != 0);
+  LTX_REQUIRE(h != nullptr, "ltx_mx_linear_tile: the result is empty or too large");
+  tile[0] = h->rows, tile[1] = h->cols, tile[2] = h->groups, tile[3] = tile[4] = 0;
+  for (const MxShape& o : kMxShapes) {
+    if (!mx_admits(o, quantized != 0)) continue;
+    tile[3] += &o < h;
+    tile[4] += 1;
+  }
+  return LTX_OK;
+}
+
 extern "C" int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_codes, const void* a_scales,
                              const void* w_codes, const void* w_scales, const void* bias, int act, void* y,
                              int64_t y_ls, void* y_scales, void* stream) {
   clear_error();
-  LTX_REQUIRE(M >= 0 && M <= 0x3FFFFFFF && N >= 0 && N <= 0x3FFFFFFF, "ltx_mx_linear: bad M or N");
-  LTX_REQUIRE(K >= kMxBlock && K % kMxBlock == 0 && K <= LTX_MX_MAX_K,
-              "ltx_mx_linear: K must be a multiple of %d, at most %d", kMxBlock, LTX_MX_MAX_K);
+  LTX_REQUIRE_MX_SIZES("ltx_mx_linear");
   LTX_REQUIRE(act == 0 || act == 1, "ltx_mx_linear: unknown activation %d", act);
   LTX_REQUIRE(y_scales == nullptr || N % kMxBlock == 0, "ltx_mx_linear: 8-bit output needs N a multiple of %d", kMxBlock);
   if (M * N == 0) return LTX_OK;
@@ -636,7 +657,9 @@ extern "C" int ltx_mx_linear(int64_t M, int64_t N, int64_t K, const void* a_code
   MxLinearArgs p{(const uint8_t*)a_codes, (const uint8_t*)a_scales, (const uint8_t*)w_codes, (const uint8_t*)w_scales,
                  (const uint16_t*)bias, y, (uint8_t*)y_scales, y_ls, (int)M, (int)N, (int)K};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  LTX_REQUIRE(act ? launch_mx<true>(p, st) : launch_mx<false>(p, st), "ltx_mx_linear: the result is too large");
+  const MxShape* const h = choose_mx(M, N, K, y_scales != nullptr);
+  LTX_REQUIRE(h != nullptr, "ltx_mx_linear: the result is too large");
+  h->launch[act](p, st);
   LTX_LAUNCH_CHECK("ltx_mx_linear");
   return LTX_OK;
 }

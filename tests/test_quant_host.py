@@ -249,3 +249,34 @@ def test_4bit_weights_near_the_smallest_scales(top):
     best = (w.double().abs()[..., None] - s.double() * grid).abs().amin(-1)
     # the value that a code stands for is a product in float32, to half of 2^-149
     assert ((q.dequantize().double() - w.double()).abs() <= best + 2.0 ** -150).all()
+
+
+def _tile(M, N, K, quantized):
+    tile = _native.i64_array([0] * 5)
+    _native.call("ltx_mx_linear_tile", M, N, K, int(quantized), ctypes.cast(tile, ctypes.c_void_p))
+    return tuple(tile)
+
+
+def test_the_size_lists_reach_every_tile():
+    """The GPU tests' sizes run every tile that a bf16 and an 8-bit result can take, and the long ones."""
+    from .test_gpu_mx_linear import TILES, TILES_OF_48
+    for quantized in (False, True):
+        seen = {}
+        for M, K, N in TILES + TILES_OF_48:
+            rows, cols, groups, at, count = _tile(M, N // 32 * 32 if quantized else N, K, quantized)
+            assert seen.setdefault(at, (rows, cols, groups)) == (rows, cols, groups)
+        assert sorted(seen) == list(range(count)) and len(set(seen.values())) == count == 11
+        assert ((16, 32, 8) in seen.values()) == quantized and ((16, 16, 8) in seen.values()) == (not quantized)
+    assert _tile(2304, 16384, 4096, True)[:2] == (192, 256) and _tile(1, 40, 32, False)[:2] == (16, 16)
+
+
+@pytest.mark.parametrize("match,call", [
+    ("null pointer", lambda: _native.call("ltx_mx_linear_tile", 1, 32, 32, 0, None)),
+    ("bad M or N", lambda: _tile(-1, 32, 32, False)),
+    ("K must be", lambda: _tile(1, 32, 33, False)),
+    ("empty or too large", lambda: _tile(0, 32, 32, False)),
+    ("empty or too large", lambda: _tile(BIG - 1, BIG - 1, 32, True)),
+])
+def test_the_tile_query_refuses(match, call):
+    with pytest.raises(_native.NativeCallError, match=match):
+        call()
