@@ -146,3 +146,53 @@ def test_silu_of_infinities(dev, M):
     y = kernels.group4_linear(x.to(dev), _to(w, dev), silu=True)
     assert (w.dequantize()[:, 5] > 0).all() and (y[0] == float("inf")).all()
     assert y[1].isnan().all() and y[M - 1].isnan().all() and torch.equal(y[2:M - 1], clean[2:M - 1])
+
+
+def check_unrounded(x, w, b, silu, y):
+    """``check`` with SiLU(x) held to 2^-16 (two bf16 parts) + 2^-20 (its float32 steps), for |x| < 6."""
+    xd, held = x.double(), 2.0 ** -20
+    if silu:
+        xd, held = torch.nn.functional.silu(xd), 2.0 ** -16 + 2 * 2.0 ** -20
+    wd = w.dequantize().double()
+    ref, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if b is not None:
+        ref, mag = ref + b.double(), mag + b.double().abs()
+    y = y.double()
+    assert y.shape == ref.shape and ((y - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * held * mag).all()
+
+
+# chunks of 128 columns that 1, 2, 4 and 8 waves share, whole and not, with the rows around the halves
+UNROUNDED = [(1, 32, 1, 32), (2, 288, 17, 32), (8, 512, 40, 128), (9, 448, 33, 64), (16, 512, 300, 32),   # 1 wave
+             (1, 544, 130, 32), (3, 576, 64, 64), (7, 640, 47, 128), (8, 1024, 100, 32), (9, 768, 515, 64),  # 2
+             (12, 896, 31, 128), (16, 1024, 999, 64), (15, 992, 18, 32),
+             (2, 1056, 50, 32), (8, 2048, 75, 64), (10, 1920, 20, 128), (16, 1600, 33, 64),   # 4
+             (4, 2080, 41, 32), (8, 4096, 66, 128), (11, 4032, 19, 64), (16, 4096, 130, 32)]   # 8
+
+
+@pytest.mark.parametrize("silu", [False, True], ids=["plain", "silu"])
+@pytest.mark.parametrize("M,K,n,group", UNROUNDED)
+def test_nothing_but_the_result_is_rounded(dev, M, K, n, group, silu):
+    g = gen(3 * M + K + n)
+    x, w = randn((M, K), g, BF).clamp(-5.96875, 5.96875), _weight(n, K, group, g)
+    b = randn((n,), g, BF) if n % 2 else None
+    y = kernels.group4_linear(x.to(dev), _to(w, dev), None if b is None else b.to(dev), silu=silu)
+    check_unrounded(x, w, b, silu, y.cpu())
+
+
+@pytest.mark.parametrize("M,silu", [(1, False), (2, True), (8, True), (9, True), (16, False)])
+@pytest.mark.parametrize("K,group", [(64, 64), (512, 128), (544, 32), (1024, 64)])
+@pytest.mark.parametrize("per", [1, 2, 4])
+def test_several_rounds_of_short_rows(dev, per, K, group, M, silu):
+    """Weights long enough that a workgroup takes 2, 3 and 5 rounds of tiles (and twice as many where
+    the rows go by halves or one workgroup fills a CU): 512 workgroups of 8 tiles of 16 rows with one
+    wave each, or of 4 with two.  Some workgroups have a round fewer than others."""
+    n = per * 512 * (8 if K <= 512 else 4) * 16 + 5 * 16 + 3
+    g = torch.Generator(device=dev).manual_seed(K + M + per)
+    tiles, chunks = -(-n // 16), -(-K // 128)
+    codes = torch.randint(0, 256, (n, K // 2), generator=g, device=dev, dtype=torch.uint8)
+    scales = torch.rand(n, K // group, generator=g, device=dev).to(BF)
+    w = quant.Group4Weight.from_codes(codes, scales)
+    assert w.codes.shape[:2] == (tiles, chunks)
+    x = torch.randn(M, K, generator=g, device=dev).clamp(-5.96875, 5.96875).to(BF)
+    b = torch.randn(n, generator=g, device=dev).to(BF)
+    check_unrounded(x, w, b, silu, kernels.group4_linear(x, w, b, silu=silu))
