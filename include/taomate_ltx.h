@@ -372,8 +372,11 @@ int ltx_adaln_mx(int64_t B, int64_t L, int64_t C, const void* x, int64_t x_bs, i
 
 /*
  * Linear layer of 8-bit rows with an 8-bit weight: y = act(a w^T + bias),
- * products and sums on the scaled matrix cores (float32 accumulators), bias,
- * activation and one rounding in the epilogue.
+ * products and sums on the scaled matrix cores, bias, activation and one rounding
+ * in the epilogue.  The matrix cores add the products of up to 8 neighbouring
+ * columns with 13 bits below the largest of them and everything else in float32: a
+ * sum may be off by 7 * 2^-13 of the sum of its products' magnitudes, so one that
+ * cancels to less has no right digits.
  *   a: 8-bit rows [M, K], w: 8-bit rows [N, K] (codes 16-byte aligned, scales
  *   4-byte aligned); K a multiple of 32, at most LTX_MX_MAX_K.  bias: bf16 [N]
  *   or NULL.  act: 0 none, 1 tanh-GELU.

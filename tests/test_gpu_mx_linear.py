@@ -624,3 +624,25 @@ def test_a_first_call_while_a_mode_is_on(dev):
     done = subprocess.run([sys.executable, "-c", _FIRST_CALL_UNDER_A_MODE], cwd=root, capture_output=True, text=True,
                           timeout=100)
     assert done.returncode == 0 and "right" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 64, 8), (20, 1024, 300), (200, 2048, 515), (300, 4096, 1000)])
+def test_sums_that_cancel(dev, M, K, N):
+    """Pairs of neighbouring columns whose products cancel, a small rest beside them: off by no more
+    than the documented part of the products' magnitudes, though that is more than the result."""
+    g = torch.Generator(device=dev).manual_seed(K)
+    rand = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    a, w = rand(M, K), rand(N, K) / K ** 0.5
+    a[:, 1::4], w[:, 1::4] = a[:, 0::4], -w[:, 0::4]
+    a[:, 2::4] *= 2.0 ** -6
+    a[:, 3::4] = 0
+    a, w = quant.quantize_mx(a), quant.quantize_mx(w)
+    ad, wd = a.dequantize().double(), w.dequantize().double()
+    ref, mag = ad @ wd.t(), ad.abs() @ wd.abs().t()
+    y = kernels.mx_linear(a, w).double()
+    assert ref.norm() < 2.0 ** -4 * mag.norm()
+    assert ((y - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * MFMA * mag).all()
+    # 1, -1 and 2^-14 side by side: the last is cut off or held, never more than that
+    a, w = torch.zeros(1, 32, device=dev), torch.zeros(1, 32, device=dev)
+    a[0, :3], w[0, :3] = torch.tensor([1, 1, 2.0 ** -7]), torch.tensor([1, -1, 2.0 ** -7])
+    assert 0.0 <= kernels.mx_linear(quant.quantize_mx(a), quant.quantize_mx(w)).item() <= 2 * 2.0 ** -13
