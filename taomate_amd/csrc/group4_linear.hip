@@ -222,11 +222,16 @@ void launch_group4(const Group4Args& a, hipStream_t st) {
   const int chunks = (a.K + 127) / 128;
   const size_t lds = (size_t)(!SILU ? a.M : a.M > 8 ? a.M + 1 : 2 * a.M) * (chunks * 16 + 1) * 16;
   const size_t all = lds + sizeof(float) * 2 * kG4Waves * (SILU ? 8 : 16) * 17;
-  // Resident workgroups per CU: two (16 waves) where the LDS holds them (4 rows of 4096
-  // -> 24576 in 15.5 us, one at a time 17.2).  Each stages x, so a large x takes one
-  // where two would have no more than a round each (8 rows of 2048 -> 12288: 7.5 us, two 8.1).
+  // Resident workgroups per CU: two (16 waves) where the LDS holds them (weights from HBM,
+  // groups of 128, SiLU: 4 rows of 4096 -> 24576 in 15.8 us, one 17.9); two that do not fit take turns
+  // and stage x twice (8 rows of it 23.6, one 19.4).  One also where SiLU of a large x is what a
+  // workgroup does most and two would have no more than a round each: 8 rows of 2048 -> 12288
+  // in 8.1, two 8.6; 7 rows 7.7 and 8.1.  Not without SiLU (8 rows 7.1, two 6.8), nor by halves
+  // (12 rows of 2048 -> 16384 10.5, two 10.0), nor for longer weights (7 rows of 2048 -> 24576
+  // 10.6, two 10.4).
   const int64_t want = ceil_div(ceil_div(a.N, 16), kG4Waves / KS);
-  const int64_t most = all > 80 * 1024 || (all > 48 * 1024 && want <= 512) ? 256 : 512;
+  const bool one = all > 80 * 1024 || (SILU && a.M <= 8 && all > 48 * 1024 && want <= 512);
+  const int64_t most = one ? 256 : 512;
   int64_t grid = want < most ? want : most;
   if (SILU && a.M > 8) grid = 2 * (want < most / 2 ? ceil_div(want, 8) * 8 : most / 2);  // whole groups of 8, 8 apart
   hipLaunchKernelGGL((group4_linear_kernel<KS, GROUP, SILU>), dim3((unsigned)grid), dim3(64 * kG4Waves), lds, st, a);
