@@ -16,14 +16,20 @@
 // may be off by 7 * 2^-13 of its products' magnitudes.  In sums that do not cancel
 // that stays under the rounding of either result (bf16 2^-8, e4m3 2^-4); in one that
 // does it can be all of it: neighbouring products 1, -1, 2^-14 give 0.  It is taken
-// because the operands themselves are rounded to 2^-4 and the results to 2^-8 or 2^-4: of the
-// 8-bit results of real sizes 0.2 % of the codes become their neighbour, and the error
-// against results that are not rounded is 0.02645 of their norm with the cut and without.
+// because the operands themselves are rounded to 2^-4 and the results to 2^-8 or 2^-4, and
+// because every product at this rate has it: the library's fp8 products cut at the same
+// bit (1.3e-5 of a result's norm for normal operands).  Of the 8-bit results of real sizes 0.2 %
+// of the codes become their neighbour, and the error against results that are not
+// rounded is 0.02645 of their norm with the cut and without.
 //
-// Bound by power at large sizes: 8192 x 8192 x 8192 in 388 us (2.83 PFLOP/s of 5.0; the matrix
-// cores busy 75 % of the cycles at 1.74 GHz), 2304 x 4096 -> 16384 with GELU and an 8-bit
-// result in 135-143 us by box, 2304 x 16384 -> 4096 in 142-147.  By the weight's read at few rows
-// (2 of 4096 -> 16384: 12.8 us, 5.4 TB/s), between them by latency.
+// Large sizes: 8192 x 8192 x 8192 in 371-400 us by box (2.75-2.96 PFLOP/s of 5.0; the matrix
+// cores busy 75-81 % of the cycles), 2304 x 4096 -> 16384 with GELU and an 8-bit result in
+// 126-143 us, 2304 x 16384 -> 4096 in 122-147 (busy 74 % of the cycles of the CUs with a tile).  The
+// loop loses what the two waves of a SIMD do not hide of its loads and LDS reads:
+// 2304 x 16384 -> 4096 takes 123 us, without the loads 98, without the reads 104, without
+// either 93 (8192^3 371, 335, 341 and 306).  Where the chip is full of tiles for long, power
+// comes on top: 1.63-1.74 GHz at 8192^3, 2.0-2.1 at the others.  By the weight's read at few rows
+// (2 of 4096 -> 16384: 12.7 us, 5.4 TB/s), between them by latency.
 //
 // Tiles of a and w travel HBM -> LDS without registers, 128 columns (one MFMA's
 // depth) per step, in rows of 128 bytes whose 16-byte chunks are exchanged by

@@ -93,7 +93,8 @@ class FeedForward(_Packs):
         """Run the two linears in 8 bits (``kernels.mx_linear``): the weights are
         packed into 8-bit rows beside the bf16 parameters, which keep their
         names and values; the activations are quantised by the norm before
-        and by the first linear's epilogue.  Call it on the device it is to run
+        and by the first linear's epilogue.  Sums hold what the 8-bit matrix cores
+        hold, as ``kernels.mx_linear`` says.  Call it on the device it is to run
         on.  Anything that changes, moves or replaces a weight afterwards ends it
         and the bf16 linears run again; so do calls that something else would see
         (gradients, autocast, hooks, compilation).  The old
