@@ -414,6 +414,115 @@ int ltx_group4_linear(int64_t M, int64_t N, int64_t K, int64_t group, const void
                       const void* codes, const void* scales, const void* bias, void* y, int64_t y_ls,
                       void* stream);
 
+/*
+ * A KV cache in blocks, for requests of different lengths (the four entry points
+ * below and ltx_prompt_attn have no counterpart in the reference, whose caches
+ * hold one length a batch).
+ *
+ * A block is `block` tokens (16, 32, 64, 128 or 256).  A request's tokens lie in
+ * the blocks of its row of `tables` (int32 [B, width], rows t_bs elements
+ * apart): position p in slot tables[b][p / block] * block + p % block.  `lens`
+ * (int32 [B]) counts the tokens that a request holds.  Blocks that no request
+ * holds are free[0, *top) of a stack of n_free entries.  All of it lies on the
+ * device: no call waits for it.
+ *
+ * ltx_kv_block_grow gives request b the blocks that fresh[b] more tokens need,
+ * from the top of the stack, request by request: its new table entries, and
+ *   starts [B + 1]      where each request's new tokens start among all of them;
+ *   slots, positions    [tokens] slot (int64) and position of every new token;
+ *                       rows behind the last one get slot -1, position 0;
+ *   lens_out, top_out   the lengths and the stack's top afterwards; lens_out may
+ *                       be lens and top_out may be top.
+ * ltx_kv_block_release puts the blocks of the requests with done[b] != 0 back
+ * on the stack; lens_out is 0 for them.  Their table rows stay as they are.
+ *
+ * When a call does not fit, nothing is given or taken: tables, stack, lengths
+ * and top stay, starts is 0, every slot is -1, and the reason is or-ed into
+ * *status (which a call that fits leaves alone):
+ *   LTX_BLOCKS_FREE    not enough free blocks (release: more than the stack holds)
+ *   LTX_BLOCKS_WIDTH   a request outgrows its table row
+ *   LTX_BLOCKS_TOKENS  more new tokens than `tokens`
+ *   LTX_BLOCKS_LENGTH  a negative length
+ * B at most LTX_MAX_REQUESTS.
+ */
+#define LTX_MAX_REQUESTS 4096
+#define LTX_BLOCKS_FREE 1
+#define LTX_BLOCKS_WIDTH 2
+#define LTX_BLOCKS_TOKENS 4
+#define LTX_BLOCKS_LENGTH 8
+int ltx_kv_block_grow(int64_t B, int64_t width, int64_t block, int32_t* tables, int64_t t_bs,
+                      const int32_t* lens, const int32_t* fresh, const int32_t* free_list, int64_t n_free,
+                      const int32_t* top, int32_t* status, int64_t tokens, int32_t* lens_out,
+                      int32_t* top_out, int32_t* starts, int64_t* slots, int32_t* positions, void* stream);
+int ltx_kv_block_release(int64_t B, int64_t width, int64_t block, const int32_t* tables, int64_t t_bs,
+                         const int32_t* lens, const uint8_t* done, int32_t* free_list, int64_t n_free,
+                         const int32_t* top, int32_t* status, int32_t* lens_out, int32_t* top_out,
+                         void* stream);
+
+/*
+ * Writes K and V of T tokens (bf16 [T, H, D], strides (ls, hs), D 64 or 128) into
+ * their slots of the pools: element (block, token, h, d) at pool + block*ps +
+ * token*ts + h*hs + d.  Tokens whose slot is negative or past the pool are
+ * skipped; slots must be distinct.
+ *   kv_dtype LTX_BF16 copies; LTX_F8E4M3 writes e4m3 codes and a float32 scale
+ *   for every token and head, at scales + block*ps + token*ts + h*hs: the row's
+ *   largest finite magnitude / 448 (1 if that is 0), codes rounded to nearest
+ *   even; values that are not finite become NaN.
+ *   Source rows 16-byte aligned, pool rows 16-byte (bf16) or 8-byte (e4m3).
+ */
+int ltx_kv_paged_append(int kv_dtype, int64_t T, int64_t H, int64_t D, const void* k, int64_t k_ls,
+                        int64_t k_hs, const void* v, int64_t v_ls, int64_t v_hs, void* k_pool,
+                        int64_t kp_ps, int64_t kp_ts, int64_t kp_hs, void* v_pool, int64_t vp_ps,
+                        int64_t vp_ts, int64_t vp_hs, float* k_scales, int64_t ks_ps, int64_t ks_ts,
+                        int64_t ks_hs, float* v_scales, int64_t vs_ps, int64_t vs_ts, int64_t vs_hs,
+                        int64_t n_blocks, int64_t block, const int64_t* slots, void* stream);
+
+/*
+ * Attention of one token of each request over its blocks: q, out bf16
+ * [B, Hk * G, D] (strides bs, hs; D 64 or 128), query head h over key head h / G of
+ * the first lens[b] tokens.  Pools and scales as ltx_kv_paged_append has them,
+ * the scales' tokens contiguous.
+ *   lens[b] counts at most width * block tokens; a request without any gets a zero
+ *   row and lse -inf.  Tokens in a table entry outside [0, n_blocks) take no part.
+ *   Memory of a block behind the last token is never used.
+ *   lse: NULL or float32 [B, Hk * G] natural-log sum-exp of the scaled logits.
+ *   scale <= 0 selects 1/sqrt(D).
+ *   workspace: ltx_paged_attn_workspace_size() bytes, 16-byte aligned (0: none).
+ *   Calls that overlap in time must use different workspaces.
+ *   Rows of q and of the pools 16-byte aligned, rows of out 8-byte; scales of a block
+ *   and head 16-byte aligned.
+ */
+int ltx_paged_attn(int kv_dtype, int64_t B, int64_t Hk, int64_t G, int64_t D, const void* q, int64_t q_bs,
+                   int64_t q_hs, const void* k_pool, int64_t k_ps, int64_t k_ts, int64_t k_hs,
+                   const void* v_pool, int64_t v_ps, int64_t v_ts, int64_t v_hs, const float* k_scales,
+                   const float* v_scales, int64_t sc_ps, int64_t sc_hs, int64_t n_blocks, int64_t block,
+                   const int32_t* tables, int64_t t_bs, int64_t width, const int32_t* lens, void* out,
+                   int64_t o_bs, int64_t o_hs, float* lse, float scale, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, int64_t D, int64_t width, int64_t block,
+                                  int64_t* bytes);
+
+/*
+ * Attention over whole prompts, packed: q, out bf16 [Tq, Hk * G, D], k, v bf16
+ * [Tk, Hk, D] (strides ls, hs; D 64 or 128).  Prompt b's rows are q[q_starts[b],
+ * q_starts[b + 1]) and its keys k[k_starts[b], k_starts[b + 1]) (int32 [B + 1] on the
+ * device, ascending from 0).
+ *   causal != 0: the last row sees every key of its prompt and each row before it
+ *   one key fewer, so with more keys than rows the prompt continues a prefix, and
+ *   with fewer the first rows see none: those get a zero row and lse -inf.
+ *   Rows of out behind q_starts[B] are zeroed if zero_tail != 0, else left as they
+ *   are.  Starts that are not ascending or pass Tq or Tk are cut, never followed.
+ *   lse: NULL or float32 [Hk * G, Tq]; scale <= 0 selects 1/sqrt(D).
+ *   Rows of every tensor 16-byte aligned.
+ *   A value that is not finite in v spoils every row of its prompt whose 128-row
+ *   tile sees its key; keys' values that a row does not see do not matter.
+ */
+int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D, const void* q,
+                    int64_t q_ls, int64_t q_hs, const void* k, int64_t k_ls, int64_t k_hs, const void* v,
+                    int64_t v_ls, int64_t v_hs, const int32_t* q_starts, const int32_t* k_starts, int causal,
+                    void* out, int64_t o_ls, int64_t o_hs, int zero_tail, float* lse, float scale,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

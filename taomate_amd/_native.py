@@ -20,6 +20,9 @@ MAX_KEYLEN_BATCH = 16  # LTX_MAX_KEYLEN_BATCH
 GROUP4_MAX_ROWS = 16  # LTX_GROUP4_MAX_ROWS
 GROUP4_MAX_COLUMNS = 4096  # LTX_SKINNY_MAX_K
 NOALLOC_SCRATCH_BYTES = 25 << 20  # LTX_NOALLOC_SCRATCH_BYTES
+MAX_REQUESTS = 4096  # LTX_MAX_REQUESTS
+# why kv_block_grow or kv_block_release left everything as it was (LTX_BLOCKS_*)
+BLOCKS_FREE, BLOCKS_WIDTH, BLOCKS_TOKENS, BLOCKS_LENGTH = 1, 2, 4, 8
 ABI_VERSION = 2
 
 _i64 = ctypes.c_int64
@@ -69,6 +72,18 @@ SIGNATURES = {
                      _ptr, _i64, _i64, _ptr, _i64, _i64, _f32, _ptr, _ptr, _ptr],
     "ltx_mx_linear": [_i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _int, _ptr, _i64, _ptr, _ptr],
     "ltx_mx_linear_tile": [_i64, _i64, _i64, _int, _ptr],
+    "ltx_kv_block_grow": [_i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr, _ptr, _ptr,
+                          _ptr, _ptr, _ptr],
+    "ltx_kv_block_release": [_i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr],
+    "ltx_kv_paged_append": [_int, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64,
+                            _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64,
+                            _ptr, _ptr],
+    "ltx_paged_attn": [_int, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64,
+                       _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _f32, _ptr,
+                       _i64, _ptr],
+    "ltx_paged_attn_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64, _ptr],
+    "ltx_prompt_attn": [_i64, _i64, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr,
+                        _ptr, _int, _ptr, _i64, _i64, _int, _ptr, _f32, _ptr],
     "ltx_group4_linear": [_i64, _i64, _i64, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _i64, _ptr],
 }
 

@@ -40,7 +40,8 @@ def _run(cmd):
 # per-source extra flags: the attention kernels' slot programs are fully
 # unrolled (#pragma unroll) and larger than LLVM's default limit for a
 # requested full unroll (16384), which would leave the fp8 instance rolled
-PER_SOURCE = {"flash_attn.hip": ["-mllvm", "-pragma-unroll-threshold=200000"]}
+_UNROLL = ["-mllvm", "-pragma-unroll-threshold=200000"]
+PER_SOURCE = {"flash_attn.hip": _UNROLL, "prompt_attn.hip": _UNROLL}
 
 
 def _host_command(out: pathlib.Path):

@@ -35,12 +35,10 @@
 #include <mutex>
 #include <type_traits>
 
-#include "ltx_common.h"
+#include "attn_common.h"
 
 namespace ltx {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
@@ -85,55 +83,15 @@ struct FlashParams {
   float scale_log2;  // scale * log2(e)
 };
 
-// Max / sum of a lane's value with lane l ^ 32's (the lane holding the other
-// 16 keys of the same query): one v_permlane32_swap, no LDS round trip.
-__device__ __forceinline__ float pair_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float pair_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// The same over the four lanes l ^ 16, l ^ 32, l ^ 48 (the pipelined kernels'
-// layout: a query's keys lie in four lanes).
-__device__ __forceinline__ float quad_max(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float quad_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
 // Which kernels can store float32 partials (FlashParams::part_f32): the launch
 // plan asks no others for them.
 constexpr bool stores_f32_partials(int D, bool pair, bool token) { return !pair || (token && D == 64); }
 
 constexpr int kBM = 128;
 constexpr int kBN = 64;
-constexpr float kLog2e = 1.4426950408889634f;
 
 // Row r of a K tile is stored at LDS row sig(r): bits 2 and 3 swapped.
 __device__ __forceinline__ int sig(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
-
-// The pipelined kernels' tile layout in LDS: rows of NC 16-byte chunks without
-// padding, chunk c of row r stored at c ^ row_swizzle(r), so that the 16 rows
-// that a fragment read touches (one chunk index each) fall on 16 different
-// 16-byte bank groups.  K rows hold keys in the order key_of_row: LDS row bits
-// (half, kbit, g1 g0, r1 r0) hold key bits (half, g1 g0, kbit, r1 r0), so that
-// a lane's scores of two adjacent 16-key blocks are 8 consecutive keys.
-template <int NC>
-__host__ __device__ constexpr int row_swizzle(int r) { return NC == 16 ? (r & 15) : ((r >> 1) & 7); }
-// chunk pairs of a token-major V tile's key rows: the 8 keys that half a
-// transposing fragment read touches (two blocks of 4, 8 keys apart, one 32-byte
-// chunk pair each) fall on 8 different 32-byte bank groups
-template <int NC>
-__host__ __device__ constexpr int key_swizzle(int r) {
-  return NC == 16 ? 2 * ((r & 3) | ((r >> 1) & 4)) : 2 * (((r >> 1) & 1) | ((r >> 2) & 2));
-}
-__host__ __device__ constexpr int key_of_row(int r) { return (r & 35) | ((r & 12) << 1) | ((r & 16) >> 2); }
 
 // Blocks are dispatched round-robin over the 8 XCDs (block id % 8).  Give each
 // XCD a contiguous range of the (batch*head, q-tile) space so the q-tiles that
@@ -798,7 +756,6 @@ __global__ void __launch_bounds__(256, 2) flash_fwd_masked_kernel(const FlashPar
                  pair_sum(l_run));
 }
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 // ---------------------------------------------------------------------------
 // Software-pipelined direct kernel (bf16; K token-major, V key- or token-major).

@@ -52,6 +52,12 @@ struct Api {
   decltype(&ltx_adaln_mx) adaln_mx;
   decltype(&ltx_mx_linear) mx_linear;
   decltype(&ltx_group4_linear) group4_linear;
+  decltype(&ltx_kv_block_grow) kv_block_grow;
+  decltype(&ltx_kv_block_release) kv_block_release;
+  decltype(&ltx_kv_paged_append) kv_paged_append;
+  decltype(&ltx_paged_attn) paged_attn;
+  decltype(&ltx_paged_attn_workspace_size) paged_attn_workspace_size;
+  decltype(&ltx_prompt_attn) prompt_attn;
 } api;
 PyObject* native_call_error = nullptr;  // taomate_amd._native.NativeCallError
 
@@ -334,6 +340,28 @@ bool capturing(void* stream) {
          st != hipStreamCaptureStatusNone;
 }
 
+// A call's workspace of `need` bytes, from construction (with the GIL released)
+// until the call's launches are in the stream.
+class Scratch {
+  std::unique_lock<std::mutex> lock_;
+  at::Tensor buf_;
+
+ public:
+  Scratch(const at::Tensor& q, void* st, int64_t need) {
+    const auto bytes = [&] { return at::empty({need}, q.options().dtype(at::kByte)); };
+    if (need > 0 && capturing(st)) {
+      buf_ = bytes();
+    } else if (need > 0) {
+      Workspace& ws = workspace(q, st);
+      lock_ = std::unique_lock<std::mutex>(ws.mu);
+      if (!ws.buf.defined() || ws.buf.numel() < need) ws.buf = bytes();
+      buf_ = ws.buf;
+    }
+  }
+  void* ptr() const { return buf_.defined() ? buf_.data_ptr() : nullptr; }
+  int64_t bytes() const { return buf_.defined() ? buf_.numel() : 0; }
+};
+
 PyObject *str_k, *str_v, *str_ks, *str_vs;
 
 // (q, segments, out, key_mask, lse, scale, frame_tokens, noalloc, key_lens, segment_batch_strides)
@@ -458,19 +486,9 @@ void flash_attn(PyObject* const* a) {
   int64_t need = 0;
   call("ltx_flash_attn_workspace_size", api.flash_attn_workspace_size, B, Lq, H, D, &need);
   released(own_bs ? "ltx_flash_attn_fwd_plain" : "ltx_flash_attn_fwd", [&] {
-    std::unique_lock<std::mutex> lock;
-    at::Tensor buf;
-    const auto bytes = [&] { return at::empty({need}, q.options().dtype(at::kByte)); };
-    if (need > 0 && capturing(st)) {
-      buf = bytes();
-    } else if (need > 0) {
-      Workspace& ws = workspace(q, st);
-      lock = std::unique_lock<std::mutex>(ws.mu);
-      if (!ws.buf.defined() || ws.buf.numel() < need) ws.buf = bytes();
-      buf = ws.buf;
-    }
-    void* wsp = buf.defined() ? buf.data_ptr() : nullptr;
-    const int64_t ws_bytes = buf.defined() ? buf.numel() : 0;
+    const Scratch ws(q, st, need);
+    void* wsp = ws.ptr();
+    const int64_t ws_bytes = ws.bytes();
     if (!own_bs) return general(api.flash_attn_fwd, wsp, ws_bytes, st);
     return api.flash_attn_fwd_plain(ptr(&q), B, Lq, H, D, q.stride(0), q.stride(1), q.stride(2), (int64_t)n, kp, vp,
                                     lens, seg_bs, k0.stride(1), k0.stride(2), ptr(&out), out.stride(0),
@@ -708,6 +726,258 @@ PyObject* group4_linear(PyObject* const* a) {
   return THPVariable_Wrap(y);
 }
 
+// ------------------------------------------------------- paged cache, prompts
+at::Tensor new_int(at::IntArrayRef shape, at::ScalarType type) {
+  return at::detail::empty_generic(shape, device_memory(), kPlain, type, std::nullopt);
+}
+
+// The number of values of a contiguous vector of `type` on the tables' device.
+int64_t vector(const char* what, const char* name, const at::Tensor& t, at::ScalarType type) {
+  if (t.scalar_type() != type) type_error(std::string(what) + ": " + name + " must be " + at::toString(type));
+  if (t.dim() != 1 || (t.size(0) > 1 && t.stride(0) != 1))
+    value_error(std::string(what) + ": " + name + " must be a contiguous vector, got " + shape(t));
+  return t.size(0);
+}
+void counted(const char* what, const char* name, const at::Tensor& t, at::ScalarType type, int64_t n) {
+  if (vector(what, name, t, type) != n)
+    value_error(std::string(what) + ": " + name + " must hold " + std::to_string(n) + " values, got " + shape(t));
+}
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
+  return a.numel() > 0 && b.numel() > 0 && p < q + b.nbytes() && q < p + a.nbytes();
+}
+// out: the tensor that a result goes to, `in` itself or memory apart from all that the call reads
+void apart(const char* what, const char* name, const at::Tensor& out, std::initializer_list<Opt> read, Opt in = nullptr) {
+  for (Opt t : read)
+    if (t != nullptr && overlap(out, *t) && !(t == in && out.data_ptr() == in->data_ptr()))
+      value_error(std::string(what) + ": " + name + " overlaps a tensor that the call reads or writes");
+}
+
+struct Tables {
+  int64_t B, width, bs;
+};
+Tables block_tables(const char* what, const at::Tensor& t) {
+  if (t.scalar_type() != at::kInt) type_error(std::string(what) + ": tables must be int32");
+  if (t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)))
+    value_error(std::string(what) + ": tables must be [requests, blocks] with contiguous rows, got " + shape(t));
+  return {t.size(0), t.size(1), t.size(0) > 1 ? t.stride(0) : t.size(1)};
+}
+
+// (tables, lens, new, free, top, status, block_size, tokens, lens_out, top_out)
+//   -> (slots, positions, starts, lens, top)
+PyObject* kv_block_grow(PyObject* const* a) {
+  const char* const what = "kv_block_grow";
+  const at::Tensor &tables = tensor(a[0]), &lens = tensor(a[1]), &fresh = tensor(a[2]), &free = tensor(a[3]);
+  const at::Tensor &top = tensor(a[4]), &status = tensor(a[5]);
+  const Opt lens_to = optional(a[8]), top_to = optional(a[9]);
+  same_device(what, tables, {&lens, &fresh, &free, &top, &status, lens_to, top_to});
+  const Tables t = block_tables(what, tables);
+  counted(what, "lens", lens, at::kInt, t.B);
+  counted(what, "new", fresh, at::kInt, t.B);
+  const int64_t n_free = vector(what, "free", free, at::kInt);
+  counted(what, "top", top, at::kInt, 1);
+  counted(what, "status", status, at::kInt, 1);
+  const int64_t block = integer(a[6]), tokens = integer(a[7]);
+  if (tokens < 0 || tokens > 0x7FFFFFFF) value_error("kv_block_grow: tokens must lie in [0, 2^31)");
+  if (lens_to != nullptr) {
+    counted(what, "lens_out", *lens_to, at::kInt, t.B);
+    apart(what, "lens_out", *lens_to, {&lens, &fresh, &free, &top, &status, &tables, top_to}, &lens);
+  }
+  if (top_to != nullptr) {
+    counted(what, "top_out", *top_to, at::kInt, 1);
+    apart(what, "top_out", *top_to, {&lens, &fresh, &free, &top, &status, &tables}, &top);
+  }
+  apart(what, "tables", tables, {&lens, &fresh, &free, &top, &status});
+  apart(what, "status", status, {&lens, &fresh, &free, &top});
+  const c10::DeviceGuard guard(tables.device());
+  const at::Tensor slots = new_int({tokens}, at::kLong), positions = new_int({tokens}, at::kInt),
+                   starts = new_int({t.B + 1}, at::kInt),
+                   lens_out = lens_to != nullptr ? *lens_to : new_int({t.B}, at::kInt),
+                   top_out = top_to != nullptr ? *top_to : new_int({1}, at::kInt);
+  call("ltx_kv_block_grow", api.kv_block_grow, t.B, t.width, block, ptr_as<int32_t>(&tables), t.bs,
+       ptr_as<const int32_t>(&lens), ptr_as<const int32_t>(&fresh), ptr_as<const int32_t>(&free), n_free,
+       ptr_as<const int32_t>(&top), ptr_as<int32_t>(&status), tokens, ptr_as<int32_t>(&lens_out),
+       ptr_as<int32_t>(&top_out), ptr_as<int32_t>(&starts), ptr_as<int64_t>(&slots), ptr_as<int32_t>(&positions),
+       stream_of(tables));
+  Ref r0(THPVariable_Wrap(slots)), r1(THPVariable_Wrap(positions)), r2(THPVariable_Wrap(starts)),
+      r3(THPVariable_Wrap(lens_out)), r4(THPVariable_Wrap(top_out));
+  return PyTuple_Pack(5, r0.o, r1.o, r2.o, r3.o, r4.o);
+}
+
+// (tables, lens, done, free, top, status, block_size, lens_out, top_out) -> (lens, top)
+PyObject* kv_block_release(PyObject* const* a) {
+  const char* const what = "kv_block_release";
+  const at::Tensor &tables = tensor(a[0]), &lens = tensor(a[1]), &done = tensor(a[2]), &free = tensor(a[3]);
+  const at::Tensor &top = tensor(a[4]), &status = tensor(a[5]);
+  const Opt lens_to = optional(a[7]), top_to = optional(a[8]);
+  same_device(what, tables, {&lens, &done, &free, &top, &status, lens_to, top_to});
+  const Tables t = block_tables(what, tables);
+  counted(what, "lens", lens, at::kInt, t.B);
+  counted(what, "done", done, at::kBool, t.B);
+  const int64_t n_free = vector(what, "free", free, at::kInt);
+  counted(what, "top", top, at::kInt, 1);
+  counted(what, "status", status, at::kInt, 1);
+  if (lens_to != nullptr) {
+    counted(what, "lens_out", *lens_to, at::kInt, t.B);
+    apart(what, "lens_out", *lens_to, {&lens, &done, &free, &top, &status, &tables, top_to}, &lens);
+  }
+  if (top_to != nullptr) {
+    counted(what, "top_out", *top_to, at::kInt, 1);
+    apart(what, "top_out", *top_to, {&lens, &done, &free, &top, &status, &tables}, &top);
+  }
+  apart(what, "free", free, {&lens, &done, &top, &status, &tables});
+  apart(what, "status", status, {&lens, &done, &top, &tables});
+  const c10::DeviceGuard guard(tables.device());
+  const at::Tensor lens_out = lens_to != nullptr ? *lens_to : new_int({t.B}, at::kInt),
+                   top_out = top_to != nullptr ? *top_to : new_int({1}, at::kInt);
+  call("ltx_kv_block_release", api.kv_block_release, t.B, t.width, integer(a[6]), ptr_as<const int32_t>(&tables), t.bs,
+       ptr_as<const int32_t>(&lens), ptr_as<const uint8_t>(&done), ptr_as<int32_t>(&free), n_free,
+       ptr_as<const int32_t>(&top), ptr_as<int32_t>(&status), ptr_as<int32_t>(&lens_out), ptr_as<int32_t>(&top_out),
+       stream_of(tables));
+  Ref r0(THPVariable_Wrap(lens_out)), r1(THPVariable_Wrap(top_out));
+  return PyTuple_Pack(2, r0.o, r1.o);
+}
+
+// Strides of pools [blocks, block tokens, heads, D]; a stride of a dimension of
+// one is of no matter and set to 0.
+struct Pool {
+  int64_t n, block, H, D, ps, ts, hs;
+  int dtype;
+};
+int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+Pool pool(const char* what, const char* name, const at::Tensor& t) {
+  const auto type = t.scalar_type();
+  if (type != at::kBFloat16 && type != at::kByte && type != at::kFloat8_e4m3fn)
+    type_error(std::string(what) + ": " + name + " must be bf16 or e4m3");
+  if (t.dim() != 4 || (t.size(3) > 1 && t.stride(3) != 1))
+    value_error(std::string(what) + ": " + name + " must be [blocks, block tokens, heads, D] with contiguous D, got " +
+                shape(t));
+  return {t.size(0), t.size(1), t.size(2), t.size(3), stride_of(t, 0), stride_of(t, 1), stride_of(t, 2), code(t)};
+}
+void pool_pair(const char* what, const at::Tensor& k, const at::Tensor& v, Opt ks, Opt vs) {
+  if (k.sizes() != v.sizes() || code(k) != code(v))
+    value_error(std::string(what) + ": pools " + shape(k) + " and " + shape(v) + " must share shape and dtype");
+  const bool fp8 = code(k) == LTX_F8E4M3;
+  if (!fp8 && (ks != nullptr || vs != nullptr)) value_error(std::string(what) + ": bf16 pools have no scales");
+  if (!fp8) return;
+  for (Opt s : {ks, vs}) {
+    if (s == nullptr || s->scalar_type() != at::kFloat || s->dim() != 3 || s->size(0) != k.size(0) ||
+        s->size(1) != k.size(1) || s->size(2) != k.size(2))
+      value_error(std::string(what) + ": e4m3 pools " + shape(k) + " need float32 scales [blocks, block tokens, heads]" +
+                  (s != nullptr ? ", got " + shape(*s) : ""));
+  }
+}
+
+// bf16 rows [T, heads, D]: token and head strides.
+struct TokenRows {
+  int64_t T, H, D, ls, hs;
+};
+TokenRows token_rows(const char* what, const char* name, const at::Tensor& t) {
+  if (t.scalar_type() != at::kBFloat16) type_error(std::string(what) + ": " + name + " must be bf16");
+  if (t.dim() != 3 || (t.size(2) > 1 && t.stride(2) != 1))
+    value_error(std::string(what) + ": " + name + " must be [tokens, heads, D] with contiguous D, got " + shape(t));
+  return {t.size(0), t.size(1), t.size(2), stride_of(t, 0), stride_of(t, 1)};
+}
+
+// (k, v, k_pool, v_pool, slots, k_scales, v_scales)
+void kv_paged_append(PyObject* const* a) {
+  const char* const what = "kv_paged_append";
+  const at::Tensor &k = tensor(a[0]), &v = tensor(a[1]), &kp = tensor(a[2]), &vp = tensor(a[3]), &slots = tensor(a[4]);
+  const Opt ks = optional(a[5]), vs = optional(a[6]);
+  same_device(what, k, {&v, &kp, &vp, &slots, ks, vs});
+  const TokenRows rk = token_rows(what, "k", k), rv = token_rows(what, "v", v);
+  const Pool pk = pool(what, "k_pool", kp), pv = pool(what, "v_pool", vp);
+  pool_pair(what, kp, vp, ks, vs);
+  if (k.sizes() != v.sizes() || rk.H != pk.H || rk.D != pk.D)
+    value_error("kv_paged_append: k " + shape(k) + ", v " + shape(v) + " for pools " + shape(kp));
+  counted(what, "slots", slots, at::kLong, rk.T);
+  const c10::DeviceGuard guard(k.device());
+  const auto st = [&](Opt s, int d) { return s != nullptr ? stride_of(*s, d) : 0; };
+  call("ltx_kv_paged_append", api.kv_paged_append, pk.dtype, rk.T, rk.H, rk.D, ptr(&k), rk.ls, rk.hs, ptr(&v), rv.ls,
+       rv.hs, ptr(&kp), pk.ps, pk.ts, pk.hs, ptr(&vp), pv.ps, pv.ts, pv.hs, ptr_as(ks), st(ks, 0), st(ks, 1), st(ks, 2),
+       ptr_as(vs), st(vs, 0), st(vs, 1), st(vs, 2), pk.n, pk.block, ptr_as<const int64_t>(&slots), stream_of(k));
+}
+
+// out as given, or new and contiguous
+at::Tensor rows_out(const char* what, Opt out, const at::Tensor& q) {
+  if (out == nullptr) return new_bf16(q.sizes());
+  if (out->scalar_type() != at::kBFloat16) type_error(std::string(what) + ": out must be bf16");
+  if (out->sizes() != q.sizes() || (q.size(2) > 1 && out->stride(2) != 1))
+    value_error(std::string(what) + ": out " + shape(*out) + " must be " + shape(q) + " with contiguous D");
+  return *out;
+}
+
+// (q, k_pool, v_pool, tables, lens, k_scales, v_scales, scale, out, lse)
+PyObject* paged_attn(PyObject* const* a) {
+  const char* const what = "paged_attn";
+  const at::Tensor &q = tensor(a[0]), &kp = tensor(a[1]), &vp = tensor(a[2]), &tables = tensor(a[3]), &lens = tensor(a[4]);
+  const Opt ks = optional(a[5]), vs = optional(a[6]), out = optional(a[8]), lse = optional(a[9]);
+  const float scale = a[7] == Py_None ? 0.0f : (float)real(a[7]);
+  same_device(what, q, {&kp, &vp, &tables, &lens, ks, vs, out, lse});
+  const TokenRows rq = token_rows(what, "q", q);
+  const Pool pk = pool(what, "k_pool", kp), pv = pool(what, "v_pool", vp);
+  pool_pair(what, kp, vp, ks, vs);
+  const Tables t = block_tables(what, tables);
+  const int64_t B = rq.T, H = rq.H, D = rq.D, G = pk.H > 0 ? H / pk.H : 0;
+  if (t.B != B || pk.D != D || G < 1 || H % pk.H != 0)
+    value_error("paged_attn: q " + shape(q) + " for pools " + shape(kp) + " and tables " + shape(tables) +
+                " (query heads a multiple of the key heads)");
+  counted(what, "lens", lens, at::kInt, B);
+  int64_t sc_ps = 0, sc_hs = 0;
+  if (ks != nullptr) {
+    sc_ps = stride_of(*ks, 0), sc_hs = stride_of(*ks, 2);
+    if (ks->stride(1) != 1 || vs->stride(1) != 1 || stride_of(*vs, 0) != sc_ps || stride_of(*vs, 2) != sc_hs)
+      value_error("paged_attn: scales must share strides, with a block's tokens contiguous");
+  }
+  if (lse != nullptr && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != B ||
+                         lse->size(1) != H || !lse->is_contiguous()))
+    value_error("paged_attn: lse must be contiguous float32 [requests, heads]");
+  const c10::DeviceGuard guard(q.device());
+  const at::Tensor o = rows_out(what, out, q);
+  int64_t need = 0;
+  call("ltx_paged_attn_workspace_size", api.paged_attn_workspace_size, B, pk.H, G, D, t.width, pk.block, &need);
+  void* st = stream_of(q);
+  released("ltx_paged_attn", [&] {
+    const Scratch ws(q, st, need);
+    return api.paged_attn(pk.dtype, B, pk.H, G, D, ptr(&q), rq.ls, rq.hs, ptr(&kp), pk.ps, pk.ts, pk.hs, ptr(&vp), pv.ps,
+                          pv.ts, pv.hs, ptr_as<const float>(ks), ptr_as<const float>(vs), sc_ps, sc_hs, pk.n, pk.block,
+                          ptr_as<const int32_t>(&tables), t.bs, t.width, ptr_as<const int32_t>(&lens), ptr(&o),
+                          stride_of(o, 0), stride_of(o, 1), ptr_as(lse), scale, ws.ptr(), ws.bytes(), st);
+  });
+  if (out == nullptr) return THPVariable_Wrap(o);
+  Py_INCREF(a[8]);
+  return a[8];
+}
+
+// (q, k, v, starts, k_starts, causal, scale, out, lse)
+PyObject* prompt_attn(PyObject* const* a) {
+  const char* const what = "prompt_attn";
+  const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &starts = tensor(a[3]);
+  const Opt given = optional(a[4]), out = optional(a[7]), lse = optional(a[8]);
+  const at::Tensor& k_starts = given != nullptr ? *given : starts;
+  const float scale = a[6] == Py_None ? 0.0f : (float)real(a[6]);
+  same_device(what, q, {&k, &v, &starts, given, out, lse});
+  const TokenRows rq = token_rows(what, "q", q), rk = token_rows(what, "k", k), rv = token_rows(what, "v", v);
+  const int64_t n = vector(what, "starts", starts, at::kInt);
+  if (n < 1) value_error("prompt_attn: starts must hold one more value than there are prompts");
+  counted(what, "k_starts", k_starts, at::kInt, n);
+  if (k.sizes() != v.sizes() || rk.D != rq.D || rk.H < 1 || rq.H < 1 || rq.H % rk.H != 0)
+    value_error("prompt_attn: q " + shape(q) + " for k " + shape(k) + " and v " + shape(v) +
+                " (query heads a multiple of the key heads)");
+  if (lse != nullptr && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != rq.H ||
+                         lse->size(1) != rq.T || !lse->is_contiguous()))
+    value_error("prompt_attn: lse must be contiguous float32 [heads, tokens]");
+  const c10::DeviceGuard guard(q.device());
+  const at::Tensor o = rows_out(what, out, q);
+  call("ltx_prompt_attn", api.prompt_attn, n - 1, rq.T, rk.T, rk.H, rq.H / rk.H, rq.D, ptr(&q), rq.ls, rq.hs, ptr(&k),
+       rk.ls, rk.hs, ptr(&v), rv.ls, rv.hs, ptr_as<const int32_t>(&starts), ptr_as<const int32_t>(&k_starts),
+       (int)truth(a[5]), ptr(&o), stride_of(o, 0), stride_of(o, 1), (int)(out == nullptr), ptr_as(lse), scale,
+       stream_of(q));
+  if (out == nullptr) return THPVariable_Wrap(o);
+  Py_INCREF(a[7]);
+  return a[7];
+}
+
 // is_eager(): whether an op on plain tensors would run as it is written, as far
 // as the thread's state tells: no gradients, autocast, torch function or dispatch
 // mode, function transform or trace (the last two and dispatch modes add keys to
@@ -808,6 +1078,12 @@ PyObject* bind(PyObject*, PyObject* args) {
   get("ltx_adaln_mx", next.adaln_mx);
   get("ltx_mx_linear", next.mx_linear);
   get("ltx_group4_linear", next.group4_linear);
+  get("ltx_kv_block_grow", next.kv_block_grow);
+  get("ltx_kv_block_release", next.kv_block_release);
+  get("ltx_kv_paged_append", next.kv_paged_append);
+  get("ltx_paged_attn", next.paged_attn);
+  get("ltx_paged_attn_workspace_size", next.paged_attn_workspace_size);
+  get("ltx_prompt_attn", next.prompt_attn);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: missing entry point addresses");
     return nullptr;
@@ -829,6 +1105,11 @@ PyMethodDef methods[] = {
     {"adaln_mx", (PyCFunction)(void*)&entry<adaln_mx, 7>, METH_FASTCALL, nullptr},
     {"mx_linear", (PyCFunction)(void*)&entry<mx_linear, 8>, METH_FASTCALL, nullptr},
     {"group4_linear", (PyCFunction)(void*)&entry<group4_linear, 7>, METH_FASTCALL, nullptr},
+    {"kv_block_grow", (PyCFunction)(void*)&entry<kv_block_grow, 10>, METH_FASTCALL, nullptr},
+    {"kv_block_release", (PyCFunction)(void*)&entry<kv_block_release, 9>, METH_FASTCALL, nullptr},
+    {"kv_paged_append", (PyCFunction)(void*)&entry<kv_paged_append, 7>, METH_FASTCALL, nullptr},
+    {"paged_attn", (PyCFunction)(void*)&entry<paged_attn, 10>, METH_FASTCALL, nullptr},
+    {"prompt_attn", (PyCFunction)(void*)&entry<prompt_attn, 9>, METH_FASTCALL, nullptr},
     {"is_eager", is_eager, METH_NOARGS, nullptr},
     {"row_operands", (PyCFunction)(void*)&row_operands, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

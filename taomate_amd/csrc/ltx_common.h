@@ -167,6 +167,17 @@ __device__ __forceinline__ float load_as_f32<uint16_t>(const uint16_t* p) {
   return bf16_bits_to_f32(*p);
 }
 
+// The last i in [0, n) with sums[i] <= x (sums ascending, sums[0] <= x).
+__device__ __forceinline__ int last_at_most(const int* sums, int n, int x) {
+  int lo = 0;
+  for (int step = n; step > 1;) {
+    const int half = step >> 1;
+    if (sums[lo + half] <= x) lo += half;
+    step -= half;
+  }
+  return lo;
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace ltx

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -207,3 +207,64 @@ def group4_linear(x: torch.Tensor, weight: Group4Weight, bias: Optional[torch.Te
     """ltx_group4_linear: act(x) @ W.T + bias for x [M <= 16, K <= 4096] bf16
     (SiLU of x first with ``silu``) and a 4-bit weight.  Computes no gradients."""
     return (N._host or N.host()).group4_linear(x, weight.codes, weight.scales, bias, silu, weight.rows, weight.columns)
+
+
+class BlockPlan(NamedTuple):
+    """What ``kv_block_grow`` returns: the slot (int64) and position (int32) of every new token, where each
+    request's tokens start among them (int32 [requests + 1]), the lengths and the stack's top afterwards."""
+    slots: torch.Tensor
+    positions: torch.Tensor
+    starts: torch.Tensor
+    lens: torch.Tensor
+    top: torch.Tensor
+
+
+def kv_block_grow(tables: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: torch.Tensor, top: torch.Tensor,
+                  status: torch.Tensor, block_size: int, tokens: int, lens_out: Optional[torch.Tensor] = None,
+                  top_out: Optional[torch.Tensor] = None) -> BlockPlan:
+    """ltx_kv_block_grow: the blocks that ``new`` (int32 [B]) more tokens of each request need, from the stack
+    ``free[:top]`` into the requests' rows of ``tables`` (int32 [B, width], in place), and the slots of those
+    tokens, ``tokens`` rows in all: rows behind the last token have slot -1 and position 0.  ``lens`` (int32 [B])
+    counts the tokens that the requests hold; ``lens_out`` and ``top_out`` may be ``lens`` and ``top`` (None: new
+    tensors).  A call that does not fit gives nothing to anyone, sets every slot to -1 and ors the reason
+    (``_native.BLOCKS_*``) into ``status`` (int32 [1]); nothing here waits for the device."""
+    return BlockPlan(*(N._host or N.host()).kv_block_grow(tables, lens, new, free, top, status, block_size, tokens,
+                                                          lens_out, top_out))
+
+
+def kv_block_release(tables: torch.Tensor, lens: torch.Tensor, done: torch.Tensor, free: torch.Tensor,
+                     top: torch.Tensor, status: torch.Tensor, block_size: int, lens_out: Optional[torch.Tensor] = None,
+                     top_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """ltx_kv_block_release: the blocks of the requests with ``done`` (bool [B]) go back on the stack ``free``
+    (in place).  Returns the lengths (0 for those requests) and the stack's top afterwards."""
+    return (N._host or N.host()).kv_block_release(tables, lens, done, free, top, status, block_size, lens_out, top_out)
+
+
+def kv_paged_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor,
+                    k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None) -> None:
+    """ltx_kv_paged_append: bf16 k, v [T, heads, D] into the slots (int64 [T], distinct; those outside the pool are
+    skipped) of pools [blocks, block tokens, heads, D]: bf16, or e4m3 codes with float32 scales [blocks, block
+    tokens, heads], one for each token and head."""
+    (N._host or N.host()).kv_paged_append(k, v, k_pool, v_pool, slots, k_scales, v_scales)
+
+
+def paged_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+               k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """ltx_paged_attn: one token of each request, bf16 q [B, heads, D], over the first ``lens`` (int32 [B]) tokens
+    of its blocks; query head h reads key head h // (heads / key heads).  Requests without tokens get zero rows
+    (``lse`` float32 [B, heads]: -inf).  Computes no gradients.  The tables' width bounds the lengths: the work
+    is planned for what they can hold, with one launch up to 1024 tokens and a joining second one beyond."""
+    return (N._host or N.host()).paged_attn(q, k_pool, v_pool, tables, lens, k_scales, v_scales, scale, out, lse)
+
+
+def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                k_starts: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None,
+                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """ltx_prompt_attn: packed prompts, bf16 q [Tq, heads, D] over k, v [Tk, key heads, D].  Prompt b's rows are
+    ``starts[b]`` to ``starts[b + 1]`` and its keys ``k_starts[b]`` to ``k_starts[b + 1]`` (int32 [prompts + 1];
+    None: as the rows).  ``causal``: the last row sees every key of its prompt, each row before it one fewer;
+    rows that see none are zero (``lse`` float32 [heads, Tq]: -inf).  Rows behind the last prompt are zero in a
+    new result and left as they are in ``out``.  Computes no gradients."""
+    return (N._host or N.host()).prompt_attn(q, k, v, starts, k_starts, causal, scale, out, lse)

@@ -1,0 +1,404 @@
+"""Block tables, paged append, attention over prompts and of single tokens, against float64 and plain loops."""
+import math
+import random
+
+import pytest
+import torch
+
+from taomate_amd import _native as N
+from taomate_amd import kernels
+
+from .paged_reference import (BF, E4, Cache, assert_attention_close, assert_lse_close, grow_reference, ints,
+                              prompt_reference, starts_of)
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ tables
+def _table_state(dev, lens, block, width, blocks, seed=0):
+    rng = random.Random(seed)
+    ids = list(range(blocks))
+    rng.shuffle(ids)
+    tables, at = [], 0
+    for n in lens:
+        held = -(-n // block)
+        tables.append(ids[at:at + held] + [-9] * (width - held))
+        at += held
+    free = ids[at:] + [0] * at
+    top = blocks - at
+    return tables, free, top
+
+
+@pytest.mark.parametrize("B,hi,new_hi,block,pad,in_place", [
+    (1, 0, 1, 16, 0, False), (1, 100, 5000, 16, 3, True), (7, 40, 60, 16, 11, False), (64, 500, 1, 32, 0, True),
+    (300, 300, 90, 64, 100, False), (300, 300, 90, 64, 100, True), (1025, 70, 3, 128, 5, False), (4096, 20, 2, 256, 0, True),
+    (5, 0, 0, 16, 4, False),
+])
+def test_grow(dev, B, hi, new_hi, block, pad, in_place):
+    rng = random.Random(B)
+    lens = [rng.randint(0, hi) for _ in range(B)]
+    new = [rng.randint(0, new_hi) for _ in range(B)]
+    width = max(-(-(a + b) // block) for a, b in zip(lens, new)) + 1
+    blocks = sum(-(-(a + b) // block) for a, b in zip(lens, new)) + 2
+    tables, free, top = _table_state(dev, lens, block, width, blocks)
+    T = sum(new) + pad
+    want = grow_reference(tables, lens, new, free, top, block, T)
+    t, le, fr, tp = ints(tables, dev), ints(lens, dev), ints(free, dev), ints([top], dev)
+    status = ints([0], dev)
+    plan = kernels.kv_block_grow(t, le, ints(new, dev), fr, tp, status, block, T, le if in_place else None,
+                                 tp if in_place else None)
+    assert status.item() == 0
+    assert t.tolist() == want[0] and plan.slots.tolist() == want[1] and plan.positions.tolist() == want[2]
+    assert plan.starts.tolist() == want[3] and plan.lens.tolist() == want[4] and plan.top.tolist() == [want[5]]
+    assert fr.tolist() == free
+    assert (le.tolist(), tp.tolist()) == ((want[4], [want[5]]) if in_place else (lens, [top]))
+
+
+@pytest.mark.parametrize("why,code", [("free", N.BLOCKS_FREE), ("width", N.BLOCKS_WIDTH), ("tokens", N.BLOCKS_TOKENS),
+                                      ("new", N.BLOCKS_LENGTH), ("len", N.BLOCKS_LENGTH), ("top", N.BLOCKS_FREE)])
+@pytest.mark.parametrize("big", [False, True])
+def test_grow_that_does_not_fit_gives_nothing(dev, why, code, big):
+    block, lens, new = 16, [5, 0, 33, 16], [20, 3000 if big else 1, 0, 1]
+    T = sum(new)
+    width, blocks = 200, 250
+    tables, free, top = _table_state(dev, lens, block, width, blocks)
+    if why == "free":
+        top = 2
+    if why == "top":
+        top = blocks + 1
+    if why == "width":
+        width = 2 if not big else 100
+        tables = [r[:width] for r in tables]
+        lens = [5, 0, 30 if not big else 33, 16]
+    if why == "tokens":
+        T -= 1
+    if why == "new":
+        new[2] = -1
+    if why == "len":
+        lens[3] = -5
+    if why == "width" and not big:
+        new[0] = 30
+        T = sum(new)
+    t, le, tp, status = ints(tables, dev), ints(lens, dev), ints([top], dev), ints([0], dev)
+    plan = kernels.kv_block_grow(t, le, ints(new, dev), ints(free, dev), tp, status, block, T)
+    assert status.item() & code
+    assert t.tolist() == tables and plan.lens.tolist() == lens and plan.top.tolist() == [top]
+    assert plan.starts.tolist() == [0] * 5 and plan.slots.tolist() == [-1] * T and plan.positions.tolist() == [0] * T
+
+
+@pytest.mark.parametrize("B,hi,block,in_place", [(1, 30, 16, False), (9, 100, 16, True), (513, 4000, 16, False),
+                                                 (513, 4000, 16, True), (3, 0, 32, False)])
+def test_release(dev, B, hi, block, in_place):
+    rng = random.Random(B)
+    lens = [rng.randint(0, hi) for _ in range(B)]
+    width = max(1, max(-(-n // block) for n in lens))
+    blocks = sum(-(-n // block) for n in lens) + 4
+    tables, free, top = _table_state(dev, lens, block, width, blocks)
+    done = [rng.random() < 0.5 for _ in range(B)]
+    want_free, want_top = list(free), top
+    for b in range(B):
+        for j in range(-(-lens[b] // block) if done[b] else 0):
+            want_free[want_top] = tables[b][j]
+            want_top += 1
+    t, le, fr, tp, status = ints(tables, dev), ints(lens, dev), ints(free, dev), ints([top], dev), ints([0], dev)
+    out, top_out = kernels.kv_block_release(t, le, torch.tensor(done, device=dev), fr, tp, status, block,
+                                            le if in_place else None, tp if in_place else None)
+    assert status.item() == 0 and fr.tolist() == want_free and top_out.tolist() == [want_top]
+    assert out.tolist() == [0 if d else n for n, d in zip(lens, done)] and t.tolist() == tables
+
+
+def test_release_of_more_than_the_stack_holds(dev):
+    t, le = ints([[0, 1], [2, 3]], dev), ints([32, 20], dev)
+    fr, status = ints([0, 1, 2, 3], dev), ints([0], dev)
+    out, top = kernels.kv_block_release(t, le, torch.tensor([True, True], device=dev), fr, ints([1], dev), status, 16)
+    assert status.item() == N.BLOCKS_FREE and out.tolist() == [32, 20] and top.tolist() == [1]
+    assert fr.tolist() == [0, 1, 2, 3]
+
+
+# ------------------------------------------------------------------ append
+@pytest.mark.parametrize("T,Hk,D,block,kv,layout", [
+    (1, 1, 64, 16, "bf16", "heads"), (77, 8, 128, 16, "bf16", "tokens"), (77, 8, 128, 16, "fp8", "heads"),
+    (130, 3, 64, 32, "fp8", "tokens"), (500, 2, 128, 256, "bf16", "heads"), (0, 2, 64, 16, "bf16", "heads"),
+])
+def test_append(dev, T, Hk, D, block, kv, layout):
+    g = torch.Generator().manual_seed(T)
+    c = Cache([max(T, 1)], Hk, D, block, kv, dev, layout=layout)
+    x = (torch.randn(T, 2 * Hk, D, generator=g) * 3).to(BF).to(dev)
+    k, v = x[:, :Hk], x[:, Hk:]                       # strided rows of one projection
+    slots = torch.randperm(c.n * block, generator=g)[:T].to(dev)
+    if T > 10:
+        slots[3], slots[7] = -1, c.n * block          # no slot; past the pool
+        k[5] = 0.0
+    pools = [c.k.clone(), c.v.clone()]
+    scales = [None if s is None else s.clone() for s in (c.k_scales, c.v_scales)]
+    kernels.kv_paged_append(k, v, c.k, c.v, slots, c.k_scales, c.v_scales)
+    ok = (slots >= 0) & (slots < c.n * block)
+    i, o = slots[ok] // block, slots[ok] % block
+    for src, pool, sc, got, got_sc in ((k, pools[0], scales[0], c.k, c.k_scales), (v, pools[1], scales[1], c.v, c.v_scales)):
+        x = src[ok]
+        if kv == "bf16":
+            pool[i, o] = x
+            assert torch.equal(got, pool)
+            continue
+        # float32 quotients by way of float64, whose double rounding is harmless (53 >= 2 * 24 + 2 bits); torch
+        # divides by a number as a product with its rounded reciprocal
+        top = x.double().abs().amax(-1)
+        s = torch.where(top > 0, top / 448, torch.ones_like(top)).float()
+        pool.view(torch.uint8)[i, o] = (x.double() / s.double()[..., None]).float().to(E4).view(torch.uint8)
+        sc[i, o] = s
+        assert torch.equal(got_sc, sc) and torch.equal(got.view(torch.uint8), pool.view(torch.uint8))
+
+
+def test_append_of_values_that_are_not_finite(dev):
+    c = Cache([16], 1, 64, 16, "fp8", dev)
+    k = torch.ones(2, 1, 64, dtype=BF, device=dev)
+    k[0, 0, 3], k[0, 0, 4], k[1] = math.inf, math.nan, math.nan
+    kernels.kv_paged_append(k, k, c.k, c.v, torch.tensor([1, 2], device=dev), c.k_scales, c.v_scales)
+    got = c.k.view(torch.uint8)[0, 1:3, 0].view(E4).float()
+    assert got[0].isnan().nonzero().flatten().tolist() == [3, 4] and (got[0][[0, 63]] == 448).all()
+    assert got[1].isnan().all() and c.k_scales[0, 1:3, 0].tolist() == [torch.tensor(1 / 448, dtype=torch.float32).item(), 1.0]
+
+
+# ------------------------------------------------------------------ prompts
+PROMPTS = [
+    # rows, keys, heads, key heads, D
+    ([1], [1], 1, 1, 64), ([1], [300], 4, 2, 128), ([77], [77], 8, 8, 64), ([128], [128], 2, 1, 128),
+    ([129, 1, 0, 64], [129, 1, 0, 64], 6, 2, 128), ([5, 200, 63, 65], [105, 200, 64, 1000], 4, 4, 64),
+    ([300], [300], 7, 1, 64), ([40, 130], [20, 100], 4, 2, 128), ([10, 10], [0, 5], 2, 2, 64),
+    ([257] * 5, [257] * 5, 16, 2, 128), ([1] * 70, list(range(70)), 3, 3, 64), ([640], [640], 24, 8, 128),
+]
+
+
+@pytest.mark.parametrize("rows,keys,H,Hk,D", PROMPTS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts(dev, rows, keys, H, Hk, D, causal):
+    g = torch.Generator().manual_seed(sum(rows))
+    q = (torch.randn(sum(rows), H, D, generator=g) * 1.5).to(BF).to(dev)
+    k, v = (torch.randn(sum(keys), Hk, D, generator=g).to(BF).to(dev) for _ in range(2))
+    ref, mag, lse_ref = prompt_reference(q, k, v, rows, keys, causal)
+    lse = torch.empty(H, sum(rows), device=dev)
+    out = kernels.prompt_attn(q, k, v, starts_of(rows, dev), starts_of(keys, dev), causal=causal, lse=lse)
+    assert_attention_close(out, ref, mag)
+    assert_lse_close(lse, lse_ref)
+
+
+def test_prompt_rows_of_a_packed_projection_and_the_rows_behind(dev):
+    """q, k, v as columns of one [T, (H + 2 Hk) D] projection; 50 rows behind the prompts; out strided."""
+    H, Hk, D, rows, T = 4, 2, 128, [70, 190], 310
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(T, H + 2 * Hk, D, generator=g).to(BF).to(dev)
+    x[260:] = math.nan
+    q, k, v = x[:, :H], x[:, H:H + Hk], x[:, H + Hk:]
+    ref, mag, _ = prompt_reference(q[:260], k[:260], v[:260], rows, rows, True)
+    starts = starts_of(rows, dev)
+    out = kernels.prompt_attn(q, k, v, starts)
+    assert_attention_close(out[:260], ref, mag)
+    assert (out[260:] == 0).all()
+    wide = torch.full((T, H, 2 * D), 7.0, dtype=BF, device=dev)
+    lse = torch.full((H, T), 5.0, device=dev)
+    assert kernels.prompt_attn(q, k, v, starts, out=wide[..., :D], lse=lse).data_ptr() == wide.data_ptr()
+    assert torch.equal(wide[:260, :, :D], out[:260]) and (wide[260:] == 7).all() and (wide[..., D:] == 7).all()
+    assert (lse[:, 260:] == 5).all()
+
+
+def test_prompt_keys_that_are_not_finite_and_lowest_scores(dev):
+    """K of a later key, and K and V of another prompt and behind the last, hold NaN and infinities; scores of
+    the first tiles are the lowest that float32 takes."""
+    D, rows = 64, [200, 100]
+    g = torch.Generator().manual_seed(4)
+    q = torch.ones(300, 1, D, dtype=BF, device=dev)
+    k, v = (torch.randn(320, 1, D, generator=g).to(BF).to(dev) for _ in range(2))
+    k[:150] = -2.0e36                                    # 64 products: scores of -1.6e37
+    k[199] = math.nan
+    k[300:], v[300:] = math.inf, math.nan
+    k[200:], v[250:300] = math.inf, math.inf
+    ref, mag, _ = prompt_reference(q[:199], k[:199], v[:199], [199], [199], True)
+    out = kernels.prompt_attn(q, k, v, starts_of(rows, dev))
+    assert_attention_close(out[:199], ref, mag)
+    assert out[199].isnan().all()
+
+
+def test_prompt_starts_outside_the_tensors_are_cut(dev):
+    q = torch.randn(64, 1, 64, device=dev).to(BF)
+    out = kernels.prompt_attn(q, q, q, ints([-5, 40, 30, 9999], dev))
+    ref, mag, _ = prompt_reference(q[:40], q[:40], q[:40], [40], [40], True)
+    assert_attention_close(out[:30], ref[:30], mag[:30])
+    assert torch.isfinite(out).all()
+
+
+# ------------------------------------------------------------------ single tokens
+TOKENS = [
+    # lens, heads, key heads, D, block
+    ([1], 1, 1, 64, 16), ([333], 8, 8, 64, 32), ([0, 1, 15, 16, 17, 31, 32, 33], 4, 2, 128, 16),
+    ([128, 129, 127, 0, 640], 12, 4, 128, 64), ([5000], 8, 2, 64, 16), ([2000, 3, 0, 7000, 129], 32, 8, 128, 128),
+    ([3100, 1500], 20, 1, 128, 16), ([900, 1100], 33, 1, 64, 256), ([40] * 300, 2, 2, 64, 16),
+    ([1] * 9 + [20000], 7, 7, 128, 32), ([4096] * 3, 16, 1, 64, 16),
+]
+
+
+@pytest.mark.parametrize("lens,H,Hk,D,block", TOKENS)
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("width", ["tight", "wide"])
+def test_tokens(dev, lens, H, Hk, D, block, kv, width):
+    """``wide``: tables that could hold far more, so that the work is cut into ranges and joined."""
+    w = None if width == "tight" else max(-(-max(lens) // block), 5000 // block) + 3
+    c = Cache(lens, Hk, D, block, kv, dev, seed=len(lens), layout="tokens" if len(lens) == 2 else "heads", width=w)
+    q = (torch.randn(len(lens), H, D, generator=torch.Generator().manual_seed(1)) * 1.5).to(BF).to(dev)
+    ref, mag, lse_ref = c.reference(q)
+    lse = torch.empty(len(lens), H, device=dev)
+    out = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales, lse=lse)
+    assert_attention_close(out, ref, mag)
+    assert_lse_close(lse, lse_ref)
+    again = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("wide", [0, 400])
+def test_token_blocks_hold_anything_behind_the_last_token(dev, kv, wide):
+    lens, block = [0, 5, 16, 45, 100], 16
+    c = Cache(lens, 2, 128, block, kv, dev, width=7 + wide)
+    q = torch.randn(5, 4, 128, device=dev).to(BF)
+    want = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales)
+    used = torch.zeros(c.n, block, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for p in range(n):
+            used[c.tables[b, p // block].item(), p % block] = True
+    used = used.to(dev)
+    for pool in (c.k, c.v):
+        if kv == "bf16":
+            pool[~used] = math.nan
+        else:
+            pool.view(torch.uint8)[~used] = 0x7F   # NaN
+    for s in (c.k_scales, c.v_scales):
+        if s is not None:
+            s[~used] = math.inf
+    got = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales)
+    assert torch.equal(got, want) and (got[0] == 0).all()
+
+
+def test_token_entries_outside_the_pool_take_no_part(dev):
+    c = Cache([100, 64], 2, 64, 16, "bf16", dev)
+    c.tables[0, 2], c.tables[0, 4], c.tables[1, 0] = -1, c.n, 1 << 30
+    q = torch.randn(2, 2, 64, device=dev).to(BF)
+    ref, mag, _ = c.reference(q)
+    assert_attention_close(kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t), ref, mag)
+
+
+def test_token_lengths_past_the_table_and_negative_are_cut(dev):
+    c = Cache([64, 64], 1, 64, 16, "bf16", dev)
+    q = torch.randn(2, 1, 64, device=dev).to(BF)
+    out = kernels.paged_attn(q, c.k, c.v, c.tables, ints([1 << 30, -3], dev))
+    want = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t)
+    assert torch.equal(out[0], want[0]) and (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_token_scores_of_any_size(dev, kv):
+    """The first keys' scores are near the lowest number of float32, all alike: they share the weight, and have
+    none once there are others."""
+    lens = [150, 260]
+    c = Cache(lens, 1, 64, 16, kv, dev)
+    for b in range(2):
+        for p in range(150):
+            i, o = c.tables[b, p // 16].item(), p % 16
+            if kv == "bf16":
+                c.k[i, o] = -2.0e36
+            else:
+                c.k.view(torch.uint8)[i, o] = 0xB8           # -1
+                c.k_scales[i, o] = 2.0e36
+    q = torch.ones(2, 1, 64, dtype=BF, device=dev)
+    ref, mag, _ = c.reference(q)
+    assert_attention_close(kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales), ref, mag)
+
+
+def test_token_offsets_past_32_bits(dev):
+    """Blocks whose distance from the pool's start passes 2^32 bytes."""
+    block, D, Hk = 256, 128, 1
+    n = (1 << 32) // (block * D * 2) + 40
+    k = torch.zeros(n, block, Hk, D, dtype=BF, device=dev)
+    v = torch.zeros_like(k)
+    x = torch.randn(300, Hk, D, device=dev).to(BF)
+    slots = torch.arange(300, device=dev) + (n - 3) * block
+    kernels.kv_paged_append(x, x, k, v, slots)
+    q = torch.randn(1, 2, D, device=dev).to(BF)
+    tables = ints([[n - 3, n - 2, 0, 0, 0, 0, 0, 0]], dev)
+    out = kernels.paged_attn(q, k, v, tables, ints([300], dev))
+    ref, mag, _ = prompt_reference(q, x, x, [1], [300], True)
+    assert_attention_close(out, ref, mag)
+
+
+# ------------------------------------------------------------------ together
+def test_prompts_then_tokens_under_a_graph(dev):
+    """Prompts admitted and attended, then tokens one at a time (a captured step, replayed), against attention
+    over everything so far; half of the requests released at the end."""
+    H, Hk, D, block, lens = 4, 2, 128, 16, [5, 31, 0, 64]
+    B, steps, width, blocks = len(lens), 20, 8, 40
+    g = torch.Generator().manual_seed(9)
+    hist = [[torch.zeros(0, Hk, D, dtype=BF, device=dev)] * 2 for _ in lens]
+    pools = [torch.full((blocks, Hk, block, D), math.nan, dtype=BF, device=dev).permute(0, 2, 1, 3) for _ in range(2)]
+    tables = torch.full((B, width), -1, dtype=torch.int32, device=dev)
+    free = torch.randperm(blocks, generator=g).int().to(dev)
+    top, status, held = ints([blocks], dev), ints([0], dev), ints([0] * B, dev)
+
+    def rows(T):
+        return [torch.randn(T, h, D, generator=g).to(BF).to(dev) for h in (H, Hk, Hk)]
+
+    q, k, v = rows(sum(lens) + 6)
+    plan = kernels.kv_block_grow(tables, held, ints(lens, dev), free, top, status, block, q.shape[0], held, top)
+    kernels.kv_paged_append(k, v, *pools, plan.slots)
+    out = kernels.prompt_attn(q, k, v, plan.starts)
+    ref, mag, _ = prompt_reference(q[:sum(lens)], k, v, lens, lens, True)
+    assert_attention_close(out[:sum(lens)], ref, mag)
+    at = 0
+    for b, n in enumerate(lens):
+        hist[b] = [k[at:at + n], v[at:at + n]]
+        at += n
+
+    one = ints([1] * B, dev)
+    sq, sk, sv = (torch.zeros(B, h, D, dtype=BF, device=dev) for h in (H, Hk, Hk))
+
+    def step():
+        p = kernels.kv_block_grow(tables, held, one, free, top, status, block, B, held, top)
+        kernels.kv_paged_append(sk, sv, *pools, p.slots)
+        return kernels.paged_attn(sq, *pools, tables, held)
+
+    graph, warm = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    save = [t.clone() for t in (tables, held, top)]
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        step()
+    torch.cuda.current_stream().wait_stream(warm)
+    for t, s in zip((tables, held, top), save):
+        t.copy_(s)
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(steps):
+        for dst, src in zip((sq, sk, sv), rows(B)):
+            dst.copy_(src)
+        graph.replay()
+        for b in range(B):
+            hist[b] = [torch.cat([hist[b][0], sk[b:b + 1]]), torch.cat([hist[b][1], sv[b:b + 1]])]
+            ref, mag, _ = prompt_reference(sq[b:b + 1], *hist[b], [1], [lens[b] + i + 1], True)
+            assert_attention_close(out[b:b + 1], ref, mag, f"step {i} request {b}")
+        torch.cuda.synchronize()
+    assert status.item() == 0 and held.tolist() == [n + steps for n in lens]
+    done = torch.tensor([True, False, True, False], device=dev)
+    kernels.kv_block_release(tables, held, done, free, top, status, block, held, top)
+    assert held.tolist() == [0, lens[1] + steps, 0, lens[3] + steps]
+    in_use = [tables[b, j].item() for b in (1, 3) for j in range(-(-held[b].item() // block))]
+    assert sorted(free[:top.item()].tolist() + in_use) == list(range(blocks)) and status.item() == 0
+
+
+def test_on_another_stream(dev):
+    c = Cache([3000, 500], 2, 128, 16, "bf16", dev)
+    q = torch.randn(2, 8, 128, device=dev).to(BF)
+    want = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append([kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t) for _ in range(4)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for outs in got for o in outs)
