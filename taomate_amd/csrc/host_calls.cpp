@@ -790,10 +790,21 @@ PyObject* kv_block_grow(PyObject* const* a) {
   apart(what, "tables", tables, {&lens, &fresh, &free, &top, &status});
   apart(what, "status", status, {&lens, &fresh, &free, &top});
   const c10::DeviceGuard guard(tables.device());
-  const at::Tensor slots = new_int({tokens}, at::kLong), positions = new_int({tokens}, at::kInt),
-                   starts = new_int({t.B + 1}, at::kInt),
-                   lens_out = lens_to != nullptr ? *lens_to : new_int({t.B}, at::kInt),
-                   top_out = top_to != nullptr ? *top_to : new_int({1}, at::kInt);
+  // one allocation for all results
+  const int64_t at[6] = {0, tokens * 8, tokens * 12, tokens * 12 + (t.B + 1) * 4, tokens * 12 + (2 * t.B + 1) * 4,
+                         tokens * 12 + (2 * t.B + 2) * 4};
+  c10::Allocator* const memory = device_memory();
+  const c10::Storage all(c10::Storage::use_byte_size_t(), (size_t)at[5], memory->allocate((size_t)at[5]), memory, true);
+  const auto part = [&](int i, int64_t n) {
+    at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all), kPlain,
+                                                            c10::scalarTypeToTypeMeta(i == 0 ? at::kLong : at::kInt));
+    r.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    r.unsafeGetTensorImpl()->set_storage_offset(at[i] / (i == 0 ? 8 : 4));
+    return r;
+  };
+  const at::Tensor slots = part(0, tokens), positions = part(1, tokens), starts = part(2, t.B + 1),
+                   lens_out = lens_to != nullptr ? *lens_to : part(3, t.B),
+                   top_out = top_to != nullptr ? *top_to : part(4, 1);
   call("ltx_kv_block_grow", api.kv_block_grow, t.B, t.width, block, ptr_as<int32_t>(&tables), t.bs,
        ptr_as<const int32_t>(&lens), ptr_as<const int32_t>(&fresh), ptr_as<const int32_t>(&free), n_free,
        ptr_as<const int32_t>(&top), ptr_as<int32_t>(&status), tokens, ptr_as<int32_t>(&lens_out),

@@ -45,26 +45,13 @@ struct TableParams {
   int64_t* slots;
   int64_t tokens, n_free;
   int B, width, shift;
-  int first, books;  // first workgroup that places tokens; whether workgroup 0 keeps the books
+  int place, books;  // whether the launch moves blocks and places tokens; whether workgroup 0 keeps the books
 };
-
-// Inclusive scan over a wave of two 64-bit sums.
-__device__ __forceinline__ void wave_scan(int64_t& a, int64_t& b) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t x = __shfl_up(a, d), y = __shfl_up(b, d);
-    if (lane >= d) {
-      a += x;
-      b += y;
-    }
-  }
-}
 
 template <bool GROW>
 __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const TableParams p) {
   __shared__ int s_blocks[LTX_MAX_REQUESTS], s_tokens[LTX_MAX_REQUESTS], s_len[LTX_MAX_REQUESTS];
-  __shared__ int64_t s_wave[2][kTableThreads / 64];
+  __shared__ uint32_t s_wave[2][kTableThreads / 64];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int top = *p.top;
   const int64_t block = (int64_t)1 << p.shift;
@@ -74,7 +61,7 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const TableP
 
   // ---- this thread's requests: their blocks and tokens, and what is wrong ----
   int bad = (top < 0 || top > p.n_free) ? LTX_BLOCKS_FREE : 0;
-  int64_t blocks = 0, tokens = 0;
+  uint32_t blocks = 0, tokens = 0;
   for (int b = b0; b < b1; ++b) {
     const int64_t len = p.lens[b], add = GROW ? p.fresh[b] : 0;
     const bool mine = GROW || p.done[b] != 0;
@@ -82,22 +69,21 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const TableP
       bad |= LTX_BLOCKS_LENGTH;
     } else {
       if (mine && blocks_of(len + add) > p.width) bad |= LTX_BLOCKS_WIDTH;
-      blocks += GROW ? blocks_of(len + add) - blocks_of(len) : mine ? blocks_of(len) : 0;
-      tokens += add;
+      blocks = add_sat(blocks, (uint32_t)(GROW ? blocks_of(len + add) - blocks_of(len) : mine ? blocks_of(len) : 0));
+      tokens = add_sat(tokens, (uint32_t)add);
     }
   }
-  int64_t sum_b = blocks, sum_t = tokens;
-  wave_scan(sum_b, sum_t);
+  uint32_t sum_b = wave_scan(blocks), sum_t = wave_scan(tokens);
   if (lane == 63) s_wave[0][wave] = sum_b, s_wave[1][wave] = sum_t;
   __syncthreads();
-  int64_t all_b = 0, all_t = 0;
+  uint32_t all_b = 0, all_t = 0;
 #pragma unroll
   for (int w = 0; w < kTableThreads / 64; ++w) {
-    if (w < wave) sum_b += s_wave[0][w], sum_t += s_wave[1][w];
-    all_b += s_wave[0][w];
-    all_t += s_wave[1][w];
+    if (w < wave) sum_b = add_sat(sum_b, s_wave[0][w]), sum_t = add_sat(sum_t, s_wave[1][w]);
+    all_b = add_sat(all_b, s_wave[0][w]);
+    all_t = add_sat(all_t, s_wave[1][w]);
   }
-  if (GROW ? all_b > top : top + all_b > p.n_free) bad |= LTX_BLOCKS_FREE;
+  if (GROW ? all_b > (int64_t)top : top + (int64_t)all_b > p.n_free) bad |= LTX_BLOCKS_FREE;
   if (GROW && all_t > p.tokens) bad |= LTX_BLOCKS_TOKENS;
   const bool keeper = p.books && blockIdx.x == 0;
 
@@ -114,10 +100,11 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const TableP
       *p.top_out = top;
       *p.status |= all;
     }
-    if (GROW)
-      for (int64_t t = (int64_t)((int)blockIdx.x - p.first) * kTableTokens + tid, i = 0;
-           i < kTableTokens / kTableThreads && (int)blockIdx.x >= p.first; ++i, t += kTableThreads)
+    if (GROW && p.place)
+      for (int i = 0; i < kTableTokens / kTableThreads; ++i) {
+        const int64_t t = (int64_t)blockIdx.x * kTableTokens + i * kTableThreads + tid;
         if (t < p.tokens) p.slots[t] = -1, p.positions[t] = 0;
+      }
     return;
   }
 
@@ -142,17 +129,17 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const TableP
   }
   __syncthreads();
 
+  if (!p.place) return;
+
   if (GROW) {
-    // ---- new table entries (workgroup 0) ----
-    if (keeper)
-      for (int e = tid; e < (int)all_b; e += kTableThreads) {
-        const int b = last_at_most(s_blocks, p.B, e);
-        const int j = (int)blocks_of(s_len[b]) + e - s_blocks[b];
-        p.tables[b * p.t_bs + j] = p.free_list[top - 1 - e];
-      }
+    // ---- new table entries, shared by all workgroups ----
+    for (int64_t e = (int64_t)blockIdx.x * kTableThreads + tid; e < all_b; e += (int64_t)gridDim.x * kTableThreads) {
+      const int b = last_at_most(s_blocks, p.B, (int)e);
+      const int j = (int)blocks_of(s_len[b]) + (int)e - s_blocks[b];
+      p.tables[b * p.t_bs + j] = p.free_list[top - 1 - e];
+    }
     // ---- slots and positions of this workgroup's tokens ----
-    if ((int)blockIdx.x < p.first) return;
-    const int64_t t0 = (int64_t)((int)blockIdx.x - p.first) * kTableTokens + tid;
+    const int64_t t0 = (int64_t)blockIdx.x * kTableTokens + tid;
 #pragma unroll
     for (int i = 0; i < kTableTokens / kTableThreads; ++i) {
       const int64_t t = t0 + i * kTableThreads;
@@ -170,17 +157,10 @@ __global__ void __launch_bounds__(kTableThreads) block_table_kernel(const TableP
       p.positions[t] = pos;
     }
   } else {
-    const int64_t e0 = (int64_t)((int)blockIdx.x - p.first) * kTableTokens + tid;
-    const int64_t step = (int64_t)((int)gridDim.x - p.first) * kTableTokens;
-    if ((int)blockIdx.x < p.first) return;
-    for (int64_t base = e0; base - tid < all_b; base += step)
-#pragma unroll
-      for (int i = 0; i < kTableTokens / kTableThreads; ++i) {
-        const int64_t e = base + i * kTableThreads;
-        if (e >= all_b) break;
-        const int b = last_at_most(s_blocks, p.B, (int)e);
-        p.free_list[top + e] = p.tables[b * p.t_bs + (e - s_blocks[b])];
-      }
+    for (int64_t e = (int64_t)blockIdx.x * kTableThreads + tid; e < all_b; e += (int64_t)gridDim.x * kTableThreads) {
+      const int b = last_at_most(s_blocks, p.B, (int)e);
+      p.free_list[top + e] = p.tables[b * p.t_bs + (e - s_blocks[b])];
+    }
   }
 }
 
@@ -273,21 +253,18 @@ static int check_tables(const char* name, int64_t B, int64_t width, int64_t t_bs
   return LTX_OK;
 }
 
-// Runs the kernel over `work` tokens or blocks.  lens_out and top_out may be
-// the inputs themselves: workgroup 0 would then change what others still read,
-// so where there are others the books are kept by a second launch after them.
+// lens_out and top_out may be the inputs themselves: workgroup 0 would then
+// change what others still read, so where there are others the books are kept
+// by a second launch after them.
 template <bool GROW>
-static int run_tables(TableParams p, int64_t work, hipStream_t st, const char* name) {
-  const int groups = (int)ceil_div(work, kTableTokens);
+static int run_tables(TableParams p, int64_t groups, hipStream_t st, const char* name) {
   const bool in_place = p.lens_out == p.lens || p.top_out == p.top;
-  const dim3 threads(kTableThreads);
-  if (groups <= 1 || !in_place) {
-    p.first = 0, p.books = 1;
-    hipLaunchKernelGGL((block_table_kernel<GROW>), dim3(groups > 0 ? groups : 1), threads, 0, st, p);
-  } else {
-    p.first = 0, p.books = 0;
-    hipLaunchKernelGGL((block_table_kernel<GROW>), dim3(groups), threads, 0, st, p);
-    p.first = 1, p.books = 1;
+  const dim3 grid((unsigned)(groups > 1 ? groups : 1)), threads(kTableThreads);
+  const bool two = groups > 1 && in_place;
+  p.place = 1, p.books = !two;
+  hipLaunchKernelGGL((block_table_kernel<GROW>), grid, threads, 0, st, p);
+  if (two) {
+    p.place = 0, p.books = 1;
     hipLaunchKernelGGL((block_table_kernel<GROW>), dim3(1), threads, 0, st, p);
   }
   LTX_LAUNCH_CHECK(name);
@@ -308,7 +285,7 @@ extern "C" int ltx_kv_block_grow(int64_t B, int64_t width, int64_t block, int32_
   p.free_list = const_cast<int32_t*>(free_list), p.top = top, p.status = status;
   p.lens_out = lens_out, p.top_out = top_out, p.starts = starts, p.slots = slots, p.positions = positions;
   p.tokens = tokens, p.n_free = n_free, p.B = (int)B, p.width = (int)width, p.shift = block_shift(block);
-  return run_tables<true>(p, tokens, reinterpret_cast<hipStream_t>(stream), "ltx_kv_block_grow");
+  return run_tables<true>(p, ceil_div(tokens, kTableTokens), reinterpret_cast<hipStream_t>(stream), "ltx_kv_block_grow");
 }
 
 extern "C" int ltx_kv_block_release(int64_t B, int64_t width, int64_t block, const int32_t* tables, int64_t t_bs,
@@ -325,10 +302,9 @@ extern "C" int ltx_kv_block_release(int64_t B, int64_t width, int64_t block, con
   p.free_list = free_list, p.top = top, p.status = status, p.lens_out = lens_out, p.top_out = top_out;
   p.n_free = n_free, p.B = (int)B, p.width = (int)width, p.shift = block_shift(block);
   // how many blocks come back is known on the device only: at most all of the
-  // tables, and 64 workgroups share more than that many shares
-  const int64_t most = B * width < n_free ? B * width : n_free;
-  const int64_t cap = 64 * kTableTokens;
-  return run_tables<false>(p, most < cap ? most : cap, reinterpret_cast<hipStream_t>(stream), "ltx_kv_block_release");
+  // tables; 64 workgroups take turns where there are more than one round of them
+  const int64_t most = ceil_div(B * width < n_free ? B * width : n_free, kTableTokens);
+  return run_tables<false>(p, most < 64 ? most : 64, reinterpret_cast<hipStream_t>(stream), "ltx_kv_block_release");
 }
 
 extern "C" int ltx_kv_paged_append(int kv_dtype, int64_t T, int64_t H, int64_t D, const void* k, int64_t k_ls,

@@ -167,6 +167,19 @@ __device__ __forceinline__ float load_as_f32<uint16_t>(const uint16_t* p) {
   return bf16_bits_to_f32(*p);
 }
 
+// Inclusive scan over a wave of sums that stop at 2^32 - 1: a sum of numbers
+// that are not negative is right or the largest there is.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  // rows of 16 lanes by shifts, then row 0 into row 1 and 2 into 3, then the first half into the second
+  x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
+  x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  return add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+}
+
 // The last i in [0, n) with sums[i] <= x (sums ascending, sums[0] <= x).
 __device__ __forceinline__ int last_at_most(const int* sums, int n, int x) {
   int lo = 0;

@@ -49,6 +49,7 @@ struct PagedAttn {
   // split form: `ranges` equal shares of all requests' tiles, each at least min_tiles
   int ranges, min_tiles, part_heads;
   float *part_o, *part_ml;     // [range][key head group][2][part_heads][D], [..][2]
+  int4* joins;                 // [range]: the request that range continues first (-1: none), its ranges, its first slot
 };
 
 template <int D, bool FP8>
@@ -64,28 +65,23 @@ struct TokenTile {
 // request, so that an empty one's result is written too), first[B] their
 // number: a scan by 256 threads.
 __device__ __forceinline__ int first_tiles(const PagedAttn& p, int* first) {
-  __shared__ int s_wave[4];
+  __shared__ uint32_t s_wave[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int each = (p.B + 255) / 256, b0 = tid * each, b1 = min(b0 + each, p.B);
   const int capacity = p.width << p.shift;
   auto tiles = [&](int b) { return max(1, (min(max(p.lens[b], 0), capacity) + kTokenTile - 1) / kTokenTile); };
-  int mine = 0;
+  uint32_t mine = 0;
   for (int b = b0; b < b1; ++b) mine += tiles(b);
-  int sum = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int x = __shfl_up(sum, d);
-    if (lane >= d) sum += x;
-  }
+  uint32_t sum = wave_scan(mine);
   if (lane == 63) s_wave[wave] = sum;
   __syncthreads();
-  int all = 0;
+  uint32_t all = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     if (w < wave) sum += s_wave[w];
     all += s_wave[w];
   }
-  int at = sum - mine;
+  int at = (int)(sum - mine);
   for (int b = b0; b < b1; ++b) {
     first[b] = at;
     at += tiles(b);
@@ -129,11 +125,15 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
   // keys [t0, t1) tiles of request b: the four waves' shares joined, then
   // written as the result (slot < 0) or as a partial one
   auto attend = [&](int b, int t0, int t1, int slot) {
-    const int len = __builtin_amdgcn_readfirstlane(length(b));
-    const int end = min(len, t1 * kTokenTile);
-    const int key_w = t0 * kTokenTile + wave * 32;  // this wave's first key
-    const int n = end > key_w ? (end - key_w + kTokenTile - 1) / kTokenTile : 0;
     const int32_t* const row = p.tables + b * p.t_bs;
+    const int key_w = t0 * kTokenTile + wave * 32;  // this wave's first key
+    // the block ids of this wave's next 32 tiles, two halves each, one a lane
+    auto ids_of = [&](int i) {
+      const int64_t key = (int64_t)key_w + (int64_t)(i + (lane >> 1)) * kTokenTile + (lane & 1) * 16;
+      const int64_t j = key >> p.shift;
+      return row[j < p.width ? j : p.width - 1];
+    };
+    int ids = ids_of(0), ids_next = 0;  // before the length is known: one wait for both
 
     bf16x8_t qf[KS];
 #pragma unroll
@@ -144,14 +144,9 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
       qf[s] = __builtin_bit_cast(bf16x8_t, x);
     }
 
-    // the block ids of this wave's next 32 tiles, two halves each, one a lane
-    auto ids_of = [&](int i) {
-      const int64_t key = (int64_t)key_w + (int64_t)(i + (lane >> 1)) * kTokenTile + (lane & 1) * 16;
-      const int64_t j = key >> p.shift;
-      return row[j < p.width ? j : p.width - 1];
-    };
-    int ids = 0, ids_next = 0;
-    if (n > 0) ids = ids_of(0);
+    const int len = __builtin_amdgcn_readfirstlane(length(b));
+    const int end = min(len, t1 * kTokenTile);
+    const int n = end > key_w ? (end - key_w + kTokenTile - 1) / kTokenTile : 0;
     if (n > 32) ids_next = ids_of(32);
 
     // tile i's loads; lim[t]: how many keys of half t take part
@@ -339,10 +334,19 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
   } else {
     const int total = first_tiles(p, s_first);
     const int per = max(p.min_tiles, (total + p.ranges - 1) / p.ranges);
-    const int64_t r0 = (int64_t)blockIdx.x * per;
-    if (r0 >= total) return;
+    const int x = (int)blockIdx.x;
+    const int64_t r0 = (int64_t)x * per;
+    const bool keeper = blockIdx.y == 0 && tid == 0;
+    if (r0 >= total) {
+      if (keeper) p.joins[x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
     const int r1 = (int)min(r0 + per, (int64_t)total);
     int b = last_at_most(s_first, p.B, (int)r0);
+    if (keeper) {  // the join's work: a request that the range before this one began
+      const int st = s_first[b], xa = st / per;
+      p.joins[x] = make_int4(st < r0 && xa + 1 == x ? b : -1, xa, (s_first[b + 1] - 1) / per, st == xa * per ? 0 : 1);
+    }
     for (int r = (int)r0; r < r1; ++b) {
       const int st = s_first[b], en = s_first[b + 1], to = min(r1, en);
       attend(b, r - st, to - st, r == st && to == en ? -1 : r == r0 ? 0 : 1);
@@ -352,33 +356,25 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
 }
 
 // Joins the partial results of the requests that several ranges share:
-// workgroup (x, key head group, head) takes the request that ends range x's
-// predecessor, if range x is the first that continues it.  Eight teams of
-// threads take every eighth partial result each.
+// workgroup (x, key head group, head) takes the request that range x is the
+// first to continue, if there is one.  Eight teams of threads take every
+// eighth partial result each.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttn p) {
   constexpr int TEAM = D / 4, TEAMS = 256 / TEAM;
   __shared__ __attribute__((aligned(16))) float s_o[TEAMS][D];
   __shared__ float s_ml[TEAMS][2];
-  extern __shared__ int s_first[];
   const int grp = (int)blockIdx.y % p.groups, kvh = (int)blockIdx.y / p.groups, h = blockIdx.z;
-  if (grp * 16 + h >= p.G) return;
-  const int total = first_tiles(p, s_first);
-  const int per = max(p.min_tiles, (total + p.ranges - 1) / p.ranges);
-  const int x = (int)blockIdx.x + 1;
-  const int64_t r0 = (int64_t)x * per;
-  if (r0 >= total) return;
-  const int b = last_at_most(s_first, p.B, (int)r0);
-  const int st = s_first[b], en = s_first[b + 1];
-  if (st == r0 || st / per + 1 != x) return;
-  const int xa = x - 1, xb = (en - 1) / per;
+  const int4 job = p.joins[blockIdx.x + 1];
+  const int b = job.x, xa = job.y, xb = job.z;
+  if (b < 0 || grp * 16 + h >= p.G) return;
 
   const int team = threadIdx.x / TEAM, d = threadIdx.x % TEAM * 4;
   float m = -INFINITY, l = 0.0f;
   f32x4_t acc{};
 #pragma unroll 4
   for (int i = xa + team; i <= xb; i += TEAMS) {
-    const int slot = i == xa && st != i * per ? 1 : 0;
+    const int slot = i == xa ? job.w : 0;
     const int64_t at = (((int64_t)i * gridDim.y + blockIdx.y) * 2 + slot) * p.part_heads + h;
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
     const f32x4_t o = *reinterpret_cast<const f32x4_t*>(p.part_o + at * D + d);
@@ -416,7 +412,8 @@ using namespace ltx;
 
 struct TokenPlan {
   int64_t y, ranges, part_heads;  // ranges 0: one workgroup a request and key head group
-  int64_t bytes() const { return ranges * y * 2 * part_heads; }
+  int64_t parts() const { return ranges * y * 2 * part_heads; }
+  int64_t bytes(int64_t D) const { return parts() * (D + 2) * 4 + ranges * 16; }
 };
 
 // Requests that can hold few tokens only take a workgroup each, one launch.
@@ -441,7 +438,7 @@ extern "C" int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, i
   LTX_REQUIRE(bytes != nullptr && B >= 0 && Hk >= 1 && G >= 1 && D >= 1 && width >= 0 && block >= 1,
               "ltx_paged_attn_workspace_size: bad argument");
   const TokenPlan t = plan_token(B, Hk, G, width * block);
-  *bytes = t.bytes() * (D + 2) * 4;
+  *bytes = t.bytes(D);
   return LTX_OK;
 }
 
@@ -455,7 +452,7 @@ static void launch_token(const PagedAttn& p, const TokenPlan& t, hipStream_t st)
   }
   hipLaunchKernelGGL((paged_attn_kernel<D, FP8, true>), dim3((unsigned)t.ranges, y), threads, lds, st, p);
   if (t.ranges > 1)
-    hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)t.ranges - 1, y, (unsigned)t.part_heads), dim3(256), lds,
+    hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)t.ranges - 1, y, (unsigned)t.part_heads), dim3(256), 0,
                        st, p);
 }
 
@@ -493,7 +490,7 @@ extern "C" int ltx_paged_attn(int kv_dtype, int64_t B, int64_t Hk, int64_t G, in
   LTX_REQUIRE(!fp8 || ((uintptr_t)k_scales % 16 == 0 && (uintptr_t)v_scales % 16 == 0 && sc_ps % 4 == 0 && sc_hs % 4 == 0),
               "%s: scales of a block and head must be 16-byte aligned", name);
   const TokenPlan t = plan_token(B, Hk, G, width * block);
-  const int64_t need = t.bytes() * (D + 2) * 4;
+  const int64_t need = t.bytes(D);
   LTX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
               "%s: needs %lld bytes of workspace", name, (long long)need);
   PagedAttn p{};
@@ -508,8 +505,11 @@ extern "C" int ltx_paged_attn(int kv_dtype, int64_t B, int64_t Hk, int64_t G, in
   p.width = (int)width, p.shift = shift, p.n_blocks = (int)n_blocks;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)D)) * kLog2e;
   p.ranges = (int)t.ranges, p.min_tiles = (int)kTokenMinTiles, p.part_heads = (int)t.part_heads;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o != nullptr ? p.part_o + t.bytes() * D : nullptr;
+  if (t.ranges > 0) {
+    p.joins = static_cast<int4*>(workspace);
+    p.part_o = reinterpret_cast<float*>(p.joins + t.ranges);
+    p.part_ml = p.part_o + t.parts() * D;
+  }
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (D == 128) {
     if (fp8) launch_token<128, true>(p, t, st);

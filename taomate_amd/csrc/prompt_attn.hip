@@ -29,6 +29,7 @@ namespace ltx {
 
 constexpr int kRows = 128;  // rows of a workgroup
 constexpr int kKeys = 64;   // keys of a tile
+constexpr int kResident = 512;  // workgroups that run at once: two a CU
 
 struct PromptAttn {
   const uint16_t* q;
@@ -39,7 +40,7 @@ struct PromptAttn {
   int64_t k_hs, v_hs;
   int k_ls, v_ls;
   const int32_t *q_starts, *k_starts;
-  int B, Tq, Tk, Hk, G, causal, zero_tail;
+  int B, Tq, Tk, Hk, G, causal, zero_tail, sorted;
   float scale_log2;
 };
 
@@ -49,36 +50,47 @@ struct PromptRows {
   int q0, k0, row0, Lq, Lk;
 };
 
-// Row tile t counted from the last tile of the last prompt backwards (late
-// rows of a causal prompt see the most keys, so the long tiles start first).
+// Row tile t in the order in which the workgroups start: a prompt's last tile
+// first (late rows of a causal prompt see the most keys), the last prompt first;
+// with `sorted` (up to 64 prompts) the prompt with the most keys first, so that a
+// grid of several rounds ends with its short tiles.
 // False: there are fewer tiles; q0 is then the first row behind the prompts and
 // row0 the distance of tile t's rows from it.
 __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows& r) {
   const int lane = threadIdx.x & 63;
   for (int b0 = p.B - 1; b0 >= 0; b0 -= 64) {
     const int b = b0 - lane;
-    int s = 0, n = 0;
+    int s = 0, n = 0, ks = 0, m = 0;
     if (b >= 0) {
-      s = min(max(p.q_starts[b], 0), p.Tq);
-      n = min(max(p.q_starts[b + 1], s), p.Tq) - s;
+      const int s0 = p.q_starts[b], s1 = p.q_starts[b + 1], k0 = p.k_starts[b], k1 = p.k_starts[b + 1];
+      s = min(max(s0, 0), p.Tq);
+      n = min(max(s1, s), p.Tq) - s;
+      ks = min(max(k0, 0), p.Tk);
+      m = min(max(k1, ks), p.Tk) - ks;
+    }
+    if (p.sorted) {
+      int rank = 0;  // lanes with more keys, or as many and before this one
+      for (int i = 0; i < p.B; ++i) {
+        const int other = __builtin_amdgcn_readlane(m, i);
+        rank += (other > m || (other == m && i < lane)) ? 1 : 0;
+      }
+      if (lane >= p.B) rank = lane;
+      s = __builtin_amdgcn_ds_permute(rank * 4, s);
+      n = __builtin_amdgcn_ds_permute(rank * 4, n);
+      ks = __builtin_amdgcn_ds_permute(rank * 4, ks);
+      m = __builtin_amdgcn_ds_permute(rank * 4, m);
     }
     const int tiles = (n + kRows - 1) / kRows;
-    int sum = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int x = __shfl_up(sum, d);
-      if (lane >= d) sum += x;
-    }
+    const int sum = (int)wave_scan((uint32_t)tiles);
     const uint64_t past = __builtin_amdgcn_ballot_w64(sum > t);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       const int before = __builtin_amdgcn_readlane(sum - tiles, at);
-      const int bb = b0 - at;
       r.q0 = __builtin_amdgcn_readlane(s, at);
       r.Lq = __builtin_amdgcn_readlane(n, at);
+      r.k0 = __builtin_amdgcn_readlane(ks, at);
+      r.Lk = __builtin_amdgcn_readlane(m, at);
       r.row0 = (__builtin_amdgcn_readlane(tiles, at) - 1 - (t - before)) * kRows;
-      r.k0 = __builtin_amdgcn_readfirstlane(min(max(p.k_starts[bb], 0), p.Tk));
-      r.Lk = __builtin_amdgcn_readfirstlane(min(max(p.k_starts[bb + 1], r.k0), p.Tk)) - r.k0;
       return true;
     }
     t -= __builtin_amdgcn_readlane(sum, 63);
@@ -129,6 +141,11 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   // keys that some row of the workgroup sees
   const int seen = p.causal ? min(w.Lk, min(w.Lq, w.row0 + kRows) + shift) : w.Lk;
   const int ntiles = seen > 0 ? (seen + BN - 1) / BN : 0;
+  // and of this wave: past the last key of its rows, or without rows, it only
+  // takes part in the loads
+  const int row_w = w.row0 + wave * 32;
+  const int wave_seen = row_w >= w.Lq ? 0 : p.causal ? min(seen, row_w + 32 + shift) : seen;
+  const int wtiles = max(1, (max(wave_seen, 0) + BN - 1) / BN);
 
   // ---- per-lane load offsets (bytes from a tile's first key), loop invariant:
   // slot i of wave w fills LDS chunks (w + 4 i) * 64 + lane, a uniform number
@@ -472,17 +489,23 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
     int j = 1;
-    for (; j + 1 < ntiles; j += 2) {
+    for (; j + 1 < wtiles; j += 2) {
       step(j, odd, sb, sa, pa, pb);
       step(j + 1, even, sa, sb, pb, pa);
     }
-    if (j < ntiles) step(j, odd, sb, sa, pa, pb);
-    // ---- epilogue: O += V(n-1)^T P(n-1) ----
+    if (j < wtiles) step(j, odd, sb, sa, pa, pb);
+    // ---- the wave's last tile: O += V(n-1)^T P(n-1); then only loads for the
+    //      waves whose rows see further ----
     publish();
-    if ((ntiles - 1) & 1)
+    if ((wtiles - 1) & 1)
       pv_tile(1, pb);
     else
       pv_tile(0, pa);
+    for (j = wtiles; j < ntiles; ++j) {
+      if (j + 2 < ntiles) issue_k(j & 1);
+      issue_v(j & 1);
+      publish();
+    }
   }
 
   // ---- normalise and store: the wave's 32 rows go through LDS (16-byte chunks
@@ -501,7 +524,6 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
           make_uint2(pack_bf16x2(oacc[d][n][0] * inv[n], oacc[d][n][1] * inv[n]),
                      pack_bf16x2(oacc[d][n][2] * inv[n], oacc[d][n][3] * inv[n]));
   __syncthreads();
-  const int row_w = w.row0 + wave * 32;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
     const int ch = i * 64 + lane, r = ch / NKC, cc = ch % NKC;
@@ -556,6 +578,8 @@ extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, in
   const int64_t tiles = ceil_div(Tq, kRows) + B;
   const int64_t grid = ceil_div(tiles * Hk, 8) * 8 * G;
   LTX_REQUIRE(grid <= 0x7FFFFFFF, "%s: too many rows and heads for one launch", name);
+  // a grid that is resident at once needs no order
+  p.sorted = B > 1 && B <= 64 && grid > kResident;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (D == 128)
     hipLaunchKernelGGL((prompt_attn_kernel<128>), dim3((unsigned)grid), dim3(256), 0, st, p);

@@ -166,6 +166,7 @@ PROMPTS = [
     ([129, 1, 0, 64], [129, 1, 0, 64], 6, 2, 128), ([5, 200, 63, 65], [105, 200, 64, 1000], 4, 4, 64),
     ([300], [300], 7, 1, 64), ([40, 130], [20, 100], 4, 2, 128), ([10, 10], [0, 5], 2, 2, 64),
     ([257] * 5, [257] * 5, 16, 2, 128), ([1] * 70, list(range(70)), 3, 3, 64), ([640], [640], 24, 8, 128),
+    ([300, 20, 700, 0, 128, 129, 1, 555], [300, 520, 700, 3, 128, 100, 1, 600], 32, 4, 64),
 ]
 
 

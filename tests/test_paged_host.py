@@ -145,5 +145,5 @@ def test_workspace_of_the_split():
     n = ctypes.c_int64()
     size = lambda *a: (_native.call("ltx_paged_attn_workspace_size", *a, ctypes.byref(n)), n.value)[1]  # noqa: E731
     assert size(64, 8, 4, 128, 64, 16) == 0                  # tables of 1024 tokens: a workgroup a request
-    assert size(64, 8, 4, 128, 65, 16) == 64 * 8 * 2 * 4 * 130 * 4
-    assert size(1, 8, 4, 128, 65, 16) == 5 * 8 * 2 * 4 * 130 * 4
+    assert size(64, 8, 4, 128, 65, 16) == 64 * 8 * 2 * 4 * 130 * 4 + 64 * 16
+    assert size(1, 8, 4, 128, 65, 16) == 5 * 8 * 2 * 4 * 130 * 4 + 5 * 16
