@@ -514,6 +514,9 @@ int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, int64_t D, i
  *   are.  Starts that are not ascending or pass Tq or Tk are cut, never followed.
  *   lse: NULL or float32 [Hk * G, Tq]; scale <= 0 selects 1/sqrt(D).
  *   Rows of every tensor 16-byte aligned.
+ *   workspace: ltx_prompt_attn_workspace_size() bytes, 16-byte aligned (0: none; few
+ *   rows over many keys share the keys among workgroups).  Calls that overlap in
+ *   time must use different workspaces.
  *   A value that is not finite in v spoils every row of its prompt whose 128-row
  *   tile sees its key; keys' values that a row does not see do not matter.
  */
@@ -521,7 +524,9 @@ int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, in
                     int64_t q_ls, int64_t q_hs, const void* k, int64_t k_ls, int64_t k_hs, const void* v,
                     int64_t v_ls, int64_t v_hs, const int32_t* q_starts, const int32_t* k_starts, int causal,
                     void* out, int64_t o_ls, int64_t o_hs, int zero_tail, float* lse, float scale,
-                    void* stream);
+                    void* workspace, int64_t workspace_bytes, void* stream);
+int ltx_prompt_attn_workspace_size(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D,
+                                   int64_t* bytes);
 
 #ifdef __cplusplus
 }

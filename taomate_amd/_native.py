@@ -83,7 +83,8 @@ SIGNATURES = {
                        _i64, _ptr],
     "ltx_paged_attn_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64, _ptr],
     "ltx_prompt_attn": [_i64, _i64, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr,
-                        _ptr, _int, _ptr, _i64, _i64, _int, _ptr, _f32, _ptr],
+                        _ptr, _int, _ptr, _i64, _i64, _int, _ptr, _f32, _ptr, _i64, _ptr],
+    "ltx_prompt_attn_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64, _ptr],
     "ltx_group4_linear": [_i64, _i64, _i64, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _i64, _ptr],
 }
 

@@ -58,6 +58,7 @@ struct Api {
   decltype(&ltx_paged_attn) paged_attn;
   decltype(&ltx_paged_attn_workspace_size) paged_attn_workspace_size;
   decltype(&ltx_prompt_attn) prompt_attn;
+  decltype(&ltx_prompt_attn_workspace_size) prompt_attn_workspace_size;
 } api;
 PyObject* native_call_error = nullptr;  // taomate_amd._native.NativeCallError
 
@@ -980,10 +981,18 @@ PyObject* prompt_attn(PyObject* const* a) {
     value_error("prompt_attn: lse must be contiguous float32 [heads, tokens]");
   const c10::DeviceGuard guard(q.device());
   const at::Tensor o = rows_out(what, out, q);
-  call("ltx_prompt_attn", api.prompt_attn, n - 1, rq.T, rk.T, rk.H, rq.H / rk.H, rq.D, ptr(&q), rq.ls, rq.hs, ptr(&k),
-       rk.ls, rk.hs, ptr(&v), rv.ls, rv.hs, ptr_as<const int32_t>(&starts), ptr_as<const int32_t>(&k_starts),
-       (int)truth(a[5]), ptr(&o), stride_of(o, 0), stride_of(o, 1), (int)(out == nullptr), ptr_as(lse), scale,
-       stream_of(q));
+  const int64_t B = n - 1, G = rq.H / rk.H;
+  int64_t need = 0;
+  call("ltx_prompt_attn_workspace_size", api.prompt_attn_workspace_size, B, rq.T, rk.T, rk.H, G, rq.D, &need);
+  const int causal = truth(a[5]);
+  void* st = stream_of(q);
+  released("ltx_prompt_attn", [&] {
+    const Scratch ws(q, st, need);
+    return api.prompt_attn(B, rq.T, rk.T, rk.H, G, rq.D, ptr(&q), rq.ls, rq.hs, ptr(&k), rk.ls, rk.hs, ptr(&v), rv.ls,
+                           rv.hs, ptr_as<const int32_t>(&starts), ptr_as<const int32_t>(&k_starts), causal, ptr(&o),
+                           stride_of(o, 0), stride_of(o, 1), (int)(out == nullptr), ptr_as(lse), scale, ws.ptr(),
+                           ws.bytes(), st);
+  });
   if (out == nullptr) return THPVariable_Wrap(o);
   Py_INCREF(a[7]);
   return a[7];
@@ -1095,6 +1104,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   get("ltx_paged_attn", next.paged_attn);
   get("ltx_paged_attn_workspace_size", next.paged_attn_workspace_size);
   get("ltx_prompt_attn", next.prompt_attn);
+  get("ltx_prompt_attn_workspace_size", next.prompt_attn_workspace_size);
   if (!ok) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: missing entry point addresses");
     return nullptr;

@@ -40,24 +40,29 @@ struct PromptAttn {
   int64_t k_hs, v_hs;
   int k_ls, v_ls;
   const int32_t *q_starts, *k_starts;
-  int B, Tq, Tk, Hk, G, causal, zero_tail, sorted;
+  int B, Tq, Tk, Hk, G, causal, zero_tail, sorted, tiles;
   float scale_log2;
+  // SPLIT: a row tile's key tiles are shared by up to `split` workgroups, whose
+  // results [workgroup][range][row][D] and (maximum, sum) are joined afterwards
+  int split;
+  float *part_o, *part_ml;
 };
 
-// Where a workgroup works: rows [row0, rows) of a prompt whose rows start at q0
-// and whose Lk keys start at k0 of the packed tensors.
+// Where a workgroup works: rows from row0 of a prompt whose Lq rows start at q0 and
+// whose Lk keys start at k0 of the packed tensors; end: the first row behind
+// all prompts.
 struct PromptRows {
-  int q0, k0, row0, Lq, Lk;
+  int q0, k0, row0, Lq, Lk, end;
 };
 
 // Row tile t in the order in which the workgroups start: a prompt's last tile
 // first (late rows of a causal prompt see the most keys), the last prompt first;
-// with `sorted` (up to 64 prompts) the prompt with the most keys first, so that a
+// with `sorted` (up to 64 prompts) the prompts with the most keys first, so that a
 // grid of several rounds ends with its short tiles.
-// False: there are fewer tiles; q0 is then the first row behind the prompts and
-// row0 the distance of tile t's rows from it.
+// False: there are fewer tiles.
 __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows& r) {
   const int lane = threadIdx.x & 63;
+  r.end = 0;
   for (int b0 = p.B - 1; b0 >= 0; b0 -= 64) {
     const int b = b0 - lane;
     int s = 0, n = 0, ks = 0, m = 0;
@@ -68,13 +73,18 @@ __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows
       ks = min(max(k0, 0), p.Tk);
       m = min(max(k1, ks), p.Tk) - ks;
     }
+    if (b0 == p.B - 1) r.end = __builtin_amdgcn_readfirstlane(s + n);
     if (p.sorted) {
-      int rank = 0;  // lanes with more keys, or as many and before this one
-      for (int i = 0; i < p.B; ++i) {
-        const int other = __builtin_amdgcn_readlane(m, i);
-        rank += (other > m || (other == m && i < lane)) ? 1 : 0;
+      // by the power of two of their number of key tiles: one ballot a power
+      const int mine = 32 - __builtin_clz(m / kKeys + 1);
+      int rank = lane, before = 0;
+      for (int power = p.sorted; power > 0; --power) {
+        const bool here = mine == power && lane < p.B;
+        const uint64_t all = __builtin_amdgcn_ballot_w64(here);
+        const int at = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+        rank = here ? at : rank;
+        before += __builtin_popcountll(all);
       }
-      if (lane >= p.B) rank = lane;
       s = __builtin_amdgcn_ds_permute(rank * 4, s);
       n = __builtin_amdgcn_ds_permute(rank * 4, n);
       ks = __builtin_amdgcn_ds_permute(rank * 4, ks);
@@ -95,12 +105,37 @@ __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows
     }
     t -= __builtin_amdgcn_readlane(sum, 63);
   }
-  r.q0 = __builtin_amdgcn_readfirstlane(min(max(p.q_starts[p.B], 0), p.Tq));
-  r.row0 = t * kRows;
   return false;
 }
 
-template <int D>
+// The row tile and heads of a workgroup.  Workgroups are dispatched round-robin
+// over the 8 XCDs.  The G heads that share a key head's keys run side by side on
+// one XCD (one L2), and the XCDs take the (row tile, key head) pairs in turn, so
+// each gets long and short ones.
+__device__ __forceinline__ int unit_of(const PromptAttn& p, int& kvh, int& h) {
+  const int slot = (int)blockIdx.x >> 3;
+  const int unit = slot / p.G * 8 + ((int)blockIdx.x & 7);
+  kvh = unit % p.Hk;
+  h = kvh * p.G + slot % p.G;
+  return unit / p.Hk;
+}
+
+// keys that some row of the tile sees
+__device__ __forceinline__ int seen_keys(const PromptAttn& p, const PromptRows& w) {
+  const int seen = p.causal ? min(w.Lk, min(w.Lq, w.row0 + kRows) + w.Lk - w.Lq) : w.Lk;
+  return max(seen, 0);
+}
+
+// How many workgroups share a row tile that sees `seen` keys, and the key tiles of each.
+constexpr int kMinPart = 4;
+__device__ __forceinline__ int parts_of(const PromptAttn& p, int seen, int& tiles) {
+  const int all = (seen + kKeys - 1) / kKeys;
+  const int parts = max(1, min(p.split, all / kMinPart));
+  tiles = (all + parts - 1) / parts;
+  return tiles > 0 ? (all + tiles - 1) / tiles : 1;
+}
+
+template <int D, bool SPLIT>
 __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   constexpr int BN = kKeys;
   constexpr int NKC = D / 8;             // 16-byte chunks of a row
@@ -116,32 +151,41 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   uint16_t* const kbuf = smem;
   uint16_t* const vbuf = smem + 2 * BUF;
 
-  // Workgroups are dispatched round-robin over the 8 XCDs.  The G heads that
-  // share a key head's keys run side by side on one XCD (one L2), and the XCDs
-  // take the (row tile, key head) pairs in turn, so each gets long and short ones.
-  const int slot = (int)blockIdx.x >> 3;
-  const int unit = slot / p.G * 8 + ((int)blockIdx.x & 7);
-  const int kvh = unit % p.Hk, h = kvh * p.G + slot % p.G;
+  int kvh, h;
+  const int unit = unit_of(p, kvh, h);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63;
   const int li = lane & 15, lg = lane >> 4;
   PromptRows w;
-  if (!find_rows(p, unit / p.Hk, w)) {
-    if (!p.zero_tail) return;
-    for (int i = threadIdx.x; i < kRows * NKC; i += 256) {
-      const int64_t row = (int64_t)w.q0 + w.row0 + i / NKC;
-      if (row >= p.Tq) break;
-      *reinterpret_cast<uint4*>(p.o + row * p.o_ls + h * p.o_hs + i % NKC * 8) = make_uint4(0, 0, 0, 0);
-      if (p.lse != nullptr && i % NKC == 0) p.lse[(int64_t)h * p.Tq + row] = -INFINITY;
-    }
-    return;
+  const bool works = find_rows(p, unit, w);
+  if (p.zero_tail && w.end < p.Tq && (!SPLIT || blockIdx.y == 0)) {
+    // rows behind the prompts, shared by all row tiles
+    for (int64_t row0 = w.end + (int64_t)unit * kRows; row0 < p.Tq; row0 += (int64_t)p.tiles * kRows)
+      for (int i = threadIdx.x; i < kRows * NKC; i += 256) {
+        const int64_t row = row0 + i / NKC;
+        if (row >= p.Tq) break;
+        *reinterpret_cast<uint4*>(p.o + row * p.o_ls + h * p.o_hs + i % NKC * 8) = make_uint4(0, 0, 0, 0);
+        if (p.lse != nullptr && i % NKC == 0) p.lse[(int64_t)h * p.Tq + row] = -INFINITY;
+      }
   }
+  if (!works) return;
   const int q0 = w.row0 + wave * 32 + li;  // this lane's queries: q0 and q0 + 16
-  const int shift = w.Lk - w.Lq;           // causal: row i sees keys up to i + shift
-  // keys that some row of the workgroup sees
-  const int seen = p.causal ? min(w.Lk, min(w.Lq, w.row0 + kRows) + shift) : w.Lk;
-  const int ntiles = seen > 0 ? (seen + BN - 1) / BN : 0;
-  // and of this wave: past the last key of its rows, or without rows, it only
+  int shift = w.Lk - w.Lq;                 // causal: row i sees keys up to i + shift
+  int seen = seen_keys(p, w);
+  int parts = 1;
+  if constexpr (SPLIT) {
+    // this workgroup's share: the prompt without the keys before and after it
+    int tiles;
+    parts = parts_of(p, seen, tiles);
+    if ((int)blockIdx.y >= parts) return;
+    const int skip = (int)blockIdx.y * tiles * BN;
+    w.k0 += skip;
+    w.Lk -= skip;
+    shift -= skip;
+    seen = min(seen - skip, tiles * BN);
+  }
+  const int ntiles = (seen + BN - 1) / BN;
+  // of this wave: past the last key of its rows, or without rows, it only
   // takes part in the loads
   const int row_w = w.row0 + wave * 32;
   const int wave_seen = row_w >= w.Lq ? 0 : p.causal ? min(seen, row_w + 32 + shift) : seen;
@@ -508,6 +552,22 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
     }
   }
 
+  if constexpr (SPLIT) {
+    if (parts > 1) {
+      const int64_t at = ((int64_t)blockIdx.x * p.split + blockIdx.y) * kRows + wave * 32 + li;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float l = quad_sum(l_run[n]);
+        if (q0 + 16 * n >= w.Lq) continue;
+#pragma unroll
+        for (int d = 0; d < CB; ++d)
+          *reinterpret_cast<f32x4_t*>(p.part_o + (at + 16 * n) * D + 16 * d + 4 * lg) = oacc[d][n];
+        if (lg == 0) *reinterpret_cast<float2*>(p.part_ml + (at + 16 * n) * 2) = make_float2(m_run[n], l);
+      }
+      return;
+    }
+  }
+
   // ---- normalise and store: the wave's 32 rows go through LDS (16-byte chunks
   // xor-swizzled by row), so that a store instruction covers whole rows ----
   const float l_tot[2] = {quad_sum(l_run[0]), quad_sum(l_run[1])};
@@ -538,20 +598,94 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
           l_tot[n] == 0.0f ? -INFINITY : (m_run[n] + __log2f(l_tot[n])) / kLog2e;
 }
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(const PromptAttn p) {
-  prompt_body<D>(p);
+  prompt_body<D, SPLIT>(p);
+}
+
+// Joins the key ranges of a row tile: a thread takes 4 channels of a row.
+template <int D>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptAttn p) {
+  int kvh, h;
+  PromptRows w;
+  if (!find_rows(p, unit_of(p, kvh, h), w)) return;
+  int tiles;
+  const int parts = parts_of(p, seen_keys(p, w), tiles);
+  const int i = (int)blockIdx.y * 256 + threadIdx.x, row = i / (D / 4), d = i % (D / 4) * 4;
+  if (parts <= 1 || w.row0 + row >= w.Lq) return;
+  const int64_t first = (int64_t)blockIdx.x * p.split;
+  float m = -INFINITY, l = 0.0f;
+  f32x4_t acc{};
+#pragma unroll 4
+  for (int r = 0; r < parts; ++r) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((first + r) * kRows + row) * 2);
+    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(p.part_o + ((first + r) * kRows + row) * D + d);
+    const float m_new = fmaxf(m, ml.x);
+    const float fa = __builtin_amdgcn_exp2f(m - m_new), fb = __builtin_amdgcn_exp2f(ml.x - m_new);
+    l = l * fa + ml.y * fb;
+    acc = acc * fa + o * fb;
+    m = m_new;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t at = w.q0 + w.row0 + row;
+  *reinterpret_cast<uint2*>(p.o + at * p.o_ls + h * p.o_hs + d) =
+      make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  if (p.lse != nullptr && d == 0)
+    p.lse[(int64_t)h * p.Tq + at] = l == 0.0f ? -INFINITY : (m + __log2f(l)) / kLog2e;
 }
 
 }  // namespace ltx
 
 using namespace ltx;
 
+// Workgroups of a call and how many may share a row tile.  Few rows over many
+// keys leave most CUs idle, so the keys are split where row tiles and heads fill
+// at most a quarter of the resident workgroups (half of them run each almost
+// twice as fast alone: 1024 rows over 4096 keys, 32 heads, 79 us split and 78
+// whole) and the prompts have keys enough to pay for the join: 768 on average,
+// 2048 above an eighth (32/8 heads x 128: 16 rows over 1024 keys 12.0 us and 20.6
+// whole, over 512 no difference; 512 rows over 2048 34 and 41, over 1024 28 and 22).
+struct PromptPlan {
+  int64_t tiles, grid, split;
+  int64_t bytes(int64_t D) const { return split > 1 ? grid * split * kRows * (D + 2) * 4 : 0; }
+};
+static PromptPlan plan_prompt(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G) {
+  // the most row tiles of B prompts with Tq rows: B of one row, and full ones
+  const int64_t some = B < Tq ? B : Tq, tiles = some + (Tq - some) / kRows;
+  PromptPlan t{tiles, ceil_div((tiles > 0 ? tiles : 1) * Hk, 8) * 8 * G, 1};
+  if (Tq > 0 && t.grid * 4 <= kResident && Tk >= B * (t.grid * 8 <= kResident ? 768 : 2048)) {
+    t.split = kResident / t.grid;
+    if (t.split > 16) t.split = 16;
+  }
+  return t;
+}
+
+extern "C" int ltx_prompt_attn_workspace_size(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D,
+                                              int64_t* bytes) {
+  clear_error();
+  LTX_REQUIRE(bytes != nullptr && B >= 0 && B <= LTX_MAX_REQUESTS && Tq >= 0 && Tk >= 0 && Tq <= 0x40000000 &&
+                  Tk <= 0x40000000 && Hk >= 1 && G >= 1 && Hk <= 65535 && G <= 65535 && D >= 1 && D <= 65535,
+              "ltx_prompt_attn_workspace_size: bad argument");
+  *bytes = plan_prompt(B, Tq, Tk, Hk, G).bytes(D);
+  return LTX_OK;
+}
+
+template <int D>
+static void launch_prompt(const PromptAttn& p, const PromptPlan& t, hipStream_t st) {
+  const dim3 threads(256);
+  if (t.split <= 1) {
+    hipLaunchKernelGGL((prompt_attn_kernel<D, false>), dim3((unsigned)t.grid), threads, 0, st, p);
+    return;
+  }
+  hipLaunchKernelGGL((prompt_attn_kernel<D, true>), dim3((unsigned)t.grid, (unsigned)t.split), threads, 0, st, p);
+  hipLaunchKernelGGL((prompt_join_kernel<D>), dim3((unsigned)t.grid, kRows * (D / 4) / 256), threads, 0, st, p);
+}
+
 extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D, const void* q,
                                int64_t q_ls, int64_t q_hs, const void* k, int64_t k_ls, int64_t k_hs, const void* v,
                                int64_t v_ls, int64_t v_hs, const int32_t* q_starts, const int32_t* k_starts, int causal,
                                void* out, int64_t o_ls, int64_t o_hs, int zero_tail, float* lse, float scale,
-                               void* stream) {
+                               void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   const char* const name = "ltx_prompt_attn";
   LTX_REQUIRE(B >= 0 && B <= LTX_MAX_REQUESTS, "%s: %lld prompts, at most %d", name, (long long)B, LTX_MAX_REQUESTS);
@@ -574,17 +708,22 @@ extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, in
   p.B = (int)B, p.Tq = (int)Tq, p.Tk = (int)Tk, p.Hk = (int)Hk, p.G = (int)G;
   p.causal = causal != 0, p.zero_tail = zero_tail != 0;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)D)) * kLog2e;
-  // row tiles: each prompt ends at most one that is not full
-  const int64_t tiles = ceil_div(Tq, kRows) + B;
-  const int64_t grid = ceil_div(tiles * Hk, 8) * 8 * G;
-  LTX_REQUIRE(grid <= 0x7FFFFFFF, "%s: too many rows and heads for one launch", name);
-  // a grid that is resident at once needs no order
-  p.sorted = B > 1 && B <= 64 && grid > kResident;
+  const PromptPlan t = plan_prompt(B, Tq, Tk, Hk, G);
+  LTX_REQUIRE(t.grid <= 0x7FFFFFFF, "%s: too many rows and heads for one launch", name);
+  const int64_t need = t.bytes(D);
+  LTX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
+              "%s: needs %lld bytes of workspace", name, (long long)need);
+  // the highest power of two of any prompt's key tiles; a grid that is resident at once needs no order
+  p.sorted = B > 1 && B <= 64 && t.grid > kResident ? 32 - __builtin_clz((unsigned)(Tk / kKeys) + 1) : 0;
+  p.tiles = (int)(t.tiles > 0 ? t.tiles : 1);
+  if (t.split > 1) {
+    p.split = (int)t.split;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + t.grid * t.split * kRows * D;
+  }
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (D == 128)
-    hipLaunchKernelGGL((prompt_attn_kernel<128>), dim3((unsigned)grid), dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((prompt_attn_kernel<64>), dim3((unsigned)grid), dim3(256), 0, st, p);
+  if (D == 128) launch_prompt<128>(p, t, st);
+  else launch_prompt<64>(p, t, st);
   LTX_LAUNCH_CHECK(name);
   return LTX_OK;
 }

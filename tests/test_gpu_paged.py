@@ -167,6 +167,9 @@ PROMPTS = [
     ([300], [300], 7, 1, 64), ([40, 130], [20, 100], 4, 2, 128), ([10, 10], [0, 5], 2, 2, 64),
     ([257] * 5, [257] * 5, 16, 2, 128), ([1] * 70, list(range(70)), 3, 3, 64), ([640], [640], 24, 8, 128),
     ([300, 20, 700, 0, 128, 129, 1, 555], [300, 520, 700, 3, 128, 100, 1, 600], 32, 4, 64),
+    # few rows over many keys: shared among workgroups
+    ([5], [3100], 8, 2, 128), ([130, 1], [2500, 4000], 4, 4, 64), ([60], [1100], 3, 1, 128),
+    ([1, 2, 3], [20, 9000, 1], 2, 1, 64), ([300, 10, 0], [200, 4500, 70], 2, 2, 128),
 ]
 
 

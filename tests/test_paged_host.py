@@ -109,7 +109,7 @@ def raw(name, **kw):
                                stream=None),
         "ltx_prompt_attn": dict(B=1, Tq=8, Tk=8, Hk=1, G=1, D=64, q=P, q_ls=64, q_hs=64, k=P, k_ls=64, k_hs=64, v=P,
                                 v_ls=64, v_hs=64, qs=P, ks=P, causal=1, out=P, o_ls=64, o_hs=64, zt=0, lse=None,
-                                scale=0.0, stream=None),
+                                scale=0.0, ws=None, wsb=0, stream=None),
         "ltx_kv_paged_append": dict(kv=1, T=4, H=1, D=64, k=P, k_ls=64, k_hs=64, v=P, v_ls=64, v_hs=64, kp=P, kp_ps=1024,
                                     kp_ts=64, kp_hs=64, vp=P, vp_ps=1024, vp_ts=64, vp_hs=64, ks=None, a=0, b=0, c=0,
                                     vs=None, d=0, e=0, f=0, n=9, block=16, slots=P, stream=None),
@@ -131,7 +131,7 @@ def raw(name, **kw):
     ("ltx_prompt_attn", dict(D=32), "head layout"), ("ltx_prompt_attn", dict(v_ls=60), "16-byte"),
     ("ltx_prompt_attn", dict(k_ls=32), "overlap"), ("ltx_prompt_attn", dict(v_ls=1 << 24), "too far"),
     ("ltx_prompt_attn", dict(B=5000), "at most 4096"), ("ltx_prompt_attn", dict(Tq=1 << 31), "2\\^30"),
-    ("ltx_prompt_attn", dict(k=None), "null"), ("ltx_prompt_attn", dict(out=P + 8), "16-byte"),
+    ("ltx_prompt_attn", dict(k=None), "null"), ("ltx_prompt_attn", dict(Tk=1024), "workspace"), ("ltx_prompt_attn", dict(out=P + 8), "16-byte"),
     ("ltx_kv_paged_append", dict(D=256), "D 64 or 128"), ("ltx_kv_paged_append", dict(block=0), "block of 0"),
     ("ltx_kv_paged_append", dict(kp_ts=66), "pools"), ("ltx_kv_paged_append", dict(k=P + 4), "rows of k and v"),
     ("ltx_kv_paged_append", dict(kv=2), "null"),
@@ -147,3 +147,8 @@ def test_workspace_of_the_split():
     assert size(64, 8, 4, 128, 64, 16) == 0                  # tables of 1024 tokens: a workgroup a request
     assert size(64, 8, 4, 128, 65, 16) == 64 * 8 * 2 * 4 * 130 * 4 + 64 * 16
     assert size(1, 8, 4, 128, 65, 16) == 5 * 8 * 2 * 4 * 130 * 4 + 5 * 16
+    rows = lambda *a: (_native.call("ltx_prompt_attn_workspace_size", *a, ctypes.byref(n)), n.value)[1]  # noqa: E731
+    assert rows(1, 128, 767, 8, 4, 128) == 0                 # too few keys to share
+    assert rows(1, 128, 768, 8, 4, 128) == 32 * 16 * 128 * 130 * 4
+    assert rows(2, 128, 1500, 8, 4, 128) == 0 and rows(8, 1024, 16384, 8, 4, 128) == 0
+    assert rows(1, 512, 2047, 8, 4, 128) == 0 and rows(1, 512, 2048, 8, 4, 128) == 128 * 4 * 128 * 130 * 4
