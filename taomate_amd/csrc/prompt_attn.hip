@@ -29,7 +29,7 @@ namespace ltx {
 
 constexpr int kRows = 128;  // rows of a workgroup
 constexpr int kKeys = 64;   // keys of a tile
-constexpr int kResident = 512;  // workgroups that run at once: two a CU
+constexpr int kResident = 512;  // workgroups that run at once: two a CU (64 channels: three)
 
 struct PromptAttn {
   const uint16_t* q;
@@ -144,6 +144,10 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   constexpr int CB = D / 16;             // 16-channel blocks of O
   constexpr int KS = D / 32;             // 32-channel steps of a score
   constexpr float kOver = 65536.0f;      // largest per-lane tile sum kept without raising m
+  // 64 channels: P(j) takes the registers of P(j-1), each word once its product
+  // is issued, so that three workgroups fit a CU (168 registers): 24 prompts of
+  // up to 1023 rows, 32 heads, 44.7 us and 51.5 with two; 128 channels have no use for it
+  constexpr bool ONE_P = D == 64;
   constexpr float kHuge = 0x1p28f;       // |m| whose last place is 2^4 or more (exp_all)
 
   // K(0), K(1), V(0), V(1), one array: the output staging spans them
@@ -267,9 +271,10 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   auto mask = [&](f32x4_t (&s)[4][2], int j) {
     const int end = w.Lk - j * BN, first = w.row0 + wave * 32 + shift + 1 - j * BN;  // of the wave's first row
     if (end >= BN && (!p.causal || first >= BN)) return;
+    const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // rare: no register held for it
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int lim = (p.causal ? min(end, first + li + 16 * n) : end) - 8 * lg;
+      const int lim = (p.causal ? min(end, first + (ln & 15) + 16 * n) : end) - 8 * (ln >> 4);
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
@@ -381,14 +386,14 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   // of both at 2q and the rest at 2q + 1 and 2q + 3, measured 1 % slower: the
   // odd slots then carry two exps, the adds and the pack).  With 16 slots
   // (D = 64) score pair p has its fma at slot p, its exp at p + 1 and its
-  // pack and adds at p + 3.  A scheduling fence closes every slot, so the exp
+  // pack and adds at p + 2.  A scheduling fence closes every slot, so the exp
   // work stays spread under the MFMAs.  The row sum adds the fp32 P
   // values: v_dot2c_f32_bf16 over the packed pair (one instruction instead
   // of two) waits for the SIMD's matrix pipeline on gfx950, about one MFMA
   // per instruction while the other wave's MFMAs run, where adds issue
   // beside them.
   constexpr int NPV = 2 * CB, NS = NPV + 4 * KS;
-  constexpr int PREF = 3;
+  constexpr int PREF = ONE_P ? 2 : 3;
   auto tile = [&](int vb, int kbf, const f32x4_t (&scur)[4][2], f32x4_t (&snext)[4][2], const uint32_t (&pprev)[16],
                   uint32_t (&pcur)[16], float (&ps)[2], const float (&neg_m)[2], auto&& loads) {
     auto frag = [&](int t) -> bf16x8_t {
@@ -453,7 +458,7 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
             e0[q] = __builtin_amdgcn_exp2f(e0[q]);
             e1[q] = __builtin_amdgcn_exp2f(e1[q]);
           }
-          if ((2 * q * NS) / 32 + 3 == t || (q == 15 && t == NS + 1 && (2 * q * NS) / 32 + 3 > NS + 1)) {
+          if (t == (q < 2 ? 4 : q + 2)) {  // from slot 4 on the words of P(j-1) below 8 are free, from slot 8 on all
             pcur[q] = pack_bf16x2(e0[q], e1[q]);
             ps[n] = ps[n] + e0[q];
             ps[n] = ps[n] + e1[q];
@@ -534,15 +539,15 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
     constexpr std::integral_constant<int, 1> odd{};
     int j = 1;
     for (; j + 1 < wtiles; j += 2) {
-      step(j, odd, sb, sa, pa, pb);
-      step(j + 1, even, sa, sb, pb, pa);
+      step(j, odd, sb, sa, pa, ONE_P ? pa : pb);
+      step(j + 1, even, sa, sb, ONE_P ? pa : pb, pa);
     }
-    if (j < wtiles) step(j, odd, sb, sa, pa, pb);
+    if (j < wtiles) step(j, odd, sb, sa, pa, ONE_P ? pa : pb);
     // ---- the wave's last tile: O += V(n-1)^T P(n-1); then only loads for the
     //      waves whose rows see further ----
     publish();
     if ((wtiles - 1) & 1)
-      pv_tile(1, pb);
+      pv_tile(1, ONE_P ? pa : pb);
     else
       pv_tile(0, pa);
     for (j = wtiles; j < ntiles; ++j) {
@@ -599,7 +604,7 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
 }
 
 template <int D, bool SPLIT>
-__global__ void __launch_bounds__(256, 2) prompt_attn_kernel(const PromptAttn p) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) prompt_attn_kernel(const PromptAttn p) {
   prompt_body<D, SPLIT>(p);
 }
 
