@@ -20,6 +20,8 @@ The public names mirror the reference's drop-in surface:
   taomate/inference/memory.py)
 * ``AVModel.quantize_linears_`` (feed-forwards in 8 bits, timestep linears in 4: ``quant``; no
   counterpart in the reference)
+* ``PagedKVCache`` (a cache in blocks for requests of different lengths, with ``kernels.prompt_attn`` and
+  ``kernels.paged_attn`` over packed prompts and single tokens; no counterpart in the reference)
 * ``load_generator`` / ``save_generator`` (taomate/inference/model_runtime.py:182-425) and the
   interactive prefix state (taomate/inference/streaming_runtime.py:1404-1500)
 
@@ -34,6 +36,7 @@ from .cache import (attach_segments, cache_segments, prune_clean_kv_to_sink_rece
                     retain_streaming_context)
 from .kv_cache import (ArenaSpec, KVArena, KVArenaFull, KVCache, KVSpanView, LayerKVCache,
                        _cat_cache, attach_arena, attach_block_arenas, init_kv_cache)
+from .paged_cache import PagedKVCache
 from .integration import ArenaPlan, Installation, init_kv_cache_for, install
 from .runtime import StreamingGenerator, denoising_sigmas
 from .rope import CausalRopeType, apply_split_rotary_emb, causal_precompute_freqs_cis, generate_freq_grid
@@ -54,5 +57,5 @@ __all__ = [
     "LearnedMemoryState", "StreamingMemory", "load_generator", "save_generator", "build_prefix_state_payload",
     "load_prefix_state", "save_prefix_state", "attach_arena", "attach_block_arenas", "ArenaPlan",
     "Installation", "init_kv_cache_for", "install", "StreamingGenerator", "denoising_sigmas",
-    "Group4Weight", "MXRows", "quantize_group4", "quantize_mx",
+    "Group4Weight", "MXRows", "quantize_group4", "quantize_mx", "PagedKVCache",
 ]

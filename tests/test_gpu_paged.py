@@ -5,8 +5,8 @@ import random
 import pytest
 import torch
 
+from taomate_amd import KVArenaFull, PagedKVCache, kernels
 from taomate_amd import _native as N
-from taomate_amd import kernels
 
 from .paged_reference import (BF, E4, Cache, assert_attention_close, assert_lse_close, grow_reference, ints,
                               prompt_reference, starts_of)
@@ -406,3 +406,63 @@ def test_on_another_stream(dev):
             got.append([kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t) for _ in range(4)])
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for outs in got for o in outs)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_cache_object(dev, kv):
+    """Prompts, continued prompts and single tokens of two layers through one cache, some requests released and
+    their blocks used again; every result against attention over the request's history as the cache holds it."""
+    H, Hk, D, R = 4, 2, 64, 5
+    c = PagedKVCache(layers=2, requests=R, blocks=21, heads=Hk, dim_head=D, max_tokens=130, block_size=16, kv_dtype=kv)
+    g = torch.Generator().manual_seed(2)
+    held = [0] * R
+    hist = [[[torch.zeros(0, Hk, D, dtype=torch.float64, device=dev)] * 2 for _ in range(R)] for _ in range(2)]
+
+    def stored(x):
+        """What the cache holds of bf16 rows."""
+        if kv == "bf16":
+            return x.double()
+        s = (x.double().abs().amax(-1, keepdim=True) / 448).float()
+        return (x.double() / s.double()).float().to(E4).double() * s.double()
+
+    def run(new, kind, behind=0):
+        T = sum(new) + behind
+        plan = c.grow(new, T)
+        for b in range(R):
+            held[b] += new[b]
+        for layer in range(2):
+            q, k, v = (torch.randn(T, h, D, generator=g).to(BF).to(dev) for h in (H, Hk, Hk))
+            c.append(layer, k, v, plan)
+            out = c.attend(layer, q) if kind == "token" else c.attend_prompts(layer, q, k, v, plan, kind == "continued")
+            at = 0
+            for b, n in enumerate(new):
+                own = [x[at:at + n] for x in (k, v)]
+                hist[layer][b] = [torch.cat([old, stored(x)]) for old, x in zip(hist[layer][b], own)]
+                keys = [x.double() for x in own] if kind == "prompt" else hist[layer][b]
+                ref, mag, _ = prompt_reference(q[at:at + n], *keys, [n], [keys[0].shape[0]], True)
+                assert_attention_close(out[at:at + n], ref, mag, f"{kind} {layer} {b}")
+                at += n
+            assert (out[at:] == 0).all()
+        assert c.lens.tolist() == held
+
+    run([33, 5, 0, 70, 16], "prompt", behind=3)
+    run([1] * R, "token")
+    run([7, 0, 20, 1, 15], "continued", behind=2)
+    c.release([True, False, False, True, False])
+    for b in (0, 3):
+        held[b], hist[0][b], hist[1][b] = 0, [x[:0] for x in hist[0][b]], [x[:0] for x in hist[1][b]]
+    run([100, 0, 0, 40, 0], "prompt")
+    run([1] * R, "token")
+    c.check()
+    before = [t.clone() for t in (c.tables, c.lens, c.top)]
+    c.grow([0, 0, 0, 100, 0], 100)          # 141 tokens fit a row of 144, but 6 more blocks are not there: 16 of 21 are taken
+    with pytest.raises(KVArenaFull, match="blocks were free"):
+        c.check()
+    c.grow([50, 0, 0, 0, 0], 50)
+    with pytest.raises(KVArenaFull, match="outgrew 144"):
+        c.check()
+    c.grow([2, 0, 0, 0, 0], 1)
+    with pytest.raises(ValueError, match="more tokens than rows"):
+        c.check()
+    assert all(torch.equal(a, b) for a, b in zip((c.tables, c.lens, c.top), before))
+    c.check()

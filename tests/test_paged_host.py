@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from taomate_amd import _native, kernels
+from taomate_amd import PagedKVCache, _native, kernels
 
 BF = torch.bfloat16
 
@@ -139,6 +139,28 @@ def raw(name, **kw):
 def test_refusals_of_the_library(name, kw, match):
     with pytest.raises(_native.NativeCallError, match=match):
         raw(name, **kw)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(dim_head=32), "dim_head"), (dict(block_size=24), "block_size"), (dict(kv_dtype="fp16"), "kv_dtype"),
+    (dict(requests=0), "requests"), (dict(requests=4097), "requests"), (dict(blocks=0), "positive"),
+    (dict(max_tokens=0), "positive"),
+])
+def test_cache_refuses(kw, match):
+    with pytest.raises(ValueError, match=match):
+        PagedKVCache(**{**dict(layers=1, requests=2, blocks=4, heads=1, dim_head=64, max_tokens=64, device="cpu"), **kw})
+
+
+def test_cache_layout():
+    c = PagedKVCache(layers=3, requests=2, blocks=5, heads=2, dim_head=64, max_tokens=100, block_size=32, kv_dtype="fp8",
+                     device="cpu")
+    k, v, ks, vs = c.pool(1)
+    assert k.shape == v.shape == (5, 32, 2, 64) and ks.shape == vs.shape == (5, 32, 2)
+    assert k.stride() == (2 * 32 * 64, 64, 32 * 64, 1) and ks.stride() == (64, 1, 32)
+    assert k.data_ptr() + 5 * 2 * 32 * 64 == v.data_ptr() and c.tables.shape == (2, 4)
+    assert sorted(c.free.tolist()) == list(range(5)) and c.top.item() == 5
+    with pytest.raises(ValueError, match="device tensors"):
+        c.grow([1, 2], 3)
 
 
 def test_workspace_of_the_split():
