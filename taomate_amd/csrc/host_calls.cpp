@@ -728,9 +728,24 @@ PyObject* group4_linear(PyObject* const* a) {
 }
 
 // ------------------------------------------------------- paged cache, prompts
-at::Tensor new_int(at::IntArrayRef shape, at::ScalarType type) {
-  return at::detail::empty_generic(shape, device_memory(), kPlain, type, std::nullopt);
-}
+// New vectors of whole numbers of so many bytes each, in one allocation.
+struct NewInts {
+  c10::Storage all;
+  int64_t at[8] = {};
+  explicit NewInts(std::initializer_list<int64_t> bytes) {
+    int i = 0;
+    for (int64_t b : bytes) at[i + 1] = at[i] + b, ++i;
+    c10::Allocator* const memory = device_memory();
+    all = c10::Storage(c10::Storage::use_byte_size_t(), (size_t)at[i], memory->allocate((size_t)at[i]), memory, true);
+  }
+  at::Tensor part(int i, at::ScalarType type) const {
+    const int64_t size = type == at::kLong ? 8 : 4;
+    at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all), kPlain, c10::scalarTypeToTypeMeta(type));
+    r.unsafeGetTensorImpl()->set_sizes_contiguous({(at[i + 1] - at[i]) / size});
+    r.unsafeGetTensorImpl()->set_storage_offset(at[i] / size);
+    return r;
+  }
+};
 
 // The number of values of a contiguous vector of `type` on the tables' device.
 int64_t vector(const char* what, const char* name, const at::Tensor& t, at::ScalarType type) {
@@ -791,21 +806,10 @@ PyObject* kv_block_grow(PyObject* const* a) {
   apart(what, "tables", tables, {&lens, &fresh, &free, &top, &status});
   apart(what, "status", status, {&lens, &fresh, &free, &top});
   const c10::DeviceGuard guard(tables.device());
-  // one allocation for all results
-  const int64_t at[6] = {0, tokens * 8, tokens * 12, tokens * 12 + (t.B + 1) * 4, tokens * 12 + (2 * t.B + 1) * 4,
-                         tokens * 12 + (2 * t.B + 2) * 4};
-  c10::Allocator* const memory = device_memory();
-  const c10::Storage all(c10::Storage::use_byte_size_t(), (size_t)at[5], memory->allocate((size_t)at[5]), memory, true);
-  const auto part = [&](int i, int64_t n) {
-    at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all), kPlain,
-                                                            c10::scalarTypeToTypeMeta(i == 0 ? at::kLong : at::kInt));
-    r.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-    r.unsafeGetTensorImpl()->set_storage_offset(at[i] / (i == 0 ? 8 : 4));
-    return r;
-  };
-  const at::Tensor slots = part(0, tokens), positions = part(1, tokens), starts = part(2, t.B + 1),
-                   lens_out = lens_to != nullptr ? *lens_to : part(3, t.B),
-                   top_out = top_to != nullptr ? *top_to : part(4, 1);
+  const NewInts made({tokens * 8, tokens * 4, (t.B + 1) * 4, lens_to != nullptr ? 0 : t.B * 4, 4});
+  const at::Tensor slots = made.part(0, at::kLong), positions = made.part(1, at::kInt), starts = made.part(2, at::kInt),
+                   lens_out = lens_to != nullptr ? *lens_to : made.part(3, at::kInt),
+                   top_out = top_to != nullptr ? *top_to : made.part(4, at::kInt);
   call("ltx_kv_block_grow", api.kv_block_grow, t.B, t.width, block, ptr_as<int32_t>(&tables), t.bs,
        ptr_as<const int32_t>(&lens), ptr_as<const int32_t>(&fresh), ptr_as<const int32_t>(&free), n_free,
        ptr_as<const int32_t>(&top), ptr_as<int32_t>(&status), tokens, ptr_as<int32_t>(&lens_out),
@@ -840,8 +844,10 @@ PyObject* kv_block_release(PyObject* const* a) {
   apart(what, "free", free, {&lens, &done, &top, &status, &tables});
   apart(what, "status", status, {&lens, &done, &top, &tables});
   const c10::DeviceGuard guard(tables.device());
-  const at::Tensor lens_out = lens_to != nullptr ? *lens_to : new_int({t.B}, at::kInt),
-                   top_out = top_to != nullptr ? *top_to : new_int({1}, at::kInt);
+  std::optional<NewInts> made;
+  if (lens_to == nullptr || top_to == nullptr) made.emplace(std::initializer_list<int64_t>{t.B * 4, 4});
+  const at::Tensor lens_out = lens_to != nullptr ? *lens_to : made->part(0, at::kInt),
+                   top_out = top_to != nullptr ? *top_to : made->part(1, at::kInt);
   call("ltx_kv_block_release", api.kv_block_release, t.B, t.width, integer(a[6]), ptr_as<const int32_t>(&tables), t.bs,
        ptr_as<const int32_t>(&lens), ptr_as<const uint8_t>(&done), ptr_as<int32_t>(&free), n_free,
        ptr_as<const int32_t>(&top), ptr_as<int32_t>(&status), ptr_as<int32_t>(&lens_out), ptr_as<int32_t>(&top_out),

@@ -198,36 +198,43 @@ __device__ __forceinline__ float lanes_max(float x) {
 template <int D, bool FP8>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppend a) {
   constexpr int CPR = D / 8, ROWS = 256 / CPR;
-  const int w = blockIdx.z, h = blockIdx.y, c = threadIdx.x % CPR;
+  const int h = blockIdx.y, c = threadIdx.x % CPR;
   const int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / CPR;
   if (t >= a.T) return;  // whole rows leave: the lanes of a row stay together
   const int64_t slot = a.slots[t];
-  const uint4 raw = *reinterpret_cast<const uint4*>(a.src[w] + t * a.s_ls[w] + h * a.s_hs[w] + c * 8);
+  uint4 raw[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+    raw[w] = *reinterpret_cast<const uint4*>(a.src[w] + t * a.s_ls[w] + h * a.s_hs[w] + c * 8);
   if (slot < 0 || slot >= a.n_slots) return;
   const int64_t page = slot >> a.shift, off = slot & (((int64_t)1 << a.shift) - 1);
-  const int64_t at = page * a.d_ps[w] + off * a.d_ts[w] + h * a.d_hs[w] + c * 8;
-  if constexpr (!FP8) {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dst[w]) + at) = raw;
-  } else {
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = bf16_bits_to_f32(u[i]), x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-    // the largest finite magnitude; NaN and infinities become NaN in their places
-    float top = 0.0f;
+  for (int w = 0; w < 2; ++w) {
+    const int64_t at = page * a.d_ps[w] + off * a.d_ts[w] + h * a.d_hs[w] + c * 8;
+    if constexpr (!FP8) {
+      store_stream(static_cast<uint16_t*>(a.dst[w]) + at, raw[w]);
+    } else {
+      const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
+      float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]) < __builtin_inff() ? fabsf(x[i]) : 0.0f);
-    top = lanes_max<CPR>(top);
-    const float sc = top > 0.0f ? __fdiv_rn(top, 448.0f) : 1.0f;
-    float q[8];
-    quotients_e4m3_bf16(x, sc, __fdiv_rn(1.0f, sc), top >= kCorrectedMinMax, q);
-    uint2 codes;
-    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-    codes.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
-    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-    codes.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.dst[w]) + at) = codes;
-    if (c == 0) a.scales[w][page * a.sc_ps[w] + off * a.sc_ts[w] + h * a.sc_hs[w]] = sc;
+      for (int i = 0; i < 4; ++i)
+        x[2 * i] = bf16_bits_to_f32(u[i]), x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      // the largest finite magnitude; NaN and infinities become NaN in their places
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]) < __builtin_inff() ? fabsf(x[i]) : 0.0f);
+      top = lanes_max<CPR>(top);
+      const float sc = top > 0.0f ? __fdiv_rn(top, 448.0f) : 1.0f;
+      float q[8];
+      quotients_e4m3_bf16(x, sc, __fdiv_rn(1.0f, sc), top >= kCorrectedMinMax, q);
+      uint2 codes;
+      int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+      codes.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+      int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+      codes.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+      store_stream(static_cast<uint8_t*>(a.dst[w]) + at, codes);
+      if (c == 0) a.scales[w][page * a.sc_ps[w] + off * a.sc_ts[w] + h * a.sc_hs[w]] = sc;
+    }
   }
 }
 
@@ -341,7 +348,7 @@ extern "C" int ltx_kv_paged_append(int kv_dtype, int64_t T, int64_t H, int64_t D
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t groups = ceil_div(T, 256 / (D / 8));
   LTX_REQUIRE(groups <= 0x7FFFFFFF, "%s: too many tokens", name);
-  const dim3 grid((unsigned)groups, (unsigned)H, 2), threads(256);
+  const dim3 grid((unsigned)groups, (unsigned)H), threads(256);
   if (D == 128) {
     if (fp8) hipLaunchKernelGGL((paged_append_kernel<128, true>), grid, threads, 0, st, a);
     else hipLaunchKernelGGL((paged_append_kernel<128, false>), grid, threads, 0, st, a);

@@ -52,6 +52,19 @@ struct PagedAttn {
   int4* joins;                 // [range]: the request that range continues first (-1: none), its ranges, its first slot
 };
 
+// Reads of the cache.  NT: more than the last-level cache holds, every byte read
+// once: non-temporal loads, which pass the caches by (a plain read of 1 GiB runs at 7.0
+// TB/s with them and at 6.2 without; 64 requests over 375 MB 68.8 us and
+// 76.3, four over 840 MB of e4m3 139 and 150).  A smaller cache that the last
+// step left in the last-level cache is slower so (10 MB: 10.5 us and 8.2).
+constexpr int64_t kLastLevelBytes = 256 << 20;
+template <bool NT, typename T>
+__device__ __forceinline__ T load_cached(const char* p) {
+  typedef unsigned int vec_t __attribute__((ext_vector_type(sizeof(T) / 4)));
+  const vec_t* const v = reinterpret_cast<const vec_t*>(p);
+  return __builtin_bit_cast(T, NT ? __builtin_nontemporal_load(v) : *v);
+}
+
 template <int D, bool FP8>
 struct TokenTile {
   static constexpr int KN = FP8 ? D / 64 : D / 32;        // 16-byte loads of a K row's lane
@@ -97,7 +110,7 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool hi) {
                                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
 }
 
-template <int D, bool FP8, bool SPLIT>
+template <int D, bool FP8, bool SPLIT, bool NT>
 __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const PagedAttn p) {
   using Tile = TokenTile<D, FP8>;
   constexpr int KS = D / 32;        // 32-channel steps of a score
@@ -166,15 +179,15 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
         const char* const kb = kh + (int64_t)id * p.k_ps + (int64_t)off * p.k_ts;
         const char* const vb = vh + (int64_t)id * p.v_ps + (int64_t)off * p.v_ts;
 #pragma unroll
-        for (int s = 0; s < Tile::KN; ++s) x.k[t][s] = *reinterpret_cast<const uint4*>(kb + k_lane + s * 64);
+        for (int s = 0; s < Tile::KN; ++s) x.k[t][s] = load_cached<NT, uint4>(kb + k_lane + s * 64);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const char* const a = vb + v_lane + r * p.v_ts;
           if constexpr (Tile::VW == 4) {
-            const uint4 y = *reinterpret_cast<const uint4*>(a);
+            const uint4 y = load_cached<NT, uint4>(a);
             x.v[t][r][0] = y.x, x.v[t][r][1] = y.y, x.v[t][r][2] = y.z, x.v[t][r][3] = y.w;
           } else if constexpr (Tile::VW == 2) {
-            const uint2 y = *reinterpret_cast<const uint2*>(a);
+            const uint2 y = load_cached<NT, uint2>(a);
             x.v[t][r][0] = y.x, x.v[t][r][1] = y.y;
           } else {
             x.v[t][r][0] = *reinterpret_cast<const uint32_t*>(a);
@@ -442,18 +455,25 @@ extern "C" int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, i
   return LTX_OK;
 }
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool NT>
 static void launch_token(const PagedAttn& p, const TokenPlan& t, hipStream_t st) {
   const dim3 threads(64 * kTokenWaves);
-  const unsigned y = (unsigned)t.y, lds = (unsigned)(p.B + 1) * 4;
+  const unsigned y = (unsigned)t.y;
   if (t.ranges == 0) {
-    hipLaunchKernelGGL((paged_attn_kernel<D, FP8, false>), dim3((unsigned)p.B, y), threads, 0, st, p);
+    hipLaunchKernelGGL((paged_attn_kernel<D, FP8, false, NT>), dim3((unsigned)p.B, y), threads, 0, st, p);
     return;
   }
-  hipLaunchKernelGGL((paged_attn_kernel<D, FP8, true>), dim3((unsigned)t.ranges, y), threads, lds, st, p);
+  hipLaunchKernelGGL((paged_attn_kernel<D, FP8, true, NT>), dim3((unsigned)t.ranges, y), threads,
+                     (unsigned)(p.B + 1) * 4, st, p);
   if (t.ranges > 1)
     hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)t.ranges - 1, y, (unsigned)t.part_heads), dim3(256), 0,
                        st, p);
+}
+template <int D, bool FP8>
+static void launch_token(const PagedAttn& p, const TokenPlan& t, hipStream_t st) {
+  const int64_t most = (int64_t)p.B * (p.width << p.shift) * p.Hk * 2 * D * (FP8 ? 1 : 2);
+  if (most > kLastLevelBytes && p.groups == 1) launch_token<D, FP8, true>(p, t, st);
+  else launch_token<D, FP8, false>(p, t, st);
 }
 
 extern "C" int ltx_paged_attn(int kv_dtype, int64_t B, int64_t Hk, int64_t G, int64_t D, const void* q, int64_t q_bs,
