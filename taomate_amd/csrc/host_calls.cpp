@@ -24,6 +24,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <map>
 #include <mutex>
@@ -897,6 +898,23 @@ TokenRows token_rows(const char* what, const char* name, const at::Tensor& t) {
   return {t.size(0), t.size(1), t.size(2), stride_of(t, 0), stride_of(t, 1)};
 }
 
+// Whether rows of D values at these (size, stride) dimensions lie apart.
+bool rows_apart(std::initializer_list<std::pair<int64_t, int64_t>> dims, int64_t D) {
+  std::pair<int64_t, int64_t> d[4];
+  int n = 0;
+  for (const auto& x : dims) {
+    if (x.first == 0) return true;
+    if (x.first > 1) d[n++] = x;
+  }
+  std::sort(d, d + n, [](const auto& a, const auto& b) { return a.second < b.second; });
+  int64_t extent = D;
+  for (int i = 0; i < n; ++i) {
+    if (d[i].second < extent) return false;
+    extent += (d[i].first - 1) * d[i].second;
+  }
+  return true;
+}
+
 // (k, v, k_pool, v_pool, slots, k_scales, v_scales)
 void kv_paged_append(PyObject* const* a) {
   const char* const what = "kv_paged_append";
@@ -909,6 +927,12 @@ void kv_paged_append(PyObject* const* a) {
   if (k.sizes() != v.sizes() || rk.H != pk.H || rk.D != pk.D)
     value_error("kv_paged_append: k " + shape(k) + ", v " + shape(v) + " for pools " + shape(kp));
   counted(what, "slots", slots, at::kLong, rk.T);
+  for (const Pool* x : {&pk, &pv})
+    if (!rows_apart({{x->n, x->ps}, {x->block, x->ts}, {x->H, x->hs}}, x->D)) value_error("kv_paged_append: rows of a pool overlap");
+  for (Opt x : {ks, vs})
+    if (x != nullptr && !rows_apart({{pk.n, stride_of(*x, 0)}, {pk.block, stride_of(*x, 1)}, {pk.H, stride_of(*x, 2)}}, 1))
+      value_error("kv_paged_append: scales overlap");
+  if (kp.numel() > 0 && kp.data_ptr() == vp.data_ptr()) value_error("kv_paged_append: k_pool and v_pool are the same memory");
   const c10::DeviceGuard guard(k.device());
   const auto st = [&](Opt s, int d) { return s != nullptr ? stride_of(*s, d) : 0; };
   call("ltx_kv_paged_append", api.kv_paged_append, pk.dtype, rk.T, rk.H, rk.D, ptr(&k), rk.ls, rk.hs, ptr(&v), rv.ls,
@@ -922,6 +946,8 @@ at::Tensor rows_out(const char* what, Opt out, const at::Tensor& q) {
   if (out->scalar_type() != at::kBFloat16) type_error(std::string(what) + ": out must be bf16");
   if (out->sizes() != q.sizes() || (q.size(2) > 1 && out->stride(2) != 1))
     value_error(std::string(what) + ": out " + shape(*out) + " must be " + shape(q) + " with contiguous D");
+  if (!rows_apart({{q.size(0), out->stride(0)}, {q.size(1), out->stride(1)}}, q.size(2)))
+    value_error(std::string(what) + ": rows of out overlap");
   return *out;
 }
 

@@ -347,7 +347,7 @@ extern "C" int ltx_kv_paged_append(int kv_dtype, int64_t T, int64_t H, int64_t D
   a.slots = slots, a.T = T, a.n_slots = n_blocks * block, a.H = (int)H, a.shift = block_shift(block);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t groups = ceil_div(T, 256 / (D / 8));
-  LTX_REQUIRE(groups <= 0x7FFFFFFF, "%s: too many tokens", name);
+  LTX_REQUIRE(groups < (1 << 24), "%s: too many tokens", name);  // 2^32 threads
   const dim3 grid((unsigned)groups, (unsigned)H), threads(256);
   if (D == 128) {
     if (fp8) hipLaunchKernelGGL((paged_append_kernel<128, true>), grid, threads, 0, st, a);

@@ -714,7 +714,7 @@ extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, in
   p.causal = causal != 0, p.zero_tail = zero_tail != 0;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)D)) * kLog2e;
   const PromptPlan t = plan_prompt(B, Tq, Tk, Hk, G);
-  LTX_REQUIRE(t.grid <= 0x7FFFFFFF, "%s: too many rows and heads for one launch", name);
+  LTX_REQUIRE(t.grid < (1 << 24), "%s: too many rows and heads for one launch", name);  // 2^32 threads
   const int64_t need = t.bytes(D);
   LTX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
               "%s: needs %lld bytes of workspace", name, (long long)need);

@@ -149,6 +149,28 @@ def test_append(dev, T, Hk, D, block, kv, layout):
         assert torch.equal(got_sc, sc) and torch.equal(got.view(torch.uint8), pool.view(torch.uint8))
 
 
+def test_append_refuses_one_memory_for_both(dev):
+    c = Cache([16], 1, 64, 16, "bf16", dev)
+    x = torch.zeros(1, 1, 64, dtype=BF, device=dev)
+    with pytest.raises(ValueError, match="same memory"):
+        kernels.kv_paged_append(x, x, c.k, c.k, torch.zeros(1, dtype=torch.int64, device=dev))
+
+
+def test_results_in_the_queries_memory(dev):
+    """out may be q itself, whole and shared among workgroups."""
+    c = Cache([300, 0, 2000], 2, 64, 16, "bf16", dev)
+    q = torch.randn(3, 4, 64, device=dev).to(BF)
+    want = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t)
+    kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, out=q)
+    assert torch.equal(q, want)
+    for rows, keys in (([200, 50], [200, 50]), ([40], [3000])):
+        q = torch.randn(sum(rows), 4, 64, device=dev).to(BF)
+        k = torch.randn(sum(keys), 2, 64, device=dev).to(BF)
+        want = kernels.prompt_attn(q, k, k, starts_of(rows, dev), starts_of(keys, dev))
+        kernels.prompt_attn(q, k, k, starts_of(rows, dev), starts_of(keys, dev), out=q)
+        assert torch.equal(q, want)
+
+
 def test_append_of_values_that_are_not_finite(dev):
     c = Cache([16], 1, 64, 16, "fp8", dev)
     k = torch.ones(2, 1, 64, dtype=BF, device=dev)
@@ -237,6 +259,8 @@ TOKENS = [
     ([128, 129, 127, 0, 640], 12, 4, 128, 64), ([5000], 8, 2, 64, 16), ([2000, 3, 0, 7000, 129], 32, 8, 128, 128),
     ([3100, 1500], 20, 1, 128, 16), ([900, 1100], 33, 1, 64, 256), ([40] * 300, 2, 2, 64, 16),
     ([1] * 9 + [20000], 7, 7, 128, 32), ([4096] * 3, 16, 1, 64, 16),
+    # tables that could hold more than the last-level cache, in both forms
+    ([33] * 120, 8, 4, 128, 16), ([1] * 129 + [1024], 8, 4, 128, 16),
 ]
 
 

@@ -87,6 +87,12 @@ def prompt(**kw):
     (lambda: prompt(k_starts=i32(4)), ValueError, "k_starts must hold 3"),
     (lambda: prompt(q=dev(7, 64, 4).transpose(1, 2)), ValueError, "contiguous D"),
     (lambda: prompt(lse=dev(7, 4, dtype=torch.float32)), ValueError, "lse"),
+    (lambda: prompt(out=dev(7, 1, 64).expand(7, 4, 64)), ValueError, "rows of out overlap"),
+    (lambda: prompt(out=dev(7 * 4 * 64).as_strided((7, 4, 64), (64, 64, 1))), ValueError, "rows of out overlap"),
+    (lambda: token(out=dev(1, 4, 64).expand(3, 4, 64)), ValueError, "rows of out overlap"),
+    (lambda: append(k_pool=dev(1, 16, 2, 64).expand(3, 16, 2, 64)), ValueError, "rows of a pool overlap"),
+    (lambda: append(v_pool=dev(3 * 16 * 2 * 64).as_strided((3, 16, 2, 64), (1024, 64, 512, 1))), ValueError,
+     "rows of a pool overlap"),
     (lambda: prompt(q=dev(7, 4, 64).requires_grad_()), RuntimeError, "computes no gradients"),
     (lambda: token(k_pool=dev(9, 16, 2, 64).requires_grad_()), RuntimeError, "computes no gradients"),
     (lambda: append(k=dev(5, 2, 64).requires_grad_()), RuntimeError, "computes no gradients"),
@@ -130,7 +136,8 @@ def raw(name, **kw):
     ("ltx_paged_attn", dict(kv=0), "bf16 or e4m3"), ("ltx_paged_attn", dict(k_ts=-64), "token stride"),
     ("ltx_prompt_attn", dict(D=32), "head layout"), ("ltx_prompt_attn", dict(v_ls=60), "16-byte"),
     ("ltx_prompt_attn", dict(k_ls=32), "overlap"), ("ltx_prompt_attn", dict(v_ls=1 << 24), "too far"),
-    ("ltx_prompt_attn", dict(B=5000), "at most 4096"), ("ltx_prompt_attn", dict(Tq=1 << 31), "2\\^30"),
+    ("ltx_prompt_attn", dict(B=5000), "at most 4096"),
+    ("ltx_prompt_attn", dict(Tq=1 << 30, G=64), "one launch"), ("ltx_kv_paged_append", dict(T=1 << 40), "too many tokens"), ("ltx_prompt_attn", dict(Tq=1 << 31), "2\\^30"),
     ("ltx_prompt_attn", dict(k=None), "null"), ("ltx_prompt_attn", dict(Tk=1024), "workspace"), ("ltx_prompt_attn", dict(out=P + 8), "16-byte"),
     ("ltx_kv_paged_append", dict(D=256), "D 64 or 128"), ("ltx_kv_paged_append", dict(block=0), "block of 0"),
     ("ltx_kv_paged_append", dict(kp_ts=66), "pools"), ("ltx_kv_paged_append", dict(k=P + 4), "rows of k and v"),
