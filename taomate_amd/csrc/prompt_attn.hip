@@ -135,6 +135,14 @@ __device__ __forceinline__ int parts_of(const PromptAttn& p, int seen, int& tile
   return tiles > 0 ? (all + tiles - 1) / tiles : 1;
 }
 
+// x where i < lim, else -inf, by bit selection: comparisons would hold a pair
+// of scalar registers each, and the key loop's own would be moved out and back
+// in every tile to make room.
+__device__ __forceinline__ float keep_below(float x, int i, int lim) {
+  const uint32_t keep = (uint32_t)((i - lim) >> 31);
+  return __uint_as_float((__float_as_uint(x) & keep) | (0xFF800000u & ~keep));
+}
+
 template <int D, bool SPLIT>
 __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   constexpr int BN = kKeys;
@@ -279,7 +287,7 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (32 * (kb >> 1) + 4 * (kb & 1) + r >= lim) s[kb][n][r] = -INFINITY;
+          s[kb][n][r] = keep_below(s[kb][n][r], 32 * (kb >> 1) + 4 * (kb & 1) + r, lim);
     }
   };
   // Largest base-2 logit of a tile for this lane's query n; a row that sees
