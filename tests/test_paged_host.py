@@ -173,9 +173,13 @@ def test_cache_layout():
 def test_workspace_of_the_split():
     n = ctypes.c_int64()
     size = lambda *a: (_native.call("ltx_paged_attn_workspace_size", *a, ctypes.byref(n)), n.value)[1]  # noqa: E731
+    part = 2 * 4 * 130 * 4
     assert size(64, 8, 4, 128, 64, 16) == 0                  # tables of 1024 tokens: a workgroup a request
-    assert size(64, 8, 4, 128, 65, 16) == 64 * 8 * 2 * 4 * 130 * 4 + 64 * 16
-    assert size(1, 8, 4, 128, 65, 16) == 5 * 8 * 2 * 4 * 130 * 4 + 5 * 16
+    assert size(64, 8, 4, 128, 65, 16) == 64 * (8 * part + 16)
+    assert size(8, 8, 4, 128, 32, 16) == 0                   # 512 tokens of a few requests
+    assert size(8, 8, 4, 128, 33, 16) == 32 * (8 * part + 16)
+    assert size(1, 8, 4, 128, 65, 16) == 9 * (8 * part + 16)
+    assert size(1, 600, 1, 128, 65, 16) == 0                 # heads enough
     rows = lambda *a: (_native.call("ltx_prompt_attn_workspace_size", *a, ctypes.byref(n)), n.value)[1]  # noqa: E731
     assert rows(1, 128, 767, 8, 4, 128) == 0                 # too few keys to share
     assert rows(1, 128, 768, 8, 4, 128) == 32 * 16 * 128 * 130 * 4
