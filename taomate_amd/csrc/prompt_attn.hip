@@ -75,11 +75,13 @@ __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows
     }
     if (b0 == p.B - 1) r.end = __builtin_amdgcn_readfirstlane(s + n);
     if (p.sorted) {
-      // by the power of two of their number of key tiles: one ballot a power
-      const int mine = 32 - __builtin_clz(m / kKeys + 1);
+      // by powers of two of their number of key tiles: the longest three, then the others
+      const int mine = lane < p.B ? 32 - __builtin_clz(m / kKeys + 1) : 0;
+      const int longest = wave_max(mine);
       int rank = lane, before = 0;
-      for (int power = p.sorted; power > 0; --power) {
-        const bool here = mine == power && lane < p.B;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool here = lane < p.B && (c < 3 ? mine == longest - c : mine < longest - 2);
         const uint64_t all = __builtin_amdgcn_ballot_w64(here);
         const int at = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
         rank = here ? at : rank;
@@ -726,8 +728,7 @@ extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, in
   const int64_t need = t.bytes(D);
   LTX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
               "%s: needs %lld bytes of workspace", name, (long long)need);
-  // the highest power of two of any prompt's key tiles; a grid that is resident at once needs no order
-  p.sorted = B > 1 && B <= 64 && t.grid > kResident ? 32 - __builtin_clz((unsigned)(Tk / kKeys) + 1) : 0;
+  p.sorted = B > 1 && B <= 64 && t.grid > kResident;  // a grid that is resident at once needs no order
   p.tiles = (int)(t.tiles > 0 ? t.tiles : 1);
   if (t.split > 1) {
     p.split = (int)t.split;
