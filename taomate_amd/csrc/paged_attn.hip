@@ -21,8 +21,9 @@
 // 8-bit caches: codes are decoded to bf16 (exact) in registers, the K scales
 // multiply the scores and the V scales P, both in float32.
 //
-// Softmax statistics, P's sum and O are float32; P is rounded to bf16 for the
-// product (half a step, 2^-8, of each weight).
+// Softmax statistics, P's sum and O are float32; P goes into its product as two
+// bf16 parts (2^-16 of each weight; one part, 2^-8, is at most 1 % faster where
+// memory bounds the kernel).
 
 #include "attn_common.h"
 
@@ -254,7 +255,12 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
         for (int e = 0; e < DV; ++e) o[e] *= alpha;
       }
       const float base = m == -INFINITY ? 0.0f : m;
-      uint32_t pw[4];
+      // P in two bf16 parts, the second holding what the first rounds away
+      uint32_t pw[4], pr[4];
+      auto split = [&](float a, float b, uint32_t& hi, uint32_t& lo) {
+        hi = pack_bf16x2(a, b);
+        lo = pack_bf16x2(a - bf16_bits_to_f32(hi & 0xFFFFu), b - __uint_as_float(hi & 0xFFFF0000u));
+      };
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -263,10 +269,11 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
           l += s[t][r];
         }
         if constexpr (FP8) s[t] *= x.vs[t];
-        pw[2 * t] = pack_bf16x2(s[t][0], s[t][1]);
-        pw[2 * t + 1] = pack_bf16x2(s[t][2], s[t][3]);
+        split(s[t][0], s[t][1], pw[2 * t], pr[2 * t]);
+        split(s[t][2], s[t][3], pw[2 * t + 1], pr[2 * t + 1]);
       }
       const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(pw[0], pw[1], pw[2], pw[3]));
+      const bf16x8_t rf = __builtin_bit_cast(bf16x8_t, make_uint4(pr[0], pr[1], pr[2], pr[3]));
 #pragma unroll
       for (int e2 = 0; e2 < DV / 2; ++e2) {  // two channels at a time: the halves of one word
         uint32_t w[2][4];
@@ -280,8 +287,9 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
           const uint4 a = make_uint4(
               __builtin_amdgcn_perm(w[0][1], w[0][0], sel), __builtin_amdgcn_perm(w[0][3], w[0][2], sel),
               __builtin_amdgcn_perm(w[1][1], w[1][0], sel), __builtin_amdgcn_perm(w[1][3], w[1][2], sel));
-          o[2 * e2 + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), pf, o[2 * e2 + u],
-                                                                  0, 0, 0);
+          f32x4_t& oe = o[2 * e2 + u];
+          oe = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), rf, oe, 0, 0, 0);
+          oe = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), pf, oe, 0, 0, 0);
         }
       }
     };

@@ -59,11 +59,12 @@ def prompt_reference(q, k, v, rows, keys, causal, scale=None):
     return out, mag, lse
 
 
-def assert_attention_close(got, out, mag, what=""):
-    """|error| <= 2^-8 (P to bf16, half a step of each weight) + 2^-8 (the result to bf16) of the weighted
-    magnitudes, and 2^-12 for the float32 scores (128 products, exp2 of a sum whose magnitude stays below 2^7)."""
+def assert_attention_close(got, out, mag, what="", weight=2 ** -8):
+    """|error| <= ``weight`` (P to bf16, half a step of each weight; two bf16 parts: 2^-16) + 2^-8 (the result to
+    bf16) of the weighted magnitudes, and 2^-12 for the float32 scores (128 products, exp2 of a sum whose
+    magnitude stays below 2^7)."""
     err = (got.double() - out).abs()
-    bound = mag * (2 ** -8 + 2 ** -8 + 2 ** -12) + 1e-30
+    bound = mag * (weight + 2 ** -8 + 2 ** -12) + 1e-30
     assert torch.isfinite(got).all(), f"{what}: not finite"
     worst = (err / bound).max().item() if err.numel() else 0.0
     assert worst <= 1.0, f"{what}: error {worst:.2f} of its bound"
