@@ -255,7 +255,8 @@ def paged_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, tabl
     """ltx_paged_attn: one token of each request, bf16 q [B, heads, D], over the first ``lens`` (int32 [B]) tokens
     of its blocks; query head h reads key head h // (heads / key heads).  Requests without tokens get zero rows
     (``lse`` float32 [B, heads]: -inf).  Computes no gradients.  The tables' width bounds the lengths: the work
-    is planned for what they can hold, with one launch up to 1024 tokens and a joining second one beyond."""
+    is planned for what they can hold, with one launch up to 1024 tokens (512 for a few requests) and a joining
+    second one beyond."""
     return (N._host or N.host()).paged_attn(q, k_pool, v_pool, tables, lens, k_scales, v_scales, scale, out, lse)
 
 

@@ -181,6 +181,21 @@ def test_append_of_values_that_are_not_finite(dev):
     assert got[1].isnan().all() and c.k_scales[0, 1:3, 0].tolist() == [torch.tensor(1 / 448, dtype=torch.float32).item(), 1.0]
 
 
+def test_append_of_tiny_and_large_rows(dev):
+    """Maxima from the smallest bf16 to its largest: scales as far as float32 goes, codes of the exact quotients."""
+    powers = torch.tensor([-133, -126, -110, -97, -96, -95, -20, 0, 60, 119], dtype=torch.float64)
+    x = (torch.randn(10, 1, 64, generator=torch.Generator().manual_seed(1)).double() * 2.0 ** powers[:, None, None])
+    x = x.to(BF).to(dev)
+    c = Cache([16], 1, 64, 16, "fp8", dev, spare=0)
+    kernels.kv_paged_append(x, x, c.k, c.v, torch.arange(10, device=dev), c.k_scales, c.v_scales)
+    top = x.double().abs().amax(-1)
+    s = torch.where(top > 0, top / 448, torch.ones_like(top)).float()
+    want = (x.double() / s.double()[..., None]).float().to(E4)
+    for pool, scales in ((c.k, c.k_scales), (c.v, c.v_scales)):
+        assert torch.equal(scales[0, :10], s)
+        assert torch.equal(pool.view(torch.uint8)[0, :10], want.view(torch.uint8))
+
+
 # ------------------------------------------------------------------ prompts
 PROMPTS = [
     # rows, keys, heads, key heads, D
@@ -416,6 +431,46 @@ def test_prompts_then_tokens_under_a_graph(dev):
     assert held.tolist() == [0, lens[1] + steps, 0, lens[3] + steps]
     in_use = [tables[b, j].item() for b in (1, 3) for j in range(-(-held[b].item() // block))]
     assert sorted(free[:top.item()].tolist() + in_use) == list(range(blocks)) and status.item() == 0
+
+
+def test_two_graphs_and_eager_calls_have_workspaces_of_their_own(dev):
+    """Calls that share keys among workgroups, captured twice with other inputs, replayed side by side on two
+    streams with eager calls between."""
+    c = Cache([3000, 20, 700], 2, 128, 16, "bf16", dev)
+    rows, keys = [20, 3], [2500, 1800]
+    starts, k_starts = starts_of(rows, dev), starts_of(keys, dev)
+    g = torch.Generator().manual_seed(5)
+    sets = []
+    for _ in range(3):
+        q1 = torch.randn(3, 8, 128, generator=g).to(BF).to(dev)
+        q2, k, v = (torch.randn(n, h, 128, generator=g).to(BF).to(dev) for n, h in ((23, 4), (4300, 2), (4300, 2)))
+        sets.append((q1, q2, k, v))
+
+    def call(q1, q2, k, v):
+        return (kernels.paged_attn(q1, c.k, c.v, c.tables, c.lens_t), kernels.prompt_attn(q2, k, v, starts, k_starts))
+
+    want = [[t.clone() for t in call(*s)] for s in sets]
+    ref, mag, _ = c.reference(sets[0][0])
+    assert_attention_close(want[0][0], ref, mag, weight=2 ** -16)
+    torch.cuda.synchronize()
+    graphs = []
+    for s in sets[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(*s)
+        graphs.append((graph, out, torch.cuda.Stream()))
+    for _ in range(4):
+        for _, out, _ in graphs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = call(*sets[2])
+        torch.cuda.synchronize()
+        for got, w in zip([graphs[0][1], graphs[1][1], eager], want):
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
 
 
 def test_on_another_stream(dev):
