@@ -29,8 +29,8 @@
 
 namespace ltx {
 
-constexpr int kTokenWaves = 4;
-constexpr int kTokenTile = 32 * kTokenWaves;  // keys of one step of a workgroup
+constexpr int kTokenWaves = 4;                // waves of a workgroup (1 where no request holds many tokens)
+constexpr int kTokenTile = 32 * kTokenWaves;  // keys of one step of such a workgroup
 
 struct PagedAttn {
   const uint16_t* q;
@@ -111,15 +111,17 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool hi) {
                                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
 }
 
-template <int D, bool FP8, bool SPLIT, bool NT>
-__global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const PagedAttn p) {
+template <int D, bool FP8, bool SPLIT, bool NT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_kernel(const PagedAttn p) {
   using Tile = TokenTile<D, FP8>;
+  static_assert(!SPLIT || WAVES == kTokenWaves, "shares are counted in kTokenTile");
+  constexpr int TILE = 32 * WAVES;  // keys of one step
   constexpr int KS = D / 32;        // 32-channel steps of a score
   constexpr int DV = D / 16;        // channels of a lane's V block = 16-channel tiles of O
   constexpr int OS = D + 4;         // row stride of the joined O in LDS
   constexpr int EB = FP8 ? 1 : 2;   // bytes of a cached value
-  __shared__ __attribute__((aligned(16))) float s_o[kTokenWaves][16][OS];
-  __shared__ float s_ml[kTokenWaves][16][2];
+  __shared__ __attribute__((aligned(16))) float s_o[WAVES][16][OS];
+  __shared__ float s_ml[WAVES][16][2];
   extern __shared__ int s_first[];  // SPLIT: first tile of each request
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -140,10 +142,10 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
   // written as the result (slot < 0) or as a partial one
   auto attend = [&](int b, int t0, int t1, int slot) {
     const int32_t* const row = p.tables + b * p.t_bs;
-    const int key_w = t0 * kTokenTile + wave * 32;  // this wave's first key
+    const int key_w = t0 * TILE + wave * 32;  // this wave's first key
     // the block ids of this wave's next 32 tiles, two halves each, one a lane
     auto ids_of = [&](int i) {
-      const int64_t key = (int64_t)key_w + (int64_t)(i + (lane >> 1)) * kTokenTile + (lane & 1) * 16;
+      const int64_t key = (int64_t)key_w + (int64_t)(i + (lane >> 1)) * TILE + (lane & 1) * 16;
       const int64_t j = key >> p.shift;
       return row[j < p.width ? j : p.width - 1];
     };
@@ -159,8 +161,8 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
     }
 
     const int len = __builtin_amdgcn_readfirstlane(length(b));
-    const int end = min(len, t1 * kTokenTile);
-    const int n = end > key_w ? (end - key_w + kTokenTile - 1) / kTokenTile : 0;
+    const int end = min(len, t1 * TILE);
+    const int n = end > key_w ? (end - key_w + TILE - 1) / TILE : 0;
     if (n > 32) ids_next = ids_of(32);
 
     // tile i's loads; lim[t]: how many keys of half t take part
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int key0 = key_w + i * kTokenTile + t * 16;
+        const int key0 = key_w + i * TILE + t * 16;
         int id = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + t);
         const bool there = (unsigned)id < (unsigned)p.n_blocks;  // an id outside the pool: keys that take no part
         lim[t] = there ? min(max(end - key0, 0), 16) : 0;
@@ -322,15 +324,15 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
       if (g == 0) s_ml[wave][c][0] = m, s_ml[wave][c][1] = l;
     }
     __syncthreads();
-    for (int i = tid; i < nh * (D / 4); i += 64 * kTokenWaves) {
+    for (int i = tid; i < nh * (D / 4); i += 64 * WAVES) {
       const int h = i / (D / 4), d = i % (D / 4) * 4;
       float mm = s_ml[0][h][0];
 #pragma unroll
-      for (int w = 1; w < kTokenWaves; ++w) mm = fmaxf(mm, s_ml[w][h][0]);
+      for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, s_ml[w][h][0]);
       f32x4_t acc{};
       float ll = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kTokenWaves; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float f = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_ml[w][h][0] - mm);
         ll += f * s_ml[w][h][1];
         acc += f * *reinterpret_cast<const f32x4_t*>(&s_o[w][h][d]);
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(64 * kTokenWaves, 2) paged_attn_kernel(const P
   };
 
   if constexpr (!SPLIT) {
-    attend((int)blockIdx.y, 0, (capacity + kTokenTile - 1) / kTokenTile, -1);
+    attend((int)blockIdx.y, 0, (capacity + TILE - 1) / TILE, -1);
   } else {
     const int total = first_tiles(p, s_first);
     const int per = max(p.min_tiles, (total + p.ranges - 1) / p.ranges);
@@ -433,22 +435,27 @@ using namespace ltx;
 
 struct TokenPlan {
   int64_t y, ranges, min_tiles, part_heads;  // ranges 0: one workgroup a request and key head group
+  bool one_wave;                             // of one wave
   int64_t parts() const { return ranges * y * 2 * part_heads; }
   int64_t bytes(int64_t D) const { return parts() * (D + 2) * 4 + ranges * 16; }
 };
 
-// Requests that can hold few tokens only take a workgroup each, one launch: up to
-// 1024 tokens, or 512 where there are few workgroups (a CU reads no more than
-// 60 GB/s, so one request of 1000 tokens with 8 key heads takes 12.7 us whole and 8.1 in
-// shares).  Otherwise all requests' tiles are cut into equal ranges: as many as
-// are resident at once (two workgroups a CU), or one a CU and down to a tile each
-// where there is little to share.
+// Requests that can hold few tokens only take a workgroup each, one launch.  Up
+// to 1024 tokens, or 512 where there are few workgroups (a CU reads no more than 60
+// GB/s: one request of 1000 tokens with 8 key heads takes 12.7 us whole and 8.1 in
+// shares).  Of one wave where there are more than fit at once and few steps'
+// keys in each, for which four waves would mostly idle (123 requests of up to
+// 60 tokens, 32 key heads: 24.9 us with four and 12.2 with one; of 250 tokens 58
+// and 51; 256 of 500, 8 key heads, 83 and 94).
+// Otherwise all requests' tiles are cut into equal ranges: as many as are
+// resident at once (two workgroups a CU), or one a CU and down to a tile each where
+// there is little to share.
 // The key heads of a request start next to each other: their rows lie side by
 // side in a block (256 requests of up to 1000 tokens, 32 heads, e4m3: 117 us, and
 // 180 with the requests side by side).
 static TokenPlan plan_token(int64_t B, int64_t Hk, int64_t G, int64_t capacity) {
   const int64_t tiles = ceil_div(capacity, kTokenTile), groups = ceil_div(G, 16), y = Hk * groups;
-  TokenPlan t{y, 0, 1, G < 16 ? G : 16};
+  TokenPlan t{y, 0, 1, G < 16 ? G : 16, B * y > 512 && capacity <= (B * y >= 2048 ? 256 : 128)};
   const bool little = B * tiles * y <= 1024;
   const int64_t resident = little ? 256 : 512;
   if (tiles <= (B * y <= 64 ? 4 : 8) || y >= resident) return t;
@@ -472,11 +479,16 @@ template <int D, bool FP8, bool NT>
 static void launch_token(const PagedAttn& p, const TokenPlan& t, hipStream_t st) {
   const dim3 threads(64 * kTokenWaves);
   const unsigned y = (unsigned)t.y;
-  if (t.ranges == 0) {
-    hipLaunchKernelGGL((paged_attn_kernel<D, FP8, false, NT>), dim3(y, (unsigned)p.B), threads, 0, st, p);
+  const dim3 each(y, (unsigned)p.B);
+  if (t.one_wave) {
+    hipLaunchKernelGGL((paged_attn_kernel<D, FP8, false, NT, 1>), each, dim3(64), 0, st, p);
     return;
   }
-  hipLaunchKernelGGL((paged_attn_kernel<D, FP8, true, NT>), dim3(y, (unsigned)t.ranges), threads,
+  if (t.ranges == 0) {
+    hipLaunchKernelGGL((paged_attn_kernel<D, FP8, false, NT, kTokenWaves>), each, threads, 0, st, p);
+    return;
+  }
+  hipLaunchKernelGGL((paged_attn_kernel<D, FP8, true, NT, kTokenWaves>), dim3(y, (unsigned)t.ranges), threads,
                      (unsigned)(p.B + 1) * 4, st, p);
   if (t.ranges > 1)
     hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)t.ranges - 1, y, (unsigned)t.part_heads), dim3(256), 0,

@@ -276,6 +276,8 @@ TOKENS = [
     ([1] * 9 + [20000], 7, 7, 128, 32), ([4096] * 3, 16, 1, 64, 16),
     # tables that could hold more than the last-level cache, in both forms
     ([33] * 120, 8, 4, 128, 16), ([1] * 129 + [1024], 8, 4, 128, 16),
+    # a wave a request and key head
+    ([0, 1, 31, 32, 33, 128, 127, 65] * 17, 12, 4, 64, 16), ([256, 0, 200, 129] * 64, 24, 8, 128, 32),
 ]
 
 
