@@ -660,6 +660,9 @@ using namespace ltx;
 // whole) and the prompts have keys enough to pay for the join: 768 on average,
 // 2048 above an eighth (32/8 heads x 128: 16 rows over 1024 keys 12.0 us and 20.6
 // whole, over 512 no difference; 512 rows over 2048 34 and 41, over 1024 28 and 22).
+// Up to 32 rows a prompt there is little to join: up to half of the workgroups, and 256 keys
+// on average, of which some prompts have more (5 prompts of 8 rows over 2000 keys
+// 21.7 us and 32.4 whole; 32 of up to 8 rows over up to 3000, 8 heads x 64, 20.3 and 27.1).
 struct PromptPlan {
   int64_t tiles, grid, split;
   int64_t bytes(int64_t D) const { return split > 1 ? grid * split * kRows * (D + 2) * 4 : 0; }
@@ -668,7 +671,9 @@ static PromptPlan plan_prompt(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int
   // the most row tiles of B prompts with Tq rows: B of one row, and full ones
   const int64_t some = B < Tq ? B : Tq, tiles = some + (Tq - some) / kRows;
   PromptPlan t{tiles, ceil_div((tiles > 0 ? tiles : 1) * Hk, 8) * 8 * G, 1};
-  if (Tq > 0 && t.grid * 4 <= kResident && Tk >= B * (t.grid * 8 <= kResident ? 768 : 2048)) {
+  const bool few = Tq <= 32 * B;
+  const int64_t least = few ? (B > 3 ? B * 256 : 768) : B * (t.grid * 8 <= kResident ? 768 : 2048);
+  if (Tq > 0 && t.grid * (few ? 2 : 4) <= kResident && Tk >= least) {
     t.split = kResident / t.grid;
     if (t.split > 16) t.split = 16;
   }

@@ -207,6 +207,7 @@ PROMPTS = [
     # few rows over many keys: shared among workgroups
     ([5], [3100], 8, 2, 128), ([130, 1], [2500, 4000], 4, 4, 64), ([60], [1100], 3, 1, 128),
     ([1, 2, 3], [20, 9000, 1], 2, 1, 64), ([300, 10, 0], [200, 4500, 70], 2, 2, 128),
+    ([8, 0, 3, 1], [900, 0, 30, 400], 8, 1, 64),
 ]
 
 

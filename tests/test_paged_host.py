@@ -181,7 +181,13 @@ def test_workspace_of_the_split():
     assert size(1, 8, 4, 128, 65, 16) == 9 * (8 * part + 16)
     assert size(1, 600, 1, 128, 65, 16) == 0                 # heads enough
     rows = lambda *a: (_native.call("ltx_prompt_attn_workspace_size", *a, ctypes.byref(n)), n.value)[1]  # noqa: E731
+    part = 128 * 130 * 4
     assert rows(1, 128, 767, 8, 4, 128) == 0                 # too few keys to share
-    assert rows(1, 128, 768, 8, 4, 128) == 32 * 16 * 128 * 130 * 4
-    assert rows(2, 128, 1500, 8, 4, 128) == 0 and rows(8, 1024, 16384, 8, 4, 128) == 0
-    assert rows(1, 512, 2047, 8, 4, 128) == 0 and rows(1, 512, 2048, 8, 4, 128) == 128 * 4 * 128 * 130 * 4
+    assert rows(1, 128, 768, 8, 4, 128) == 32 * 16 * part
+    assert rows(2, 128, 1535, 8, 4, 128) == 0 and rows(8, 1024, 16384, 8, 4, 128) == 0
+    assert rows(1, 512, 2047, 8, 4, 128) == 0 and rows(1, 512, 2048, 8, 4, 128) == 128 * 4 * part
+    assert rows(1, 1024, 8192, 8, 4, 128) == 0               # half of the resident workgroups
+    # up to 32 rows a prompt
+    assert rows(4, 128, 1023, 8, 4, 128) == 0 and rows(4, 128, 1024, 8, 4, 128) == 128 * 4 * part
+    assert rows(8, 8, 2048, 8, 4, 128) == 256 * 2 * part and rows(9, 9, 4096, 8, 4, 128) == 0
+    assert rows(2, 64, 767, 8, 4, 128) == 0 and rows(2, 64, 768, 8, 4, 128) == 64 * 8 * part
