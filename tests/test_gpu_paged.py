@@ -57,7 +57,8 @@ def test_grow(dev, B, hi, new_hi, block, pad, in_place):
 @pytest.mark.parametrize("why,code", [("free", N.BLOCKS_FREE), ("width", N.BLOCKS_WIDTH), ("tokens", N.BLOCKS_TOKENS),
                                       ("new", N.BLOCKS_LENGTH), ("len", N.BLOCKS_LENGTH), ("top", N.BLOCKS_FREE)])
 @pytest.mark.parametrize("big", [False, True])
-def test_grow_that_does_not_fit_gives_nothing(dev, why, code, big):
+@pytest.mark.parametrize("in_place", [False, True])
+def test_grow_that_does_not_fit_gives_nothing(dev, why, code, big, in_place):
     block, lens, new = 16, [5, 0, 33, 16], [20, 3000 if big else 1, 0, 1]
     T = sum(new)
     width, blocks = 200, 250
@@ -80,7 +81,8 @@ def test_grow_that_does_not_fit_gives_nothing(dev, why, code, big):
         new[0] = 30
         T = sum(new)
     t, le, tp, status = ints(tables, dev), ints(lens, dev), ints([top], dev), ints([0], dev)
-    plan = kernels.kv_block_grow(t, le, ints(new, dev), ints(free, dev), tp, status, block, T)
+    plan = kernels.kv_block_grow(t, le, ints(new, dev), ints(free, dev), tp, status, block, T, le if in_place else None,
+                                 tp if in_place else None)
     assert status.item() & code
     assert t.tolist() == tables and plan.lens.tolist() == lens and plan.top.tolist() == [top]
     assert plan.starts.tolist() == [0] * 5 and plan.slots.tolist() == [-1] * T and plan.positions.tolist() == [0] * T
@@ -208,6 +210,7 @@ PROMPTS = [
     ([5], [3100], 8, 2, 128), ([130, 1], [2500, 4000], 4, 4, 64), ([60], [1100], 3, 1, 128),
     ([1, 2, 3], [20, 9000, 1], 2, 1, 64), ([300, 10, 0], [200, 4500, 70], 2, 2, 128),
     ([8, 0, 3, 1], [900, 0, 30, 400], 8, 1, 64),
+    ([1, 0, 3, 2] * 250, [5, 2, 3, 1] * 250, 1, 1, 64),
 ]
 
 
