@@ -63,6 +63,15 @@ struct PromptRows {
 __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows& r) {
   const int lane = threadIdx.x & 63;
   r.end = 0;
+  if (p.B == 1) {  // no search: scalar loads
+    r.q0 = min(max(p.q_starts[0], 0), p.Tq);
+    r.end = min(max(p.q_starts[1], r.q0), p.Tq);
+    r.k0 = min(max(p.k_starts[0], 0), p.Tk);
+    r.Lk = min(max(p.k_starts[1], r.k0), p.Tk) - r.k0;
+    r.Lq = r.end - r.q0;
+    r.row0 = ((r.Lq + kRows - 1) / kRows - 1 - t) * kRows;
+    return r.row0 >= 0;
+  }
   for (int b0 = p.B - 1; b0 >= 0; b0 -= 64) {
     const int b = b0 - lane;
     int s = 0, n = 0, ks = 0, m = 0;

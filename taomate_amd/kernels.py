@@ -267,5 +267,6 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch
     ``starts[b]`` to ``starts[b + 1]`` and its keys ``k_starts[b]`` to ``k_starts[b + 1]`` (int32 [prompts + 1];
     None: as the rows).  ``causal``: the last row sees every key of its prompt, each row before it one fewer;
     rows that see none are zero (``lse`` float32 [heads, Tq]: -inf).  Rows behind the last prompt are zero in a
-    new result and left as they are in ``out``.  Computes no gradients."""
+    new result and left as they are in ``out``.  A value of v that is not finite makes NaN of earlier rows of its
+    prompt within the same 128 rows.  Computes no gradients."""
     return (N._host or N.host()).prompt_attn(q, k, v, starts, k_starts, causal, scale, out, lse)

@@ -269,6 +269,10 @@ def test_prompt_starts_outside_the_tensors_are_cut(dev):
     ref, mag, _ = prompt_reference(q[:40], q[:40], q[:40], [40], [40], True)
     assert_attention_close(out[:30], ref[:30], mag[:30])
     assert torch.isfinite(out).all()
+    assert torch.equal(kernels.prompt_attn(q, q, q, ints([-5, 40], dev))[:30], out[:30])
+    assert (kernels.prompt_attn(q, q, q, ints([0, 0], dev)) == 0).all()
+    assert (kernels.prompt_attn(q, q, q, ints([50, 20], dev)) == 0)[50:].all()
+    assert (kernels.prompt_attn(q, q, q, ints([0], dev)) == 0).all()
 
 
 # ------------------------------------------------------------------ single tokens
