@@ -222,15 +222,16 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   const int voff = krow0 * p.v_ls + ((lane % NKC) ^ key_swizzle<NKC>(krow0)) * 16;
   const char* kptr = p.k + kvh * p.k_hs + (int64_t)w.k0 * p.k_ls;
   const char* vptr = p.v + kvh * p.v_hs + (int64_t)w.k0 * p.v_ls;
-  int krem = w.Lk, vrem = w.Lk;  // keys from the next K (V) tile on
+  int krem = seen, vrem = seen;  // seen keys from the next K (V) tile on
   auto lds_slot0 = [&](uint16_t* buf0) {
     uint32_t a = (uint32_t)(uintptr_t)(lds_ptr_t)(buf0 + wave * 512);
     asm volatile("" : "+s"(a));  // one address, not one scalar register for each slot and buffer
     return a;
   };
-  // A tile's loads.  Rows past the prompt's end lie outside the partial tile's
-  // buffer range: those lanes load zeros, so nothing of the next prompt or of
-  // memory behind the tensor is read, and their scores are masked.  A whole
+  // A tile's loads.  Rows past the last key that any row here sees lie outside the
+  // partial tile's buffer range: those lanes load zeros, so nothing of later keys, of
+  // the next prompt or of memory behind the tensor is read, and their scores are
+  // masked.  A whole
   // tile's slots take their uniform offset from a scalar register; a partial
   // tile adds it per lane, so that the range check sees all of it.
   auto issue = [&](uint16_t* buf0, const char*& ptr, int& rem, int off0, int row_bytes, auto keys_of_slot) {

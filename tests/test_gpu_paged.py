@@ -263,6 +263,21 @@ def test_prompt_keys_that_are_not_finite_and_lowest_scores(dev):
     assert out[199].isnan().all()
 
 
+@pytest.mark.parametrize("past", [0, 10, 70])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_values_that_are_not_finite_stay_within_their_128_rows(dev, past, D):
+    n = 300
+    g = torch.Generator().manual_seed(past)
+    q = torch.randn(n, 2, D, generator=g).to(BF).to(dev)
+    k, v = (torch.randn(n + past, 1, D, generator=g).to(BF).to(dev) for _ in range(2))
+    starts, k_starts = starts_of([n], dev), starts_of([n + past], dev)
+    want = kernels.prompt_attn(q, k, v, starts, k_starts)
+    v[past + 128:past + 256] = math.nan               # the keys of rows 128 to 255
+    v[past + 270] = math.inf
+    got = kernels.prompt_attn(q, k, v, starts, k_starts)
+    assert torch.equal(got[:128], want[:128]) and got[128:].isnan().any(-1).all()
+
+
 def test_prompt_starts_outside_the_tensors_are_cut(dev):
     q = torch.randn(64, 1, 64, device=dev).to(BF)
     out = kernels.prompt_attn(q, q, q, ints([-5, 40, 30, 9999], dev))
