@@ -759,9 +759,15 @@ void counted(const char* what, const char* name, const at::Tensor& t, at::Scalar
   if (vector(what, name, t, type) != n)
     value_error(std::string(what) + ": " + name + " must hold " + std::to_string(n) + " values, got " + shape(t));
 }
+// Whether the memory from a's first to its last element meets b's.
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
-  return a.numel() > 0 && b.numel() > 0 && p < q + b.nbytes() && q < p + a.nbytes();
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return static_cast<const char*>(a.data_ptr()) < end(b) && static_cast<const char*>(b.data_ptr()) < end(a);
 }
 // out: the tensor that a result goes to, `in` itself or memory apart from all that the call reads
 void apart(const char* what, const char* name, const at::Tensor& out, std::initializer_list<Opt> read, Opt in = nullptr) {
@@ -933,6 +939,8 @@ void kv_paged_append(PyObject* const* a) {
     if (x != nullptr && !rows_apart({{pk.n, stride_of(*x, 0)}, {pk.block, stride_of(*x, 1)}, {pk.H, stride_of(*x, 2)}}, 1))
       value_error("kv_paged_append: scales overlap");
   if (kp.numel() > 0 && kp.data_ptr() == vp.data_ptr()) value_error("kv_paged_append: k_pool and v_pool are the same memory");
+  if (ks != nullptr && ks->numel() > 0 && ks->data_ptr() == vs->data_ptr())
+    value_error("kv_paged_append: k_scales and v_scales are the same memory");
   const c10::DeviceGuard guard(k.device());
   const auto st = [&](Opt s, int d) { return s != nullptr ? stride_of(*s, d) : 0; };
   call("ltx_kv_paged_append", api.kv_paged_append, pk.dtype, rk.T, rk.H, rk.D, ptr(&k), rk.ls, rk.hs, ptr(&v), rv.ls,

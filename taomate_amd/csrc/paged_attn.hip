@@ -519,7 +519,7 @@ extern "C" int ltx_paged_attn(int kv_dtype, int64_t B, int64_t Hk, int64_t G, in
   LTX_REQUIRE(shift > 0, "%s: block of %lld tokens (16, 32, 64, 128 or 256)", name, (long long)block);
   LTX_REQUIRE(n_blocks >= 1 && n_blocks <= 0x7FFFFFFF, "%s: a pool holds at least one block", name);
   LTX_REQUIRE(width >= 1 && width * block <= 0x40000000, "%s: a table row holds 1 to 2^30 tokens", name);
-  LTX_REQUIRE(B * ceil_div(width * block, kTokenTile) <= 0x7FFFFFFF, "%s: the tables hold too many tokens", name);
+  LTX_REQUIRE(B * ceil_div(width * block, kTokenTile) <= 0x40000000, "%s: the tables hold too many tokens", name);
   if (B == 0) return LTX_OK;
   const bool fp8 = kv_dtype == LTX_F8E4M3;
   LTX_REQUIRE(q && k_pool && v_pool && tables && lens && out && (!fp8 || (k_scales && v_scales)), "%s: null pointer", name);

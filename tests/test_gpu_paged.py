@@ -88,6 +88,19 @@ def test_grow_that_does_not_fit_gives_nothing(dev, why, code, big, in_place):
     assert plan.starts.tolist() == [0] * 5 and plan.slots.tolist() == [-1] * T and plan.positions.tolist() == [0] * T
 
 
+def test_tables_in_wide_rows_lie_apart_from_the_other_operands(dev):
+    memory = torch.zeros(8, 100, dtype=torch.int32, device=dev)
+    inside = memory[7, 4:]   # behind the first 8 * 20 elements, within the last row's
+    new, free, top, status = ints([0] * 8, dev), ints([0, 1], dev), ints([2], dev), ints([0], dev)
+    done = torch.zeros(8, dtype=torch.bool, device=dev)
+    for lens, stack in ((inside[:8], free), (ints([0] * 8, dev), inside[:2])):
+        with pytest.raises(ValueError, match="overlaps"):
+            kernels.kv_block_grow(memory[:, :20], lens, new, stack, top, status, 16, 4)
+    with pytest.raises(ValueError, match="free overlaps"):
+        kernels.kv_block_release(memory[:, :20], new, done, inside[:2], top, status, 16)
+    assert int(memory.abs().sum()) == 0 and status.item() == 0
+
+
 @pytest.mark.parametrize("B,hi,block,in_place", [(1, 30, 16, False), (9, 100, 16, True), (513, 4000, 16, False),
                                                  (513, 4000, 16, True), (3, 0, 32, False)])
 def test_release(dev, B, hi, block, in_place):
@@ -156,6 +169,13 @@ def test_append_refuses_one_memory_for_both(dev):
     x = torch.zeros(1, 1, 64, dtype=BF, device=dev)
     with pytest.raises(ValueError, match="same memory"):
         kernels.kv_paged_append(x, x, c.k, c.k, torch.zeros(1, dtype=torch.int64, device=dev))
+
+
+def test_append_refuses_one_memory_for_both_scales(dev):
+    c = Cache([16], 1, 64, 16, "fp8", dev)
+    x = torch.zeros(1, 1, 64, dtype=BF, device=dev)
+    with pytest.raises(ValueError, match="k_scales and v_scales are the same memory"):
+        kernels.kv_paged_append(x, x, c.k, c.v, torch.zeros(1, dtype=torch.int64, device=dev), c.k_scales, c.k_scales)
 
 
 def test_results_in_the_queries_memory(dev):
