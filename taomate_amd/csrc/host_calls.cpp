@@ -959,12 +959,21 @@ at::Tensor rows_out(const char* what, Opt out, const at::Tensor& q) {
   return *out;
 }
 
+// The factor of the logits; None: 0, for which the library takes 1/sqrt(D).
+float logit_scale(const char* what, PyObject* o) {
+  if (o == Py_None) return 0.0f;
+  const float s = (float)real(o);
+  if (!(s > 0.0f && s <= 2e38f))  // times log2(e) it is a float32 too
+    value_error(std::string(what) + ": scale must be a finite float32 above 0, up to 2e38 (None: 1/sqrt(D))");
+  return s;
+}
+
 // (q, k_pool, v_pool, tables, lens, k_scales, v_scales, scale, out, lse)
 PyObject* paged_attn(PyObject* const* a) {
   const char* const what = "paged_attn";
   const at::Tensor &q = tensor(a[0]), &kp = tensor(a[1]), &vp = tensor(a[2]), &tables = tensor(a[3]), &lens = tensor(a[4]);
   const Opt ks = optional(a[5]), vs = optional(a[6]), out = optional(a[8]), lse = optional(a[9]);
-  const float scale = a[7] == Py_None ? 0.0f : (float)real(a[7]);
+  const float scale = logit_scale(what, a[7]);
   same_device(what, q, {&kp, &vp, &tables, &lens, ks, vs, out, lse});
   const TokenRows rq = token_rows(what, "q", q);
   const Pool pk = pool(what, "k_pool", kp), pv = pool(what, "v_pool", vp);
@@ -1007,7 +1016,7 @@ PyObject* prompt_attn(PyObject* const* a) {
   const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &starts = tensor(a[3]);
   const Opt given = optional(a[4]), out = optional(a[7]), lse = optional(a[8]);
   const at::Tensor& k_starts = given != nullptr ? *given : starts;
-  const float scale = a[6] == Py_None ? 0.0f : (float)real(a[6]);
+  const float scale = logit_scale(what, a[6]);
   same_device(what, q, {&k, &v, &starts, given, out, lse});
   const TokenRows rq = token_rows(what, "q", q), rk = token_rows(what, "k", k), rv = token_rows(what, "v", v);
   const int64_t n = vector(what, "starts", starts, at::kInt);

@@ -254,9 +254,10 @@ def paged_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, tabl
                lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """ltx_paged_attn: one token of each request, bf16 q [B, heads, D], over the first ``lens`` (int32 [B]) tokens
     of its blocks; query head h reads key head h // (heads / key heads).  Requests without tokens get zero rows
-    (``lse`` float32 [B, heads]: -inf).  ``out`` may be ``q`` but share no other memory that the call reads.
-    Computes no gradients.  The tables' width bounds the lengths: the work is planned for what they can hold, with
-    one launch up to 1024 tokens (512 for a few requests) and a joining second one beyond."""
+    (``lse`` float32 [B, heads]: -inf).  ``scale`` must be above 0 (None: 1/sqrt(D)).  ``out`` may be ``q`` but
+    share no other memory that the call reads.  Computes no gradients.  The tables' width bounds the lengths: the
+    work is planned for what they can hold, with one launch up to 1024 tokens (512 for a few requests) and a joining
+    second one beyond."""
     return (N._host or N.host()).paged_attn(q, k_pool, v_pool, tables, lens, k_scales, v_scales, scale, out, lse)
 
 
@@ -268,6 +269,6 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch
     None: as the rows).  ``causal``: the last row sees every key of its prompt, each row before it one fewer;
     rows that see none are zero (``lse`` float32 [heads, Tq]: -inf).  Rows behind the last prompt are zero in a
     new result and left as they are in ``out``.  A value of v that is not finite makes NaN of earlier rows of its
-    prompt within the same 128 rows.  ``out`` may be ``q`` but share no other memory that the call reads.
-    Computes no gradients."""
+    prompt within the same 128 rows.  ``scale`` must be above 0 (None: 1/sqrt(D)).  ``out`` may be ``q`` but share
+    no other memory that the call reads.  Computes no gradients."""
     return (N._host or N.host()).prompt_attn(q, k, v, starts, k_starts, causal, scale, out, lse)

@@ -191,3 +191,10 @@ def test_workspace_of_the_split():
     assert rows(4, 128, 1023, 8, 4, 128) == 0 and rows(4, 128, 1024, 8, 4, 128) == 128 * 4 * part
     assert rows(8, 8, 2048, 8, 4, 128) == 256 * 2 * part and rows(9, 9, 4096, 8, 4, 128) == 0
     assert rows(2, 64, 767, 8, 4, 128) == 0 and rows(2, 64, 768, 8, 4, 128) == 64 * 8 * part
+
+
+@pytest.mark.parametrize("call", [token, prompt])
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 1e39, 3e38, 1e-60])
+def test_scales_that_are_no_positive_float32_are_refused(call, scale):
+    with pytest.raises(ValueError, match="scale must be a finite float32 above 0"):
+        call(scale=scale)
