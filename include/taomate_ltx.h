@@ -506,12 +506,13 @@ int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, int64_t D, i
  * Attention over whole prompts, packed: q, out bf16 [Tq, Hk * G, D], k, v bf16
  * [Tk, Hk, D] (strides ls, hs; D 64 or 128).  Prompt b's rows are q[q_starts[b],
  * q_starts[b + 1]) and its keys k[k_starts[b], k_starts[b + 1]) (int32 [B + 1] on the
- * device, ascending from 0).
+ * device, ascending).
  *   causal != 0: the last row sees every key of its prompt and each row before it
  *   one key fewer, so with more keys than rows the prompt continues a prefix, and
  *   with fewer the first rows see none: those get a zero row and lse -inf.
- *   Rows of out behind q_starts[B] are zeroed if zero_tail != 0, else left as they
- *   are.  Starts that are not ascending or pass Tq or Tk are cut, never followed.
+ *   Rows of out before q_starts[0] and behind q_starts[B] are zeroed (lse -inf) if
+ *   zero_rest != 0, else left as they are.  Starts that are not ascending or pass Tq
+ *   or Tk are cut, never followed.
  *   lse: NULL or float32 [Hk * G, Tq]; scale <= 0 selects 1/sqrt(D).
  *   Rows of every tensor 16-byte aligned.
  *   workspace: ltx_prompt_attn_workspace_size() bytes, 16-byte aligned (0: none; few
@@ -523,7 +524,7 @@ int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, int64_t D, i
 int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D, const void* q,
                     int64_t q_ls, int64_t q_hs, const void* k, int64_t k_ls, int64_t k_hs, const void* v,
                     int64_t v_ls, int64_t v_hs, const int32_t* q_starts, const int32_t* k_starts, int causal,
-                    void* out, int64_t o_ls, int64_t o_hs, int zero_tail, float* lse, float scale,
+                    void* out, int64_t o_ls, int64_t o_hs, int zero_rest, float* lse, float scale,
                     void* workspace, int64_t workspace_bytes, void* stream);
 int ltx_prompt_attn_workspace_size(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D,
                                    int64_t* bytes);

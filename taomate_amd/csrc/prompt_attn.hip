@@ -40,7 +40,7 @@ struct PromptAttn {
   int64_t k_hs, v_hs;
   int k_ls, v_ls;
   const int32_t *q_starts, *k_starts;
-  int B, Tq, Tk, Hk, G, causal, zero_tail, sorted, tiles;
+  int B, Tq, Tk, Hk, G, causal, zero_rest, sorted, tiles;
   float scale_log2;
   // SPLIT: a row tile's key tiles are shared by up to `split` workgroups, whose
   // results [workgroup][range][row][D] and (maximum, sum) are joined afterwards
@@ -49,10 +49,10 @@ struct PromptAttn {
 };
 
 // Where a workgroup works: rows from row0 of a prompt whose Lq rows start at q0 and
-// whose Lk keys start at k0 of the packed tensors; end: the first row behind
-// all prompts.
+// whose Lk keys start at k0 of the packed tensors; begin, end: the first row of
+// all prompts and the first one behind them.
 struct PromptRows {
-  int q0, k0, row0, Lq, Lk, end;
+  int q0, k0, row0, Lq, Lk, begin, end;
 };
 
 // Row tile t in the order in which the workgroups start: a prompt's last tile
@@ -62,9 +62,9 @@ struct PromptRows {
 // False: there are fewer tiles.
 __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows& r) {
   const int lane = threadIdx.x & 63;
-  r.end = 0;
+  r.begin = r.end = 0;
   if (p.B == 1) {  // no search: scalar loads
-    r.q0 = min(max(p.q_starts[0], 0), p.Tq);
+    r.begin = r.q0 = min(max(p.q_starts[0], 0), p.Tq);
     r.end = min(max(p.q_starts[1], r.q0), p.Tq);
     r.k0 = min(max(p.k_starts[0], 0), p.Tk);
     r.Lk = min(max(p.k_starts[1], r.k0), p.Tk) - r.k0;
@@ -82,7 +82,10 @@ __device__ __forceinline__ bool find_rows(const PromptAttn& p, int t, PromptRows
       ks = min(max(k0, 0), p.Tk);
       m = min(max(k1, ks), p.Tk) - ks;
     }
-    if (b0 == p.B - 1) r.end = __builtin_amdgcn_readfirstlane(s + n);
+    if (b0 == p.B - 1) {
+      r.end = __builtin_amdgcn_readfirstlane(s + n);
+      r.begin = p.B <= 64 ? __builtin_amdgcn_readlane(s, p.B - 1) : min(max(p.q_starts[0], 0), p.Tq);
+    }
     if (p.sorted) {
       // by powers of two of their number of key tiles: the longest three, then the others
       const int mine = lane < p.B ? 32 - __builtin_clz(m / kKeys + 1) : 0;
@@ -181,12 +184,14 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   const int li = lane & 15, lg = lane >> 4;
   PromptRows w;
   const bool works = find_rows(p, unit, w);
-  if (p.zero_tail && w.end < p.Tq && (!SPLIT || blockIdx.y == 0)) {
-    // rows behind the prompts, shared by all row tiles
-    for (int64_t row0 = w.end + (int64_t)unit * kRows; row0 < p.Tq; row0 += (int64_t)p.tiles * kRows)
+  const int rest = w.begin + p.Tq - w.end;
+  if (p.zero_rest && rest > 0 && (!SPLIT || blockIdx.y == 0)) {
+    // rows before and behind the prompts, shared by all row tiles
+    for (int64_t row0 = (int64_t)unit * kRows; row0 < rest; row0 += (int64_t)p.tiles * kRows)
       for (int i = threadIdx.x; i < kRows * NKC; i += 256) {
-        const int64_t row = row0 + i / NKC;
-        if (row >= p.Tq) break;
+        int64_t row = row0 + i / NKC;
+        if (row >= rest) break;
+        if (row >= w.begin) row += w.end - w.begin;
         *reinterpret_cast<uint4*>(p.o + row * p.o_ls + h * p.o_hs + i % NKC * 8) = make_uint4(0, 0, 0, 0);
         if (p.lse != nullptr && i % NKC == 0) p.lse[(int64_t)h * p.Tq + row] = -INFINITY;
       }
@@ -714,7 +719,7 @@ static void launch_prompt(const PromptAttn& p, const PromptPlan& t, hipStream_t 
 extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, int64_t G, int64_t D, const void* q,
                                int64_t q_ls, int64_t q_hs, const void* k, int64_t k_ls, int64_t k_hs, const void* v,
                                int64_t v_ls, int64_t v_hs, const int32_t* q_starts, const int32_t* k_starts, int causal,
-                               void* out, int64_t o_ls, int64_t o_hs, int zero_tail, float* lse, float scale,
+                               void* out, int64_t o_ls, int64_t o_hs, int zero_rest, float* lse, float scale,
                                void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   const char* const name = "ltx_prompt_attn";
@@ -736,7 +741,7 @@ extern "C" int ltx_prompt_attn(int64_t B, int64_t Tq, int64_t Tk, int64_t Hk, in
   p.v = static_cast<const char*>(v), p.v_ls = (int)(Tk > 1 ? v_ls : D) * 2, p.v_hs = v_hs * 2;
   p.q_starts = q_starts, p.k_starts = k_starts;
   p.B = (int)B, p.Tq = (int)Tq, p.Tk = (int)Tk, p.Hk = (int)Hk, p.G = (int)G;
-  p.causal = causal != 0, p.zero_tail = zero_tail != 0;
+  p.causal = causal != 0, p.zero_rest = zero_rest != 0;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)D)) * kLog2e;
   const PromptPlan t = plan_prompt(B, Tq, Tk, Hk, G);
   LTX_REQUIRE(t.grid < (1 << 24), "%s: too many rows and heads for one launch", name);  // 2^32 threads

@@ -267,8 +267,8 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch
     """ltx_prompt_attn: packed prompts, bf16 q [Tq, heads, D] over k, v [Tk, key heads, D].  Prompt b's rows are
     ``starts[b]`` to ``starts[b + 1]`` and its keys ``k_starts[b]`` to ``k_starts[b + 1]`` (int32 [prompts + 1];
     None: as the rows).  ``causal``: the last row sees every key of its prompt, each row before it one fewer;
-    rows that see none are zero (``lse`` float32 [heads, Tq]: -inf).  Rows behind the last prompt are zero in a
-    new result and left as they are in ``out``.  A value of v that is not finite makes NaN of earlier rows of its
+    rows that see none are zero (``lse`` float32 [heads, Tq]: -inf).  Rows before the first prompt and behind the
+    last are zero in a new result (``lse`` -inf) and left as they are, ``lse`` too, with ``out``.  A value of v that is not finite makes NaN of earlier rows of its
     prompt within the same 128 rows.  ``scale`` must be above 0 (None: 1/sqrt(D)).  ``out`` may be ``q`` but share
     no other memory that the call reads.  Computes no gradients."""
     return (N._host or N.host()).prompt_attn(q, k, v, starts, k_starts, causal, scale, out, lse)

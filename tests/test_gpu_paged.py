@@ -590,3 +590,32 @@ def test_cache_object(dev, kv):
         c.check()
     assert all(torch.equal(a, b) for a, b in zip((c.tables, c.lens, c.top), before))
     c.check()
+
+
+@pytest.mark.parametrize("first,rows,keys", [(50, [14], None), (300, [200, 0, 30], None), (64, [20], [3000]),
+                                             (17, [], None), (40, [3] * 70, None)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_rows_before_the_first_prompt(dev, first, rows, keys, D):
+    """A call over some of the prompts: the rows of the others are zero in a new result, and left in one given."""
+    T = first + sum(rows) + 9
+    g = torch.Generator().manual_seed(first)
+    q = torch.randn(T, 4, D, generator=g).to(BF).to(dev)
+    k, v = (torch.randn(sum(keys or rows) + first, 2, D, generator=g).to(BF).to(dev) for _ in range(2))
+    starts = starts_of(rows, dev) + first
+    k_starts = starts_of(keys or rows, dev) + first
+    mine = slice(first, first + sum(rows))
+    ref, mag, lse_ref = prompt_reference(q[mine], k[first:], v[first:], rows, keys or rows, True)
+    given = torch.full_like(q, 3.0)
+    kernels.prompt_attn(q, k, v, starts, k_starts, out=given)
+    lse = torch.full((4, T), 5.0, device=dev)
+    dirty = torch.full_like(q, math.nan)
+    at = dirty.data_ptr()
+    del dirty                                            # the new result takes this memory
+    out = kernels.prompt_attn(q, k, v, starts, k_starts, lse=lse)
+    assert out.data_ptr() == at
+    assert_attention_close(out[mine], ref, mag)
+    assert_lse_close(lse[:, mine], lse_ref)
+    rest = torch.ones(T, dtype=torch.bool, device=dev)
+    rest[mine] = False
+    assert (out[rest] == 0).all() and (lse[:, rest] == -math.inf).all()
+    assert torch.equal(given[mine], out[mine]) and (given[rest] == 3).all()
