@@ -463,7 +463,8 @@ int ltx_kv_block_release(int64_t B, int64_t width, int64_t block, const int32_t*
  * Writes K and V of T tokens (bf16 [T, H, D], strides (ls, hs), D 64 or 128) into
  * their slots of the pools: element (block, token, h, d) at pool + block*ps +
  * token*ts + h*hs + d.  Tokens whose slot is negative or past the pool are
- * skipped; slots must be distinct.
+ * skipped; slots must be distinct, and the pools and scales share no memory with
+ * each other, k, v and slots.
  *   kv_dtype LTX_BF16 copies; LTX_F8E4M3 writes e4m3 codes and a float32 scale
  *   for every token and head, at scales + block*ps + token*ts + h*hs: the row's
  *   largest finite magnitude / 448 (1 if that is 0), codes rounded to nearest

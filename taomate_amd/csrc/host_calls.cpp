@@ -759,21 +759,70 @@ void counted(const char* what, const char* name, const at::Tensor& t, at::Scalar
   if (vector(what, name, t, type) != n)
     value_error(std::string(what) + ": " + name + " must hold " + std::to_string(n) + " values, got " + shape(t));
 }
-// Whether the memory from a's first to its last element meets b's.
-bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto end = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
-  };
-  return static_cast<const char*>(a.data_ptr()) < end(b) && static_cast<const char*>(b.data_ptr()) < end(a);
+// A tensor's memory: `width` bytes at each of `count` steps of `step` bytes in up
+// to four dimensions, steps ascending.
+struct Extent {
+  struct Dim {
+    int64_t step, count;
+  } d[4];
+  int n = 0;
+  int64_t width;
+
+  explicit Extent(const at::Tensor& t) : width(t.element_size()) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) > 0) d[n++] = {t.stride(i) * width, t.size(i)};
+    std::sort(d, d + n, [](const Dim& a, const Dim& b) { return a.step < b.step; });
+  }
+  int64_t bytes(int dims) const {
+    int64_t all = width;
+    for (int i = 0; i < dims; ++i) all += d[i].step * (d[i].count - 1);
+    return all;
+  }
+};
+// Whether a's inner `na` dimensions meet b's, which start `delta` bytes further.
+// Views that take turns in memory (columns of one projection, K and V of one
+// pool) have the widest step in common: they meet where their rows do at one of the
+// two distances below a step.  Shapes that do not nest so count as one piece.
+bool meet(const Extent& a, int na, const Extent& b, int nb, int64_t delta) {
+  if (delta >= a.bytes(na) || -delta >= b.bytes(nb)) return false;
+  const int64_t sa = na > 0 ? a.d[na - 1].step : 0, sb = nb > 0 ? b.d[nb - 1].step : 0, step = std::max(sa, sb);
+  if (step == 0) return true;
+  const int ia = na - (sa == step), ib = nb - (sb == step);
+  if (a.bytes(ia) > step || b.bytes(ib) > step) return true;
+  const int64_t most = sb == step ? b.d[nb - 1].count - 1 : 0, least = sa == step ? 1 - a.d[na - 1].count : 0;
+  const int64_t under = delta >= 0 ? delta % step : (step - -delta % step) % step;
+  for (int64_t r : {under, under - step}) {
+    const int64_t steps = (r - delta) / step;  // rows of b less rows of a at this distance
+    if (steps >= least && steps <= most && meet(a, ia, b, ib, r)) return true;
+  }
+  return false;
 }
-// out: the tensor that a result goes to, `in` itself or memory apart from all that the call reads
+// The memory from a tensor's first to its last element.
+struct Span {
+  const char *first, *end;
+  explicit Span(const at::Tensor& t) {
+    if (t.numel() == 0) {
+      first = end = nullptr;
+      return;
+    }
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t last = 1;
+    for (size_t d = 0; d < sizes.size(); ++d) last += (sizes[d] - 1) * strides[d];
+    first = static_cast<const char*>(t.data_ptr());
+    end = first + last * (int64_t)t.element_size();
+  }
+};
+// out: the tensor that a result goes to (of up to four dimensions), `in` itself or memory apart from all that the call reads
 void apart(const char* what, const char* name, const at::Tensor& out, std::initializer_list<Opt> read, Opt in = nullptr) {
-  for (Opt t : read)
-    if (t != nullptr && overlap(out, *t) && !(t == in && out.data_ptr() == in->data_ptr()))
+  const Span o(out);
+  for (Opt t : read) {
+    if (t == nullptr) continue;
+    const Span r(*t);
+    if (r.first >= o.end || o.first >= r.end || (t == in && r.first == o.first)) continue;
+    const Extent x(out), y(*t);
+    if (meet(x, x.n, y, y.n, r.first - o.first))
       value_error(std::string(what) + ": " + name + " overlaps a tensor that the call reads or writes");
+  }
 }
 
 struct Tables {
@@ -941,6 +990,12 @@ void kv_paged_append(PyObject* const* a) {
   if (kp.numel() > 0 && kp.data_ptr() == vp.data_ptr()) value_error("kv_paged_append: k_pool and v_pool are the same memory");
   if (ks != nullptr && ks->numel() > 0 && ks->data_ptr() == vs->data_ptr())
     value_error("kv_paged_append: k_scales and v_scales are the same memory");
+  apart(what, "k_pool", kp, {&k, &v, &vp, &slots, ks, vs});
+  apart(what, "v_pool", vp, {&k, &v, &slots, ks, vs});
+  if (ks != nullptr) {
+    apart(what, "k_scales", *ks, {&k, &v, &slots, vs});
+    apart(what, "v_scales", *vs, {&k, &v, &slots});
+  }
   const c10::DeviceGuard guard(k.device());
   const auto st = [&](Opt s, int d) { return s != nullptr ? stride_of(*s, d) : 0; };
   call("ltx_kv_paged_append", api.kv_paged_append, pk.dtype, rk.T, rk.H, rk.D, ptr(&k), rk.ls, rk.hs, ptr(&v), rv.ls,

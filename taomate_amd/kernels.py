@@ -244,7 +244,8 @@ def kv_paged_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_po
                     k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None) -> None:
     """ltx_kv_paged_append: bf16 k, v [T, heads, D] into the slots (int64 [T], distinct; those outside the pool are
     skipped) of pools [blocks, block tokens, heads, D]: bf16, or e4m3 codes with float32 scales [blocks, block
-    tokens, heads], one for each token and head."""
+    tokens, heads], one for each token and head.  What is written may share no memory with the rest; pools may take turns
+    in one storage (K and V of a block or of a token side by side)."""
     (N._host or N.host()).kv_paged_append(k, v, k_pool, v_pool, slots, k_scales, v_scales)
 
 

@@ -619,3 +619,73 @@ def test_prompt_rows_before_the_first_prompt(dev, first, rows, keys, D):
     rest[mine] = False
     assert (out[rest] == 0).all() and (lse[:, rest] == -math.inf).all()
     assert torch.equal(given[mine], out[mine]) and (given[rest] == 3).all()
+
+
+def _share(a, b):
+    """Whether two views of one storage have an element in common."""
+    def elements(t):
+        at = torch.tensor([t.storage_offset()])
+        for n, step in zip(t.shape, t.stride()):
+            at = (at[:, None] + torch.arange(n) * step).flatten()
+        return set(at.tolist())
+    return bool(elements(a) & elements(b))
+
+
+def test_append_refuses_pools_that_overlap_and_takes_pools_that_take_turns(dev):
+    """No rows, so nothing is launched: whether K's and V's pools share memory, against their elements."""
+    none, slots = torch.empty(0, 2, 64, dtype=BF, device=dev), torch.empty(0, dtype=torch.int64, device=dev)
+    memory = torch.empty(1 << 16, dtype=BF, device=dev)
+    rng = random.Random(3)
+    refused = 0
+    for _ in range(300):
+        sizes = {"n": rng.choice([1, 2, 3]), "t": 16, "h": 2}
+        order = rng.sample(["n", "t", "h", "pair"], 4)     # from the innermost dimension; "pair": K, then V
+        step, strides = 64, {}
+        for d in order:
+            strides[d] = step
+            step = step * sizes.get(d, 2) + rng.choice([0, 0, 8])
+        at = strides["pair"] if rng.random() < 0.5 else 8 * rng.randint(1, step // 4)
+        shape, st = (sizes["n"], 16, 2, 64), (strides["n"], strides["t"], strides["h"], 1)
+        k, v = memory.as_strided(shape, st), memory.as_strided(shape, st, at)
+        if _share(k, v):
+            refused += 1
+            with pytest.raises(ValueError, match="k_pool overlaps"):
+                kernels.kv_paged_append(none, none, k, v, slots)
+            with pytest.raises(ValueError, match="k_pool overlaps"):
+                kernels.kv_paged_append(none, none, v, k, slots)
+        else:
+            kernels.kv_paged_append(none, none, k, v, slots)
+            kernels.kv_paged_append(none, none, v, k, slots)
+    assert 50 < refused < 250
+
+
+def test_append_refuses_rows_and_scales_inside_the_pools(dev):
+    c = Cache([40], 2, 64, 16, "fp8", dev, layout="tokens")
+    x = torch.zeros(4, 2, 64, dtype=BF, device=dev)
+    slots = torch.arange(4, device=dev)
+    before = [t.view(torch.uint8).clone() for t in (c.k, c.v)]
+    inside = c.k.view(torch.uint8).flatten()[:1024].view(BF).view(4, 2, 64)
+    for k, v, match in ((inside, x, "k_pool overlaps"), (x, inside, "k_pool overlaps")):
+        with pytest.raises(ValueError, match=match):
+            kernels.kv_paged_append(k, v, c.k, c.v, slots, c.k_scales, c.v_scales)
+    scales = c.k.view(torch.uint8).flatten().view(torch.float32)[:c.n * 32].view(c.n, 2, 16).permute(0, 2, 1)
+    assert scales.data_ptr() == c.k.data_ptr()
+    with pytest.raises(ValueError, match="k_pool overlaps"):
+        kernels.kv_paged_append(x, x, c.k, c.v, slots, scales, c.v_scales)
+    both = torch.empty(c.n * 32 + 16, device=dev)
+    first, second = (both[o:o + c.n * 32].view(c.n, 2, 16).permute(0, 2, 1) for o in (0, 16))
+    with pytest.raises(ValueError, match="k_scales overlaps"):
+        kernels.kv_paged_append(x, x, c.k, c.v, slots, first, second)
+    assert all(torch.equal(t.view(torch.uint8), b) for t, b in zip((c.k, c.v), before))
+
+
+def test_append_into_pools_that_take_turns(dev):
+    """K and V of a block, or of a token, side by side in one storage."""
+    for shape, pair, dims in (((5, 2, 2, 16, 64), 1, (0, 2, 1, 3)), ((5, 16, 2, 2, 64), 2, (0, 1, 2, 3))):
+        store = torch.zeros(shape, dtype=BF, device=dev)
+        k_pool, v_pool = (store.select(pair, i).permute(dims) for i in (0, 1))
+        x = torch.randn(20, 4, 64, device=dev).to(BF)
+        slots = torch.randperm(80, device=dev)[:20]
+        kernels.kv_paged_append(x[:, :2], x[:, 2:], k_pool, v_pool, slots)
+        assert torch.equal(k_pool[slots // 16, slots % 16], x[:, :2])
+        assert torch.equal(v_pool[slots // 16, slots % 16], x[:, 2:])
