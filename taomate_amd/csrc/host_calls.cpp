@@ -1014,6 +1014,20 @@ at::Tensor rows_out(const char* what, Opt out, const at::Tensor& q) {
   return *out;
 }
 
+// Results given by the caller: out is q itself, or shares memory with nothing that the call reads; nor does lse.
+void results_apart(const char* what, const at::Tensor& q, Opt out, Opt lse, std::initializer_list<Opt> read) {
+  if (out != nullptr) {
+    const bool same = out->data_ptr() == q.data_ptr() && stride_of(*out, 0) == stride_of(q, 0) &&
+                      stride_of(*out, 1) == stride_of(q, 1);
+    apart(what, "out", *out, read);
+    apart(what, "out", *out, {same ? nullptr : &q, lse});
+  }
+  if (lse != nullptr) {
+    apart(what, "lse", *lse, read);
+    apart(what, "lse", *lse, {&q});
+  }
+}
+
 // The factor of the logits; None: 0, for which the library takes 1/sqrt(D).
 float logit_scale(const char* what, PyObject* o) {
   if (o == Py_None) return 0.0f;
@@ -1050,6 +1064,7 @@ PyObject* paged_attn(PyObject* const* a) {
     value_error("paged_attn: lse must be contiguous float32 [requests, heads]");
   const c10::DeviceGuard guard(q.device());
   const at::Tensor o = rows_out(what, out, q);
+  results_apart(what, q, out, lse, {&kp, &vp, &tables, &lens, ks, vs});
   int64_t need = 0;
   call("ltx_paged_attn_workspace_size", api.paged_attn_workspace_size, B, pk.H, G, D, t.width, pk.block, &need);
   void* st = stream_of(q);
@@ -1085,6 +1100,7 @@ PyObject* prompt_attn(PyObject* const* a) {
     value_error("prompt_attn: lse must be contiguous float32 [heads, tokens]");
   const c10::DeviceGuard guard(q.device());
   const at::Tensor o = rows_out(what, out, q);
+  results_apart(what, q, out, lse, {&k, &v, &starts, given});
   const int64_t B = n - 1, G = rq.H / rk.H;
   int64_t need = 0;
   call("ltx_prompt_attn_workspace_size", api.prompt_attn_workspace_size, B, rq.T, rk.T, rk.H, G, rq.D, &need);

@@ -244,8 +244,8 @@ def kv_paged_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_po
                     k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None) -> None:
     """ltx_kv_paged_append: bf16 k, v [T, heads, D] into the slots (int64 [T], distinct; those outside the pool are
     skipped) of pools [blocks, block tokens, heads, D]: bf16, or e4m3 codes with float32 scales [blocks, block
-    tokens, heads], one for each token and head.  What is written may share no memory with the rest; pools may take turns
-    in one storage (K and V of a block or of a token side by side)."""
+    tokens, heads], one for each token and head.  What is written may share no memory with the rest; pools may
+    take turns in one storage (K and V of a block or of a token side by side)."""
     (N._host or N.host()).kv_paged_append(k, v, k_pool, v_pool, slots, k_scales, v_scales)
 
 
@@ -255,10 +255,10 @@ def paged_attn(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, tabl
                lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """ltx_paged_attn: one token of each request, bf16 q [B, heads, D], over the first ``lens`` (int32 [B]) tokens
     of its blocks; query head h reads key head h // (heads / key heads).  Requests without tokens get zero rows
-    (``lse`` float32 [B, heads]: -inf).  ``scale`` must be above 0 (None: 1/sqrt(D)).  ``out`` may be ``q`` but
-    share no other memory that the call reads.  Computes no gradients.  The tables' width bounds the lengths: the
-    work is planned for what they can hold, with one launch up to 1024 tokens (512 for a few requests) and a joining
-    second one beyond."""
+    (``lse`` float32 [B, heads]: -inf).  ``scale`` must be above 0 (None: 1/sqrt(D)).  ``out`` may be ``q`` but may
+    share no other memory with what the call reads.  Computes no gradients.  The tables' width bounds the lengths:
+    the work is planned for what they can hold, with one launch up to 1024 tokens (512 for a few requests) and a
+    joining second one beyond."""
     return (N._host or N.host()).paged_attn(q, k_pool, v_pool, tables, lens, k_scales, v_scales, scale, out, lse)
 
 
@@ -269,7 +269,8 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch
     ``starts[b]`` to ``starts[b + 1]`` and its keys ``k_starts[b]`` to ``k_starts[b + 1]`` (int32 [prompts + 1];
     None: as the rows).  ``causal``: the last row sees every key of its prompt, each row before it one fewer;
     rows that see none are zero (``lse`` float32 [heads, Tq]: -inf).  Rows before the first prompt and behind the
-    last are zero in a new result (``lse`` -inf) and left as they are, ``lse`` too, with ``out``.  A value of v that is not finite makes NaN of earlier rows of its
-    prompt within the same 128 rows.  ``scale`` must be above 0 (None: 1/sqrt(D)).  ``out`` may be ``q`` but share
-    no other memory that the call reads.  Computes no gradients."""
+    last are zero in a new result (``lse`` -inf) and left as they are, ``lse`` too, with ``out``.  A value of v that
+    is not finite makes NaN of earlier rows of its prompt within the same 128 rows.  ``scale`` must be above 0 (None:
+    1/sqrt(D)).  ``out`` may be ``q`` but may share no other memory with what the call reads.  Computes no
+    gradients."""
     return (N._host or N.host()).prompt_attn(q, k, v, starts, k_starts, causal, scale, out, lse)

@@ -689,3 +689,55 @@ def test_append_into_pools_that_take_turns(dev):
         kernels.kv_paged_append(x[:, :2], x[:, 2:], k_pool, v_pool, slots)
         assert torch.equal(k_pool[slots // 16, slots % 16], x[:, :2])
         assert torch.equal(v_pool[slots // 16, slots % 16], x[:, 2:])
+
+
+def test_results_over_what_the_call_reads_are_refused(dev):
+    c = Cache([30, 5], 2, 64, 16, "fp8", dev, layout="tokens")
+    q = torch.randn(2, 2, 64, device=dev).to(BF)
+
+    def token(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales, **kw)
+
+    in_pool = c.v.view(torch.uint8).flatten()
+    token("out overlaps", out=in_pool[256:768].view(BF).view(2, 2, 64))
+    token("lse overlaps", lse=in_pool[:16].view(torch.float32).view(2, 2))
+    token("lse overlaps", lse=q.flatten()[:8].view(torch.float32).view(2, 2))
+    wide = torch.zeros(3, 2, 64, device=dev, dtype=BF)
+    q = wide[:2]
+    token("out overlaps", out=wide[1:])                      # q's rows, one further
+    token("out overlaps", out=wide.flatten()[:256].view(2, 2, 64).transpose(0, 1))
+    out = torch.zeros(2, 2, 64, device=dev, dtype=BF)
+    token("out overlaps", out=out, lse=out.flatten()[:8].view(torch.float32).view(2, 2))
+
+    x = torch.randn(40, 4, 64, device=dev).to(BF)
+    starts = starts_of([30, 10], dev)
+    k, v = x[:, :2], x[:, 2:]
+
+    def prompt(match, q, k, v, **kw):
+        with pytest.raises(ValueError, match=match):
+            kernels.prompt_attn(q, k, v, starts, **kw)
+
+    q = torch.randn(40, 2, 64, device=dev).to(BF)
+    prompt("out overlaps", q, k, v, out=x[:, 1:3])
+    prompt("out overlaps", q, q, v, out=q)                    # the queries' memory, but the keys' as well
+    prompt("out overlaps", q, k, v, out=x.flatten()[64:64 + 40 * 128].view(40, 2, 64))
+    prompt("lse overlaps", q, k, v, lse=x.flatten()[:160].view(torch.float32).view(2, 40))
+
+
+def test_results_between_what_the_call_reads(dev):
+    """q, k, v and the result take turns in one storage, rows of one prompt among others."""
+    T, D, rows = 150, 64, [100, 50]
+    x = torch.randn(T, 10, D, generator=torch.Generator().manual_seed(1)).to(BF).to(dev)
+    q, k, v, out = x[:, :4], x[:, 4:5], x[:, 5:6], x[:, 6:]
+    starts = starts_of(rows, dev)
+    want, kv = kernels.prompt_attn(q, k, v, starts), x[:, :6].clone()
+    kernels.prompt_attn(q, k, v, starts, out=out)
+    assert torch.equal(out, want) and torch.equal(x[:, :6], kv)
+    kernels.prompt_attn(q, k, v, starts, out=q)
+    assert torch.equal(q, want) and torch.equal(x[:, 4:6], kv[:, 4:])
+    # one row over all keys: its result lies between the keys' rows
+    one, at = ints([0, 1], dev), ints([0, T], dev)
+    want = kernels.prompt_attn(q[70:71], k, v, one, at)
+    kernels.prompt_attn(q[70:71], k, v, one, at, out=out[70:71])
+    assert torch.equal(out[70:71], want) and torch.equal(x[:, 4:6], kv[:, 4:])
