@@ -107,12 +107,12 @@ class PagedKVCache:
         kp, vp, ks, vs = self.pool(layer)
         rows = torch.arange(q.shape[0], dtype=torch.int32, device=q.device)
         request = torch.searchsorted(plan.starts[1:], rows, right=True).clamp_(max=self.requests - 1)
-        tables = self.tables[request]
         lens = torch.where(plan.slots >= 0, plan.positions + 1, torch.zeros_like(plan.positions))
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         for a in range(0, q.shape[0], _ROWS):
             part = slice(a, a + _ROWS)
-            kernels.paged_attn(q[part], kp, vp, tables[part], lens[part], ks, vs, scale=scale, out=out[part])
+            tables = self.tables[request[part]]   # of this part's rows only: a row can have thousands of entries
+            kernels.paged_attn(q[part], kp, vp, tables, lens[part], ks, vs, scale=scale, out=out[part])
         return out
 
     def check(self) -> None:

@@ -741,3 +741,22 @@ def test_results_between_what_the_call_reads(dev):
     want = kernels.prompt_attn(q[70:71], k, v, one, at)
     kernels.prompt_attn(q[70:71], k, v, one, at, out=out[70:71])
     assert torch.equal(out[70:71], want) and torch.equal(x[:, 4:6], kv[:, 4:])
+
+
+def test_continued_prompts_gather_the_tables_of_one_call_at_a_time(dev):
+    """9000 rows of two requests with table rows of 4096 entries: 64 MiB of tables for each 4096 rows."""
+    rows, H, D = [8000, 1000], 1, 64
+    c = PagedKVCache(layers=1, requests=2, blocks=600, heads=1, dim_head=D, max_tokens=4096 * 16, block_size=16)
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(sum(rows) + 5, H, D, generator=g).to(BF).to(dev) for _ in range(3))
+    plan = c.grow(rows, sum(rows) + 5)
+    c.append(0, k, v, plan)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = c.attend_prompts(0, q, k, v, plan, continued=True)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 96 << 20
+    ref, mag, _ = prompt_reference(q[:9000], k[:9000], v[:9000], rows, rows, True)
+    assert_attention_close(out[:9000], ref, mag, weight=2 ** -16)
+    assert (out[9000:] == 0).all()
