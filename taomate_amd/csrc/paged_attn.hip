@@ -53,11 +53,17 @@ struct PagedAttn {
   int4* joins;                 // [range]: the request that range continues first (-1: none), its ranges, its first slot
 };
 
-// Reads of the cache.  NT: more than the last-level cache holds, every byte read
-// once: non-temporal loads, which pass the caches by (a plain read of 1 GiB runs at 7.0
+// Reads of the cache.  NT: the tables could name more than the last-level cache
+// holds: non-temporal loads, which pass the caches by (a plain read of 1 GiB runs at 7.0
 // TB/s with them and at 6.2 without; 64 requests over 375 MB 68.8 us and
 // 76.3, four over 840 MB of e4m3 139 and 150).  A smaller cache that the last
 // step left in the last-level cache is slower so (10 MB: 10.5 us and 8.2).
+// The tables' width bounds what is read, and mostly from far above; a bound by the
+// pool as well would be closer and is not better, since the layers of a model take
+// turns and none finds its blocks in that cache again (tables of 16384 tokens, 8
+// heads x 128: 64 requests of 900, 243 MB, six layers in turn 44 us and 49, one
+// layer alone 43 and 40; 64 of 300, twelve layers 19 and 21, one 18 and 18.5).
+// Rows that share blocks (64 rows over 4096 tokens) take 96 us either way.
 constexpr int64_t kLastLevelBytes = 256 << 20;
 template <bool NT, typename T>
 __device__ __forceinline__ T load_cached(const char* p) {
