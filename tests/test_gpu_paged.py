@@ -760,3 +760,79 @@ def test_continued_prompts_gather_the_tables_of_one_call_at_a_time(dev):
     ref, mag, _ = prompt_reference(q[:9000], k[:9000], v[:9000], rows, rows, True)
     assert_attention_close(out[:9000], ref, mag, weight=2 ** -16)
     assert (out[9000:] == 0).all()
+
+
+EARLIER = 1 << 8   # a bit of the status word that an earlier call may have left
+
+
+@pytest.mark.parametrize("big", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("change,code", [
+    ({}, 0), ({"top": 2}, N.BLOCKS_FREE), ({"top": -1}, N.BLOCKS_FREE), ({"top": 251}, N.BLOCKS_FREE),
+    ({"width": 2, "new": 30}, N.BLOCKS_WIDTH), ({"tokens": -1}, N.BLOCKS_TOKENS),
+    ({"len": -5}, N.BLOCKS_LENGTH), ({"new": -1, "tokens": 100}, N.BLOCKS_LENGTH),
+    ({"top": 1, "width": 2, "new": 30, "tokens": -1}, N.BLOCKS_FREE | N.BLOCKS_WIDTH | N.BLOCKS_TOKENS),
+])
+def test_grow_notes_every_reason_and_no_other(dev, change, code, big, in_place):
+    block, lens, new = 16, [5, 0, 30, 16], [20, 1, 2, 1]
+    if big:
+        new[1] = 3000 if "width" not in change else 1
+    new[0] = change.get("new", new[0])
+    lens[3] = change.get("len", lens[3])
+    T = sum(new) + change.get("tokens", 0) + (2000 if big and "width" in change and "tokens" not in change else 0)
+    width, blocks = change.get("width", 200), 250
+    tables, free, top = _table_state(dev, [max(n, 0) for n in lens], block, width, blocks)
+    top = change.get("top", top)
+    t, le, fr, tp, status = ints(tables, dev), ints(lens, dev), ints(free, dev), ints([top], dev), ints([EARLIER], dev)
+    plan = kernels.kv_block_grow(t, le, ints(new, dev), fr, tp, status, block, T, le if in_place else None,
+                                 tp if in_place else None)
+    assert status.item() == EARLIER | code
+    if code == 0:
+        want = grow_reference(tables, lens, new, free, top, block, T)
+        assert t.tolist() == want[0] and plan.slots.tolist() == want[1] and plan.top.tolist() == [want[5]]
+        return
+    assert t.tolist() == tables and plan.lens.tolist() == lens and plan.top.tolist() == [top] and fr.tolist() == free
+    assert plan.starts.tolist() == [0] * 5 and plan.slots.tolist() == [-1] * T and plan.positions.tolist() == [0] * T
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("change,code", [
+    ({}, 0), ({"top": 2}, N.BLOCKS_FREE), ({"top": -1}, N.BLOCKS_FREE),
+    ({"kept": 1 << 30}, 0),                                   # a row that is not released may hold anything
+    ({"released": 16 * 5000}, N.BLOCKS_WIDTH | N.BLOCKS_FREE), ({"released": -1}, N.BLOCKS_LENGTH),
+    ({"kept": -1}, N.BLOCKS_LENGTH), ({"released": 16 * 5000, "kept": -1, "top": 0},
+                                      N.BLOCKS_WIDTH | N.BLOCKS_FREE | N.BLOCKS_LENGTH),
+])
+def test_release_notes_every_reason_and_no_other(dev, change, code, wide, in_place):
+    """``wide``: tables and a stack of more than 1024 blocks, so that the books are kept by a second launch."""
+    block, lens, done = 16, [40, 0, 17, 100], [True, True, False, True]
+    width, blocks = (1000, 3000) if wide else (8, 16)
+    tables, free, top = _table_state(dev, lens, block, width, blocks)
+    if "top" in change:
+        top = change["top"] if change["top"] <= 0 else blocks - change["top"]
+    lens[0], lens[2] = change.get("released", lens[0]), change.get("kept", lens[2])
+    t, le, fr, tp, status = ints(tables, dev), ints(lens, dev), ints(free, dev), ints([top], dev), ints([EARLIER], dev)
+    out, top_out = kernels.kv_block_release(t, le, torch.tensor(done, device=dev), fr, tp, status, block,
+                                            le if in_place else None, tp if in_place else None)
+    assert status.item() == EARLIER | code and t.tolist() == tables
+    if code == 0:
+        back = [tables[b][j] for b in (0, 3) for j in range(-(-lens[b] // block))]
+        assert out.tolist() == [0, 0, lens[2], 0] and top_out.tolist() == [top + len(back)]
+        assert fr.tolist() == free[:top] + back + free[top + len(back):]
+    else:
+        assert out.tolist() == lens and top_out.tolist() == [top] and fr.tolist() == free
+
+
+@pytest.mark.parametrize("kv,requests", [("bf16", 257), ("fp8", 514)])
+def test_token_a_wave_a_request_of_tables_past_the_last_level_cache(dev, kv, requests):
+    """Tables of 256 tokens a request, 8 heads x 128: just past 256 MiB."""
+    rng = random.Random(requests)
+    lens = [rng.choice([0, 1, 31, 32, 33, 64, 256, rng.randint(1, 60)]) for _ in range(requests)]
+    c = Cache(lens, 8, 128, 16, kv, dev, width=16)
+    q = (torch.randn(requests, 8, 128, generator=torch.Generator().manual_seed(1)) * 1.5).to(BF).to(dev)
+    ref, mag, lse_ref = c.reference(q)
+    lse = torch.empty(requests, 8, device=dev)
+    out = kernels.paged_attn(q, c.k, c.v, c.tables, c.lens_t, c.k_scales, c.v_scales, lse=lse)
+    assert_attention_close(out, ref, mag, weight=2 ** -16)
+    assert_lse_close(lse, lse_ref)
