@@ -812,7 +812,8 @@ struct Span {
     end = first + last * (int64_t)t.element_size();
   }
 };
-// out: the tensor that a result goes to (of up to four dimensions), `in` itself or memory apart from all that the call reads
+// out: the tensor that a result goes to, `in` itself or memory apart from all that
+// the call reads (all of shapes that were checked: up to four dimensions)
 void apart(const char* what, const char* name, const at::Tensor& out, std::initializer_list<Opt> read, Opt in = nullptr) {
   const Span o(out);
   for (Opt t : read) {
@@ -851,14 +852,11 @@ PyObject* kv_block_grow(PyObject* const* a) {
   counted(what, "status", status, at::kInt, 1);
   const int64_t block = integer(a[6]), tokens = integer(a[7]);
   if (tokens < 0 || tokens > 0x7FFFFFFF) value_error("kv_block_grow: tokens must lie in [0, 2^31)");
-  if (lens_to != nullptr) {
-    counted(what, "lens_out", *lens_to, at::kInt, t.B);
+  if (lens_to != nullptr) counted(what, "lens_out", *lens_to, at::kInt, t.B);
+  if (top_to != nullptr) counted(what, "top_out", *top_to, at::kInt, 1);
+  if (lens_to != nullptr)
     apart(what, "lens_out", *lens_to, {&lens, &fresh, &free, &top, &status, &tables, top_to}, &lens);
-  }
-  if (top_to != nullptr) {
-    counted(what, "top_out", *top_to, at::kInt, 1);
-    apart(what, "top_out", *top_to, {&lens, &fresh, &free, &top, &status, &tables}, &top);
-  }
+  if (top_to != nullptr) apart(what, "top_out", *top_to, {&lens, &fresh, &free, &top, &status, &tables}, &top);
   apart(what, "tables", tables, {&lens, &fresh, &free, &top, &status});
   apart(what, "status", status, {&lens, &fresh, &free, &top});
   const c10::DeviceGuard guard(tables.device());
@@ -889,14 +887,11 @@ PyObject* kv_block_release(PyObject* const* a) {
   const int64_t n_free = vector(what, "free", free, at::kInt);
   counted(what, "top", top, at::kInt, 1);
   counted(what, "status", status, at::kInt, 1);
-  if (lens_to != nullptr) {
-    counted(what, "lens_out", *lens_to, at::kInt, t.B);
+  if (lens_to != nullptr) counted(what, "lens_out", *lens_to, at::kInt, t.B);
+  if (top_to != nullptr) counted(what, "top_out", *top_to, at::kInt, 1);
+  if (lens_to != nullptr)
     apart(what, "lens_out", *lens_to, {&lens, &done, &free, &top, &status, &tables, top_to}, &lens);
-  }
-  if (top_to != nullptr) {
-    counted(what, "top_out", *top_to, at::kInt, 1);
-    apart(what, "top_out", *top_to, {&lens, &done, &free, &top, &status, &tables}, &top);
-  }
+  if (top_to != nullptr) apart(what, "top_out", *top_to, {&lens, &done, &free, &top, &status, &tables}, &top);
   apart(what, "free", free, {&lens, &done, &top, &status, &tables});
   apart(what, "status", status, {&lens, &done, &top, &tables});
   const c10::DeviceGuard guard(tables.device());

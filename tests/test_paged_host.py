@@ -198,3 +198,11 @@ def test_workspace_of_the_split():
 def test_scales_that_are_no_positive_float32_are_refused(call, scale):
     with pytest.raises(ValueError, match="scale must be a finite float32 above 0"):
         call(scale=scale)
+
+
+@pytest.mark.parametrize("call", [grow, release])
+@pytest.mark.parametrize("kw", [dict(lens_out=i32(2, 2, 2, 2, 2, 2)), dict(top_out=i32(2, 2, 2, 2, 2, 2)),
+                                dict(lens_out=i32(3), top_out=i32(2, 2, 2, 2, 2, 2))])
+def test_results_of_table_calls_are_vectors(call, kw):
+    with pytest.raises(ValueError, match="_out must be a contiguous vector"):
+        call(**kw)
