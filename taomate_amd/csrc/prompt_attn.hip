@@ -168,7 +168,8 @@ __device__ __forceinline__ void prompt_body(const PromptAttn& p) {
   constexpr float kOver = 65536.0f;      // largest per-lane tile sum kept without raising m
   // 64 channels: P(j) takes the registers of P(j-1), each word once its product
   // is issued, so that three workgroups fit a CU (168 registers): 24 prompts of
-  // up to 1023 rows, 32 heads, 44.7 us and 51.5 with two; 128 channels have no use for it
+  // up to 1023 rows, 32 heads, 44.7 us and 51.5 with two (at the start of a run; 37.7
+  // once the clock has risen); 128 channels have no use for it
   constexpr bool ONE_P = D == 64;
   constexpr float kHuge = 0x1p28f;       // |m| whose last place is 2^4 or more (exp_all)
 
@@ -669,7 +670,8 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptAttn p) {
 using namespace ltx;
 
 // Workgroups of a call and how many may share a row tile.  Few rows over many
-// keys leave most CUs idle, so the keys are split where row tiles and heads fill
+// keys leave most CUs idle, so the keys are split where row tiles and heads (pairs of a
+// row tile and a key head counted by eights, as the grid has them) fill
 // at most a quarter of the resident workgroups (half of them run each almost
 // twice as fast alone: 1024 rows over 4096 keys, 32 heads, 79 us split and 78
 // whole) and the prompts have keys enough to pay for the join: 768 on average,

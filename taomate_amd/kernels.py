@@ -211,7 +211,8 @@ def group4_linear(x: torch.Tensor, weight: Group4Weight, bias: Optional[torch.Te
 
 class BlockPlan(NamedTuple):
     """What ``kv_block_grow`` returns: the slot (int64) and position (int32) of every new token, where each
-    request's tokens start among them (int32 [requests + 1]), the lengths and the stack's top afterwards."""
+    request's tokens start among them (int32 [requests + 1]), the lengths and the stack's top afterwards.  They share
+    one allocation: clone what outlives the plan by far, such as a top or lengths that are new tensors."""
     slots: torch.Tensor
     positions: torch.Tensor
     starts: torch.Tensor

@@ -101,7 +101,8 @@ class PagedKVCache:
         """Causal attention of a plan's rows, q [tokens, query heads, dim_head].  The rows' own ``k`` and ``v`` are all
         that they see, as for requests that were empty before the plan; with ``continued`` they see everything
         that their request holds up to themselves, read from the cache after ``append`` (every row as a token of
-        its own: for a few rows a request).  Rows without a slot are zero."""
+        its own: for a few rows a request).  Rows without a slot are zero.  Without ``continued``, rows of a request
+        that held tokens before do not see them and nothing says so: the lengths lie on the device."""
         if not continued:
             return kernels.prompt_attn(q, k, v, plan.starts, scale=scale)
         kp, vp, ks, vs = self.pool(layer)
