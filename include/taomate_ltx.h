@@ -492,6 +492,8 @@ int ltx_kv_paged_append(int kv_dtype, int64_t T, int64_t H, int64_t D, const voi
  *   Calls that overlap in time must use different workspaces.
  *   Rows of q and of the pools 16-byte aligned, rows of out 8-byte; scales of a block
  *   and head 16-byte aligned.
+ *   out may be q (the same rows), and shares no other memory with what is read; nor
+ *   does lse.
  */
 int ltx_paged_attn(int kv_dtype, int64_t B, int64_t Hk, int64_t G, int64_t D, const void* q, int64_t q_bs,
                    int64_t q_hs, const void* k_pool, int64_t k_ps, int64_t k_ts, int64_t k_hs,
@@ -515,7 +517,8 @@ int ltx_paged_attn_workspace_size(int64_t B, int64_t Hk, int64_t G, int64_t D, i
  *   zero_rest != 0, else left as they are.  Starts that are not ascending or pass Tq
  *   or Tk are cut, never followed.
  *   lse: NULL or float32 [Hk * G, Tq]; scale <= 0 selects 1/sqrt(D).
- *   Rows of every tensor 16-byte aligned.
+ *   Rows of every tensor 16-byte aligned.  out may be q (the same rows), and shares
+ *   no other memory with what is read; nor does lse.
  *   workspace: ltx_prompt_attn_workspace_size() bytes, 16-byte aligned (0: none; few
  *   rows over many keys share the keys among workgroups).  Calls that overlap in
  *   time must use different workspaces.
