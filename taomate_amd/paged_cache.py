@@ -112,8 +112,9 @@ class PagedKVCache:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         for a in range(0, q.shape[0], _ROWS):
             part = slice(a, a + _ROWS)
-            tables = self.tables[request[part]]   # of this part's rows only: a row can have thousands of entries
-            kernels.paged_attn(q[part], kp, vp, tables, lens[part], ks, vs, scale=scale, out=out[part])
+            # table rows of thousands of entries: gathered for one part, and gone before the next one's
+            kernels.paged_attn(q[part], kp, vp, self.tables[request[part]], lens[part], ks, vs, scale=scale,
+                               out=out[part])
         return out
 
     def check(self) -> None:
